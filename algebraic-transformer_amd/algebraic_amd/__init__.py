@@ -7,3 +7,6 @@ Public entry points keep the reference's signatures:
 
 from .kernels.flash import flash_attention, make_variant  # noqa: F401
 from .kernels.fused_head import fused_head  # noqa: F401
+from .kernels.norm import add_rms_norm, add_rms_norm_fp8, rms_norm  # noqa: F401
+from .kernels.packed import packed_flash_attention  # noqa: F401
+from .kernels.paged import paged_append, paged_flash_attention  # noqa: F401

@@ -11,7 +11,7 @@ from pathlib import Path
 _HERE = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("ALGEBRAIC_HIP_LIB", _HERE / "libalgebraic_hip.so"))
 
-ABI_VERSION = 3  # ALG_ABI_VERSION of include/algebraic_hip.h these signatures follow
+ABI_VERSION = 4  # ALG_ABI_VERSION of include/algebraic_hip.h these signatures follow
 
 ALG_OK, ALG_ERR_INVALID, ALG_ERR_UNSUPPORTED, ALG_ERR_HIP = 0, 1, 2, 3
 DTYPE_BF16, DTYPE_F32 = 0, 1
@@ -68,6 +68,19 @@ _SIGNATURES = {
                                _S]),
     "alg_rms_norm_fwd": (_I, [_P, _I, _I, _P, _P, _F, _P, _P]),
     "alg_rms_norm_bwd": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _S]),
+    "alg_add_rms_norm_fwd": (_I, [_P, _I, _I, _P, _P, _P, _F, _P, _P, _P]),
+    "alg_add_rms_norm_fp8": (_I, [_P, _I, _I, _P, _P, _P, _F, _P, _P, _P]),
+    "alg_add_rms_norm_bwd": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _S]),
+    "alg_packed_attn_fwd": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _F, _I, _P,
+                                 _P]),
+    "alg_packed_attn_bwd_workspace_size": (_S, [_I, _I, _I, _I]),
+    "alg_packed_attn_bwd": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _F, _I, _P,
+                                 _P, _P, _L, _L, _P, _P, _P, _P, _P, _S]),
+    "alg_paged_attn_workspace_size": (_S, [_I, _I, _I, _I, _I, _I, _I]),
+    "alg_paged_attn": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _P, _I, _P,
+                            _P, _P, _I, _F, _I, _P, _P, _S]),
+    "alg_paged_append": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _L, _P, _L, _L,
+                              _L, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _F, _P]),
     "alg_timer_enable": (None, [_I]),
     "alg_timer_report": (_S, [ctypes.c_char_p, _S]),
 }
@@ -153,6 +166,27 @@ def stream_of(t):
     2 to 13 us to make, in the backward's thread above all)."""
     import torch
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+class _Here:
+    """The device is the current one already: nothing to switch and nothing to switch back."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_ALREADY = _Here()
+
+
+def device_of(t):
+    """A context in which ``t``'s device is the current one, as a launch on its stream wants."""
+    import torch
+    if t.get_device() == torch._C._cuda_getDevice():
+        return _HERE_ALREADY
+    return torch.cuda.device(t.get_device())
 
 
 def align256(nbytes):

@@ -5,7 +5,14 @@ as the model uses it before the head (src/algebraic/model.py:208): bfloat16 rows
 statistics, one rounding to bfloat16; differentiable in x and the gain, with the VJP JAX's
 autodiff forms for that expression. Both passes are HIP kernels (one wave per row); compose
 with the head as ``fused_head(rms_norm(x, g), E, t, ...)``. No CPU fallback.
+
+``add_rms_norm`` takes the residual stream's addition in front of a norm with it
+(src/algebraic/model.py:182-187: ``x = x + ...`` and the next block's ``rms_norm``), one pass
+instead of two each way; ``add_rms_norm_fp8`` leaves the norm in 8 bits with a scale per row, for
+products of 8-bit operands in inference.
 """
+
+import math
 
 import torch
 
@@ -55,3 +62,100 @@ def rms_norm(x, gain=None, eps: float = 1e-5):
     if not x.is_cuda:
         raise RuntimeError("rms_norm needs a GPU tensor (no CPU fallback)")
     return _RmsNormFn.apply(x, gain, float(eps))
+
+
+class _AddRmsNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, gain, eps):
+        lib = _lib.load()
+        d = x.shape[-1]
+        x2, r2 = _lib.aligned16(x).reshape(-1, d), _lib.aligned16(residual).reshape(-1, d)
+        rows = x2.shape[0]
+        g = _f32_gain(gain, x)
+        y, s = torch.empty_like(x2), torch.empty_like(x2)
+        tau = torch.empty(rows, dtype=torch.float32, device=x.device)
+        p = _lib.ptr
+        if rows:
+            with _lib.device_of(x2):
+                _lib.check(lib.alg_add_rms_norm_fwd(_lib.stream_of(x2), rows, d, p(x2), p(r2), p(g), eps, p(s), p(y),
+                                                    p(tau)), "add_rms_norm")
+        s = s.reshape(x.shape)
+        ctx.save_for_backward(s, g, tau)
+        ctx.gain_meta = None if gain is None else (gain.shape, gain.dtype)
+        ctx.set_materialize_grads(False)
+        return y.reshape(x.shape), s
+
+    @staticmethod
+    def backward(ctx, dy, ds):
+        s, g, tau = ctx.saved_tensors
+        if dy is None:  # the norm was not used
+            return ds, ds, None, None
+        lib = _lib.load()
+        d = s.shape[-1]
+        rows = tau.shape[0]
+        dy2 = _lib.aligned16(dy.to(s.dtype))
+        ds2 = None if ds is None else _lib.aligned16(ds.to(s.dtype))
+        dx = torch.empty_like(s, memory_format=torch.contiguous_format)
+        wants_gain = g is not None and ctx.needs_input_grad[2]
+        dg = torch.zeros(d, dtype=torch.float32, device=s.device) if wants_gain else None
+        nbytes = lib.alg_rms_norm_workspace_size(rows, d) if wants_gain else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
+        p = _lib.ptr
+        if rows:
+            with _lib.device_of(s):
+                _lib.check(lib.alg_add_rms_norm_bwd(_lib.stream_of(s), rows, d, p(s), p(g), p(tau), p(dy2), p(ds2),
+                                                    p(dx), p(dg), p(ws), nbytes), "add_rms_norm backward")
+        dgain = None if dg is None else dg.reshape(ctx.gain_meta[0]).to(ctx.gain_meta[1])
+        return dx, dx, dgain, None
+
+
+def _f32_gain(gain, x):
+    return None if gain is None else _lib.aligned16(gain.detach().to(device=x.device, dtype=torch.float32))
+
+
+def _check_add(x, residual, gain, eps, what):
+    if x.dtype != torch.bfloat16 or residual.dtype != torch.bfloat16:
+        raise NotImplementedError(f"dtypes {x.dtype}, {residual.dtype}: the gfx950 norm takes bfloat16 rows")
+    if x.shape != residual.shape or x.dim() == 0:
+        raise ValueError(f"x {tuple(x.shape)} and residual {tuple(residual.shape)} must share a shape of rows")
+    if x.device != residual.device:
+        raise ValueError(f"residual must be on {x.device}")
+    if gain is not None and gain.numel() != x.shape[-1]:
+        raise ValueError(f"gain must have {x.shape[-1]} entries")
+    if not (eps > 0) or not math.isfinite(eps):
+        raise ValueError("eps must be positive and finite")
+    if x.shape[-1] == 0 or x.shape[-1] % 8 or x.shape[-1] > 4096:
+        raise NotImplementedError(f"rows of {x.shape[-1]}: the gfx950 norm takes multiples of 8 up to 4096")
+    if not x.is_cuda:
+        raise RuntimeError(f"{what} needs GPU tensors (no CPU fallback)")
+
+
+def add_rms_norm(x, residual, gain=None, eps: float = 1e-5):
+    """``(rms_norm(s, gain), s)`` with ``s = x + residual`` rounded to bfloat16, in one pass.
+
+    bfloat16 rows of up to 4096 elements over the last axis; the norm is of the stored s.
+    Differentiable in x, residual (which have the one gradient) and the gain.
+    """
+    _check_add(x, residual, gain, eps, "add_rms_norm")
+    return _AddRmsNormFn.apply(x, residual, gain, float(eps))
+
+
+def add_rms_norm_fp8(x, residual, gain=None, eps: float = 1e-5):
+    """``(y8, scale, s)``: ``add_rms_norm`` with the norm in float8_e4m3fn and a float32 scale per
+    row, (..., 1): ``y8.float() * scale`` is the norm, its largest value of the row at 448. No
+    gradient (inference)."""
+    _check_add(x, residual, gain, eps, "add_rms_norm_fp8")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, gain)):
+        raise NotImplementedError("add_rms_norm_fp8 has no gradient: call it under torch.no_grad() or on detached tensors")
+    d = x.shape[-1]
+    x2, r2 = _lib.aligned16(x), _lib.aligned16(residual)
+    g = _f32_gain(gain, x)
+    y8 = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    s = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+    p = _lib.ptr
+    if scale.numel():
+        with _lib.device_of(x2):
+            _lib.check(_lib.load().alg_add_rms_norm_fp8(_lib.stream_of(x2), scale.numel(), d, p(x2), p(r2), p(g),
+                                                        float(eps), p(s), p(y8), p(scale)), "add_rms_norm_fp8")
+    return y8, scale, s

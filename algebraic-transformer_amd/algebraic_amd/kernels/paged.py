@@ -1,0 +1,156 @@
+"""Serving: algebraic attention of new tokens over a paged key and value cache on MI355X.
+
+The reference scores and samples by running whole rows (src/algebraic/benchmarking.py:170-190);
+here a step takes only the new tokens. One layer's step is
+
+    q = paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens,
+                     q_gain, k_gain, cos, sin)               # norm, rotation, and into the cache
+    o = paged_flash_attention(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, sink, n=n, c=c)
+
+for new tokens packed one sequence after the other (one each, chunks of prompts, or both). The
+attention is ``flash_attention``'s (src/algebraic/kernels/flash.py:763-857, ``kind="asinh"``), the
+norm and rotation those of src/algebraic/model.py:170-174. bfloat16, hand-written HIP
+(csrc/paged_decode.hip, packed_fwd.hip, paged_append.hip), no CPU fallback and no gradient. Neither
+call reads device data on the host, so a captured graph of a step serves any lengths.
+
+The cache: ``k_pages``, ``v_pages`` (pages, Hkv, page, D), strides in any order with a contiguous
+last axis ((pages, page, Hkv, D) storage is a transposed view), page a multiple of 16, D 64 or 128.
+``page_table`` (S, width) int32: position i of sequence s lies in page ``page_table[s, i // page]``;
+entries behind a sequence's end are not read, sequences may share pages that are only read.
+``cu_seqlens`` (S + 1) int32: sequence s's new tokens are ``cu_seqlens[s]:cu_seqlens[s + 1]``.
+``kv_lens`` (S) int32: the keys it holds, the new tokens (its last) among them.
+"""
+
+import math
+from typing import Optional
+
+import torch
+
+from .. import _lib
+from .flash import _sink_input
+from .packed import _check_heads, _check_index, _check_scale, _check_sink, _rows, _strided
+
+
+def _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != Hkv or k_pages.shape[3] != q.shape[2]:
+        raise ValueError(f"k_pages and v_pages must share the shape (pages, Hkv, page, {q.shape[2]})")
+    pages, _, page, D = k_pages.shape
+    if D not in (64, 128):
+        raise NotImplementedError(f"head_dim {D}: the gfx950 cache kernels are built for 64 and 128")
+    if pages == 0 or page == 0 or page % 16:
+        raise NotImplementedError(f"{pages} pages of {page} positions: pages hold a positive multiple of 16")
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if t.dtype != torch.bfloat16:
+            raise NotImplementedError(f"dtype {t.dtype}: the gfx950 cache kernels take bfloat16")
+        if t.device != q.device:
+            raise ValueError(f"{name} must be on {q.device}")
+        ps, hs, ts, one = t.stride()
+        if one != 1 or ps % 8 or hs % 8 or ts % 8 or min(ps, ts) < D or (hs < D and t.shape[1] > 1) or t.data_ptr() % 16:
+            raise ValueError(f"{name}: the last axis must be contiguous and the others start on 16 bytes")
+    if kv_lens.dim() != 1:
+        raise ValueError("kv_lens must be (S,)")
+    S = kv_lens.shape[0]
+    _check_index("kv_lens", kv_lens, (S,), q)
+    _check_index("cu_seqlens", cu_seqlens, (S + 1,), q)
+    if page_table.dim() != 2 or page_table.shape[0] != S or page_table.shape[1] == 0:
+        raise ValueError(f"page_table must be ({S}, width)")
+    _check_index("page_table", page_table, tuple(page_table.shape), q)
+
+
+def _no_gradient(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def _page_args(t):
+    return t.data_ptr(), t.stride(0), max(t.stride(1), t.shape[3]), t.stride(2)
+
+
+def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, q_gain=None, k_gain=None, cos=None,
+                 sin=None, *, eps: float = 1e-5):
+    """Norm and rotate the new tokens' q (N, H, D) and k (N, Hkv, D) and put k and v into the cache.
+
+    Token t of sequence s stands at position ``kv_lens[s] - new + t``, ``new`` the number of its new
+    tokens; q and k become ``rot(x / rms(x) gain)`` in f32, rounded once, with the tables' row of that
+    position (``cos``, ``sin`` (>= width page, D/2) float32, or both None: no rotation) and gains (D,)
+    or None. Returns the queries (N, H, D); ``k_pages`` and ``v_pages`` are written in place, one
+    place a token. A token whose position or page number is out of range is not written; its query,
+    and those behind the last sequence, are zero. Two tokens in one place: either is kept.
+    """
+    _check_heads(q, k, v)
+    _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, k.shape[1])
+    if not (eps > 0) or not math.isfinite(eps):
+        raise ValueError("eps must be positive and finite")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin are given together")
+    N, H, D = q.shape
+    reach = page_table.shape[1] * k_pages.shape[2]
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t is not None and (t.dim() != 2 or t.shape[0] < reach or t.shape[1] != D // 2):
+            raise ValueError(f"{name} must be (>= {reach}, {D // 2})")
+    for name, g in (("q_gain", q_gain), ("k_gain", k_gain)):
+        if g is not None and g.numel() != D:
+            raise ValueError(f"{name} must have {D} entries")
+    _no_gradient("paged_append", q, k, v, k_pages, v_pages, q_gain, k_gain)
+    if not q.is_cuda:
+        raise RuntimeError("paged_append needs GPU tensors (no CPU fallback)")
+    out = torch.empty((N, H, D), dtype=q.dtype, device=q.device)
+    if N == 0:
+        return out
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    page_table, cu, kv = page_table.contiguous(), cu_seqlens.contiguous(), kv_lens.contiguous()
+    f32 = lambda t: None if t is None else _lib.aligned16(t.detach().to(device=q.device, dtype=torch.float32))  # noqa: E731
+    gq, gk, cs, sn = f32(q_gain), f32(k_gain), f32(cos), f32(sin)
+    rows = 0 if cs is None else min(cs.shape[0], sn.shape[0])
+    p = _lib.ptr
+    with _lib.device_of(q):
+        _lib.check(_lib.load().alg_paged_append(
+            _lib.stream_of(q), N, kv.shape[0], H, k.shape[1], D, *_strided(q), *_strided(k), *_strided(v),
+            *_page_args(k_pages), *_page_args(v_pages), k_pages.shape[0], k_pages.shape[2], p(page_table),
+            page_table.shape[1], p(cu), p(kv), p(gq), p(gk), p(cs), p(sn), rows, eps, p(out)), "paged_append")
+    return out
+
+
+def paged_flash_attention(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, sink_logit: Optional[torch.Tensor] = None,
+                          *, n: int = 16, c: float = 16.0):
+    """Attention of the new tokens q (N, H, D) over the keys their sequences hold, (N, H, D).
+
+    Token t of sequence s attends to positions up to ``kv_lens[s] - new + t``; query head h reads key
+    head ``h // (H // Hkv)``. q's strides as in ``packed_flash_attention``; ``sink_logit`` broadcasts
+    to (H,). Tokens behind the last sequence, or before position 0, get zeros. What pages hold behind
+    a sequence's end is not read; a page number outside the cache makes the outputs that would have
+    read it NaN. The order of every sum is fixed by the shapes.
+    """
+    if k_pages.dim() != 4:
+        raise ValueError("k_pages and v_pages must be (pages, Hkv, page, D)")
+    if q.dim() != 3:
+        raise ValueError("q must be (tokens, heads, D)")
+    if q.dtype != torch.bfloat16:
+        raise NotImplementedError(f"dtype {q.dtype}: the gfx950 cache kernels take bfloat16")
+    N, H, D = q.shape
+    Hkv = k_pages.shape[1]
+    if H == 0 or Hkv == 0 or H % Hkv:
+        raise ValueError(f"{H} query heads do not share {Hkv} key heads evenly")
+    _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv)
+    _check_scale(n, c)
+    _check_sink(sink_logit, q)
+    _no_gradient("paged_flash_attention", q, k_pages, v_pages, sink_logit)
+    if not q.is_cuda:
+        raise RuntimeError("paged_flash_attention needs GPU tensors (no CPU fallback)")
+    o = torch.empty((N, H, D), dtype=q.dtype, device=q.device)
+    if N == 0:
+        return o
+    lib = _lib.load()
+    q = _rows(q)
+    page_table, cu, kv = page_table.contiguous(), cu_seqlens.contiguous(), kv_lens.contiguous()
+    S, width, page = kv.shape[0], page_table.shape[1], k_pages.shape[2]
+    sink = _sink_input(sink_logit, H, q.device)
+    nbytes = lib.alg_paged_attn_workspace_size(N, S, H, Hkv, D, width, page)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    p = _lib.ptr
+    with _lib.device_of(q):
+        _lib.check(lib.alg_paged_attn(
+            _lib.stream_of(q), N, S, H, Hkv, D, *_strided(q), *_page_args(k_pages), *_page_args(v_pages),
+            k_pages.shape[0], page, p(page_table), width, p(cu), p(kv), p(sink), 0 if sink is None else sink.numel(),
+            float(c), int(n), p(o), p(ws), nbytes), "paged_flash_attention")
+    return o

@@ -826,34 +826,6 @@ __global__ __launch_bounds__(256, bwd_bf16_waves_per_simd<D>()) void attn_bwd_bf
   if (blockIdx.x == gridDim.x - 1) attn_sink_grad(p, ceil_div(T_, SINK_ROWS));
 }
 
-// LDS layout of the 16-key dK/dV kernel's Q / dO tiles (64 rows of D bf16) and the lane
-// mapping of its fragments, chosen with the bank-conflict counter so that both kinds of
-// fragment read are conflict-free (each alternative listed cost 2-4 extra cycles per read):
-//   D = 128: chunk c of row r at c ^ (4(r&3) + ((r>>2)&3)) (the attention kernels' swizzle);
-//            MFMA row m of a 16-query block is tile row sigma(m) (0..7 -> {0..3, 8..11}, 8..15
-//            -> {4..7, 12..15}); lane group g reads k chunk 4g + s at step s (not 4s + g);
-//            the transposed reads' row quads are qoff(g) = 0, 8, 4, 12 (not 4g);
-//   D = 64:  chunk c of row r at c ^ (r & 7) (the attention kernels' D = 64 swizzle costs 4
-//            extra cycles per row-fragment read with every mapping tried); identity rows, k
-//            chunk 4s + g, quads 4g.
-// Lane group g then owns queries 16 b + quad(g) + i in register i of query block b.
-template <int D>
-struct Dkdv16Lay;
-template <>
-struct Dkdv16Lay<128> {
-  static __device__ __forceinline__ int swz(int r) { return swz_chunk<16>(r); }
-  static __device__ __forceinline__ int arow(int m) { return (m & 3) | ((m & 4) << 1) | ((m & 8) >> 1); }
-  static __device__ __forceinline__ int dcol(int g, int s) { return 32 * g + 8 * s; }
-  static __device__ __forceinline__ int quad(int g) { return 4 * (((g & 1) << 1) | (g >> 1)); }
-};
-template <>
-struct Dkdv16Lay<64> {
-  static __device__ __forceinline__ int swz(int r) { return r & 7; }
-  static __device__ __forceinline__ int arow(int m) { return m; }
-  static __device__ __forceinline__ int dcol(int g, int s) { return 32 * s + 8 * g; }
-  static __device__ __forceinline__ int quad(int g) { return 4 * g; }
-};
-
 // dK/dV kernel for bf16 inputs built for two or more waves per SIMD: 16 keys per wave on
 // v_mfma_f32_16x16x32_bf16, NW waves per workgroup (16 NW keys of one head). At D = 128 a
 // wave's dK/dV accumulators take 64 registers (16 keys x 128 d x 2 / 64 lanes) and its K/V

@@ -311,7 +311,7 @@ int noalloc_scratch(void** out) {
 extern "C" {
 
 const char* alg_last_error(void) { return g_err.c_str(); }
-const char* alg_version(void) { return "algebraic_hip 0.3 gfx950 (ABI 3)"; }
+const char* alg_version(void) { return "algebraic_hip 0.4 gfx950 (ABI 4)"; }
 int alg_abi_version(void) { return ALG_ABI_VERSION; }
 
 size_t alg_attn_workspace_size(int dtype, int B, int H, int T, int D) {
@@ -1124,6 +1124,294 @@ int alg_head_bwd_streamed(alg_stream_t stream, int dtype, int N, int d, int V, c
   p.dh_part = ws.nchunks > 1 ? reinterpret_cast<float*>(w + ws.acc) : nullptr;
   p.de_part = ws.has_de_part ? reinterpret_cast<float*>(w + ws.de_part) : nullptr;
   return hip_status(alg::launch_head_bwd_streamed(p, ws.chunk, (hipStream_t)stream), "alg_head_bwd_streamed");
+}
+
+// ---- residual norm ----------------------------------------------------------------------------
+
+static alg::RmsNormParams add_norm_params(int rows, int d, const void* x, const void* res, const float* gain, float eps,
+                                          void* sum) {
+  alg::RmsNormParams p;
+  std::memset(&p, 0, sizeof p);
+  p.x = static_cast<const bf16*>(x); p.res = static_cast<const bf16*>(res); p.gain = gain;
+  p.sum = static_cast<bf16*>(sum);
+  p.rows = rows; p.d = d; p.eps = eps;
+  return p;
+}
+
+int alg_add_rms_norm_fwd(alg_stream_t stream, int rows, int d, const void* x, const void* res, const float* gain,
+                         float eps, void* sum, void* y, float* tau) {
+  const int rc = check_rms_norm(rows, d, eps);
+  if (rc) return rc;
+  if (!x || !res || !sum || !y || !tau) return fail(ALG_ERR_INVALID, "x, res, sum, y and tau are required");
+  if (!aligned16({x, res, gain, sum, y})) return fail(ALG_ERR_INVALID, "matrices and gain must be 16-byte aligned");
+  alg::RmsNormParams p = add_norm_params(rows, d, x, res, gain, eps, sum);
+  p.y = static_cast<bf16*>(y); p.tau = tau;
+  return hip_status(alg::launch_add_rms_norm(p, (hipStream_t)stream), "alg_add_rms_norm_fwd");
+}
+
+int alg_add_rms_norm_fp8(alg_stream_t stream, int rows, int d, const void* x, const void* res, const float* gain,
+                         float eps, void* sum, void* y8, float* scale) {
+  const int rc = check_rms_norm(rows, d, eps);
+  if (rc) return rc;
+  if (!x || !res || !sum || !y8 || !scale) return fail(ALG_ERR_INVALID, "x, res, sum, y8 and scale are required");
+  if (!aligned16({x, res, gain, sum, y8})) return fail(ALG_ERR_INVALID, "matrices and gain must be 16-byte aligned");
+  alg::RmsNormParams p = add_norm_params(rows, d, x, res, gain, eps, sum);
+  p.y8 = static_cast<unsigned char*>(y8); p.scale = scale;
+  return hip_status(alg::launch_add_rms_norm(p, (hipStream_t)stream), "alg_add_rms_norm_fp8");
+}
+
+int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, const float* gain, const float* tau,
+                         const void* dy, const void* dsum, void* dx, float* dgain, void* workspace,
+                         size_t workspace_bytes) {
+  const int rc = check_rms_norm(rows, d, 1.0f);
+  if (rc) return rc;
+  if (!sum || !tau || !dy || !dx) return fail(ALG_ERR_INVALID, "sum, tau, dy and dx are required");
+  if (!aligned16({sum, gain, dy, dsum, dx})) return fail(ALG_ERR_INVALID, "matrices and gain must be 16-byte aligned");
+  if (dgain && !gain) return fail(ALG_ERR_INVALID, "a gain gradient needs the gain it differentiates");
+  const size_t need = alg_rms_norm_workspace_size(rows, d);
+  if (dgain && (!workspace || workspace_bytes < need))
+    return fail(ALG_ERR_INVALID, "workspace too small: need %zu bytes", need);
+  alg::RmsNormParams p;
+  std::memset(&p, 0, sizeof p);
+  p.x = static_cast<const bf16*>(sum); p.gain = gain; p.tau = const_cast<float*>(tau);
+  p.dy = static_cast<const bf16*>(dy); p.dsum = static_cast<const bf16*>(dsum); p.dx = static_cast<bf16*>(dx);
+  p.gpart = dgain ? static_cast<float*>(workspace) : nullptr;
+  p.rows = rows; p.d = d;
+  return hip_status(alg::launch_rms_norm_bwd(p, dgain, (hipStream_t)stream), "alg_add_rms_norm_bwd");
+}
+
+// ---- packed sequences and paged caches --------------------------------------------------------
+
+// The arithmetic of one call's weights (packed_common.h): R = 4 holds |x| up to 1.875 in the plain
+// form, R = 2 up to 0.75 for n = 32; larger exponents would leave f32 and take the careful form.
+static alg::AttnScale attn_scale(int n, float c, int D) {
+  alg::AttnScale s;
+  s.log2n = log2_pow2(n);
+  const double alpha = 1.0 / (std::sqrt((double)D) * (double)c);
+  const double R = n <= 16 ? 4.0 : (n == 32 ? 2.0 : 1.0);
+  const int e = (int)std::ceil(std::log2(R / alpha));
+  const double a = std::ldexp(alpha, e);
+  s.qmul = (float)std::ldexp(1.0, -e);
+  s.a = (float)a;
+  s.b = (float)(1.0 / (a * a));
+  s.bound = n <= 32 ? (float)(0.5 * (R - 1.0 / R) / a) : -1.0f;
+  return s;
+}
+
+static int check_packed(int N, int S, int H, int Hkv, int D, float c, int n, const int* cu, const float* sink,
+                        int sink_count) {
+  if (N < 0 || S < 0) return fail(ALG_ERR_INVALID, "N and S must not be negative (got %d, %d)", N, S);
+  if (H <= 0 || Hkv <= 0 || H % Hkv) return fail(ALG_ERR_INVALID, "H = %d must be a positive multiple of Hkv = %d", H, Hkv);
+  if (D != 64 && D != 128) return fail(ALG_ERR_UNSUPPORTED, "head_dim %d: gfx950 kernels are built for D in {64, 128}", D);
+  if (H / Hkv > 128) return fail(ALG_ERR_UNSUPPORTED, "%d query heads to a key head: at most 128", H / Hkv);
+  // Rows are counted in 32 bits, and so are a grid's workgroups (a slot and key head each) and their
+  // threads.
+  if ((double)N * H >= 2147483648.0 - 1024.0) return fail(ALG_ERR_UNSUPPORTED, "N H = %d %d rows: at most 2^31 - 1024", N, H);
+  if (((double)N * H / 16.0 + (S + 1.0) * Hkv + H) * 256.0 >= 4294967296.0)
+    return fail(ALG_ERR_UNSUPPORTED, "too many rows and sequences for one launch");
+  if (const int rc = check_n(n)) return rc;
+  if (!(c > 0.0f) || !std::isfinite(c)) return fail(ALG_ERR_INVALID, "asinh scale c must be positive and finite");
+  if (c < 0x1p-30f || c > 0x1p30f) return fail(ALG_ERR_UNSUPPORTED, "asinh scale c = %g: built for 2^-30 to 2^30", (double)c);
+  if (!cu) return fail(ALG_ERR_INVALID, "cu_seqlens is required");
+  if (sink && sink_count != 1 && sink_count != H) return fail(ALG_ERR_INVALID, "sink_count must be 1 or H");
+  return ALG_OK;
+}
+
+// Strides in elements of rows that are read 16 bytes a lane: multiples of 8, rows that do not
+// overlap, 64 tokens and a group's heads within 32-bit byte offsets.
+static int check_strides(const char* name, const void* base, long ts, long hs, int heads, int D) {
+  if (!aligned16({base})) return fail(ALG_ERR_INVALID, "%s must be 16-byte aligned", name);
+  if (ts % 8 || hs % 8 || ts < D || (heads > 1 && hs < D))
+    return fail(ALG_ERR_INVALID, "%s: strides (%ld, %ld) must be multiples of 8 and at least %d", name, ts, hs, D);
+  if (66.0 * (double)ts + (double)heads * (double)hs + D >= 1073741824.0)
+    return fail(ALG_ERR_UNSUPPORTED, "%s: strides (%ld, %ld) pass 32-bit offsets", name, ts, hs);
+  return ALG_OK;
+}
+
+int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                        const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
+                        const float* sink, int sink_count, float c, int n, void* o, float* stat) {
+  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_count);
+  if (rc) return rc;
+  if (N == 0) return ALG_OK;
+  if (!q || !k || !v || !o || !stat) return fail(ALG_ERR_INVALID, "null argument");
+  rc = check_strides("q", q, q_ts, q_hs, H, D);
+  if (!rc) rc = check_strides("k", k, k_ts, k_hs, Hkv, D);
+  if (!rc) rc = check_strides("v", v, v_ts, v_hs, Hkv, D);
+  if (!rc) rc = check_strides("o", o, (long)H * D, D, H, D);
+  if (rc) return rc;
+  alg::PackedParams p;
+  std::memset(&p, 0, sizeof p);
+  p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
+  p.o = static_cast<bf16*>(o); p.stat = stat;
+  p.sink = sink; p.sink_count = sink_count; p.c = c; p.cu = cu;
+  p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
+  p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
+  p.sc = attn_scale(n, c, D);
+  p.nsplit = 1;
+  return hip_status(alg::launch_packed_fwd(p, D, false, (hipStream_t)stream), "alg_packed_attn_fwd");
+}
+
+// Backward workspace: [di f32 N H][the slots' forms i32].
+struct PackedBwdWs {
+  size_t care, total;
+};
+static PackedBwdWs packed_bwd_ws(int N, int S, int H, int Hkv) {
+  PackedBwdWs w;
+  w.care = align256((size_t)N * H * sizeof(float));
+  w.total = w.care + align256((size_t)alg::packed_slots(N, H / Hkv, S, alg::PK_ROWS) * Hkv * sizeof(int));
+  return w;
+}
+
+size_t alg_packed_attn_bwd_workspace_size(int N, int S, int H, int Hkv) {
+  if (N <= 0 || S < 0 || H <= 0 || Hkv <= 0 || H % Hkv) return 0;
+  return packed_bwd_ws(N, S, H, Hkv).total;
+}
+
+int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                        const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
+                        const float* sink, int sink_count, float c, int n, const void* o, const float* stat,
+                        const void* dO, long do_ts, long do_hs, void* dq, void* dk, void* dv, float* dsink,
+                        void* workspace, size_t workspace_bytes) {
+  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_count);
+  if (rc) return rc;
+  if (dsink && !sink) return fail(ALG_ERR_INVALID, "a sink gradient needs the sink it differentiates");
+  if (N == 0) return dsink ? fail(ALG_ERR_INVALID, "a sink gradient needs tokens") : ALG_OK;
+  if (!q || !k || !v || !o || !stat || !dO || !dq || !dk || !dv) return fail(ALG_ERR_INVALID, "null argument");
+  rc = check_strides("q", q, q_ts, q_hs, H, D);
+  if (!rc) rc = check_strides("k", k, k_ts, k_hs, Hkv, D);
+  if (!rc) rc = check_strides("v", v, v_ts, v_hs, Hkv, D);
+  if (!rc) rc = check_strides("dO", dO, do_ts, do_hs, H, D);
+  if (rc) return rc;
+  if (!aligned16({o, dq, dk, dv, workspace})) return fail(ALG_ERR_INVALID, "o, dq, dk, dv and workspace must be 16-byte aligned");
+  const PackedBwdWs ws = packed_bwd_ws(N, S, H, Hkv);
+  if (!workspace || workspace_bytes < ws.total)
+    return fail(ALG_ERR_INVALID, "workspace too small: need %zu bytes", ws.total);
+  alg::PackedBwdParams p;
+  std::memset(&p, 0, sizeof p);
+  p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
+  p.o = static_cast<const bf16*>(o); p.dO = static_cast<const bf16*>(dO); p.stat = stat;
+  p.di = static_cast<float*>(workspace);
+  p.care = reinterpret_cast<int*>(static_cast<char*>(workspace) + ws.care);
+  p.sink = sink; p.sink_count = sink_count; p.c = c; p.cu = cu;
+  p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
+  p.do_ts = do_ts; p.do_hs = do_hs;
+  p.dq = static_cast<bf16*>(dq); p.dk = static_cast<bf16*>(dk); p.dv = static_cast<bf16*>(dv); p.dsink = dsink;
+  p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
+  p.sc = attn_scale(n, c, D);
+  return hip_status(alg::launch_packed_bwd(p, D, (hipStream_t)stream), "alg_packed_attn_bwd");
+}
+
+static int check_pages(const char* name, const void* base, long ps, long hs, long ts, int Hkv, int page, int D) {
+  int rc = check_strides(name, base, ts, hs, Hkv, D);
+  if (!rc && (ps % 8 || ps < D)) rc = fail(ALG_ERR_INVALID, "%s: page stride %ld must be a multiple of 8 and at least %d", name, ps, D);
+  if (!rc && (page <= 0 || page % 16)) rc = fail(ALG_ERR_UNSUPPORTED, "pages of %d positions: a positive multiple of 16", page);
+  return rc;
+}
+static int check_table(int width, int page, int pages) {
+  if (width <= 0 || pages <= 0) return fail(ALG_ERR_INVALID, "the page table's width and the pages must be positive");
+  if ((double)width * page > 2147483647.0 - 256.0) return fail(ALG_ERR_UNSUPPORTED, "%d pages of %d positions a sequence: at most 2^31", width, page);
+  return ALG_OK;
+}
+
+// How a paged call runs: which kernel, on rows per workgroup, and over how many ranges of keys.
+// Rows: a sequence's average, since the lengths are on the device. Up to 16 or 32 of them take the
+// kernel whose waves split the keys; more, the one whose waves split 128 rows. Ranges: as many as
+// bring the launch to two workgroups a CU, while a range keeps 512 keys (or 1024 of the larger
+// kernel, whose partial sums are 128 rows) of a sequence as long as the table allows.
+struct PagedPlan {
+  int row_tiles;  // 1, 2: 16 or 32 rows (paged_decode); 0: 128 (packed_fwd)
+  int nsplit;
+  size_t zt, total;  // workspace: [partial sums f32][Z, T f32]
+};
+static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int page) {
+  PagedPlan pl;
+  const long G = H / Hkv, rows = N * G, each = (rows + std::max(S, 1) - 1) / std::max(S, 1);
+  pl.row_tiles = each <= 16 ? 1 : (each <= 32 ? 2 : 0);
+  const long tile = pl.row_tiles ? 16 * pl.row_tiles : alg::PK_ROWS;
+  const long groups = std::max(1L, std::max((rows + tile - 1) / tile, (long)std::min(S, N)) * Hkv);
+  const long cap = (long)width * page, least = pl.row_tiles ? 512 : 1024;
+  pl.nsplit = (int)std::max(1L, std::min(std::min((512 + groups - 1) / groups, 64L), cap / least));
+  const size_t parts = pl.nsplit > 1 ? (size_t)pl.nsplit * N * H : 0;
+  pl.zt = align256(parts * D * sizeof(float));
+  pl.total = pl.zt + align256(parts * 2 * sizeof(float));
+  return pl;
+}
+
+size_t alg_paged_attn_workspace_size(int N, int S, int H, int Hkv, int D, int width, int page) {
+  if (N <= 0 || S < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || width <= 0 || page <= 0) return 0;
+  return paged_plan(N, S, H, Hkv, D, width, page).total;
+}
+
+int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                   const void* k_pages, long k_ps, long k_hs, long k_ts, const void* v_pages, long v_ps, long v_hs,
+                   long v_ts, int pages, int page, const int* table, int width, const int* cu, const int* kv_lens,
+                   const float* sink, int sink_count, float c, int n, void* o, void* workspace, size_t workspace_bytes) {
+  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_count);
+  if (!rc) rc = check_table(width, page, pages);
+  if (rc) return rc;
+  if (N == 0) return ALG_OK;
+  if (!q || !k_pages || !v_pages || !o || !table || !kv_lens) return fail(ALG_ERR_INVALID, "null argument");
+  rc = check_strides("q", q, q_ts, q_hs, H, D);
+  if (!rc) rc = check_pages("k_pages", k_pages, k_ps, k_hs, k_ts, Hkv, page, D);
+  if (!rc) rc = check_pages("v_pages", v_pages, v_ps, v_hs, v_ts, Hkv, page, D);
+  if (!rc) rc = check_strides("o", o, (long)H * D, D, H, D);
+  if (rc) return rc;
+  const PagedPlan pl = paged_plan(N, S, H, Hkv, D, width, page);
+  if (pl.total && (!workspace || workspace_bytes < pl.total))
+    return fail(ALG_ERR_INVALID, "workspace too small: need %zu bytes", pl.total);
+  if (!aligned16({workspace})) return fail(ALG_ERR_INVALID, "workspace must be 16-byte aligned");
+  alg::PackedParams p;
+  std::memset(&p, 0, sizeof p);
+  p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k_pages); p.v = static_cast<const bf16*>(v_pages);
+  p.o = static_cast<bf16*>(o);
+  p.sink = sink; p.sink_count = sink_count; p.c = c; p.cu = cu; p.kv_lens = kv_lens;
+  p.table = table; p.width = width; p.page = page; p.pages = pages;
+  p.q_ts = q_ts; p.q_hs = q_hs;
+  p.k_ts = k_ts; p.k_hs = k_hs; p.k_ps = k_ps; p.v_ts = v_ts; p.v_hs = v_hs; p.v_ps = v_ps;
+  p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
+  p.sc = attn_scale(n, c, D);
+  p.nsplit = pl.nsplit;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_zt = pl.total ? reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.zt) : nullptr;
+  return hip_status(pl.row_tiles ? alg::launch_paged_decode(p, D, pl.row_tiles, (hipStream_t)stream)
+                                 : alg::launch_packed_fwd(p, D, true, (hipStream_t)stream),
+                    "alg_paged_attn");
+}
+
+int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                     const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
+                     long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, int pages, int page,
+                     const int* table, int width, const int* cu, const int* kv_lens, const float* q_gain,
+                     const float* k_gain, const float* cos, const float* sin, int table_rows, float eps, void* q_out) {
+  int rc = check_packed(N, S, H, Hkv, D, 1.0f, 2, cu, nullptr, 0);
+  if (!rc) rc = check_table(width, page, pages);
+  if (rc) return rc;
+  if (!(eps > 0.0f) || !std::isfinite(eps)) return fail(ALG_ERR_INVALID, "eps must be positive and finite");
+  if (!cos != !sin) return fail(ALG_ERR_INVALID, "cos and sin are given together");
+  if (cos && (long)table_rows < (long)width * page)
+    return fail(ALG_ERR_INVALID, "rotation tables of %d rows for %ld positions", table_rows, (long)width * page);
+  if (N == 0) return ALG_OK;
+  if (!q || !k || !v || !k_pages || !v_pages || !q_out || !table || !kv_lens) return fail(ALG_ERR_INVALID, "null argument");
+  rc = check_strides("q", q, q_ts, q_hs, H, D);
+  if (!rc) rc = check_strides("k", k, k_ts, k_hs, Hkv, D);
+  if (!rc) rc = check_strides("v", v, v_ts, v_hs, Hkv, D);
+  if (!rc) rc = check_pages("k_pages", k_pages, k_ps, kp_hs, kp_ts, Hkv, page, D);
+  if (!rc) rc = check_pages("v_pages", v_pages, v_ps, vp_hs, vp_ts, Hkv, page, D);
+  if (rc) return rc;
+  if (!aligned16({q_out, q_gain, k_gain, cos, sin}))
+    return fail(ALG_ERR_INVALID, "q_out, gains and tables must be 16-byte aligned");
+  alg::PagedAppendParams p;
+  std::memset(&p, 0, sizeof p);
+  p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
+  p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
+  p.kp = static_cast<bf16*>(k_pages); p.vp = static_cast<bf16*>(v_pages);
+  p.kp_ps = k_ps; p.kp_hs = kp_hs; p.kp_ts = kp_ts; p.vp_ps = v_ps; p.vp_hs = vp_hs; p.vp_ts = vp_ts;
+  p.qo = static_cast<bf16*>(q_out);
+  p.cu = cu; p.kv_lens = kv_lens; p.table = table; p.width = width; p.page = page; p.pages = pages;
+  p.q_gain = q_gain; p.k_gain = k_gain; p.cos = cos; p.sin = sin; p.eps = eps;
+  p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.D = D;
+  return hip_status(alg::launch_paged_append(p, (hipStream_t)stream), "alg_paged_append");
 }
 
 }  // extern "C"

@@ -135,6 +135,12 @@ struct RmsNormParams {
   float* gpart;         // VJP: (nblocks, d) gain-gradient partials and their group sums, or nullptr
   int rows, d;
   float eps;
+  // With the residual's addition (x: the block's output).
+  const bf16* res = nullptr;  // the residual stream (rows, d)
+  bf16* sum = nullptr;        // round(x + res)
+  unsigned char* y8 = nullptr;  // e4m3 output (rows, d) and its scales (rows,), in the place of y
+  float* scale = nullptr;
+  const bf16* dsum = nullptr;  // VJP: cotangent of sum, or nullptr
 };
 
 }  // namespace alg

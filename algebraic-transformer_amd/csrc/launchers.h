@@ -7,6 +7,7 @@
 #include "attn_common.h"
 #include "attn_prep.h"
 #include "head_params.h"
+#include "packed_common.h"
 
 namespace alg {
 
@@ -100,5 +101,11 @@ int ffn_gate_up_tile(int N, int F, int d);
 int ffn_dy_tile(int N, int F, int dm);
 hipError_t launch_ffn_gemm(const FfnGemmParams& g, int a_mode, int b_mode, hipStream_t st);
 hipError_t launch_rms_norm_bwd(const RmsNormParams& p, float* dgain, hipStream_t st);
+hipError_t launch_add_rms_norm(const RmsNormParams& p, hipStream_t st);
+hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t st);
+hipError_t launch_packed_bwd(const PackedBwdParams& p, int D, hipStream_t st);
+hipError_t launch_packed_fwd(const PackedParams& p, int D, bool paged, hipStream_t st);
+hipError_t launch_packed_combine(const PackedParams& p, int D, hipStream_t st);
+hipError_t launch_paged_decode(const PackedParams& p, int D, int row_tiles, hipStream_t st);
 
 }  // namespace alg

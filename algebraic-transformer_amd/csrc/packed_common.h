@@ -1,0 +1,167 @@
+// Attention over packed sequences and over a paged cache: parameters, the weights' arithmetic and
+// the mapping of workgroups to sequences, shared by packed_fwd.hip, packed_bwd.hip and
+// paged_decode.hip.
+//
+// Weights without a pass ahead of them. With x = q.k alpha, alpha = 1/(sqrt(D) c), the weight of a
+// key is rho(x)^n, rho(x) = x + sqrt(1 + x^2). The kernels form s = (q 2^-e).k (a power of two:
+// exact) and t = s + sqrt(s^2 + b), b = 1/a^2, a = alpha 2^e; then t = rho(x) / a, and the factor
+// a^-n, common to a row's weights and its sink, cancels in the normalisation. No rounding of a
+// scaled query and no multiplication per score is left. e makes a in [R, 2 R), R the rho of the
+// bound X on |x| (AttnScale): inside the bound t is at most 1, and t^n at least 2^-80 at n = 16
+// (2^-96 at n = 32), so plain f32 sums of t^n and of t^n v neither overflow nor vanish. A
+// workgroup keeps the largest |s| that it sees (half an instruction per score); if one lies
+// outside the bound, it does its rows again in the careful form: a running maximum per row, and
+// rho of a negative x as 1/rho(-x), which plain f32 would lose to cancellation.
+// The row statistic is rs = (row's shift) Z^(-1/n), so that a normalised weight is (t rs)^n in
+// either form; its sign tells the backward pass which form the row took (negative: careful).
+//
+// Rows. The H query heads share Hkv key heads in groups of G = H / Hkv. The G queries of one token
+// at one key head are neighbours in a row index r = t G + g of the sequence, so that a tile of 128
+// rows holds 128 / G tokens, K and V are read once for the group, dK and dV add up over the group
+// inside one workgroup, and a single token's G queries share a tile.
+//
+// Sequences. cu[s] is the first token of sequence s. Sequence s owns the work slots from
+// cu[s] G / ROWS + s on: at least as many as it has tiles, so that a workgroup finds its sequence
+// by a search over cu, without a list made ahead; a slot past a sequence's tiles ends at once
+// (at most one a sequence). The tokens from cu[S] on belong to no sequence: their outputs and
+// gradients are zero.
+#pragma once
+
+#include "attn_common.h"
+
+namespace alg {
+
+constexpr int PK_ROWS = 128;  // rows (token, head of the group) per workgroup of the prompt kernels
+constexpr int PK_BK = 64;     // keys per LDS tile
+
+// How scores become weights for one call (host: attn_scale).
+struct AttnScale {
+  int log2n;
+  float qmul;   // 2^-e, applied to the queries (exact in bf16 but for subnormals)
+  float a;      // alpha 2^e: x = a s
+  float b;      // 1 / a^2
+  float bound;  // largest |s| of the plain form; negative: every row takes the careful form
+};
+
+struct PackedParams {
+  const bf16* q;   // (N, H, D)
+  const bf16* k;   // packed: (N, Hkv, D); paged: pages of (Hkv, page, D)
+  const bf16* v;
+  bf16* o;         // (N, H, D), contiguous
+  float* stat;     // (Hkv, N G) row statistics, or nullptr
+  const float* sink;  // logits, `sink_count` (1 or H) of them, or nullptr
+  int sink_count;
+  float c;
+  const int* cu;   // (S + 1)
+  const int* kv_lens;  // paged: (S) keys held, the new tokens among them
+  const int* table;    // paged: (S, width) page numbers
+  int width, page, pages;
+  long q_ts, q_hs;             // elements between tokens, between heads
+  long k_ts, k_hs, k_ps;       // tokens, heads, pages
+  long v_ts, v_hs, v_ps;
+  int N, S, H, Hkv, G;
+  AttnScale sc;
+  // Keys in `nsplit` ranges, each with its own partial row: f32 sums of t^n v, then per row Z and
+  // the shift's reciprocal.
+  int nsplit;
+  float* part_o;   // (nsplit, Hkv N G, D)
+  float* part_zt;  // (nsplit, Hkv N G, 2)
+};
+
+// New tokens' queries, keys and values on their way into a paged cache (paged_append.hip).
+struct PagedAppendParams {
+  const bf16 *q, *k, *v;  // raw projections (N, H or Hkv, D)
+  long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+  bf16 *kp, *vp;          // pages of (Hkv, page, D)
+  long kp_ps, kp_hs, kp_ts, vp_ps, vp_hs, vp_ts;
+  bf16* qo;               // (N, H, D) contiguous
+  const int *cu, *kv_lens, *table;
+  int width, page, pages;
+  const float *q_gain, *k_gain;  // (D) or nullptr
+  const float *cos, *sin;        // (>= width page, D / 2) or nullptr
+  float eps;
+  int N, S, H, Hkv, D;
+};
+
+struct PackedBwdParams {
+  const bf16 *q, *k, *v, *o, *dO;
+  const float* stat;  // (Hkv, N G)
+  float* di;          // (Hkv, N G), written by the dQ kernel
+  int* care;          // (slots, Hkv): whether the slot's rows took the careful form, likewise
+  const float* sink;
+  int sink_count;
+  float c;
+  const int* cu;
+  long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, do_ts, do_hs;
+  bf16 *dq, *dk, *dv;  // contiguous
+  float* dsink;        // (H) gradients per head, or nullptr
+  int N, S, H, Hkv, G;
+  AttnScale sc;
+};
+
+__device__ __forceinline__ float sink_score(const float* sink, int count, int head, float c, float a) {
+  return sink[count == 1 ? 0 : head] / (c * a);
+}
+
+// t and r = 1/sqrt(s^2 + b) of the plain form.
+__device__ __forceinline__ float weight_t(float s, float b, float& r) {
+  const float rad = __builtin_fmaf(s, s, b);
+  r = rsq(rad);
+  return __builtin_fmaf(rad, r, s);
+}
+// The careful form, as exact for either sign: t = b / (|s| + sqrt(s^2 + b)) below zero. Past
+// |s| = 2^60 the square root is |s| itself (b is at most 1), and rad would overflow.
+__device__ __forceinline__ float weight_t_careful(float s, float b, float& r) {
+  const float as = __builtin_fabsf(s);
+  const bool far = as > 0x1p60f;
+  const float rad = __builtin_fmaf(s, s, b);
+  r = far ? __builtin_amdgcn_rcpf(as) : rsq(rad);
+  const float u = as + (far ? as : rad * r);
+  return s < 0.0f ? b * __builtin_amdgcn_rcpf(u) : u;
+}
+
+// Slots of a launch, and the sequence of slot `slot` (S: the tokens behind the last sequence).
+__host__ __device__ inline int packed_slots(int N, int G, int S, int rows) { return (int)((long)N * G / rows) + S + 1; }
+
+struct PackedSeq {
+  int s;      // S: behind the last sequence
+  int start;  // first token
+  int len;    // tokens
+  int tile;   // tile of `rows` rows within the sequence
+};
+// First token of entry s, whatever the caller wrote there: in [0, N].
+__device__ __forceinline__ int packed_start(const int* cu, int s, int N) {
+  return s == 0 ? 0 : min(max(cu[s], 0), N);
+}
+__device__ __forceinline__ PackedSeq packed_find(const int* cu, int N, int S, int G, int rows, int slot) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = S + 1;
+  while (n > 1) {  // 64 candidates at a time: one step up to 63 sequences, two up to 4095
+    const int step = (n + 63) / 64;
+    const int at = lane * step;
+    bool ok = false;
+    if (at < n) {
+      const int s = lo + at;
+      ok = packed_start(cu, s, N) * G / rows + s <= slot;
+    }
+    const int c = max((int)__popcll(__ballot(ok)), 1) - 1;
+    lo += c * step;
+    n = min(step, n - c * step);
+  }
+  PackedSeq f;
+  f.s = __builtin_amdgcn_readfirstlane(min(lo, S));
+  f.start = __builtin_amdgcn_readfirstlane(packed_start(cu, f.s, N));
+  const int end = f.s == S ? N : __builtin_amdgcn_readfirstlane(packed_start(cu, f.s + 1, N));
+  f.len = max(end - f.start, 0);
+  f.tile = slot - (f.start * G / rows + f.s);
+  return f;
+}
+
+// One 16-row group of a K / V tile: where its rows start, and how many of them exist.
+struct KvGroup {
+  const bf16* k;
+  const bf16* v;
+  int rows;
+};
+
+}  // namespace alg

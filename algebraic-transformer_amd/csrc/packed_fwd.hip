@@ -1,0 +1,487 @@
+// Causal algebraic attention over packed sequences of different lengths, or of new tokens over a
+// paged cache, with grouped heads, bf16: the forward pass for many rows (packed_common.h has the
+// arithmetic, the row order and the mapping of workgroups; paged_decode.hip the few rows of single
+// tokens).
+//
+// One workgroup = 4 waves = 128 rows (token, head of the group) of one sequence and key head; a
+// wave owns 32 rows and streams K and V through LDS in 64-key tiles, as the (B, H, T, D) forward
+// does: S^T = K Q^T (32x32x16 MFMA, lane = row), t^n in registers, O^T += V^T P^T with V^T read
+// transposed from LDS, two buffer sets, each filled by direct global -> LDS copies while the other
+// is consumed. What differs:
+//   * a wave copies 16 consecutive keys of a tile, through a buffer descriptor made for those keys:
+//     they start anywhere (packed rows: a 64-bit base per tile, so no length passes an offset's 32
+//     bits; pages: one table entry, since a page holds a multiple of 16 keys), and keys past the
+//     sequence read as zeros, whatever memory holds there;
+//   * the rows of a tile end at different positions, so the number of masked tiles is not fixed;
+//   * nothing is known of the scores' range in advance: see the two forms in packed_common.h.
+// With nsplit > 1 the keys of a row are split over workgroups, whose sums are joined by
+// packed_combine_kernel.
+#include <type_traits>
+
+#include "launchers.h"
+#include "packed_common.h"
+
+namespace alg {
+
+template <int D, int L2N, bool PAGED>
+__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
+  static_assert(D == 64 || D == 128, "head_dim");
+  constexpr int BK = PK_BK, CPR = D / 8, NDB = D / 32, NF = D / 16;
+  constexpr int RPI = 64 / CPR;       // keys per copy instruction
+  constexpr int PW = 16 / RPI;        // copy instruction pairs per wave and tile: 16 keys
+  __shared__ __attribute__((aligned(16))) bf16 Ks0[BK * D];
+  __shared__ __attribute__((aligned(16))) bf16 Ks1[BK * D];
+  __shared__ __attribute__((aligned(16))) bf16 Vs0[BK * D];
+  __shared__ __attribute__((aligned(16))) bf16 Vs1[BK * D];
+  __shared__ int bad_page;
+
+  const int lane = threadIdx.x & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
+  const int kvh = blockIdx.x % p.Hkv, slot = (gridDim.x - 1 - blockIdx.x) / p.Hkv;  // longest rows first
+  const PackedSeq f = packed_find(p.cu, p.N, p.S, p.G, PK_ROWS, slot);
+  const int G = p.G;
+  const int R = f.len * G;           // rows of the sequence
+  const int r0 = f.tile * PK_ROWS;   // this workgroup's first row
+  if (f.tile < 0 || r0 >= R) return;
+  const int myr = r0 + wave * 32 + l32;
+  const bool live = myr < R;
+  const int tok = min(myr, R - 1) / G, head = kvh * G + (min(myr, R - 1) - tok * G);
+  const size_t orow = ((size_t)(f.start + tok) * p.H + head) * D;
+  const size_t srow = (size_t)kvh * p.N * G + (size_t)f.start * G + min(myr, R - 1);
+
+  if (f.s == p.S) {  // tokens behind the last sequence
+    if (live && blockIdx.y == 0) {
+      const bf16x8 z = {};
+      for (int d = 8 * h; d < D; d += 16) *reinterpret_cast<bf16x8*>(p.o + orow + d) = z;
+      if (p.stat && h == 0) p.stat[srow] = 0.0f;
+    }
+    return;
+  }
+
+  // Keys of the sequence, and the position of its first token among them.
+  const int L = PAGED ? min(max(p.kv_lens[f.s], 0), p.width * p.page) : f.len;
+  const int off = L - f.len;
+  const int mypos = live ? off + tok : -1;
+  const int rlast = min(r0 + PK_ROWS, R) - 1;
+  const int posmin = off + r0 / G, posmax = off + rlast / G;
+  const int wave_posmax = off + min(r0 + wave * 32 + 31, R - 1) / G;
+  int kt0 = 0, kt1 = posmax < 0 ? 0 : posmax / BK + 1;  // this workgroup's key tiles
+  if (p.nsplit > 1) {
+    const int per = ceil_div(kt1, p.nsplit);
+    kt0 = min((int)blockIdx.y * per, kt1);
+    kt1 = min(kt0 + per, kt1);
+  }
+  const int nfull = posmin < 0 ? 0 : (posmin + 1) / BK;  // tiles before every row's position
+
+  // The 16 keys of tile kt that this wave copies. Pages: one table entry, read a tile ahead.
+  const bf16* kbase = p.k + (size_t)kvh * p.k_hs + (PAGED ? 0 : (size_t)f.start * p.k_ts);
+  const bf16* vbase = p.v + (size_t)kvh * p.v_hs + (PAGED ? 0 : (size_t)f.start * p.v_ts);
+  int pidx = 0, prow = 0;  // page of the group within the sequence, and row in the page
+  if constexpr (PAGED) {
+    const int key = kt0 * BK + 16 * wave;
+    pidx = key / p.page;
+    prow = key - pidx * p.page;
+  }
+  // Constant address space: a scalar load, which does not wait in the order of the copies.
+  const auto* trow = (const __attribute__((address_space(4))) int*)(PAGED ? p.table + (size_t)f.s * p.width : nullptr);
+  int next_id = PAGED && pidx < p.width && kt0 < kt1 ? trow[pidx] : 0;
+  bool bad = false;
+  auto group = [&](int kt) {
+    KvGroup g;
+    const int key = kt * BK + 16 * wave;
+    g.rows = kt < kt1 ? min(max(L - key, 0), 16) : 0;
+    if constexpr (PAGED) {
+      int id = __builtin_amdgcn_readfirstlane(next_id);
+      if (g.rows > 0 && (unsigned)id >= (unsigned)p.pages) {  // never read; the rows' results become NaN
+        bad = true;
+        g.rows = 0;
+      }
+      id = g.rows > 0 ? id : 0;
+      g.k = kbase + (size_t)id * p.k_ps + (size_t)prow * p.k_ts;
+      g.v = vbase + (size_t)id * p.v_ps + (size_t)prow * p.v_ts;
+      prow += BK;
+      while (prow >= p.page) {
+        prow -= p.page;
+        ++pidx;
+      }
+      next_id = pidx < p.width && kt + 1 < kt1 ? trow[pidx] : 0;
+    } else {
+      const int k = g.rows > 0 ? key : 0;
+      g.k = kbase + (size_t)k * p.k_ts;
+      g.v = vbase + (size_t)k * p.v_ts;
+    }
+    return g;
+  };
+  const int lrow = lane / CPR, lchunk = lane % CPR;
+  const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
+  const int chunkb = 16 * (lchunk ^ swz_chunk<CPR>(lrow));
+  auto dma = [&](bf16* la, bf16* lb, const KvGroup& g, int j) {
+    const int kn = g.rows > 0 ? ((g.rows - 1) * (int)p.k_ts + D) * 2 : 0;
+    const int vn = g.rows > 0 ? ((g.rows - 1) * (int)p.v_ts + D) * 2 : 0;
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)g.k, (short)0, kn, BUF_RSRC_WORD3);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)g.v, (short)0, vn, BUF_RSRC_WORD3);
+    auto lla = LDS_PTR(bf16, la);
+    auto llb = LDS_PTR(bf16, lb);
+    asm volatile("" : "+s"(lla), "+s"(llb));
+    const int J = wave * PW + j;
+    const int col = chunkb ^ (16 * swz_chunk<CPR>(RPI * J));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lla + J * 512, 16, RPI * j * (int)p.k_ts * 2 + k_row + col, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, llb + J * 512, 16, RPI * j * (int)p.v_ts * 2 + v_row + col, 0, 0, 0);
+  };
+
+  if constexpr (PAGED) {
+    if (threadIdx.x == 0) bad_page = 0;
+  }
+  {
+    const KvGroup g = group(kt0);
+#pragma unroll
+    for (int j = 0; j < PW; ++j) dma(Ks0, Vs0, g, j);
+  }
+  // Query fragments (B operand of S^T = K Q^T), held for the whole kernel; dead rows are zero.
+  bf16x8 qf[NF];
+  {
+    const bf16* Q = p.q + (size_t)(f.start + tok) * p.q_ts + (size_t)head * p.q_hs;
+#pragma unroll
+    for (int s = 0; s < NF; ++s) qf[s] = ld8(Q + 16 * s + 8 * h);
+    keep_own_row<NF>(qf, live);
+#pragma unroll
+    for (int s = 0; s < NF; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) qf[s][j] = f2bf((float)qf[s][j] * p.sc.qmul);
+  }
+  const int log2n = p.sc.log2n;
+  const float b2 = p.sc.b;
+  floatx16 oacc[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) oacc[db] = floatx16{};
+  float lsum = 0.0f, smax = 0.0f;
+
+  const int tr = (lane & 15) >> 2;
+  int row_off[NF];  // row fragments of K: row l32, k chunk 2 st + h
+#pragma unroll
+  for (int st = 0; st < NF; ++st) row_off[st] = swz_at<CPR>(l32, 16 * st + 8 * h);
+  int tv_lo[NDB], tv_hi[NDB];  // transposed V fragments: rows 4h + (0..3), 4h + 8 + (0..3)
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) {
+    tv_lo[db] = swz_at<CPR>(4 * h + tr, tr_col(db * 32, lane));
+    tv_hi[db] = swz_at<CPR>(4 * h + 8 + tr, tr_col(db * 32, lane));
+  }
+
+  bf16x8 rk3[3];  // row fragments of K, two steps ahead
+  __builtin_amdgcn_s_waitcnt(VMCNT0);
+  __syncthreads();
+  rk3[0] = ld8(Ks0 + row_off[0]);
+  rk3[1] = ld8(Ks0 + row_off[1]);
+  constexpr int VE = 11;  // VALU instructions per weight (scheduling hint)
+
+  // One key tile in the plain form, software-pipelined over its two 32-key blocks:
+  //   R1 S^T of keys 0..31 | the next tile's copy    R2 S^T of 32..63 | weights of 0..31
+  //   R3 O^T over 0..31 | weights of 32..63          R4 O^T over 32..63
+  auto tile = [&](auto bufc, auto maskc, int kt) {
+    constexpr int BUF = decltype(bufc)::value;
+    constexpr bool MASKED = decltype(maskc)::value;
+    const bf16* Ks = BUF ? Ks1 : Ks0;
+    const bf16* Vs = BUF ? Vs1 : Vs0;
+    bf16* Kn = BUF ? Ks0 : Ks1;
+    bf16* Vn = BUF ? Vs0 : Vs1;
+    const int kb0 = kt * BK;
+    const KvGroup gn = group(kt + 1);
+    if constexpr (MASKED) {
+      if (kb0 > wave_posmax) {  // every key lies after this wave's rows
+#pragma unroll
+        for (int j = 0; j < PW; ++j) dma(Kn, Vn, gn, j);
+        __builtin_amdgcn_s_waitcnt(VMCNT0);
+        __syncthreads();
+        rk3[0] = ld8(Kn + row_off[0]);
+        rk3[1] = ld8(Kn + row_off[1]);
+        return;
+      }
+    }
+    floatx16 s[2];
+    bf16x8 pf[2][2];
+    float w[16];
+    auto s_step = [&](int g) {
+      const int blk = g / NF, st = g % NF;
+      const int gx = g + 2;
+      if (gx < 2 * NF) rk3[gx % 3] = ld8(Ks + (gx / NF) * 32 * D + row_off[gx % NF]);
+      s[blk] = mfma_bf16(rk3[g % 3], qf[st], s[blk]);
+    };
+    auto elem = [&](int blk, int i) {
+      const bool dead = MASKED && kb0 + blk * 32 + 8 * (i >> 2) + 4 * h + (i & 3) > mypos;
+      const float x = dead ? 0.0f : s[blk][i];
+      smax = fmaxf(smax, __builtin_fabsf(x));
+      float r;
+      float wi = pow2n<L2N>(weight_t(x, b2, r), log2n);
+      if (dead) wi = 0.0f;
+      lsum += wi;
+      w[i] = wi;
+      if (i & 1) {
+        pf[blk][i >> 3][(i & 7) - 1] = f2bf(w[i - 1]);
+        pf[blk][i >> 3][i & 7] = f2bf(w[i]);
+      }
+    };
+    bf16x8 ft[2][2];
+    auto pv_load = [&](int blk, int db, bf16x8 (&fr)[2]) {
+      const bf16* vb = Vs + blk * 32 * D;
+      fr[0] = tr_frag_at(vb, tv_lo[db], tv_hi[db]);
+      fr[1] = tr_frag_at(vb + 16 * D, tv_lo[db], tv_hi[db]);
+    };
+    s[0] = floatx16{};
+    s[1] = floatx16{};
+#pragma unroll
+    for (int g = 0; g < NF; ++g) {
+      s_step(g);
+      if (g < PW) dma(Kn, Vn, gn, g);
+      step_order<1, 0, 2, 0>();
+    }
+    constexpr int E2 = 16 / NF;
+#pragma unroll
+    for (int g = NF; g < 2 * NF; ++g) {
+      s_step(g);
+#pragma unroll
+      for (int k = 0; k < E2; ++k) elem(0, E2 * (g - NF) + k);
+      if (g == 2 * NF - 1) pv_load(0, 0, ft[0]);
+      step_order<1, VE * E2, 2, 0>();
+    }
+    constexpr int E3 = 16 / NDB;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const int c = db & 1;
+      if (db + 1 < NDB) pv_load(0, db + 1, ft[c ^ 1]);
+      else pv_load(1, 0, ft[c ^ 1]);
+      oacc[db] = mfma_bf16(ft[c][0], pf[0][0], oacc[db]);
+      oacc[db] = mfma_bf16(ft[c][1], pf[0][1], oacc[db]);
+#pragma unroll
+      for (int k = 0; k < E3; ++k) elem(1, E3 * db + k);
+      step_order<2, VE * E3, 4, 0>();
+    }
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const int c = (db + NDB) & 1;
+      if (db + 1 < NDB) pv_load(1, db + 1, ft[c ^ 1]);
+      oacc[db] = mfma_bf16(ft[c][0], pf[1][0], oacc[db]);
+      oacc[db] = mfma_bf16(ft[c][1], pf[1][1], oacc[db]);
+      step_order<2, 0, 4, 0>();
+    }
+    __builtin_amdgcn_s_waitcnt(VMCNT0);  // this wave's copies of the next tile have landed
+    __syncthreads();                     // the next tile is complete; this buffer set is free
+    rk3[0] = ld8(Kn + row_off[0]);
+    rk3[1] = ld8(Kn + row_off[1]);
+  };
+
+  const bool has_sink = p.sink != nullptr && p.nsplit == 1;  // split: the sink joins in the combination
+  const float ss = has_sink ? sink_score(p.sink, p.sink_count, head, p.c, p.sc.a) : 0.0f;
+  const float bound = p.sc.bound;
+  bool careful = bound < 0.0f;
+  if (!careful) {
+    // The tiles in pairs (buffer sets 0 and 1); the last pair may be half one, and a pair counts as
+    // masked when one of its tiles does. No branch chooses a buffer set inside the loops: the
+    // accumulators' registers stay put.
+    const int full = kt0 + (max(min(nfull, kt1) - kt0, 0) & ~1);
+    int kt = kt0;
+    for (; kt < full; kt += 2) {
+      tile(std::integral_constant<int, 0>{}, std::false_type{}, kt);
+      tile(std::integral_constant<int, 1>{}, std::false_type{}, kt + 1);
+    }
+    for (; kt < kt1; kt += 2) {
+      tile(std::integral_constant<int, 0>{}, std::true_type{}, kt);
+      if (kt + 1 >= kt1) break;
+      tile(std::integral_constant<int, 1>{}, std::true_type{}, kt + 1);
+    }
+    // A score that is no number needs no other form: its row's results are NaN in either.
+    careful = __syncthreads_or(smax > bound || __builtin_fabsf(ss) > bound) != 0;
+  }
+
+  float shift = 1.0f, tmax = 1.0f;  // the row's weights are (t shift)^n; tmax = 1 / shift
+  if (careful) {
+    // The rows again, with a running maximum of the scores per row (the sink a first key).
+    float m = has_sink ? ss : -INFINITY;
+    lsum = has_sink && h == 0 ? 1.0f : 0.0f;
+    {
+      float r;
+      tmax = has_sink ? weight_t_careful(ss, b2, r) : 0.0f;
+      shift = has_sink ? 1.0f / tmax : 0.0f;
+    }
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) oacc[db] = floatx16{};
+    if constexpr (PAGED) {
+      const int key = kt0 * BK + 16 * wave;
+      pidx = key / p.page;
+      prow = key - pidx * p.page;
+      next_id = pidx < p.width && kt0 < kt1 ? trow[pidx] : 0;
+    }
+    for (int kt = kt0; kt < kt1; ++kt) {
+      __syncthreads();  // every wave is done with the tile before
+      const KvGroup g = group(kt);
+#pragma unroll
+      for (int j = 0; j < PW; ++j) dma(Ks0, Vs0, g, j);
+      __builtin_amdgcn_s_waitcnt(VMCNT0);
+      __syncthreads();
+      for (int blk = 0; blk < 2; ++blk) {
+        const int kb = kt * BK + 32 * blk;
+        if (kb > wave_posmax) continue;
+        floatx16 s = {};
+#pragma unroll
+        for (int st = 0; st < NF; ++st) s = mfma_bf16(ld8(Ks0 + blk * 32 * D + row_off[st]), qf[st], s);
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (kb + 8 * (i >> 2) + 4 * h + (i & 3) <= mypos) top = fmaxf(top, s[i]);
+        top = fmaxf(top, xor32(top));
+        if (top > m) {
+          float r;
+          const float t = weight_t_careful(top, b2, r);
+          const float fall = m == -INFINITY ? 0.0f : pow2n<0>(tmax / t, log2n);
+          m = top;
+          tmax = t;
+          shift = 1.0f / t;
+          lsum *= fall;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) oacc[db][i] *= fall;
+        }
+        bf16x8 pf[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool dead = kb + 8 * (i >> 2) + 4 * h + (i & 3) > mypos;
+          float r;
+          float w = pow2n<0>(weight_t_careful(dead ? 0.0f : s[i], b2, r) * shift, log2n);
+          if (dead) w = 0.0f;
+          lsum += w;
+          pf[i >> 3][i & 7] = f2bf(w);
+        }
+        const bf16* vb = Vs0 + blk * 32 * D;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          oacc[db] = mfma_bf16(tr_frag_at(vb, tv_lo[db], tv_hi[db]), pf[0], oacc[db]);
+          oacc[db] = mfma_bf16(tr_frag_at(vb + 16 * D, tv_lo[db], tv_hi[db]), pf[1], oacc[db]);
+        }
+      }
+    }
+  }
+
+  float Z = lsum + xor32(lsum);
+  if constexpr (PAGED) {
+    if (bad) bad_page = 1;
+    __syncthreads();
+    if (bad_page) Z = __builtin_nanf("");
+  }
+  if (!live) return;
+  if (p.nsplit > 1) {
+    const size_t part = (size_t)blockIdx.y * p.Hkv * p.N * G + srow;
+    float* O = p.part_o + part * D;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        floatx4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = oacc[db][4 * g + e];
+        *reinterpret_cast<floatx4*>(O + db * 32 + 8 * g + 4 * h) = v;
+      }
+    if (h == 0) {
+      p.part_zt[2 * part] = Z;
+      p.part_zt[2 * part + 1] = tmax;
+    }
+    return;
+  }
+  if (!careful && has_sink) {
+    float r;
+    Z += pow2n<L2N>(weight_t(ss, b2, r), log2n);
+  }
+  const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;  // a row without keys and sink is zero
+  bf16* O = p.o + orow;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      bf16x4 ob;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ob[e] = f2bf(oacc[db][4 * g + e] * inv);
+      *reinterpret_cast<bf16x4*>(O + db * 32 + 8 * g + 4 * h) = ob;
+    }
+  if (p.stat && h == 0) {
+    const float rs = Z == 0.0f ? 0.0f : shift * inv_root(Z, 1 << log2n);
+    p.stat[srow] = careful ? -rs : rs;
+  }
+}
+
+// Rows whose keys were split: o = sum_i f_i O_i / (sum_i f_i Z_i + sink), f_i = (T_i / T)^n with
+// T_i the range's shift and T the largest of them and the sink's. One wave a row, at most 64 ranges;
+// a range without keys for the row has Z_i = 0 and counts for nothing. The order of the sums is
+// fixed.
+template <int D>
+__global__ __launch_bounds__(256) void packed_combine_kernel(PackedParams p) {
+  const int lane = threadIdx.x & 63;
+  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // token N, head H
+  if (row >= p.N * p.H) return;
+  const int tok = row / p.H, head = row - tok * p.H, kvh = head / p.G;
+  const int total = packed_start(p.cu, p.S, p.N);
+  if (p.S == 0 || tok >= total) return;  // written as zeros by the first range's workgroups
+  const size_t rows = (size_t)p.Hkv * p.N * p.G;
+  const size_t srow = (size_t)kvh * p.N * p.G + (size_t)tok * p.G + (head - kvh * p.G);
+  const int log2n = p.sc.log2n;
+  float ts = 0.0f, T = 0.0f;
+  if (p.sink) {
+    float r;
+    ts = weight_t_careful(sink_score(p.sink, p.sink_count, head, p.c, p.sc.a), p.sc.b, r);
+    T = ts;
+  }
+  float2 zt = make_float2(0.0f, 0.0f);  // lane i: range i
+  if (lane < p.nsplit) zt = *reinterpret_cast<const float2*>(p.part_zt + 2 * (lane * rows + srow));
+  if (zt.x != 0.0f) T = fmaxf(T, zt.y);
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) T = fmaxf(T, __shfl_xor(T, m, 64));
+  const float f = zt.x != 0.0f ? pow2n<0>(zt.y / T, log2n) : 0.0f;
+  float Z = f * zt.x;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) Z += __shfl_xor(Z, m, 64);
+  if (p.sink) Z += pow2n<0>(ts / T, log2n);
+  constexpr int E = D / 64;  // columns a lane
+  typedef float fvec __attribute__((ext_vector_type(E)));
+  fvec acc = 0.0f;
+  for (int i0 = 0; i0 < p.nsplit; i0 += 8) {  // eight ranges' loads in flight
+    fvec o[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      o[k] = *reinterpret_cast<const fvec*>(p.part_o + (min(i0 + k, p.nsplit - 1) * rows + srow) * D + lane * E);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float fi = __shfl(f, (i0 + k) & 63, 64);  // 0 past the last range, and where none was written
+      if (i0 + k < p.nsplit && fi != 0.0f) acc += fi * o[k];
+    }
+  }
+  const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
+  bf16* O = p.o + (size_t)row * D + lane * E;
+  if constexpr (E == 2) *reinterpret_cast<unsigned*>(O) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  else O[0] = f2bf(acc[0] * inv);
+}
+
+template <int D, bool PAGED>
+static void launch_fwd(const PackedParams& p, dim3 grid, hipStream_t st) {
+  if (p.sc.log2n == 4) hipLaunchKernelGGL((packed_fwd_kernel<D, 4, PAGED>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((packed_fwd_kernel<D, 0, PAGED>), grid, dim3(256), 0, st, p);
+}
+
+hipError_t launch_packed_combine(const PackedParams& p, int D, hipStream_t st) {
+  KTimer t("packed_combine", st);
+  const dim3 grid((unsigned)(((long)p.N * p.H + 3) / 4));
+  if (D == 64) hipLaunchKernelGGL(packed_combine_kernel<64>, grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(packed_combine_kernel<128>, grid, dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+hipError_t launch_packed_fwd(const PackedParams& p, int D, bool paged, hipStream_t st) {
+  const dim3 grid(p.Hkv * packed_slots(p.N, p.G, p.S, PK_ROWS), p.nsplit);
+  {
+    KTimer t(paged ? "paged_fwd" : "packed_fwd", st);
+    if (D == 64) paged ? launch_fwd<64, true>(p, grid, st) : launch_fwd<64, false>(p, grid, st);
+    else paged ? launch_fwd<128, true>(p, grid, st) : launch_fwd<128, false>(p, grid, st);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.nsplit == 1) return e;
+  return launch_packed_combine(p, D, st);
+}
+
+}  // namespace alg

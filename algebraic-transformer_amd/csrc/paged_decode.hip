@@ -1,0 +1,323 @@
+// Attention of a few new tokens per sequence over a paged cache, bf16: a token's G queries at one
+// key head (times the tokens, where there are several) make 16 or 32 rows, and the work is reading
+// the held keys and values once.
+//
+// One workgroup = 4 waves = the rows of one sequence and key head over one range of its keys (the
+// ranges are joined by packed_combine_kernel). Each wave takes every fourth block of 32 keys and
+// keeps a state of its own, so that nothing synchronises until the waves' states are joined
+// through LDS at the end:
+//   S^T = K Q^T (16x16x32 MFMA; A = K straight from memory to registers: lane l holds 8 elements
+//   of key l % 16), weights in registers, O^T += V^T P^T, where the 32 keys are numbered
+//   (lane group g, slot j) -> 4 g + j % 4 + 16 (j / 4), the order in which S^T leaves the MFMA;
+//   V comes through a private LDS tile (direct copies) and is read transposed.
+// While a block is computed the next one's 16 KB are in flight: 8 waves a CU hold up to 128 KB.
+// A group of 16 keys lies in one page (pages hold a multiple of 16 keys): its page number is one
+// scalar load, whose counter is not the vector loads', so that looking a page up never waits for
+// the keys and values in flight.
+// Keys past the range read as zeros (buffer descriptors end there) and have no weight.
+// The weights' two forms: packed_common.h. Here a wave changes to the careful form at the first
+// block that needs it and goes on from the sums it has, whose shift is 1.
+#include "launchers.h"
+#include "packed_common.h"
+
+namespace alg {
+
+template <int D, int RT, int L2N>
+__global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
+  static_assert(D == 64 || D == 128, "head_dim");
+  constexpr int NS = D / 32, NDB = D / 16, CPR = D / 8, RPI = 64 / CPR, PW = 16 / RPI;
+  constexpr int LOADS = 2 * NS + 2 * PW;  // vector loads and copies of one block of 32 keys
+  constexpr int ROWS = 16 * RT;
+  constexpr int BLK = 32;
+  __shared__ __attribute__((aligned(16))) bf16 Vs[4 * 2 * BLK * D];
+  __shared__ float jT[4][ROWS], jZ[4][ROWS];
+  static_assert(4 * ROWS * D * sizeof(float) <= sizeof(Vs), "the waves' sums fit the V tiles");
+
+  const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = blockIdx.x % p.Hkv;
+  const PackedSeq f = packed_find(p.cu, p.N, p.S, p.G, ROWS, blockIdx.x / p.Hkv);
+  const int G = p.G, R = f.len * G, r0 = f.tile * ROWS;
+  if (f.tile < 0 || r0 >= R) return;
+  const int nrow = min(ROWS, R - r0);  // live rows of the tile
+  if (f.s == p.S) {                    // tokens behind the last sequence
+    if (blockIdx.y == 0)
+      for (int i = threadIdx.x; i < nrow * (D / 8); i += 256) {
+        const int r = r0 + i / (D / 8), tok = r / G, head = kvh * G + r - tok * G;
+        const bf16x8 z = {};
+        *reinterpret_cast<bf16x8*>(p.o + ((size_t)(f.start + tok) * p.H + head) * D + 8 * (i % (D / 8))) = z;
+      }
+    return;
+  }
+  const int L = min(max(p.kv_lens[f.s], 0), p.width * p.page);
+  const int off = L - f.len;
+  const int kend = max(off + (r0 + nrow - 1) / G + 1, 0);  // keys that some row sees: [0, kend)
+  // This workgroup's blocks of 32 keys: an equal share, of at least 4 blocks a wave.
+  int b0 = 0, b1 = ceil_div(kend, BLK);
+  if (p.nsplit > 1) {
+    const int per = max(ceil_div(b1, p.nsplit), 16);
+    b0 = min((int)blockIdx.y * per, b1);
+    b1 = min(b0 + per, b1);
+  }
+
+  bf16x8 qf[RT][NS];
+  int mypos[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = r0 + 16 * rt + l16;
+    const bool live = r < R;
+    const int rc = min(r, R - 1), tok = rc / G, head = kvh * G + rc - tok * G;
+    mypos[rt] = live ? off + tok : -1;
+    const bf16* Q = p.q + (size_t)(f.start + tok) * p.q_ts + (size_t)head * p.q_hs + 8 * g;
+#pragma unroll
+    for (int st = 0; st < NS; ++st) qf[rt][st] = ld8(Q + 32 * st);
+    keep_own_row<NS>(qf[rt], live);
+#pragma unroll
+    for (int st = 0; st < NS; ++st)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) qf[rt][st][j] = f2bf((float)qf[rt][st][j] * p.sc.qmul);
+  }
+
+  const int log2n = p.sc.log2n;
+  const float b2 = p.sc.b, bound = p.sc.bound;
+  const auto* trow = (const __attribute__((address_space(4))) int*)(p.table + (size_t)f.s * p.width);
+  const bf16* kbase = p.k + (size_t)kvh * p.k_hs;
+  const bf16* vbase = p.v + (size_t)kvh * p.v_hs;
+  bf16* vbuf = Vs + wave * 2 * BLK * D;
+  const int lrow = lane / CPR;
+  const int k_off = (l16 * (int)p.k_ts + 8 * g) * 2;
+  const int v_off = lrow * (int)p.v_ts * 2;
+  const int chunkb = 16 * ((lane % CPR) ^ swz_chunk<CPR>(lrow));
+  int t_off[NDB];  // transposed V fragments: keys 4 g + (0..3), columns 16 db + (0..15)
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) t_off[db] = swz_at<CPR>(4 * g + (l16 >> 2), 16 * db + 4 * (lane & 3));
+
+  bool bad = false;
+  typedef bf16x8 KBlock[2][NS];
+  auto load = [&](int blk, KBlock& kf, bf16* vl) {
+    auto ll = LDS_PTR(bf16, vl);
+    asm volatile("" : "+s"(ll));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = blk * BLK + 16 * u;
+      int rows = blk < b1 ? min(max(kend - key, 0), 16) : 0;
+      int id = 0, prow = 0;
+      if (rows > 0) {
+        const int pi = key / p.page;
+        prow = key - pi * p.page;
+        id = trow[pi];
+        if ((unsigned)id >= (unsigned)p.pages) {  // never read; the rows' results become NaN
+          bad = true;
+          id = rows = 0;
+        }
+      }
+      const bf16* K = kbase + (size_t)id * p.k_ps + (size_t)prow * p.k_ts;
+      const bf16* V = vbase + (size_t)id * p.v_ps + (size_t)prow * p.v_ts;
+      const int kn = rows > 0 ? ((rows - 1) * (int)p.k_ts + D) * 2 : 0, vn = rows > 0 ? ((rows - 1) * (int)p.v_ts + D) * 2 : 0;
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)K, (short)0, kn, BUF_RSRC_WORD3);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)V, (short)0, vn, BUF_RSRC_WORD3);
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(rk, k_off + 64 * st, 0, 0);
+        const uint4 raw = make_uint4(v[0], v[1], v[2], v[3]);
+        kf[u][st] = *reinterpret_cast<const bf16x8*>(&raw);
+      }
+#pragma unroll
+      for (int j = 0; j < PW; ++j) {
+        const int J = u * PW + j;
+        const int col = chunkb ^ (16 * swz_chunk<CPR>(RPI * j));
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, ll + J * 512, 16, RPI * j * (int)p.v_ts * 2 + v_off + col, 0, 0, 0);
+      }
+    }
+  };
+
+  floatx4 oacc[RT][NDB];
+  float lsum[RT], T[RT], shift[RT];  // weights (t shift)^n, T = 1 / shift (0: no key yet)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    lsum[rt] = 0.0f;
+    T[rt] = shift[rt] = 1.0f;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) oacc[rt][db] = floatx4{};
+  }
+  bool careful = false;
+
+  auto compute = [&](int blk, const KBlock& kf, const bf16* vl) {
+    floatx4 s[RT][2];
+    float smax = 0.0f;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[rt][u] = floatx4{};
+#pragma unroll
+        for (int st = 0; st < NS; ++st) s[rt][u] = mfma16_bf16(kf[u][st], qf[rt][st], s[rt][u]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          smax = fmaxf(smax, blk * BLK + 16 * u + 4 * g + i > mypos[rt] ? 0.0f : __builtin_fabsf(s[rt][u][i]));
+      }
+    if (!careful && __any(smax > bound)) {
+      careful = true;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {  // a row without a key yet takes its first key's shift
+        float z = lsum[rt];
+        z += __shfl_xor(z, 16, 64);
+        z += __shfl_xor(z, 32, 64);
+        if (z == 0.0f) T[rt] = shift[rt] = 0.0f;
+      }
+    }
+    bf16x8 pf[RT];
+    if (!careful) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int u = j >> 2, i = j & 3;
+          float r;
+          float w = pow2n<L2N>(weight_t(s[rt][u][i], b2, r), log2n);
+          if (blk * BLK + 16 * u + 4 * g + i > mypos[rt]) w = 0.0f;
+          lsum[rt] += w;
+          pf[rt][j] = f2bf(w);
+        }
+    } else {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float t[8], top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int u = j >> 2, i = j & 3;
+          float r;
+          const bool dead = blk * BLK + 16 * u + 4 * g + i > mypos[rt];
+          t[j] = dead ? 0.0f : weight_t_careful(s[rt][u][i], b2, r);
+          top = fmaxf(top, t[j]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (top > T[rt]) {
+          const float fall = pow2n<0>(T[rt] / top, log2n);
+          T[rt] = top;
+          shift[rt] = 1.0f / top;
+          lsum[rt] *= fall;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) oacc[rt][db][i] *= fall;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float w = pow2n<0>(t[j] * shift[rt], log2n);
+          lsum[rt] += w;
+          pf[rt][j] = f2bf(w);
+        }
+      }
+    }
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const bf16x8 vf = tr_frag_at(vl, t_off[db], t_off[db] + 16 * D);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) oacc[rt][db] = mfma16_bf16(vf, pf[rt], oacc[rt][db]);
+    }
+    // The block's V tile is read before the next copy into it is issued.
+    __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(63));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  // Blocks b0 + wave, + 4, ...; a block past the range loads nothing (empty descriptors).
+  KBlock ka, kb;
+  load(b0 + wave, ka, vbuf);
+  for (int blk = b0 + wave; blk < b1; blk += 8) {
+    load(blk + 4, kb, vbuf + BLK * D);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
+    __builtin_amdgcn_sched_barrier(0);
+    compute(blk, ka, vbuf);
+    load(blk + 8, ka, vbuf);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
+    __builtin_amdgcn_sched_barrier(0);
+    if (blk + 4 < b1) compute(blk + 4, kb, vbuf + BLK * D);
+  }
+  __builtin_amdgcn_s_waitcnt(VMCNT0);  // copies into the tiles that the join overwrites
+
+  // The waves' states, joined in wave order.
+  float* sO = reinterpret_cast<float*>(Vs);
+  __syncthreads();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    float z = lsum[rt];
+    z += __shfl_xor(z, 16, 64);
+    z += __shfl_xor(z, 32, 64);
+    if (bad) z = __builtin_nanf("");
+    if (g == 0) {
+      jT[wave][16 * rt + l16] = T[rt];
+      jZ[wave][16 * rt + l16] = z;
+    }
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+      *reinterpret_cast<floatx4*>(sO + ((wave * ROWS) + 16 * rt + l16) * D + 16 * db + 4 * g) = oacc[rt][db];
+  }
+  __syncthreads();
+  constexpr int TPR = 256 / ROWS, CPT = D / TPR;  // threads a row, columns a thread
+  const int row = threadIdx.x / TPR, c0 = (threadIdx.x % TPR) * CPT;
+  const int r = r0 + row;
+  if (r >= R) return;
+  const int tok = r / G, head = kvh * G + r - tok * G;
+  const bool sink = p.sink != nullptr && p.nsplit == 1;  // split: the sink joins in the combination
+  float Tm = 0.0f, ts = 0.0f;
+  if (sink) {
+    float rr;
+    Tm = ts = weight_t_careful(sink_score(p.sink, p.sink_count, head, p.c, p.sc.a), b2, rr);
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    if (jZ[w][row] != 0.0f) Tm = fmaxf(Tm, jT[w][row]);
+  float Z = sink ? pow2n<0>(ts / Tm, log2n) : 0.0f;
+  float acc[CPT] = {};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (jZ[w][row] == 0.0f) continue;
+    const float fw = pow2n<0>(jT[w][row] / Tm, log2n);
+    Z += fw * jZ[w][row];
+#pragma unroll
+    for (int e = 0; e < CPT; ++e) acc[e] += fw * sO[(w * ROWS + row) * D + c0 + e];
+  }
+  if (p.nsplit > 1) {
+    const size_t part = (size_t)blockIdx.y * p.Hkv * p.N * G + (size_t)kvh * p.N * G + (size_t)f.start * G + r;
+    if (c0 == 0) {
+      p.part_zt[2 * part] = Z;
+      p.part_zt[2 * part + 1] = Tm;
+    }
+    if (Z != 0.0f)  // an empty range's sums are not read
+#pragma unroll
+      for (int e = 0; e < CPT; e += 4)
+        *reinterpret_cast<floatx4*>(p.part_o + part * D + c0 + e) = floatx4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+    return;
+  }
+  const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
+  bf16* O = p.o + ((size_t)(f.start + tok) * p.H + head) * D + c0;
+#pragma unroll
+  for (int e = 0; e < CPT; e += 4) {
+    bf16x4 ob;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ob[i] = f2bf(acc[e + i] * inv);
+    *reinterpret_cast<bf16x4*>(O + e) = ob;
+  }
+}
+
+template <int D, int RT>
+static void launch_decode(const PackedParams& p, hipStream_t st) {
+  const dim3 grid(p.Hkv * packed_slots(p.N, p.G, p.S, 16 * RT), p.nsplit);
+  if (p.sc.log2n == 4) hipLaunchKernelGGL((paged_decode_kernel<D, RT, 4>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((paged_decode_kernel<D, RT, 0>), grid, dim3(256), 0, st, p);
+}
+
+hipError_t launch_paged_decode(const PackedParams& p, int D, int row_tiles, hipStream_t st) {
+  {
+    KTimer t("paged_decode", st);
+    if (D == 64) row_tiles == 1 ? launch_decode<64, 1>(p, st) : launch_decode<64, 2>(p, st);
+    else row_tiles == 1 ? launch_decode<128, 1>(p, st) : launch_decode<128, 2>(p, st);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.nsplit == 1) return e;
+  return launch_packed_combine(p, D, st);
+}
+
+}  // namespace alg

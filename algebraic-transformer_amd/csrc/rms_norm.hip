@@ -8,6 +8,11 @@
 // for the VJP. VJP (JAX autodiff of the same expression, in f32): a = g dy,
 // dx = round(a tau - x tau^3 sum(a x) / d); dgain = sum over rows of dy x tau, as per-workgroup
 // partials (the workgroup's waves summed in order) reduced per column in block order.
+//
+// With the residual's addition (add_rms_norm): s = round(x + res) is stored, and the norm is of
+// the stored s, so that the VJP, which reads s alone, differentiates what the forward computed:
+// d(x) = d(res) = round(dx of the norm + ds). The 8-bit output is y / scale in e4m3, scale =
+// max|y| / 448 of the row (1 for a row of zeros), from the unrounded y: one rounding.
 #include "launchers.h"
 
 #pragma clang fp contract(off)
@@ -107,12 +112,93 @@ __global__ __launch_bounds__(256) void rms_norm_fwd_kernel(RmsNormParams p) {
   if (lane == 0) p.tau[row] = tau;
 }
 
+// s = round(x + res), y = round((s tau) g) or its e4m3 form; one row per wave, as above.
+template <int NC, bool FP8>
+__global__ __launch_bounds__(256) void add_rms_norm_kernel(RmsNormParams p) {
+  const int lane = threadIdx.x & 63;
+  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
+  if (row >= p.rows) return;
+  const int nch = p.d / 8;
+  const size_t at = (size_t)row * p.d;
+  uint4 xr[NC], rr[NC];
+  load_row<NC>(p.x + at, lane, nch, xr);
+  load_row<NC>(p.res + at, lane, nch, rr);
+  float g[NC][8];
+  load_gain<NC>(p.gain, lane, nch, g);
+  float s[NC][8];
+  float ss = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    float a[8], b[8];
+    bf16 out[8];
+    cvt8(xr[c], a);
+    cvt8(rr[c], b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      out[e] = f2bf(a[e] + b[e]);
+      s[c][e] = (float)out[e];
+      ss += s[c][e] * s[c][e];
+    }
+    const int ch = lane + 64 * c;
+    if (ch < nch) *reinterpret_cast<uint4*>(p.sum + at + 8 * ch) = *reinterpret_cast<uint4*>(out);
+  }
+  ss = wave_sum(ss);
+  const float tau = 1.0f / sqrtf(ss * (1.0f / (float)p.d) + p.eps);
+  if constexpr (!FP8) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int ch = lane + 64 * c;
+      if (ch < nch) {
+        bf16 out[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = f2bf(__fmul_rn(__fmul_rn(s[c][e], tau), g[c][e]));
+        *reinterpret_cast<uint4*>(p.y + at + 8 * ch) = *reinterpret_cast<uint4*>(out);
+      }
+    }
+    if (lane == 0) p.tau[row] = tau;
+  } else {
+    float top = 0.0f;  // a NaN of the row is in every y, and in the scale's product with it
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s[c][e] = __fmul_rn(__fmul_rn(s[c][e], tau), g[c][e]);
+        top = fmaxf(top, __builtin_fabsf(s[c][e]));
+      }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+    // Below 2^-100 the quotient would leave the normal numbers: such a row is zeros.
+    const float scale = top > 0x1p-100f ? top * (1.0f / 448.0f) : 1.0f;
+    const float mul = top > 0x1p-100f ? 448.0f / top : 1.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int ch = lane + 64 * c;
+      if (ch < nch) {
+        // The conversion saturates nothing: |y mul| passes 448 by a rounding at most, and is cut.
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = s[c][e] * mul;
+          v[e] = v[e] > 448.0f ? 448.0f : (v[e] < -448.0f ? -448.0f : v[e]);  // a NaN stays
+        }
+        int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+        int hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
+        *reinterpret_cast<int2*>(p.y8 + at + 8 * ch) = make_int2(lo, hi);
+      }
+    }
+    if (lane == 0) p.scale[row] = scale;
+  }
+}
+
 // Rows in a grid-stride loop, one row per wave at a time (the gain gradient is a
 // per-workgroup partial). The gain sits in LDS and the per-element values (x, dy, a = g dy)
 // are formed again from the raw row for the output, so a wave holds only its row's raw
 // chunks and its gain-gradient accumulators: about 100 registers at d = 2048, four waves
 // per SIMD, whose row loads keep enough bytes in flight without a software prefetch.
-template <int NC>
+// ADD: the cotangent of the sum, dsum, is added to dx before its rounding.
+template <int NC, bool ADD>
 __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(RmsNormParams p) {
   __shared__ __attribute__((aligned(16))) float gs[NC * 512];
   __shared__ float red[NC * 512];
@@ -137,9 +223,10 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(RmsNormParams p) {
   const float inv_d = 1.0f / (float)p.d;
   const int stride = gridDim.x * 4;
   for (int row = blockIdx.x * 4 + wave; row < p.rows; row += stride) {
-    uint4 xr[NC], dyr[NC];
+    uint4 xr[NC], dyr[NC], dsr[ADD ? NC : 1];
     load_row<NC>(p.x + (size_t)row * p.d, lane, nch, xr);
     load_row<NC>(p.dy + (size_t)row * p.d, lane, nch, dyr);
+    if constexpr (ADD) load_row<NC>(p.dsum + (size_t)row * p.d, lane, nch, dsr);
     const float tau = p.tau[row];
     float s = 0.0f;
 #pragma unroll
@@ -174,9 +261,14 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(RmsNormParams p) {
         cvt8(dyr[c], dy);
         const float* g = gs + 8 * ch;
         bf16 out[8];
+        float ds[8];
+        if constexpr (ADD) cvt8(dsr[c], ds);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          out[e] = f2bf(__fsub_rn(__fmul_rn(__fmul_rn(g[e], dy[e]), tau), __fmul_rn(x[e], coef)));
+        for (int e = 0; e < 8; ++e) {
+          float v = __fsub_rn(__fmul_rn(__fmul_rn(g[e], dy[e]), tau), __fmul_rn(x[e], coef));
+          if constexpr (ADD) v += ds[e];
+          out[e] = f2bf(v);
+        }
         *reinterpret_cast<uint4*>(dxr + 8 * ch) = *reinterpret_cast<uint4*>(out);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -240,19 +332,31 @@ static int rms_norm_nc(int d) { return (d / 8 + 63) / 64; }
 
 #define RN_DISPATCH(KERNEL, GRID, ...)                                                          \
   switch (rms_norm_nc(p.d)) {                                                                 \
-    case 1: hipLaunchKernelGGL(KERNEL<1>, GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
-    case 2: hipLaunchKernelGGL(KERNEL<2>, GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
-    case 3: hipLaunchKernelGGL(KERNEL<3>, GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
-    case 4: hipLaunchKernelGGL(KERNEL<4>, GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
-    case 5: hipLaunchKernelGGL(KERNEL<5>, GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
-    case 6: hipLaunchKernelGGL(KERNEL<6>, GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
-    case 7: hipLaunchKernelGGL(KERNEL<7>, GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
-    default: hipLaunchKernelGGL(KERNEL<8>, GRID, dim3(256), 0, st, __VA_ARGS__); break;        \
+    case 1: hipLaunchKernelGGL((KERNEL(1)), GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
+    case 2: hipLaunchKernelGGL((KERNEL(2)), GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
+    case 3: hipLaunchKernelGGL((KERNEL(3)), GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
+    case 4: hipLaunchKernelGGL((KERNEL(4)), GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
+    case 5: hipLaunchKernelGGL((KERNEL(5)), GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
+    case 6: hipLaunchKernelGGL((KERNEL(6)), GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
+    case 7: hipLaunchKernelGGL((KERNEL(7)), GRID, dim3(256), 0, st, __VA_ARGS__); break;         \
+    default: hipLaunchKernelGGL((KERNEL(8)), GRID, dim3(256), 0, st, __VA_ARGS__); break;        \
   }
+#define RN_FWD(NC) rms_norm_fwd_kernel<NC>
+#define RN_BWD(NC) rms_norm_bwd_kernel<NC, false>
+#define RN_BWD_ADD(NC) rms_norm_bwd_kernel<NC, true>
+#define RN_ADD(NC) add_rms_norm_kernel<NC, false>
+#define RN_ADD_FP8(NC) add_rms_norm_kernel<NC, true>
 
 hipError_t launch_rms_norm_fwd(const RmsNormParams& p, hipStream_t st) {
   KTimer t("rms_norm_fwd", st);
-  RN_DISPATCH(rms_norm_fwd_kernel, dim3((p.rows + 3) / 4), p);
+  RN_DISPATCH(RN_FWD, dim3((p.rows + 3) / 4), p);
+  return hipGetLastError();
+}
+
+hipError_t launch_add_rms_norm(const RmsNormParams& p, hipStream_t st) {
+  KTimer t(p.y8 ? "add_rms_norm_fp8" : "add_rms_norm", st);
+  const dim3 grid((p.rows + 3) / 4);
+  if (p.y8) RN_DISPATCH(RN_ADD_FP8, grid, p) else RN_DISPATCH(RN_ADD, grid, p)
   return hipGetLastError();
 }
 
@@ -260,7 +364,7 @@ hipError_t launch_rms_norm_bwd(const RmsNormParams& p, float* dgain, hipStream_t
   const int nb = rms_norm_blocks(p.rows);
   {
     KTimer t("rms_norm_bwd", st);
-    RN_DISPATCH(rms_norm_bwd_kernel, dim3(nb), p);
+    if (p.dsum) RN_DISPATCH(RN_BWD_ADD, dim3(nb), p) else RN_DISPATCH(RN_BWD, dim3(nb), p)
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !dgain) return e;

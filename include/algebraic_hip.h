@@ -63,8 +63,10 @@ enum { ALG_ATTN_INRANGE = 0, ALG_ATTN_CLIPPED = 1, ALG_ATTN_SHIFTED = 2, ALG_ATT
 /* Version 2: alg_attn_workspace_size and alg_head_* take a leading dtype argument and
  * alg_attn_bwd has no o_precise argument (version 1 had one).
  * Version 3: adds alg_attn_bwd_sink_logit, alg_head_eval_index64, alg_ffn_block_*, alg_head_plan
- * and alg_ffn_plan; nothing else changed. */
-#define ALG_ABI_VERSION 3
+ * and alg_ffn_plan; nothing else changed.
+ * Version 4: adds alg_add_rms_norm_*, alg_packed_attn_*, alg_paged_attn* and alg_paged_append;
+ * nothing else changed. */
+#define ALG_ABI_VERSION 4
 
 const char* alg_last_error(void);
 const char* alg_version(void);
@@ -330,6 +332,66 @@ int alg_head_bwd_streamed(alg_stream_t stream, int dtype, int N, int d, int V,
                           const void* h, const void* E, const int32_t* targets, const float* stat,
                           const float* g, int n, float c, int vocab_chunk, void* dh, void* dE, int dE_dtype,
                           void* workspace, size_t workspace_bytes);
+
+/* The residual stream's addition with the norm that follows it: sum = round(x + res), then
+ * alg_rms_norm's y and tau of sum (bf16), or y in 8 bits: y8 = e4m3(y / scale) of the unrounded y,
+ * scale (rows) f32 = max|y| / 448 (1 for rows without a value above 2^-100). Backward: dx, the
+ * gradient of x and of res alike, = round(dx of the norm + dsum), dsum (the cotangent of sum) may
+ * be NULL; dgain and workspace as in alg_rms_norm_bwd. Same sizes and alignment as alg_rms_norm;
+ * gain 16-byte aligned. No counterpart in the reference, whose compiler fuses the addition
+ * (src/algebraic/model.py:182-193). */
+int alg_add_rms_norm_fwd(alg_stream_t stream, int rows, int d, const void* x, const void* res, const float* gain,
+                         float eps, void* sum, void* y, float* tau);
+int alg_add_rms_norm_fp8(alg_stream_t stream, int rows, int d, const void* x, const void* res, const float* gain,
+                         float eps, void* sum, void* y8, float* scale);
+int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, const float* gain, const float* tau,
+                         const void* dy, const void* dsum, void* dx, float* dgain, void* workspace,
+                         size_t workspace_bytes);
+
+/* Causal algebraic attention (the function of alg_attn_fwd_guarded) over packed sequences with
+ * grouped heads, bf16: q, o (N, H, D), k, v (N, Hkv, D), H a multiple of Hkv, query head h reading
+ * key head h / (H / Hkv); D in {64, 128}. cu (S + 1) int32 on the device: sequence s is the tokens
+ * [cu[s], cu[s+1]), not decreasing, cu[0] = 0, cu[S] <= N; the tokens from cu[S] on get zeros.
+ * Strides are in elements between tokens (_ts) and heads (_hs), multiples of 8, the last axis
+ * contiguous, bases 16-byte aligned; o, dq, dk, dv are contiguous. sink: (sink_count = 1 or H)
+ * logits, f32, or NULL. stat (Hkv N (H / Hkv)) f32: the rows' statistics for the backward pass,
+ * which also takes o and dO; dsink (H) f32 = dL/dlogit per head, or NULL. Scores of any size:
+ * |q.k| / (sqrt(D) c) up to 2^60 is exact to f32 rounding, without a guard ahead. */
+int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                        const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
+                        const float* sink, int sink_count, float c, int n, void* o, float* stat);
+size_t alg_packed_attn_bwd_workspace_size(int N, int S, int H, int Hkv);
+int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                        const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
+                        const float* sink, int sink_count, float c, int n, const void* o, const float* stat,
+                        const void* dO, long do_ts, long do_hs, void* dq, void* dk, void* dv, float* dsink,
+                        void* workspace, size_t workspace_bytes);
+
+/* The same attention of new tokens over a paged cache, forward only: sequence s holds kv_lens[s]
+ * keys, of which its cu[s+1] - cu[s] tokens here are the last, token t at position
+ * kv_lens[s] - (cu[s+1] - cu[s]) + t; position i lies in page table[s width + i / page], place
+ * i % page, of k_pages and v_pages (pages, Hkv, page, D) with strides between pages (_ps), heads
+ * (_hs) and places (_ts) in any order; page a multiple of 16. What lies in a page behind a
+ * sequence's end is not read. A token before position 0 gets zeros; a page number outside
+ * [0, pages) is never followed, and makes the outputs that would have read it NaN. Split over
+ * ranges of keys where few rows would leave CUs idle; workspace: alg_paged_attn_workspace_size
+ * bytes (0: none). */
+size_t alg_paged_attn_workspace_size(int N, int S, int H, int Hkv, int D, int width, int page);
+int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                   const void* k_pages, long k_ps, long k_hs, long k_ts, const void* v_pages, long v_ps, long v_hs,
+                   long v_ts, int pages, int page, const int* table, int width, const int* cu, const int* kv_lens,
+                   const float* sink, int sink_count, float c, int n, void* o, void* workspace, size_t workspace_bytes);
+
+/* What precedes it: the new tokens' QK RMS norm with gain and Cayley rotation at their positions
+ * (model.py:170-174), y = rot((x tau) gain) in f32 rounded once; queries to q_out (N, H, D)
+ * contiguous, rotated keys and the values to their pages. Gains (D) f32 or NULL; cos, sin
+ * (table_rows >= width page, D / 2) f32, or both NULL. A token whose position or page number is
+ * out of range is not written; behind the last sequence, or out of range, its query is zero. */
+int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                     const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
+                     long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, int pages, int page,
+                     const int* table, int width, const int* cu, const int* kv_lens, const float* q_gain,
+                     const float* k_gain, const float* cos, const float* sin, int table_rows, float eps, void* q_out);
 
 /* Measurement hook (no counterpart in the reference; for benchmarks and profilers):
  * while enabled, every kernel launch of this library records a HIP event pair on its
