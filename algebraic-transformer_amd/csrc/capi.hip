@@ -1317,8 +1317,8 @@ static int check_table(int width, int page, int pages) {
 // How a paged call runs: which kernel, on rows per workgroup, and over how many ranges of keys.
 // Rows: a sequence's average, since the lengths are on the device. Up to 16 or 32 of them take the
 // kernel whose waves split the keys; more, the one whose waves split 128 rows. Ranges: as many as
-// bring the launch to two workgroups a CU, while a range keeps 512 keys (or 1024 of the larger
-// kernel, whose partial sums are 128 rows) of a sequence as long as the table allows.
+// bring the launch to two workgroups a CU, while a range keeps DECODE_RANGE keys (or 1024 of the
+// larger kernel, whose partial sums are 128 rows) of a sequence as long as the table allows.
 struct PagedPlan {
   int row_tiles;  // 1, 2: 16 or 32 rows (paged_decode); 0: 128 (packed_fwd)
   int nsplit;
@@ -1330,8 +1330,9 @@ static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int 
   pl.row_tiles = each <= 16 ? 1 : (each <= 32 ? 2 : 0);
   const long tile = pl.row_tiles ? 16 * pl.row_tiles : alg::PK_ROWS;
   const long groups = std::max(1L, std::max((rows + tile - 1) / tile, (long)std::min(S, N)) * Hkv);
-  const long cap = (long)width * page, least = pl.row_tiles ? 512 : 1024;
-  pl.nsplit = (int)std::max(1L, std::min(std::min((512 + groups - 1) / groups, 64L), cap / least));
+  const long cap = (long)width * page, least = pl.row_tiles ? alg::DECODE_RANGE : 1024;
+  const long most = std::min((512 + groups - 1) / groups, (long)alg::MAX_RANGES);
+  pl.nsplit = (int)std::max(1L, std::min(most, cap / least));
   const size_t parts = pl.nsplit > 1 ? (size_t)pl.nsplit * N * H : 0;
   pl.zt = align256(parts * D * sizeof(float));
   pl.total = pl.zt + align256(parts * 2 * sizeof(float));

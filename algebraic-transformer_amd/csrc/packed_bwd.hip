@@ -34,6 +34,7 @@ __device__ __forceinline__ void packed_elem(float s, float dp, float rs, float d
   const float t = CARE ? weight_t_careful(s, b, r) : weight_t(s, b, r);
   pw = pow2n<L2N>(t * __builtin_fabsf(rs), log2n);
   ds = pw * (dp - di) * r;
+  keep_here(pw, ds);
   if (dead) pw = ds = 0.0f;
 }
 
@@ -48,8 +49,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
 
   const int lane = threadIdx.x & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
-  const int kvh = blockIdx.x % p.Hkv, slot = (gridDim.x - 1 - blockIdx.x) / p.Hkv;  // longest rows first
-  const PackedSeq f = packed_find(p.cu, p.N, p.S, p.G, PK_ROWS, slot);
+  const int kvh = blockIdx.x % p.Hkv;
+  const PackedSeq f = packed_find<true>(p.cu, p.N, p.S, p.G, PK_ROWS, blockIdx.x / p.Hkv, gridDim.x / p.Hkv);
   const int G = p.G, R = f.len * G, r0 = f.tile * PK_ROWS;
   if (f.tile < 0 || r0 >= R) return;
   const int myr = r0 + wave * 32 + l32;
@@ -73,9 +74,6 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
 
   const bf16* kbase = p.k + (size_t)kvh * p.k_hs + (size_t)f.start * p.k_ts;
   const bf16* vbase = p.v + (size_t)kvh * p.v_hs + (size_t)f.start * p.v_ts;
-  const int lrow = lane / CPR;
-  const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
-  const int chunkb = 16 * ((lane % CPR) ^ swz_chunk<CPR>(lrow));
   // The 16 keys of tile kt that this wave copies; past the sequence they read as zeros.
   auto group = [&](int kt) {
     KvGroup g;
@@ -95,6 +93,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
     auto llb = LDS_PTR(bf16, lb);
     asm volatile("" : "+s"(lla), "+s"(llb));
     const int J = wave * PW + j;
+    int lrow = lane / CPR, chunkb = 16 * ((lane % CPR) ^ swz_chunk<CPR>(lane / CPR));
+    asm volatile("" : "+v"(lrow), "+v"(chunkb));  // computed here, not kept live
+    const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
     const int col = chunkb ^ (16 * swz_chunk<CPR>(RPI * J));
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lla + J * 512, 16, RPI * j * (int)p.k_ts * 2 + k_row + col, 0, 0, 0);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, llb + J * 512, 16, RPI * j * (int)p.v_ts * 2 + v_row + col, 0, 0, 0);
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   const float rs = live ? p.stat[srow] : 0.0f;
   if (live && h == 0) p.di[srow] = di;
   const bool careful = __syncthreads_or(rs < 0.0f) != 0;
-  if (threadIdx.x == 0) p.care[(size_t)slot * p.Hkv + kvh] = careful;
+  if (threadIdx.x == 0) p.care[(size_t)packed_slot(f, G, PK_ROWS) * p.Hkv + kvh] = careful;
   const int log2n = p.sc.log2n;
   const float b2 = p.sc.b;
   // Plain form: dS = (t^n r) fma(rs^n, dP, - rs^n di), one instruction less than P (dP - di) r.
@@ -201,7 +202,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
       const bool dead = MASKED && kb0 + blk * 32 + 8 * (i >> 2) + 4 * h + (i & 3) > mytok;
       float r;
       const float w = pow2n<L2N>(weight_t(s[blk][i], b2, r), log2n);
-      dsv[i] = dead ? 0.0f : (w * r) * __builtin_fmaf(pz, dp[blk][i], nzd);
+      float ds = (w * r) * __builtin_fmaf(pz, dp[blk][i], nzd);
+      if constexpr (MASKED) keep_here(ds);
+      dsv[i] = dead ? 0.0f : ds;
       if (i & 1) {
         da[blk][i >> 3][(i & 7) - 1] = f2bf(dsv[i - 1]);
         da[blk][i >> 3][i & 7] = f2bf(dsv[i]);
@@ -364,19 +367,20 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   __shared__ __attribute__((aligned(16))) float di1[BQ];
 
   const int kvh = blockIdx.x % p.Hkv, G = p.G;
-  int slot = blockIdx.x / p.Hkv;
+  int item = blockIdx.x / p.Hkv;
   if (p.dsink) {
-    if (slot < G) {
-      packed_sink_grad(p, kvh, slot);
+    if (item < G) {
+      packed_sink_grad(p, kvh, item);
       return;
     }
-    slot -= G;
+    item -= G;
   }
   const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
-  const PackedSeq f = packed_find(p.cu, p.N, p.S, 1, PK_KEYS, slot);  // keys: one row a token
-  const int k0 = f.tile * PK_KEYS;
-  if (f.tile < 0 || k0 >= f.len) return;
+  // Keys: one row a token; the first keys of a sequence, which the most rows see, are its last tile.
+  const PackedSeq f = packed_find_heavy(p.cu, p.N, p.S, 1, PK_KEYS, item, packed_slots(p.N, 1, p.S, PK_KEYS));
+  const int k0 = ((f.len + PK_KEYS - 1) / PK_KEYS - 1 - f.tile) * PK_KEYS;
+  if (f.tile < 0 || k0 < 0) return;
   const size_t dk_base = ((size_t)f.start * p.Hkv + kvh) * D;
   if (f.s == p.S) {  // tokens behind the last sequence
     const bf16x8 z = {};
@@ -410,10 +414,24 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
     const bf16 *q, *o;
     int rem, left;  // first row's head; rows left from the tile's first
   };
-  auto source = [&](int j) {
-    const int r = j * BQ, tb = r / G;
-    const size_t t = r < rows ? tb : 0;
-    return Tile{qbase + t * p.q_ts, dobase + t * p.do_ts, r - tb * G, rows - r};
+  // The tiles from the last rows to the first: workgroups of one sequence and head that run at the
+  // same time then read the same rows, out of the L2, wherever their keys lie (packed documents of
+  // 16384 tokens, 16 heads over 4, D = 128: 545 us from the first rows on, 418 us so). The next
+  // tile's first token and head are kept up without a division.
+  const int step_t = BQ / G, step_h = BQ - step_t * G;
+  int next_r = (nq - 1) * BQ, next_t = next_r / G, next_h = next_r - next_t * G;
+  auto source = [&]() {
+    const bool some = next_r >= 0;
+    const size_t t = some ? next_t : 0;
+    const Tile now{qbase + t * p.q_ts, dobase + t * p.do_ts, next_h, some ? rows - next_r : 0};
+    next_r -= BQ;
+    next_t -= step_t;
+    next_h -= step_h;
+    if (next_h < 0) {
+      next_h += G;
+      --next_t;
+    }
+    return now;
   };
   auto dma_part = [&](bf16* la, bf16* lb, const Tile& t, int j) {
     const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)t.q, (short)0, 0x7ffffff0, BUF_RSRC_WORD3);
@@ -431,10 +449,10 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, lla + J * 512, 16, qo, 0, 0, 0);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(ro, llb + J * 512, 16, oo, 0, 0, 0);
   };
-  // Statistics of row tile j (stat by wave 0, di by wave 1); rows past the sequence are zeros.
-  auto stat_dma = [&](float* ls, float* ld, int j) {
-    const int left = min(max(rows - j * BQ, 0), BQ);
-    const size_t at = sbase + (left > 0 ? j * BQ : 0);
+  // Statistics of a row tile (stat by wave 0, di by wave 1); rows past the sequence are zeros.
+  auto stat_dma = [&](float* ls, float* ld, const Tile& t) {
+    const int left = min(max(t.left, 0), BQ);
+    const size_t at = sbase + (left > 0 ? rows - t.left : 0);
     const __amdgpu_buffer_rsrc_t rst = __builtin_amdgcn_make_buffer_rsrc((void*)(p.stat + at), (short)0, left * 4, BUF_RSRC_WORD3);
     const __amdgpu_buffer_rsrc_t rdi = __builtin_amdgcn_make_buffer_rsrc((void*)(p.di + at), (short)0, left * 4, BUF_RSRC_WORD3);
     if (wave == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(rst, LDS_PTR(void, ls), 4, lane * 4, 0, 0, 0);
@@ -442,10 +460,10 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   };
   auto lds_at = [](int row, int col) { return row * D + (((col >> 3) ^ Lay::swz(row)) << 3) + (col & 7); };
   {
-    const Tile t = source(0);
+    const Tile t = source();
 #pragma unroll
     for (int j = 0; j < PW; ++j) dma_part(Qs0, dOs0, t, j);
-    stat_dma(st0, di0, 0);
+    stat_dma(st0, di0, t);
   }
   // K (scaled as the queries are in the forward: an exact power of two) and V fragments of this
   // wave's keys; keys past the sequence are zero.
@@ -502,7 +520,8 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
     float* din = BUF ? di0 : di1;
     const float* sts = BUF ? st1 : st0;
     const float* dis = BUF ? di1 : di0;
-    const Tile next = source(qt + 1);
+    const Tile next = source();
+    const int row0 = (nq - 1 - qt) * BQ;  // the tile's first row
     floatx4 s[4], dp[4];
     floatx4 sv[2], dvv[2];  // stat and di of a block's rows (slot = block & 1)
     bf16x8 pa[2], da[2];
@@ -524,7 +543,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
     };
     // P and dS of row 16 b + qoff + i of the tile.
     auto elem = [&](int b, int i) {
-      const bool dead = MASKED && qt * BQ + 16 * b + qoff + i < dead_below;
+      const bool dead = MASKED && row0 + 16 * b + qoff + i < dead_below;
       packed_elem<L2N, false>(s[b][i], dp[b][i], sv[b & 1][i], dvv[b & 1][i], b2, log2n, dead, pw[i], dsx[i]);
       const int c = b >> 1, j0 = 4 * (b & 1);
       if (i & 1) {
@@ -562,7 +581,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
         if (st == NS - 1) {
 #pragma unroll
           for (int j = NS; j < PW; ++j) dma_part(Qn, dOn, next, j);
-          stat_dma(stn, din, qt + 1);
+          stat_dma(stn, din, next);
         }
         step_order_r<2, 0>(t + PF < 4 * NS ? 2 : 0);
       } else {
@@ -601,26 +620,27 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   }
   if (!careful) {
     // In pairs of tiles, as in the forward.
+    const int full = (nq - nmask) & ~1;
     int qt = 0;
-    while (qt < nmask) {
-      tile(std::integral_constant<int, 0>{}, std::true_type{}, qt);
-      if (++qt >= nq) break;
-      tile(std::integral_constant<int, 1>{}, std::true_type{}, qt);
-      ++qt;
-    }
-    while (qt < nq) {
+    for (; qt < full; qt += 2) {
       tile(std::integral_constant<int, 0>{}, std::false_type{}, qt);
-      if (++qt >= nq) break;
-      tile(std::integral_constant<int, 1>{}, std::false_type{}, qt);
-      ++qt;
+      tile(std::integral_constant<int, 1>{}, std::false_type{}, qt + 1);
+    }
+    for (; qt < nq; qt += 2) {
+      tile(std::integral_constant<int, 0>{}, std::true_type{}, qt);
+      if (qt + 1 >= nq) break;
+      tile(std::integral_constant<int, 1>{}, std::true_type{}, qt + 1);
     }
   } else {
+    next_r = (nq - 1) * BQ;
+    next_t = next_r / G;
+    next_h = next_r - next_t * G;
     for (int qt = 0; qt < nq; ++qt) {
       __syncthreads();  // every wave is done with the tile before
-      const Tile now = source(qt);
+      const Tile now = source();
 #pragma unroll
       for (int j = 0; j < PW; ++j) dma_part(Qs0, dOs0, now, j);
-      stat_dma(st0, di0, qt);
+      stat_dma(st0, di0, now);
       __builtin_amdgcn_s_waitcnt(VMCNT0);
       __syncthreads();
       for (int c = 0; c < 2; ++c) {  // halves of 32 rows
@@ -638,7 +658,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
           for (int i = 0; i < 4; ++i) {
             const int x = 16 * b + qoff + i;
             float pw, ds;
-            packed_elem<0, true>(s[i], dp[i], st0[x], di0[x], b2, log2n, qt * BQ + x < dead_below, pw, ds);
+            packed_elem<0, true>(s[i], dp[i], st0[x], di0[x], b2, log2n, (nq - 1 - qt) * BQ + x < dead_below, pw, ds);
             pa[4 * u + i] = f2bf(pw);
             da[4 * u + i] = f2bf(ds);
           }

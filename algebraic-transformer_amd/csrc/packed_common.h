@@ -33,6 +33,8 @@ namespace alg {
 
 constexpr int PK_ROWS = 128;  // rows (token, head of the group) per workgroup of the prompt kernels
 constexpr int PK_BK = 64;     // keys per LDS tile
+constexpr int DECODE_RANGE = 256;  // keys that a range of paged_decode's holds at least
+constexpr int MAX_RANGES = 256;    // ranges that packed_combine_kernel joins
 
 // How scores become weights for one call (host: attn_scale).
 struct AttnScale {
@@ -99,6 +101,11 @@ struct PackedBwdParams {
   AttnScale sc;
 };
 
+// Values formed here whatever is selected of them afterwards: without it the arithmetic of a masked
+// element moves behind a branch of its own, a branch an element.
+__device__ __forceinline__ void keep_here(float& a) { asm volatile("" : "+v"(a)); }
+__device__ __forceinline__ void keep_here(float& a, float& b) { asm volatile("" : "+v"(a), "+v"(b)); }
+
 __device__ __forceinline__ float sink_score(const float* sink, int count, int head, float c, float a) {
   return sink[count == 1 ? 0 : head] / (c * a);
 }
@@ -133,10 +140,57 @@ struct PackedSeq {
 __device__ __forceinline__ int packed_start(const int* cu, int s, int N) {
   return s == 0 ? 0 : min(max(cu[s], 0), N);
 }
-__device__ __forceinline__ PackedSeq packed_find(const int* cu, int N, int S, int G, int rows, int slot) {
+// Up to 64 sequences, one a lane of the wave: the tiles are counted by a sum over the lanes, and a
+// launch's first items are tiles, without the gaps of the slots (empty workgroups between others
+// leave the CUs unevenly filled: 8 requests of 8000 keys, 8 heads in 4 ranges, 58 us instead of 47).
+// The tokens behind the last sequence come last.
+struct PackedLanes {
+  int start, len, tiles;  // of the lane's sequence
+};
+__device__ __forceinline__ PackedLanes packed_lanes(const int* cu, int N, int S, int G, int rows) {
   const int lane = threadIdx.x & 63;
+  PackedLanes a{0, 0, 0};
+  if (lane < S) {
+    a.start = packed_start(cu, lane, N);
+    a.len = max(packed_start(cu, lane + 1, N) - a.start, 0);
+  }
+  a.tiles = (a.len * G + rows - 1) / rows;
+  return a;
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readfirstlane(__shfl(v, lane, 64)); }
+__device__ __forceinline__ PackedSeq packed_tail(const int* cu, int N, int S, int tile) {
+  PackedSeq f;
+  f.s = S;
+  f.start = __builtin_amdgcn_readfirstlane(packed_start(cu, S, N));
+  f.len = N - f.start;
+  f.tile = tile;
+  return f;
+}
+// Item `item` of a launch of `slots` of them: sequence after sequence, or backwards.
+template <bool BACKWARDS>
+__device__ __forceinline__ PackedSeq packed_find(const int* cu, int N, int S, int G, int rows, int item, int slots) {
+  const int lane = threadIdx.x & 63;
+  if (S <= 64) {
+    const PackedLanes a = packed_lanes(cu, N, S, G, rows);
+    int upto = a.tiles;  // tiles of the sequences up to the lane's
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int below = __shfl_up(upto, m, 64);
+      if (lane >= m) upto += below;
+    }
+    const int total = lane_value(upto, 63);
+    if (item >= total) return packed_tail(cu, N, S, item - total);
+    if (BACKWARDS) item = total - 1 - item;
+    PackedSeq f;
+    f.s = __builtin_amdgcn_readfirstlane(__popcll(__ballot(upto <= item)));
+    f.start = lane_value(a.start, f.s);
+    f.len = lane_value(a.len, f.s);
+    f.tile = item - lane_value(upto - a.tiles, f.s);
+    return f;
+  }
+  const int slot = BACKWARDS ? slots - 1 - item : item;
   int lo = 0, n = S + 1;
-  while (n > 1) {  // 64 candidates at a time: one step up to 63 sequences, two up to 4095
+  while (n > 1) {  // 64 candidates at a time: two steps up to 4095 sequences
     const int step = (n + 63) / 64;
     const int at = lane * step;
     bool ok = false;
@@ -155,6 +209,44 @@ __device__ __forceinline__ PackedSeq packed_find(const int* cu, int N, int S, in
   f.len = max(end - f.start, 0);
   f.tile = slot - (f.start * G / rows + f.s);
   return f;
+}
+// A tile's slot.
+__device__ __forceinline__ int packed_slot(const PackedSeq& f, int G, int rows) { return f.start * G / rows + f.s + f.tile; }
+
+// The same for a kernel whose work grows with the tile's number: by falling tile number over all
+// sequences, so that the longest work starts first wherever its sequence lies. With f(l) the number
+// of tiles numbered l or more, item i has the largest l with f(l) > i, found by halving. From 65
+// sequences on, packed_find's order backwards. (dK/dV of nine documents, 16384 tokens, 16 heads over
+// 4, D = 128: 454 us, 486 us in packed_find's order; of 13 documents, 8161 tokens, 16 heads, D = 64,
+// which are more workgroups of more equal work: 63 and 60.)
+__device__ __forceinline__ PackedSeq packed_find_heavy(const int* cu, int N, int S, int G, int rows, int item, int slots) {
+  if (S > 64) return packed_find<true>(cu, N, S, G, rows, item, slots);
+  const int lane = threadIdx.x & 63;
+  const PackedLanes a = packed_lanes(cu, N, S, G, rows);
+  const auto f = [&](int l) {
+    int c = max(a.tiles - l, 0);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) c += __shfl_xor(c, m, 64);
+    return __builtin_amdgcn_readfirstlane(c);
+  };
+  const int total = f(0);
+  if (item >= total) return packed_tail(cu, N, S, item - total);
+  int lo = 0, hi = slots;  // f(lo) > item, f(hi) <= item: every tile's number is below `slots`
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (f(mid) > item) lo = mid;
+    else hi = mid;
+  }
+  const int k = item - f(lo + 1);  // k-th of the sequences that have a tile `lo`
+  const unsigned long long has = __ballot(a.tiles > lo);
+  const int before = __popcll(has & ((1ull << lane) - 1));
+  const unsigned long long at = __ballot(a.tiles > lo && before == k);
+  PackedSeq r;
+  r.s = __builtin_amdgcn_readfirstlane(at ? __builtin_ctzll(at) : 0);
+  r.start = lane_value(a.start, r.s);
+  r.len = lane_value(a.len, r.s);
+  r.tile = at ? lo : -1;
+  return r;
 }
 
 // One 16-row group of a K / V tile: where its rows start, and how many of them exist.

@@ -37,8 +37,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
 
   const int lane = threadIdx.x & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
-  const int kvh = blockIdx.x % p.Hkv, slot = (gridDim.x - 1 - blockIdx.x) / p.Hkv;  // longest rows first
-  const PackedSeq f = packed_find(p.cu, p.N, p.S, p.G, PK_ROWS, slot);
+  // Workgroups: key head, range of keys, item; a sequence's longest rows first.
+  const int kvh = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv, range = unit % p.nsplit;
+  const PackedSeq f = packed_find<true>(p.cu, p.N, p.S, p.G, PK_ROWS, unit / p.nsplit, gridDim.x / p.Hkv / p.nsplit);
   const int G = p.G;
   const int R = f.len * G;           // rows of the sequence
   const int r0 = f.tile * PK_ROWS;   // this workgroup's first row
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   const size_t srow = (size_t)kvh * p.N * G + (size_t)f.start * G + min(myr, R - 1);
 
   if (f.s == p.S) {  // tokens behind the last sequence
-    if (live && blockIdx.y == 0) {
+    if (live && range == 0) {
       const bf16x8 z = {};
       for (int d = 8 * h; d < D; d += 16) *reinterpret_cast<bf16x8*>(p.o + orow + d) = z;
       if (p.stat && h == 0) p.stat[srow] = 0.0f;
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   int kt0 = 0, kt1 = posmax < 0 ? 0 : posmax / BK + 1;  // this workgroup's key tiles
   if (p.nsplit > 1) {
     const int per = ceil_div(kt1, p.nsplit);
-    kt0 = min((int)blockIdx.y * per, kt1);
+    kt0 = min(range * per, kt1);
     kt1 = min(kt0 + per, kt1);
   }
   const int nfull = posmin < 0 ? 0 : (posmin + 1) / BK;  // tiles before every row's position
@@ -112,10 +113,10 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     }
     return g;
   };
-  const int lrow = lane / CPR, lchunk = lane % CPR;
-  const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
-  const int chunkb = 16 * (lchunk ^ swz_chunk<CPR>(lrow));
   auto dma = [&](bf16* la, bf16* lb, const KvGroup& g, int j) {
+    int lrow = lane / CPR, chunkb = 16 * ((lane % CPR) ^ swz_chunk<CPR>(lane / CPR));
+    asm volatile("" : "+v"(lrow), "+v"(chunkb));  // computed here, not kept live
+    const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
     const int kn = g.rows > 0 ? ((g.rows - 1) * (int)p.k_ts + D) * 2 : 0;
     const int vn = g.rows > 0 ? ((g.rows - 1) * (int)p.v_ts + D) * 2 : 0;
     const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)g.k, (short)0, kn, BUF_RSRC_WORD3);
@@ -212,6 +213,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
       smax = fmaxf(smax, __builtin_fabsf(x));
       float r;
       float wi = pow2n<L2N>(weight_t(x, b2, r), log2n);
+      if constexpr (MASKED) keep_here(wi);
       if (dead) wi = 0.0f;
       lsum += wi;
       w[i] = wi;
@@ -347,6 +349,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
           const bool dead = kb + 8 * (i >> 2) + 4 * h + (i & 3) > mypos;
           float r;
           float w = pow2n<0>(weight_t_careful(dead ? 0.0f : s[i], b2, r) * shift, log2n);
+          keep_here(w);
           if (dead) w = 0.0f;
           lsum += w;
           pf[i >> 3][i & 7] = f2bf(w);
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   }
   if (!live) return;
   if (p.nsplit > 1) {
-    const size_t part = (size_t)blockIdx.y * p.Hkv * p.N * G + srow;
+    const size_t part = (size_t)range * p.Hkv * p.N * G + srow;
     float* O = p.part_o + part * D;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
@@ -408,54 +411,95 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
 }
 
 // Rows whose keys were split: o = sum_i f_i O_i / (sum_i f_i Z_i + sink), f_i = (T_i / T)^n with
-// T_i the range's shift and T the largest of them and the sink's. One wave a row, at most 64 ranges;
-// a range without keys for the row has Z_i = 0 and counts for nothing. The order of the sums is
-// fixed.
-template <int D>
+// T_i the range's shift and T the largest of them and the sink's; a range without keys for the row
+// has Z_i = 0 and counts for nothing (its sums are not read: they may not be written). The order of
+// the sums is fixed. Latency is all of it, so every load that can be is issued before a result is
+// waited for. WIDE: a workgroup a row, thread i range i, its waves a quarter of the ranges' sums each
+// (16 rows of 64 ranges: 12.7 us by one wave a row, of which launches are about 5). Else, up to 8
+// ranges, a wave a row, every lane all of the ranges' factors.
+template <int D, bool WIDE>
 __global__ __launch_bounds__(256) void packed_combine_kernel(PackedParams p) {
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // token N, head H
+  constexpr int E = D / 64;  // columns a lane
+  typedef float fvec __attribute__((ext_vector_type(E)));
+  __shared__ float fs[MAX_RANGES], red[2][4];
+  __shared__ fvec part[WIDE ? 4 : 1][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = WIDE ? blockIdx.x : blockIdx.x * 4 + wave;  // token, head
   if (row >= p.N * p.H) return;
   const int tok = row / p.H, head = row - tok * p.H, kvh = head / p.G;
   const int total = packed_start(p.cu, p.S, p.N);
-  if (p.S == 0 || tok >= total) return;  // written as zeros by the first range's workgroups
+  if (tok >= total) return;  // behind the last sequence: zeros, written by the first range's workgroups
   const size_t rows = (size_t)p.Hkv * p.N * p.G;
   const size_t srow = (size_t)kvh * p.N * p.G + (size_t)tok * p.G + (head - kvh * p.G);
+  const float* O = p.part_o + srow * D + lane * E;
   const int log2n = p.sc.log2n;
-  float ts = 0.0f, T = 0.0f;
+  float T = 0.0f, ts = 0.0f;
   if (p.sink) {
     float r;
-    ts = weight_t_careful(sink_score(p.sink, p.sink_count, head, p.c, p.sc.a), p.sc.b, r);
-    T = ts;
+    T = ts = weight_t_careful(sink_score(p.sink, p.sink_count, head, p.c, p.sc.a), p.sc.b, r);
   }
-  float2 zt = make_float2(0.0f, 0.0f);  // lane i: range i
-  if (lane < p.nsplit) zt = *reinterpret_cast<const float2*>(p.part_zt + 2 * (lane * rows + srow));
-  if (zt.x != 0.0f) T = fmaxf(T, zt.y);
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) T = fmaxf(T, __shfl_xor(T, m, 64));
-  const float f = zt.x != 0.0f ? pow2n<0>(zt.y / T, log2n) : 0.0f;
-  float Z = f * zt.x;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) Z += __shfl_xor(Z, m, 64);
-  if (p.sink) Z += pow2n<0>(ts / T, log2n);
-  constexpr int E = D / 64;  // columns a lane
-  typedef float fvec __attribute__((ext_vector_type(E)));
+  float Z;
   fvec acc = 0.0f;
-  for (int i0 = 0; i0 < p.nsplit; i0 += 8) {  // eight ranges' loads in flight
+  if constexpr (WIDE) {
+    const bool mine = (int)threadIdx.x < p.nsplit;
+    const float2 zt = mine ? *reinterpret_cast<const float2*>(p.part_zt + 2 * (threadIdx.x * rows + srow)) : make_float2(0.0f, 0.0f);
+    if (zt.x != 0.0f) T = fmaxf(T, zt.y);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) T = fmaxf(T, __shfl_xor(T, m, 64));
+    if (lane == 0) red[0][wave] = T;
+    __syncthreads();
+    T = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float f = zt.x != 0.0f ? pow2n<0>(zt.y / T, log2n) : 0.0f;
+    fs[threadIdx.x] = f;
+    Z = f * zt.x;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) Z += __shfl_xor(Z, m, 64);
+    if (lane == 0) red[1][wave] = Z;
+    __syncthreads();
+    Z = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    for (int i0 = wave; i0 < p.nsplit; i0 += 32) {  // eight ranges' loads in flight
+      fvec o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        o[k] = *reinterpret_cast<const fvec*>(O + min(i0 + 4 * k, p.nsplit - 1) * rows * D);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float fi = i0 + 4 * k < p.nsplit ? fs[i0 + 4 * k] : 0.0f;
+        if (fi != 0.0f) acc += fi * o[k];
+      }
+    }
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0) return;
+    acc = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+  } else {
+    float2 zt[8];
     fvec o[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      o[k] = *reinterpret_cast<const fvec*>(p.part_o + (min(i0 + k, p.nsplit - 1) * rows + srow) * D + lane * E);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float fi = __shfl(f, (i0 + k) & 63, 64);  // 0 past the last range, and where none was written
-      if (i0 + k < p.nsplit && fi != 0.0f) acc += fi * o[k];
+    for (int i = 0; i < 8; ++i) {
+      const size_t at = (size_t)min(i, p.nsplit - 1) * rows;
+      zt[i] = *reinterpret_cast<const float2*>(p.part_zt + 2 * (at + srow));
+      o[i] = *reinterpret_cast<const fvec*>(O + at * D);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i >= p.nsplit) zt[i].x = 0.0f;
+      if (zt[i].x != 0.0f) T = fmaxf(T, zt[i].y);
+    }
+    Z = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (zt[i].x != 0.0f) {
+        const float f = pow2n<0>(zt[i].y / T, log2n);
+        Z += f * zt[i].x;
+        acc += f * o[i];
+      }
   }
+  if (p.sink) Z += pow2n<0>(ts / T, log2n);
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
-  bf16* O = p.o + (size_t)row * D + lane * E;
-  if constexpr (E == 2) *reinterpret_cast<unsigned*>(O) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-  else O[0] = f2bf(acc[0] * inv);
+  bf16* out = p.o + (size_t)row * D + lane * E;
+  if constexpr (E == 2) *reinterpret_cast<unsigned*>(out) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  else out[0] = f2bf(acc[0] * inv);
 }
 
 template <int D, bool PAGED>
@@ -464,16 +508,22 @@ static void launch_fwd(const PackedParams& p, dim3 grid, hipStream_t st) {
   else hipLaunchKernelGGL((packed_fwd_kernel<D, 0, PAGED>), grid, dim3(256), 0, st, p);
 }
 
+template <int D>
+static void launch_combine(const PackedParams& p, hipStream_t st) {
+  const long rows = (long)p.N * p.H;
+  if (p.nsplit > 8) hipLaunchKernelGGL((packed_combine_kernel<D, true>), dim3((unsigned)rows), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((packed_combine_kernel<D, false>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
+}
+
 hipError_t launch_packed_combine(const PackedParams& p, int D, hipStream_t st) {
   KTimer t("packed_combine", st);
-  const dim3 grid((unsigned)(((long)p.N * p.H + 3) / 4));
-  if (D == 64) hipLaunchKernelGGL(packed_combine_kernel<64>, grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(packed_combine_kernel<128>, grid, dim3(256), 0, st, p);
+  if (D == 64) launch_combine<64>(p, st);
+  else launch_combine<128>(p, st);
   return hipGetLastError();
 }
 
 hipError_t launch_packed_fwd(const PackedParams& p, int D, bool paged, hipStream_t st) {
-  const dim3 grid(p.Hkv * packed_slots(p.N, p.G, p.S, PK_ROWS), p.nsplit);
+  const dim3 grid(p.Hkv * p.nsplit * packed_slots(p.N, p.G, p.S, PK_ROWS));
   {
     KTimer t(paged ? "paged_fwd" : "packed_fwd", st);
     if (D == 64) paged ? launch_fwd<64, true>(p, grid, st) : launch_fwd<64, false>(p, grid, st);

@@ -10,7 +10,9 @@
 //   of key l % 16), weights in registers, O^T += V^T P^T, where the 32 keys are numbered
 //   (lane group g, slot j) -> 4 g + j % 4 + 16 (j / 4), the order in which S^T leaves the MFMA;
 //   V comes through a private LDS tile (direct copies) and is read transposed.
-// While a block is computed the next one's 16 KB are in flight: 8 waves a CU hold up to 128 KB.
+// While a wave computes a block, the next one's 16 KB (D = 128) are under way: up to 128 KB a CU.
+// (One workgroup of 16 waves for a whole short sequence, without a launch to join ranges, was slower
+// than ranges: a CU alone reads about 50 GB/s, and 16 heads' 1024 keys took 23 us, 17 us in ranges.)
 // A group of 16 keys lies in one page (pages hold a multiple of 16 keys): its page number is one
 // scalar load, whose counter is not the vector loads', so that looking a page up never waits for
 // the keys and values in flight.
@@ -25,24 +27,26 @@ namespace alg {
 template <int D, int RT, int L2N>
 __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
   static_assert(D == 64 || D == 128, "head_dim");
+  constexpr int WAVES = 4;
   constexpr int NS = D / 32, NDB = D / 16, CPR = D / 8, RPI = 64 / CPR, PW = 16 / RPI;
   constexpr int LOADS = 2 * NS + 2 * PW;  // vector loads and copies of one block of 32 keys
   constexpr int ROWS = 16 * RT;
   constexpr int BLK = 32;
-  __shared__ __attribute__((aligned(16))) bf16 Vs[4 * 2 * BLK * D];
-  __shared__ float jT[4][ROWS], jZ[4][ROWS];
-  static_assert(4 * ROWS * D * sizeof(float) <= sizeof(Vs), "the waves' sums fit the V tiles");
+  __shared__ __attribute__((aligned(16))) bf16 Vs[WAVES * 2 * BLK * D];
+  __shared__ float jT[WAVES][ROWS], jZ[WAVES][ROWS];
+  static_assert(WAVES * ROWS * D * sizeof(float) <= sizeof(Vs), "the waves' sums fit the V tiles");
 
   const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kvh = blockIdx.x % p.Hkv;
-  const PackedSeq f = packed_find(p.cu, p.N, p.S, p.G, ROWS, blockIdx.x / p.Hkv);
+  // Workgroups: key head, range of keys, item.
+  const int kvh = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv, range = unit % p.nsplit;
+  const PackedSeq f = packed_find<false>(p.cu, p.N, p.S, p.G, ROWS, unit / p.nsplit, gridDim.x / p.Hkv / p.nsplit);
   const int G = p.G, R = f.len * G, r0 = f.tile * ROWS;
   if (f.tile < 0 || r0 >= R) return;
   const int nrow = min(ROWS, R - r0);  // live rows of the tile
   if (f.s == p.S) {                    // tokens behind the last sequence
-    if (blockIdx.y == 0)
-      for (int i = threadIdx.x; i < nrow * (D / 8); i += 256) {
+    if (range == 0)
+      for (int i = threadIdx.x; i < nrow * (D / 8); i += 64 * WAVES) {
         const int r = r0 + i / (D / 8), tok = r / G, head = kvh * G + r - tok * G;
         const bf16x8 z = {};
         *reinterpret_cast<bf16x8*>(p.o + ((size_t)(f.start + tok) * p.H + head) * D + 8 * (i % (D / 8))) = z;
@@ -52,11 +56,11 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
   const int L = min(max(p.kv_lens[f.s], 0), p.width * p.page);
   const int off = L - f.len;
   const int kend = max(off + (r0 + nrow - 1) / G + 1, 0);  // keys that some row sees: [0, kend)
-  // This workgroup's blocks of 32 keys: an equal share, of at least 4 blocks a wave.
+  // This workgroup's blocks of 32 keys: an equal share, of at least DECODE_RANGE keys.
   int b0 = 0, b1 = ceil_div(kend, BLK);
   if (p.nsplit > 1) {
-    const int per = max(ceil_div(b1, p.nsplit), 16);
-    b0 = min((int)blockIdx.y * per, b1);
+    const int per = max(ceil_div(b1, p.nsplit), DECODE_RANGE / BLK);
+    b0 = min(range * per, b1);
     b1 = min(b0 + per, b1);
   }
 
@@ -175,6 +179,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
           const int u = j >> 2, i = j & 3;
           float r;
           float w = pow2n<L2N>(weight_t(s[rt][u][i], b2, r), log2n);
+          keep_here(w);
           if (blk * BLK + 16 * u + 4 * g + i > mypos[rt]) w = 0.0f;
           lsum[rt] += w;
           pf[rt][j] = f2bf(w);
@@ -222,18 +227,18 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  // Blocks b0 + wave, + 4, ...; a block past the range loads nothing (empty descriptors).
+  // Blocks b0 + wave, + WAVES, ...; a block past the range loads nothing (empty descriptors).
   KBlock ka, kb;
   load(b0 + wave, ka, vbuf);
-  for (int blk = b0 + wave; blk < b1; blk += 8) {
-    load(blk + 4, kb, vbuf + BLK * D);
+  for (int blk = b0 + wave; blk < b1; blk += 2 * WAVES) {
+    load(blk + WAVES, kb, vbuf + BLK * D);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
     __builtin_amdgcn_sched_barrier(0);
     compute(blk, ka, vbuf);
-    load(blk + 8, ka, vbuf);
+    load(blk + 2 * WAVES, ka, vbuf);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
     __builtin_amdgcn_sched_barrier(0);
-    if (blk + 4 < b1) compute(blk + 4, kb, vbuf + BLK * D);
+    if (blk + WAVES < b1) compute(blk + WAVES, kb, vbuf + BLK * D);
   }
   __builtin_amdgcn_s_waitcnt(VMCNT0);  // copies into the tiles that the join overwrites
 
@@ -255,7 +260,9 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
       *reinterpret_cast<floatx4*>(sO + ((wave * ROWS) + 16 * rt + l16) * D + 16 * db + 4 * g) = oacc[rt][db];
   }
   __syncthreads();
-  constexpr int TPR = 256 / ROWS, CPT = D / TPR;  // threads a row, columns a thread
+  constexpr int TPR = 64 * WAVES / ROWS, CPT = D / TPR;  // threads a row, columns a thread
+  typedef float fvec __attribute__((ext_vector_type(CPT)));
+  typedef bf16 bvec __attribute__((ext_vector_type(CPT)));
   const int row = threadIdx.x / TPR, c0 = (threadIdx.x % TPR) * CPT;
   const int r = r0 + row;
   if (r >= R) return;
@@ -267,44 +274,36 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
     Tm = ts = weight_t_careful(sink_score(p.sink, p.sink_count, head, p.c, p.sc.a), b2, rr);
   }
 #pragma unroll
-  for (int w = 0; w < 4; ++w)
+  for (int w = 0; w < WAVES; ++w)
     if (jZ[w][row] != 0.0f) Tm = fmaxf(Tm, jT[w][row]);
   float Z = sink ? pow2n<0>(ts / Tm, log2n) : 0.0f;
-  float acc[CPT] = {};
+  fvec acc = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (jZ[w][row] == 0.0f) continue;
-    const float fw = pow2n<0>(jT[w][row] / Tm, log2n);
-    Z += fw * jZ[w][row];
-#pragma unroll
-    for (int e = 0; e < CPT; ++e) acc[e] += fw * sO[(w * ROWS + row) * D + c0 + e];
+  for (int w = 0; w < WAVES; ++w) {
+    const float z = jZ[w][row];
+    const float fw = z != 0.0f ? pow2n<0>(jT[w][row] / Tm, log2n) : 0.0f;
+    Z += fw * z;
+    acc += fw * *reinterpret_cast<const fvec*>(sO + (w * ROWS + row) * D + c0);  // zeros where z is
   }
   if (p.nsplit > 1) {
-    const size_t part = (size_t)blockIdx.y * p.Hkv * p.N * G + (size_t)kvh * p.N * G + (size_t)f.start * G + r;
+    const size_t part = (size_t)range * p.Hkv * p.N * G + (size_t)kvh * p.N * G + (size_t)f.start * G + r;
     if (c0 == 0) {
       p.part_zt[2 * part] = Z;
       p.part_zt[2 * part + 1] = Tm;
     }
-    if (Z != 0.0f)  // an empty range's sums are not read
-#pragma unroll
-      for (int e = 0; e < CPT; e += 4)
-        *reinterpret_cast<floatx4*>(p.part_o + part * D + c0 + e) = floatx4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+    if (Z != 0.0f) *reinterpret_cast<fvec*>(p.part_o + part * D + c0) = acc;  // an empty range's is not read
     return;
   }
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
-  bf16* O = p.o + ((size_t)(f.start + tok) * p.H + head) * D + c0;
+  bvec out;
 #pragma unroll
-  for (int e = 0; e < CPT; e += 4) {
-    bf16x4 ob;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ob[i] = f2bf(acc[e + i] * inv);
-    *reinterpret_cast<bf16x4*>(O + e) = ob;
-  }
+  for (int e = 0; e < CPT; ++e) out[e] = f2bf(acc[e] * inv);
+  *reinterpret_cast<bvec*>(p.o + ((size_t)(f.start + tok) * p.H + head) * D + c0) = out;
 }
 
 template <int D, int RT>
 static void launch_decode(const PackedParams& p, hipStream_t st) {
-  const dim3 grid(p.Hkv * packed_slots(p.N, p.G, p.S, 16 * RT), p.nsplit);
+  const dim3 grid(p.Hkv * p.nsplit * packed_slots(p.N, p.G, p.S, 16 * RT));
   if (p.sc.log2n == 4) hipLaunchKernelGGL((paged_decode_kernel<D, RT, 4>), grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL((paged_decode_kernel<D, RT, 0>), grid, dim3(256), 0, st, p);
 }
