@@ -68,19 +68,19 @@ _SIGNATURES = {
                                _S]),
     "alg_rms_norm_fwd": (_I, [_P, _I, _I, _P, _P, _F, _P, _P]),
     "alg_rms_norm_bwd": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _S]),
-    "alg_add_rms_norm_fwd": (_I, [_P, _I, _I, _P, _P, _P, _F, _P, _P, _P]),
-    "alg_add_rms_norm_fp8": (_I, [_P, _I, _I, _P, _P, _P, _F, _P, _P, _P]),
-    "alg_add_rms_norm_bwd": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _S]),
-    "alg_packed_attn_fwd": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _F, _I, _P,
-                                 _P]),
+    "alg_add_rms_norm_fwd": (_I, [_P, _I, _I, _P, _P, _P, _I, _F, _P, _P, _P]),
+    "alg_add_rms_norm_fp8": (_I, [_P, _I, _I, _P, _P, _P, _I, _F, _P, _P, _P]),
+    "alg_add_rms_norm_bwd": (_I, [_P, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _S]),
+    "alg_packed_attn_fwd": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _F, _I,
+                                 _P, _P]),
     "alg_packed_attn_bwd_workspace_size": (_S, [_I, _I, _I, _I]),
-    "alg_packed_attn_bwd": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _F, _I, _P,
-                                 _P, _P, _L, _L, _P, _P, _P, _P, _P, _S]),
+    "alg_packed_attn_bwd": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _F, _I,
+                                 _P, _P, _P, _L, _L, _P, _P, _P, _P, _I, _P, _S]),
     "alg_paged_attn_workspace_size": (_S, [_I, _I, _I, _I, _I, _I, _I]),
     "alg_paged_attn": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _P, _I, _P,
-                            _P, _P, _I, _F, _I, _P, _P, _S]),
+                            _P, _P, _I, _I, _F, _I, _P, _P, _S]),
     "alg_paged_append": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _L, _P, _L, _L,
-                              _L, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _F, _P]),
+                              _L, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P, _P, _I, _F, _P]),
     "alg_timer_enable": (None, [_I]),
     "alg_timer_report": (_S, [ctypes.c_char_p, _S]),
 }

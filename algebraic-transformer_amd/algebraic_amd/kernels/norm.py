@@ -64,26 +64,29 @@ def rms_norm(x, gain=None, eps: float = 1e-5):
     return _RmsNormFn.apply(x, gain, float(eps))
 
 
+_BF16, _F32 = torch.bfloat16, torch.float32
+_WEIGHTS = {_BF16: _lib.DTYPE_BF16, _F32: _lib.DTYPE_F32}
+
+
 class _AddRmsNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, gain, eps):
         lib = _lib.load()
+        x, residual = _lib.aligned16(x), _lib.aligned16(residual)
         d = x.shape[-1]
-        x2, r2 = _lib.aligned16(x).reshape(-1, d), _lib.aligned16(residual).reshape(-1, d)
-        rows = x2.shape[0]
-        g = _f32_gain(gain, x)
-        y, s = torch.empty_like(x2), torch.empty_like(x2)
-        tau = torch.empty(rows, dtype=torch.float32, device=x.device)
+        rows = x.numel() // d
+        g, gain_dtype = _gain_vector(gain, x.device)
+        y, s = torch.empty_like(x), torch.empty_like(x)
+        tau = torch.empty(rows, dtype=_F32, device=x.device)
         p = _lib.ptr
         if rows:
-            with _lib.device_of(x2):
-                _lib.check(lib.alg_add_rms_norm_fwd(_lib.stream_of(x2), rows, d, p(x2), p(r2), p(g), eps, p(s), p(y),
-                                                    p(tau)), "add_rms_norm")
-        s = s.reshape(x.shape)
+            with _lib.device_of(x):
+                _lib.check(lib.alg_add_rms_norm_fwd(_lib.stream_of(x), rows, d, p(x), p(residual), p(g), gain_dtype, eps,
+                                                    p(s), p(y), p(tau)), "add_rms_norm")
         ctx.save_for_backward(s, g, tau)
         ctx.gain_meta = None if gain is None else (gain.shape, gain.dtype)
         ctx.set_materialize_grads(False)
-        return y.reshape(x.shape), s
+        return y, s
 
     @staticmethod
     def backward(ctx, dy, ds):
@@ -91,41 +94,55 @@ class _AddRmsNormFn(torch.autograd.Function):
         if dy is None:  # the norm was not used
             return ds, ds, None, None
         lib = _lib.load()
-        d = s.shape[-1]
-        rows = tau.shape[0]
-        dy2 = _lib.aligned16(dy.to(s.dtype))
-        ds2 = None if ds is None else _lib.aligned16(ds.to(s.dtype))
-        dx = torch.empty_like(s, memory_format=torch.contiguous_format)
-        wants_gain = g is not None and ctx.needs_input_grad[2]
-        dg = torch.zeros(d, dtype=torch.float32, device=s.device) if wants_gain else None
-        nbytes = lib.alg_rms_norm_workspace_size(rows, d) if wants_gain else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
+        d, rows = s.shape[-1], tau.shape[0]
+        dy = _lib.aligned16(dy if dy.dtype is _BF16 else dy.to(_BF16))
+        if ds is not None:
+            ds = _lib.aligned16(ds if ds.dtype is _BF16 else ds.to(_BF16))
+        dx = torch.empty_like(s)
+        dg, ws, nbytes, gain_dtype = None, None, 0, 1
+        if g is not None:
+            gain_dtype = _WEIGHTS[g.dtype]
+            if ctx.needs_input_grad[2]:
+                dg = torch.empty_like(g) if rows else torch.zeros_like(g)
+                nbytes = lib.alg_rms_norm_workspace_size(rows, d)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
         p = _lib.ptr
         if rows:
             with _lib.device_of(s):
-                _lib.check(lib.alg_add_rms_norm_bwd(_lib.stream_of(s), rows, d, p(s), p(g), p(tau), p(dy2), p(ds2),
-                                                    p(dx), p(dg), p(ws), nbytes), "add_rms_norm backward")
-        dgain = None if dg is None else dg.reshape(ctx.gain_meta[0]).to(ctx.gain_meta[1])
-        return dx, dx, dgain, None
+                _lib.check(lib.alg_add_rms_norm_bwd(_lib.stream_of(s), rows, d, p(s), p(g), gain_dtype, p(tau), p(dy),
+                                                    p(ds), p(dx), p(dg), p(ws), nbytes), "add_rms_norm backward")
+        if dg is not None:
+            shape, dtype = ctx.gain_meta
+            dg = dg.reshape(shape)
+            if dg.dtype is not dtype:
+                dg = dg.to(dtype)
+        return dx, dx, dg, None
 
 
-def _f32_gain(gain, x):
-    return None if gain is None else _lib.aligned16(gain.detach().to(device=x.device, dtype=torch.float32))
+def _gain_vector(gain, device):
+    """The gain, f32 or bf16, contiguous and aligned, and its type's code."""
+    if gain is None:
+        return None, 1
+    g = gain.detach()
+    if g.dtype not in _WEIGHTS or g.device != device:
+        g = g.to(device=device, dtype=_F32)
+    return _lib.aligned16(g.reshape(-1)), _WEIGHTS[g.dtype]
 
 
 def _check_add(x, residual, gain, eps, what):
-    if x.dtype != torch.bfloat16 or residual.dtype != torch.bfloat16:
+    if x.dtype is not _BF16 or residual.dtype is not _BF16:
         raise NotImplementedError(f"dtypes {x.dtype}, {residual.dtype}: the gfx950 norm takes bfloat16 rows")
     if x.shape != residual.shape or x.dim() == 0:
         raise ValueError(f"x {tuple(x.shape)} and residual {tuple(residual.shape)} must share a shape of rows")
     if x.device != residual.device:
         raise ValueError(f"residual must be on {x.device}")
-    if gain is not None and gain.numel() != x.shape[-1]:
-        raise ValueError(f"gain must have {x.shape[-1]} entries")
+    d = x.shape[-1]
+    if gain is not None and gain.numel() != d:
+        raise ValueError(f"gain must have {d} entries")
     if not (eps > 0) or not math.isfinite(eps):
         raise ValueError("eps must be positive and finite")
-    if x.shape[-1] == 0 or x.shape[-1] % 8 or x.shape[-1] > 4096:
-        raise NotImplementedError(f"rows of {x.shape[-1]}: the gfx950 norm takes multiples of 8 up to 4096")
+    if d == 0 or d % 8 or d > 4096:
+        raise NotImplementedError(f"rows of {d}: the gfx950 norm takes multiples of 8 up to 4096")
     if not x.is_cuda:
         raise RuntimeError(f"{what} needs GPU tensors (no CPU fallback)")
 
@@ -147,15 +164,16 @@ def add_rms_norm_fp8(x, residual, gain=None, eps: float = 1e-5):
     _check_add(x, residual, gain, eps, "add_rms_norm_fp8")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, gain)):
         raise NotImplementedError("add_rms_norm_fp8 has no gradient: call it under torch.no_grad() or on detached tensors")
-    d = x.shape[-1]
-    x2, r2 = _lib.aligned16(x), _lib.aligned16(residual)
-    g = _f32_gain(gain, x)
+    x, residual = _lib.aligned16(x), _lib.aligned16(residual)
+    g, gain_dtype = _gain_vector(gain, x.device)
     y8 = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    s = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+    s = torch.empty_like(x)
+    scale = torch.empty((*x.shape[:-1], 1), dtype=_F32, device=x.device)
+    rows = scale.numel()
     p = _lib.ptr
-    if scale.numel():
-        with _lib.device_of(x2):
-            _lib.check(_lib.load().alg_add_rms_norm_fp8(_lib.stream_of(x2), scale.numel(), d, p(x2), p(r2), p(g),
-                                                        float(eps), p(s), p(y8), p(scale)), "add_rms_norm_fp8")
+    if rows:
+        with _lib.device_of(x):
+            _lib.check(_lib.load().alg_add_rms_norm_fp8(_lib.stream_of(x), rows, x.shape[-1], p(x), p(residual), p(g),
+                                                        gain_dtype, float(eps), p(s), p(y8), p(scale)),
+                       "add_rms_norm_fp8")
     return y8, scale, s

@@ -27,43 +27,70 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .flash import _sink_input
-from .packed import _check_heads, _check_index, _check_scale, _check_sink, _rows, _strided
+from .packed import _BF16, _F32, _WEIGHTS, _check_heads, _check_index, _check_scale, _rows, _sink_vector, _strided
 
 
 def _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv):
+    """Checks a cache, its table and lengths; returns (pages, page, S, width, the pages' arguments)."""
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != Hkv or k_pages.shape[3] != q.shape[2]:
         raise ValueError(f"k_pages and v_pages must share the shape (pages, Hkv, page, {q.shape[2]})")
     pages, _, page, D = k_pages.shape
-    if D not in (64, 128):
+    dev = q.device
+    if D != 128 and D != 64:
         raise NotImplementedError(f"head_dim {D}: the gfx950 cache kernels are built for 64 and 128")
     if pages == 0 or page == 0 or page % 16:
         raise NotImplementedError(f"{pages} pages of {page} positions: pages hold a positive multiple of 16")
+    args = []
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dtype != torch.bfloat16:
+        if t.dtype is not _BF16:
             raise NotImplementedError(f"dtype {t.dtype}: the gfx950 cache kernels take bfloat16")
-        if t.device != q.device:
-            raise ValueError(f"{name} must be on {q.device}")
-        ps, hs, ts, one = t.stride()
-        if one != 1 or ps % 8 or hs % 8 or ts % 8 or min(ps, ts) < D or (hs < D and t.shape[1] > 1) or t.data_ptr() % 16:
+        if t.device != dev:
+            raise ValueError(f"{name} must be on {dev}")
+        (ps, hs, ts, one), at = t.stride(), t.data_ptr()
+        if one != 1 or (ps | hs | ts) & 7 or ps < D or ts < D or (hs < D and Hkv > 1) or at & 15:
             raise ValueError(f"{name}: the last axis must be contiguous and the others start on 16 bytes")
+        args += (at, ps, hs if hs >= D else D, ts)
     if kv_lens.dim() != 1:
         raise ValueError("kv_lens must be (S,)")
     S = kv_lens.shape[0]
-    _check_index("kv_lens", kv_lens, (S,), q)
-    _check_index("cu_seqlens", cu_seqlens, (S + 1,), q)
+    _check_index("kv_lens", kv_lens, (S,), dev)
+    _check_index("cu_seqlens", cu_seqlens, (S + 1,), dev)
     if page_table.dim() != 2 or page_table.shape[0] != S or page_table.shape[1] == 0:
         raise ValueError(f"page_table must be ({S}, width)")
-    _check_index("page_table", page_table, tuple(page_table.shape), q)
+    width = page_table.shape[1]
+    _check_index("page_table", page_table, (S, width), dev)
+    return pages, page, S, width, args
 
 
 def _no_gradient(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(f"{what} has no gradient: call it under torch.no_grad() or on detached "
+                                          "tensors")
 
 
-def _page_args(t):
-    return t.data_ptr(), t.stride(0), max(t.stride(1), t.shape[3]), t.stride(2)
+def _gains(q_gain, k_gain, device):
+    """Both gains in one of the types that the kernel reads, 16-byte aligned, and its code."""
+    gains = [None if g is None else g.detach() for g in (q_gain, k_gain)]
+    types = {g.dtype for g in gains if g is not None}
+    same = types.pop() if len(types) == 1 else _F32
+    if same not in _WEIGHTS:
+        same = _F32
+    for i, g in enumerate(gains):
+        if g is not None:
+            if g.dtype is not same or g.device != device:
+                g = g.to(device=device, dtype=same)
+            gains[i] = _lib.aligned16(g)
+    return (*gains, _WEIGHTS[same])
+
+
+def _table(t, device):
+    if t is None:
+        return None
+    if t.dtype is not _F32 or t.device != device or t.requires_grad:
+        t = t.detach().to(device=device, dtype=_F32)
+    return _lib.aligned16(t)
 
 
 def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, q_gain=None, k_gain=None, cos=None,
@@ -78,36 +105,37 @@ def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, q_g
     and those behind the last sequence, are zero. Two tokens in one place: either is kept.
     """
     _check_heads(q, k, v)
-    _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, k.shape[1])
+    (N, H, D), Hkv, dev = q.shape, k.shape[1], q.device
+    pages, page, S, width, where = _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv)
     if not (eps > 0) or not math.isfinite(eps):
         raise ValueError("eps must be positive and finite")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin are given together")
-    N, H, D = q.shape
-    reach = page_table.shape[1] * k_pages.shape[2]
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t is not None and (t.dim() != 2 or t.shape[0] < reach or t.shape[1] != D // 2):
-            raise ValueError(f"{name} must be (>= {reach}, {D // 2})")
+    reach, rows = width * page, 0
+    if cos is not None:
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dim() != 2 or t.shape[0] < reach or t.shape[1] != D // 2:
+                raise ValueError(f"{name} must be (>= {reach}, {D // 2})")
+        rows = min(cos.shape[0], sin.shape[0])
     for name, g in (("q_gain", q_gain), ("k_gain", k_gain)):
         if g is not None and g.numel() != D:
             raise ValueError(f"{name} must have {D} entries")
     _no_gradient("paged_append", q, k, v, k_pages, v_pages, q_gain, k_gain)
     if not q.is_cuda:
         raise RuntimeError("paged_append needs GPU tensors (no CPU fallback)")
-    out = torch.empty((N, H, D), dtype=q.dtype, device=q.device)
+    out = torch.empty((N, H, D), dtype=_BF16, device=dev)
     if N == 0:
         return out
     q, k, v = _rows(q), _rows(k), _rows(v)
     page_table, cu, kv = page_table.contiguous(), cu_seqlens.contiguous(), kv_lens.contiguous()
-    f32 = lambda t: None if t is None else _lib.aligned16(t.detach().to(device=q.device, dtype=torch.float32))  # noqa: E731
-    gq, gk, cs, sn = f32(q_gain), f32(k_gain), f32(cos), f32(sin)
-    rows = 0 if cs is None else min(cs.shape[0], sn.shape[0])
+    gq, gk, gain_dtype = _gains(q_gain, k_gain, dev)
+    cs, sn = _table(cos, dev), _table(sin, dev)
     p = _lib.ptr
     with _lib.device_of(q):
         _lib.check(_lib.load().alg_paged_append(
-            _lib.stream_of(q), N, kv.shape[0], H, k.shape[1], D, *_strided(q), *_strided(k), *_strided(v),
-            *_page_args(k_pages), *_page_args(v_pages), k_pages.shape[0], k_pages.shape[2], p(page_table),
-            page_table.shape[1], p(cu), p(kv), p(gq), p(gk), p(cs), p(sn), rows, eps, p(out)), "paged_append")
+            _lib.stream_of(q), N, S, H, Hkv, D, *_strided(q), *_strided(k), *_strided(v), *where, pages, page,
+            p(page_table), width, p(cu), p(kv), p(gq), p(gk), gain_dtype, p(cs), p(sn), rows, eps, p(out)),
+            "paged_append")
     return out
 
 
@@ -125,32 +153,28 @@ def paged_flash_attention(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, 
         raise ValueError("k_pages and v_pages must be (pages, Hkv, page, D)")
     if q.dim() != 3:
         raise ValueError("q must be (tokens, heads, D)")
-    if q.dtype != torch.bfloat16:
+    if q.dtype is not _BF16:
         raise NotImplementedError(f"dtype {q.dtype}: the gfx950 cache kernels take bfloat16")
-    N, H, D = q.shape
-    Hkv = k_pages.shape[1]
+    (N, H, D), Hkv, dev = q.shape, k_pages.shape[1], q.device
     if H == 0 or Hkv == 0 or H % Hkv:
         raise ValueError(f"{H} query heads do not share {Hkv} key heads evenly")
-    _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv)
+    pages, page, S, width, where = _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv)
     _check_scale(n, c)
-    _check_sink(sink_logit, q)
+    sink, sink_dtype, count = _sink_vector(sink_logit, H, dev)
     _no_gradient("paged_flash_attention", q, k_pages, v_pages, sink_logit)
     if not q.is_cuda:
         raise RuntimeError("paged_flash_attention needs GPU tensors (no CPU fallback)")
-    o = torch.empty((N, H, D), dtype=q.dtype, device=q.device)
+    o = torch.empty((N, H, D), dtype=_BF16, device=dev)
     if N == 0:
         return o
     lib = _lib.load()
     q = _rows(q)
     page_table, cu, kv = page_table.contiguous(), cu_seqlens.contiguous(), kv_lens.contiguous()
-    S, width, page = kv.shape[0], page_table.shape[1], k_pages.shape[2]
-    sink = _sink_input(sink_logit, H, q.device)
     nbytes = lib.alg_paged_attn_workspace_size(N, S, H, Hkv, D, width, page)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     p = _lib.ptr
     with _lib.device_of(q):
         _lib.check(lib.alg_paged_attn(
-            _lib.stream_of(q), N, S, H, Hkv, D, *_strided(q), *_page_args(k_pages), *_page_args(v_pages),
-            k_pages.shape[0], page, p(page_table), width, p(cu), p(kv), p(sink), 0 if sink is None else sink.numel(),
-            float(c), int(n), p(o), p(ws), nbytes), "paged_flash_attention")
+            _lib.stream_of(q), N, S, H, Hkv, D, *_strided(q), *where, pages, page, p(page_table), width, p(cu), p(kv),
+            p(sink), sink_dtype, count, float(c), int(n), p(o), p(ws), nbytes), "paged_flash_attention")
     return o

@@ -1128,44 +1128,48 @@ int alg_head_bwd_streamed(alg_stream_t stream, int dtype, int N, int d, int V, c
 
 // ---- residual norm ----------------------------------------------------------------------------
 
-static alg::RmsNormParams add_norm_params(int rows, int d, const void* x, const void* res, const float* gain, float eps,
-                                          void* sum) {
+static alg::RmsNormParams add_norm_params(int rows, int d, const void* x, const void* res, const void* gain,
+                                          int gain_dtype, float eps, void* sum) {
   alg::RmsNormParams p;
   std::memset(&p, 0, sizeof p);
-  p.x = static_cast<const bf16*>(x); p.res = static_cast<const bf16*>(res); p.gain = gain;
+  p.x = static_cast<const bf16*>(x); p.res = static_cast<const bf16*>(res);
+  p.gain = static_cast<const float*>(gain); p.gain_bf16 = gain_dtype == ALG_DTYPE_BF16;
   p.sum = static_cast<bf16*>(sum);
   p.rows = rows; p.d = d; p.eps = eps;
   return p;
 }
 
-int alg_add_rms_norm_fwd(alg_stream_t stream, int rows, int d, const void* x, const void* res, const float* gain,
-                         float eps, void* sum, void* y, float* tau) {
+int alg_add_rms_norm_fwd(alg_stream_t stream, int rows, int d, const void* x, const void* res, const void* gain,
+                         int gain_dtype, float eps, void* sum, void* y, float* tau) {
   const int rc = check_rms_norm(rows, d, eps);
   if (rc) return rc;
   if (!x || !res || !sum || !y || !tau) return fail(ALG_ERR_INVALID, "x, res, sum, y and tau are required");
+  if (gain && !is_weight_dtype(gain_dtype)) return fail(ALG_ERR_INVALID, "gain must be bf16 or f32");
   if (!aligned16({x, res, gain, sum, y})) return fail(ALG_ERR_INVALID, "matrices and gain must be 16-byte aligned");
-  alg::RmsNormParams p = add_norm_params(rows, d, x, res, gain, eps, sum);
+  alg::RmsNormParams p = add_norm_params(rows, d, x, res, gain, gain_dtype, eps, sum);
   p.y = static_cast<bf16*>(y); p.tau = tau;
   return hip_status(alg::launch_add_rms_norm(p, (hipStream_t)stream), "alg_add_rms_norm_fwd");
 }
 
-int alg_add_rms_norm_fp8(alg_stream_t stream, int rows, int d, const void* x, const void* res, const float* gain,
-                         float eps, void* sum, void* y8, float* scale) {
+int alg_add_rms_norm_fp8(alg_stream_t stream, int rows, int d, const void* x, const void* res, const void* gain,
+                         int gain_dtype, float eps, void* sum, void* y8, float* scale) {
   const int rc = check_rms_norm(rows, d, eps);
   if (rc) return rc;
   if (!x || !res || !sum || !y8 || !scale) return fail(ALG_ERR_INVALID, "x, res, sum, y8 and scale are required");
+  if (gain && !is_weight_dtype(gain_dtype)) return fail(ALG_ERR_INVALID, "gain must be bf16 or f32");
   if (!aligned16({x, res, gain, sum, y8})) return fail(ALG_ERR_INVALID, "matrices and gain must be 16-byte aligned");
-  alg::RmsNormParams p = add_norm_params(rows, d, x, res, gain, eps, sum);
+  alg::RmsNormParams p = add_norm_params(rows, d, x, res, gain, gain_dtype, eps, sum);
   p.y8 = static_cast<unsigned char*>(y8); p.scale = scale;
   return hip_status(alg::launch_add_rms_norm(p, (hipStream_t)stream), "alg_add_rms_norm_fp8");
 }
 
-int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, const float* gain, const float* tau,
-                         const void* dy, const void* dsum, void* dx, float* dgain, void* workspace,
+int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, const void* gain, int gain_dtype,
+                         const float* tau, const void* dy, const void* dsum, void* dx, void* dgain, void* workspace,
                          size_t workspace_bytes) {
   const int rc = check_rms_norm(rows, d, 1.0f);
   if (rc) return rc;
   if (!sum || !tau || !dy || !dx) return fail(ALG_ERR_INVALID, "sum, tau, dy and dx are required");
+  if (gain && !is_weight_dtype(gain_dtype)) return fail(ALG_ERR_INVALID, "gain must be bf16 or f32");
   if (!aligned16({sum, gain, dy, dsum, dx})) return fail(ALG_ERR_INVALID, "matrices and gain must be 16-byte aligned");
   if (dgain && !gain) return fail(ALG_ERR_INVALID, "a gain gradient needs the gain it differentiates");
   const size_t need = alg_rms_norm_workspace_size(rows, d);
@@ -1173,7 +1177,8 @@ int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, 
     return fail(ALG_ERR_INVALID, "workspace too small: need %zu bytes", need);
   alg::RmsNormParams p;
   std::memset(&p, 0, sizeof p);
-  p.x = static_cast<const bf16*>(sum); p.gain = gain; p.tau = const_cast<float*>(tau);
+  p.x = static_cast<const bf16*>(sum);
+  p.gain = static_cast<const float*>(gain); p.gain_bf16 = gain_dtype == ALG_DTYPE_BF16; p.tau = const_cast<float*>(tau);
   p.dy = static_cast<const bf16*>(dy); p.dsum = static_cast<const bf16*>(dsum); p.dx = static_cast<bf16*>(dx);
   p.gpart = dgain ? static_cast<float*>(workspace) : nullptr;
   p.rows = rows; p.d = d;
@@ -1198,8 +1203,8 @@ static alg::AttnScale attn_scale(int n, float c, int D) {
   return s;
 }
 
-static int check_packed(int N, int S, int H, int Hkv, int D, float c, int n, const int* cu, const float* sink,
-                        int sink_count) {
+static int check_packed(int N, int S, int H, int Hkv, int D, float c, int n, const int* cu, const void* sink,
+                        int sink_dtype, int sink_count) {
   if (N < 0 || S < 0) return fail(ALG_ERR_INVALID, "N and S must not be negative (got %d, %d)", N, S);
   if (H <= 0 || Hkv <= 0 || H % Hkv) return fail(ALG_ERR_INVALID, "H = %d must be a positive multiple of Hkv = %d", H, Hkv);
   if (D != 64 && D != 128) return fail(ALG_ERR_UNSUPPORTED, "head_dim %d: gfx950 kernels are built for D in {64, 128}", D);
@@ -1214,6 +1219,7 @@ static int check_packed(int N, int S, int H, int Hkv, int D, float c, int n, con
   if (c < 0x1p-30f || c > 0x1p30f) return fail(ALG_ERR_UNSUPPORTED, "asinh scale c = %g: built for 2^-30 to 2^30", (double)c);
   if (!cu) return fail(ALG_ERR_INVALID, "cu_seqlens is required");
   if (sink && sink_count != 1 && sink_count != H) return fail(ALG_ERR_INVALID, "sink_count must be 1 or H");
+  if (sink && !is_weight_dtype(sink_dtype)) return fail(ALG_ERR_INVALID, "sink must be bf16 or f32");
   return ALG_OK;
 }
 
@@ -1230,8 +1236,8 @@ static int check_strides(const char* name, const void* base, long ts, long hs, i
 
 int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                         const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
-                        const float* sink, int sink_count, float c, int n, void* o, float* stat) {
-  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_count);
+                        const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, float* stat) {
+  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_dtype, sink_count);
   if (rc) return rc;
   if (N == 0) return ALG_OK;
   if (!q || !k || !v || !o || !stat) return fail(ALG_ERR_INVALID, "null argument");
@@ -1244,7 +1250,7 @@ int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D
   std::memset(&p, 0, sizeof p);
   p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
   p.o = static_cast<bf16*>(o); p.stat = stat;
-  p.sink = sink; p.sink_count = sink_count; p.c = c; p.cu = cu;
+  p.sink = sink; p.sink_count = sink_count; p.sink_bf16 = sink_dtype == ALG_DTYPE_BF16; p.c = c; p.cu = cu;
   p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
   p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
   p.sc = attn_scale(n, c, D);
@@ -1270,12 +1276,13 @@ size_t alg_packed_attn_bwd_workspace_size(int N, int S, int H, int Hkv) {
 
 int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                         const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
-                        const float* sink, int sink_count, float c, int n, const void* o, const float* stat,
-                        const void* dO, long do_ts, long do_hs, void* dq, void* dk, void* dv, float* dsink,
-                        void* workspace, size_t workspace_bytes) {
-  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_count);
+                        const void* sink, int sink_dtype, int sink_count, float c, int n, const void* o, const float* stat,
+                        const void* dO, long do_ts, long do_hs, void* dq, void* dk, void* dv, void* dsink,
+                        int dsink_dtype, void* workspace, size_t workspace_bytes) {
+  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_dtype, sink_count);
   if (rc) return rc;
   if (dsink && !sink) return fail(ALG_ERR_INVALID, "a sink gradient needs the sink it differentiates");
+  if (dsink && !is_weight_dtype(dsink_dtype)) return fail(ALG_ERR_INVALID, "the sink gradient must be bf16 or f32");
   if (N == 0) return dsink ? fail(ALG_ERR_INVALID, "a sink gradient needs tokens") : ALG_OK;
   if (!q || !k || !v || !o || !stat || !dO || !dq || !dk || !dv) return fail(ALG_ERR_INVALID, "null argument");
   rc = check_strides("q", q, q_ts, q_hs, H, D);
@@ -1293,18 +1300,21 @@ int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D
   p.o = static_cast<const bf16*>(o); p.dO = static_cast<const bf16*>(dO); p.stat = stat;
   p.di = static_cast<float*>(workspace);
   p.care = reinterpret_cast<int*>(static_cast<char*>(workspace) + ws.care);
-  p.sink = sink; p.sink_count = sink_count; p.c = c; p.cu = cu;
+  p.sink = sink; p.sink_count = sink_count; p.sink_bf16 = sink_dtype == ALG_DTYPE_BF16; p.c = c; p.cu = cu;
   p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
   p.do_ts = do_ts; p.do_hs = do_hs;
-  p.dq = static_cast<bf16*>(dq); p.dk = static_cast<bf16*>(dk); p.dv = static_cast<bf16*>(dv); p.dsink = dsink;
+  p.dq = static_cast<bf16*>(dq); p.dk = static_cast<bf16*>(dk); p.dv = static_cast<bf16*>(dv);
+  p.dsink = dsink; p.dsink_bf16 = dsink_dtype == ALG_DTYPE_BF16;
   p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
   p.sc = attn_scale(n, c, D);
   return hip_status(alg::launch_packed_bwd(p, D, (hipStream_t)stream), "alg_packed_attn_bwd");
 }
 
+// Pages: only the places of a page (16 at a time) are reached by 32-bit offsets.
 static int check_pages(const char* name, const void* base, long ps, long hs, long ts, int Hkv, int page, int D) {
-  int rc = check_strides(name, base, ts, hs, Hkv, D);
-  if (!rc && (ps % 8 || ps < D)) rc = fail(ALG_ERR_INVALID, "%s: page stride %ld must be a multiple of 8 and at least %d", name, ps, D);
+  int rc = check_strides(name, base, ts, D, 1, D);
+  if (!rc && (hs % 8 || (Hkv > 1 && hs < D) || ps % 8 || ps < D))
+    rc = fail(ALG_ERR_INVALID, "%s: page and head strides (%ld, %ld) must be multiples of 8 and at least %d", name, ps, hs, D);
   if (!rc && (page <= 0 || page % 16)) rc = fail(ALG_ERR_UNSUPPORTED, "pages of %d positions: a positive multiple of 16", page);
   return rc;
 }
@@ -1316,9 +1326,12 @@ static int check_table(int width, int page, int pages) {
 
 // How a paged call runs: which kernel, on rows per workgroup, and over how many ranges of keys.
 // Rows: a sequence's average, since the lengths are on the device. Up to 16 or 32 of them take the
-// kernel whose waves split the keys; more, the one whose waves split 128 rows. Ranges: as many as
-// bring the launch to two workgroups a CU, while a range keeps DECODE_RANGE keys (or 1024 of the
-// larger kernel, whose partial sums are 128 rows) of a sequence as long as the table allows.
+// kernel whose waves split the keys; more, the one whose waves split 128 rows.
+// Ranges, the former: at most one workgroup a CU, none under DECODE_RANGE keys of a sequence as long
+// as the table allows. One token over 131001 keys, 4 heads of 128: 64 workgroups 82 us, 128 to 256
+// 47 to 49, 320 60, 512 50; over 8000 keys, 8 heads: 64 20 us, 256 (250 keys each) 14, 512 17.
+// The latter, whose partial sums are 128 rows: two workgroups a CU, ranges of 1024 keys (2100 tokens
+// of 3 requests over 24000 keys, 16 heads over 4: 226 us whole, 2 ranges 200, 4 ranges 210).
 struct PagedPlan {
   int row_tiles;  // 1, 2: 16 or 32 rows (paged_decode); 0: 128 (packed_fwd)
   int nsplit;
@@ -1331,7 +1344,7 @@ static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int 
   const long tile = pl.row_tiles ? 16 * pl.row_tiles : alg::PK_ROWS;
   const long groups = std::max(1L, std::max((rows + tile - 1) / tile, (long)std::min(S, N)) * Hkv);
   const long cap = (long)width * page, least = pl.row_tiles ? alg::DECODE_RANGE : 1024;
-  const long most = std::min((512 + groups - 1) / groups, (long)alg::MAX_RANGES);
+  const long most = pl.row_tiles ? std::min(256 / groups, (long)alg::MAX_RANGES) : (512 + groups - 1) / groups;
   pl.nsplit = (int)std::max(1L, std::min(most, cap / least));
   const size_t parts = pl.nsplit > 1 ? (size_t)pl.nsplit * N * H : 0;
   pl.zt = align256(parts * D * sizeof(float));
@@ -1347,8 +1360,9 @@ size_t alg_paged_attn_workspace_size(int N, int S, int H, int Hkv, int D, int wi
 int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                    const void* k_pages, long k_ps, long k_hs, long k_ts, const void* v_pages, long v_ps, long v_hs,
                    long v_ts, int pages, int page, const int* table, int width, const int* cu, const int* kv_lens,
-                   const float* sink, int sink_count, float c, int n, void* o, void* workspace, size_t workspace_bytes) {
-  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_count);
+                   const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, void* workspace,
+                   size_t workspace_bytes) {
+  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_dtype, sink_count);
   if (!rc) rc = check_table(width, page, pages);
   if (rc) return rc;
   if (N == 0) return ALG_OK;
@@ -1366,7 +1380,7 @@ int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, con
   std::memset(&p, 0, sizeof p);
   p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k_pages); p.v = static_cast<const bf16*>(v_pages);
   p.o = static_cast<bf16*>(o);
-  p.sink = sink; p.sink_count = sink_count; p.c = c; p.cu = cu; p.kv_lens = kv_lens;
+  p.sink = sink; p.sink_count = sink_count; p.sink_bf16 = sink_dtype == ALG_DTYPE_BF16; p.c = c; p.cu = cu; p.kv_lens = kv_lens;
   p.table = table; p.width = width; p.page = page; p.pages = pages;
   p.q_ts = q_ts; p.q_hs = q_hs;
   p.k_ts = k_ts; p.k_hs = k_hs; p.k_ps = k_ps; p.v_ts = v_ts; p.v_hs = v_hs; p.v_ps = v_ps;
@@ -1383,12 +1397,13 @@ int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, con
 int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                      const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
                      long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, int pages, int page,
-                     const int* table, int width, const int* cu, const int* kv_lens, const float* q_gain,
-                     const float* k_gain, const float* cos, const float* sin, int table_rows, float eps, void* q_out) {
-  int rc = check_packed(N, S, H, Hkv, D, 1.0f, 2, cu, nullptr, 0);
+                     const int* table, int width, const int* cu, const int* kv_lens, const void* q_gain,
+                     const void* k_gain, int gain_dtype, const float* cos, const float* sin, int table_rows, float eps, void* q_out) {
+  int rc = check_packed(N, S, H, Hkv, D, 1.0f, 2, cu, nullptr, 0, 0);
   if (!rc) rc = check_table(width, page, pages);
   if (rc) return rc;
   if (!(eps > 0.0f) || !std::isfinite(eps)) return fail(ALG_ERR_INVALID, "eps must be positive and finite");
+  if ((q_gain || k_gain) && !is_weight_dtype(gain_dtype)) return fail(ALG_ERR_INVALID, "gains must be bf16 or f32");
   if (!cos != !sin) return fail(ALG_ERR_INVALID, "cos and sin are given together");
   if (cos && (long)table_rows < (long)width * page)
     return fail(ALG_ERR_INVALID, "rotation tables of %d rows for %ld positions", table_rows, (long)width * page);
@@ -1410,7 +1425,7 @@ int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, c
   p.kp_ps = k_ps; p.kp_hs = kp_hs; p.kp_ts = kp_ts; p.vp_ps = v_ps; p.vp_hs = vp_hs; p.vp_ts = vp_ts;
   p.qo = static_cast<bf16*>(q_out);
   p.cu = cu; p.kv_lens = kv_lens; p.table = table; p.width = width; p.page = page; p.pages = pages;
-  p.q_gain = q_gain; p.k_gain = k_gain; p.cos = cos; p.sin = sin; p.eps = eps;
+  p.q_gain = q_gain; p.k_gain = k_gain; p.gain_bf16 = gain_dtype == ALG_DTYPE_BF16; p.cos = cos; p.sin = sin; p.eps = eps;
   p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.D = D;
   return hip_status(alg::launch_paged_append(p, (hipStream_t)stream), "alg_paged_append");
 }

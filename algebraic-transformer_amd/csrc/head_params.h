@@ -135,6 +135,7 @@ struct RmsNormParams {
   float* gpart;         // VJP: (nblocks, d) gain-gradient partials and their group sums, or nullptr
   int rows, d;
   float eps;
+  int gain_bf16 = 0;  // the gain, and its gradient, are bf16
   // With the residual's addition (x: the block's output).
   const bf16* res = nullptr;  // the residual stream (rows, d)
   bf16* sum = nullptr;        // round(x + res)

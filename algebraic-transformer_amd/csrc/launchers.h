@@ -100,7 +100,7 @@ FfnGemmPlan ffn_gemm_plan(int M, int N, int K);
 int ffn_gate_up_tile(int N, int F, int d);
 int ffn_dy_tile(int N, int F, int dm);
 hipError_t launch_ffn_gemm(const FfnGemmParams& g, int a_mode, int b_mode, hipStream_t st);
-hipError_t launch_rms_norm_bwd(const RmsNormParams& p, float* dgain, hipStream_t st);
+hipError_t launch_rms_norm_bwd(const RmsNormParams& p, void* dgain, hipStream_t st);
 hipError_t launch_add_rms_norm(const RmsNormParams& p, hipStream_t st);
 hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t st);
 hipError_t launch_packed_bwd(const PackedBwdParams& p, int D, hipStream_t st);

@@ -328,7 +328,7 @@ __device__ __forceinline__ void packed_sink_grad(const PackedBwdParams& p, int k
   __shared__ float red[4];
   const int head = kvh * p.G + g;
   float r;
-  const float t = weight_t_careful(sink_score(p.sink, p.sink_count, head, p.c, p.sc.a), p.sc.b, r);
+  const float t = weight_t_careful(sink_score(p, head), p.sc.b, r);
   const size_t base = (size_t)kvh * p.N * p.G + g;
   float sum = 0.0f;
 #pragma unroll 8
@@ -340,8 +340,11 @@ __device__ __forceinline__ void packed_sink_grad(const PackedBwdParams& p, int k
   for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x == 0)
-    p.dsink[head] = -(red[0] + red[1] + red[2] + red[3]) * (float)(1 << p.sc.log2n) * (r / p.sc.a) / p.c;
+  if (threadIdx.x == 0) {
+    const float d = -(red[0] + red[1] + red[2] + red[3]) * (float)(1 << p.sc.log2n) * (r / p.sc.a) / p.c;
+    if (p.dsink_bf16) static_cast<bf16*>(p.dsink)[head] = f2bf(d);
+    else static_cast<float*>(p.dsink)[head] = d;
+  }
 }
 
 template <int D>

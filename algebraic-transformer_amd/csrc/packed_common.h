@@ -51,8 +51,8 @@ struct PackedParams {
   const bf16* v;
   bf16* o;         // (N, H, D), contiguous
   float* stat;     // (Hkv, N G) row statistics, or nullptr
-  const float* sink;  // logits, `sink_count` (1 or H) of them, or nullptr
-  int sink_count;
+  const void* sink;  // logits, `sink_count` (1 or H) of them, f32 or bf16, or nullptr
+  int sink_count, sink_bf16;
   float c;
   const int* cu;   // (S + 1)
   const int* kv_lens;  // paged: (S) keys held, the new tokens among them
@@ -79,7 +79,8 @@ struct PagedAppendParams {
   bf16* qo;               // (N, H, D) contiguous
   const int *cu, *kv_lens, *table;
   int width, page, pages;
-  const float *q_gain, *k_gain;  // (D) or nullptr
+  const void *q_gain, *k_gain;   // (D), f32 or bf16, or nullptr
+  int gain_bf16;
   const float *cos, *sin;        // (>= width page, D / 2) or nullptr
   float eps;
   int N, S, H, Hkv, D;
@@ -90,13 +91,14 @@ struct PackedBwdParams {
   const float* stat;  // (Hkv, N G)
   float* di;          // (Hkv, N G), written by the dQ kernel
   int* care;          // (slots, Hkv): whether the slot's rows took the careful form, likewise
-  const float* sink;
-  int sink_count;
+  const void* sink;
+  int sink_count, sink_bf16;
   float c;
   const int* cu;
   long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, do_ts, do_hs;
   bf16 *dq, *dk, *dv;  // contiguous
-  float* dsink;        // (H) gradients per head, or nullptr
+  void* dsink;         // (H) gradients per head, f32 or bf16, or nullptr
+  int dsink_bf16;
   int N, S, H, Hkv, G;
   AttnScale sc;
 };
@@ -106,8 +108,11 @@ struct PackedBwdParams {
 __device__ __forceinline__ void keep_here(float& a) { asm volatile("" : "+v"(a)); }
 __device__ __forceinline__ void keep_here(float& a, float& b) { asm volatile("" : "+v"(a), "+v"(b)); }
 
-__device__ __forceinline__ float sink_score(const float* sink, int count, int head, float c, float a) {
-  return sink[count == 1 ? 0 : head] / (c * a);
+template <typename P>
+__device__ __forceinline__ float sink_score(const P& p, int head) {
+  const int i = p.sink_count == 1 ? 0 : head;
+  const float logit = p.sink_bf16 ? (float)static_cast<const bf16*>(p.sink)[i] : static_cast<const float*>(p.sink)[i];
+  return logit / (p.c * p.sc.a);
 }
 
 // t and r = 1/sqrt(s^2 + b) of the plain form.

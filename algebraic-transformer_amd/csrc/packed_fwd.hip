@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   };
 
   const bool has_sink = p.sink != nullptr && p.nsplit == 1;  // split: the sink joins in the combination
-  const float ss = has_sink ? sink_score(p.sink, p.sink_count, head, p.c, p.sc.a) : 0.0f;
+  const float ss = has_sink ? sink_score(p, head) : 0.0f;
   const float bound = p.sc.bound;
   bool careful = bound < 0.0f;
   if (!careful) {
@@ -436,7 +436,7 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(PackedParams p) {
   float T = 0.0f, ts = 0.0f;
   if (p.sink) {
     float r;
-    T = ts = weight_t_careful(sink_score(p.sink, p.sink_count, head, p.c, p.sc.a), p.sc.b, r);
+    T = ts = weight_t_careful(sink_score(p, head), p.sc.b, r);
   }
   float Z;
   fvec acc = 0.0f;

@@ -98,13 +98,16 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) 
     for (int m = 1; m < LPR; m <<= 1) ss += __shfl_xor(ss, m, 64);
     if (!isv) {
       const float tau = 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
-      const float* gain = isq ? p.q_gain : p.k_gain;
+      const void* gain = isq ? p.q_gain : p.k_gain;
       float ga[8], gb[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) ga[e] = gb[e] = 1.0f;
-      if (gain) {
-        loadf8(gain + c0, ga);
-        loadf8(gain + HALF + c0, gb);
+      if (gain && p.gain_bf16) {
+        load8(static_cast<const bf16*>(gain) + c0, ga);
+        load8(static_cast<const bf16*>(gain) + HALF + c0, gb);
+      } else if (gain) {
+        loadf8(static_cast<const float*>(gain) + c0, ga);
+        loadf8(static_cast<const float*>(gain) + HALF + c0, gb);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

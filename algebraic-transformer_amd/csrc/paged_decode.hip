@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
   float Tm = 0.0f, ts = 0.0f;
   if (sink) {
     float rr;
-    Tm = ts = weight_t_careful(sink_score(p.sink, p.sink_count, head, p.c, p.sc.a), b2, rr);
+    Tm = ts = weight_t_careful(sink_score(p, head), b2, rr);
   }
 #pragma unroll
   for (int w = 0; w < WAVES; ++w)

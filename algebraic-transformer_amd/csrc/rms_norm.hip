@@ -50,9 +50,17 @@ __device__ __forceinline__ void load_row(const bf16* r, int lane, int nch, uint4
   }
 }
 
-// Gain of this lane's chunks (1 without a gain; zeros past the row's end, where x is zero).
+// Gain of this lane's chunks (1 without a gain; zeros past the row's end, where x is zero), f32 or,
+// with `gain_bf16`, bf16.
 template <int NC>
-__device__ __forceinline__ void load_gain(const float* gain, int lane, int nch, float (&g)[NC][8]) {
+__device__ __forceinline__ void load_gain(const float* gain, int lane, int nch, float (&g)[NC][8], bool gain_bf16 = false) {
+  if (gain && gain_bf16) {
+    uint4 raw[NC];
+    load_row<NC>(reinterpret_cast<const bf16*>(gain), lane, nch, raw);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) cvt8(raw[c], g[c]);
+    return;
+  }
   if (!gain) {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -124,7 +132,7 @@ __global__ __launch_bounds__(256) void add_rms_norm_kernel(RmsNormParams p) {
   load_row<NC>(p.x + at, lane, nch, xr);
   load_row<NC>(p.res + at, lane, nch, rr);
   float g[NC][8];
-  load_gain<NC>(p.gain, lane, nch, g);
+  load_gain<NC>(p.gain, lane, nch, g, p.gain_bf16);
   float s[NC][8];
   float ss = 0.0f;
 #pragma unroll
@@ -206,7 +214,7 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(RmsNormParams p) {
   const int nch = p.d / 8;
   {
     float g[NC][8];  // chunk lane + 64 c of the gain, as the rows are laid out
-    load_gain<NC>(p.gain, lane, nch, g);
+    load_gain<NC>(p.gain, lane, nch, g, p.gain_bf16);
     if (wave == 0) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -316,10 +324,13 @@ __global__ __launch_bounds__(256) void rms_norm_gain_part_kernel(const float* gp
   tmp[(size_t)blockIdx.y * d + i] = rn_sum_rows(gpart, b0, min(nblocks, b0 + RN_GROUP), d, i);
 }
 
-__global__ __launch_bounds__(256) void rms_norm_gain_reduce_kernel(const float* tmp, int ngroups, int d, float* dgain) {
+__global__ __launch_bounds__(256) void rms_norm_gain_reduce_kernel(const float* tmp, int ngroups, int d, void* dgain,
+                                                                   int as_bf16) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= d) return;
-  dgain[i] = rn_sum_rows(tmp, 0, ngroups, d, i);
+  const float s = rn_sum_rows(tmp, 0, ngroups, d, i);
+  if (as_bf16) static_cast<bf16*>(dgain)[i] = f2bf(s);
+  else static_cast<float*>(dgain)[i] = s;
 }
 
 int rms_norm_max_d() { return RN_MAXC * 512; }
@@ -360,7 +371,7 @@ hipError_t launch_add_rms_norm(const RmsNormParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-hipError_t launch_rms_norm_bwd(const RmsNormParams& p, float* dgain, hipStream_t st) {
+hipError_t launch_rms_norm_bwd(const RmsNormParams& p, void* dgain, hipStream_t st) {
   const int nb = rms_norm_blocks(p.rows);
   {
     KTimer t("rms_norm_bwd", st);
@@ -373,7 +384,8 @@ hipError_t launch_rms_norm_bwd(const RmsNormParams& p, float* dgain, hipStream_t
   float* tmp = p.gpart + ((size_t)nb * p.d + 63) / 64 * 64;
   KTimer t("rms_norm_gain_reduce", st);
   hipLaunchKernelGGL(rms_norm_gain_part_kernel, dim3((p.d + 255) / 256, ng), dim3(256), 0, st, p.gpart, nb, p.d, tmp);
-  hipLaunchKernelGGL(rms_norm_gain_reduce_kernel, dim3((p.d + 255) / 256), dim3(256), 0, st, tmp, ng, p.d, dgain);
+  hipLaunchKernelGGL(rms_norm_gain_reduce_kernel, dim3((p.d + 255) / 256), dim3(256), 0, st, tmp, ng, p.d, dgain,
+                     p.gain_bf16);
   return hipGetLastError();
 }
 

@@ -340,12 +340,12 @@ int alg_head_bwd_streamed(alg_stream_t stream, int dtype, int N, int d, int V,
  * be NULL; dgain and workspace as in alg_rms_norm_bwd. Same sizes and alignment as alg_rms_norm;
  * gain 16-byte aligned. No counterpart in the reference, whose compiler fuses the addition
  * (src/algebraic/model.py:182-193). */
-int alg_add_rms_norm_fwd(alg_stream_t stream, int rows, int d, const void* x, const void* res, const float* gain,
-                         float eps, void* sum, void* y, float* tau);
-int alg_add_rms_norm_fp8(alg_stream_t stream, int rows, int d, const void* x, const void* res, const float* gain,
-                         float eps, void* sum, void* y8, float* scale);
-int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, const float* gain, const float* tau,
-                         const void* dy, const void* dsum, void* dx, float* dgain, void* workspace,
+int alg_add_rms_norm_fwd(alg_stream_t stream, int rows, int d, const void* x, const void* res, const void* gain,
+                         int gain_dtype, float eps, void* sum, void* y, float* tau);
+int alg_add_rms_norm_fp8(alg_stream_t stream, int rows, int d, const void* x, const void* res, const void* gain,
+                         int gain_dtype, float eps, void* sum, void* y8, float* scale);
+int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, const void* gain, int gain_dtype,
+                         const float* tau, const void* dy, const void* dsum, void* dx, void* dgain, void* workspace,
                          size_t workspace_bytes);
 
 /* Causal algebraic attention (the function of alg_attn_fwd_guarded) over packed sequences with
@@ -359,13 +359,13 @@ int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, 
  * |q.k| / (sqrt(D) c) up to 2^60 is exact to f32 rounding, without a guard ahead. */
 int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                         const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
-                        const float* sink, int sink_count, float c, int n, void* o, float* stat);
+                        const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, float* stat);
 size_t alg_packed_attn_bwd_workspace_size(int N, int S, int H, int Hkv);
 int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                         const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
-                        const float* sink, int sink_count, float c, int n, const void* o, const float* stat,
-                        const void* dO, long do_ts, long do_hs, void* dq, void* dk, void* dv, float* dsink,
-                        void* workspace, size_t workspace_bytes);
+                        const void* sink, int sink_dtype, int sink_count, float c, int n, const void* o, const float* stat,
+                        const void* dO, long do_ts, long do_hs, void* dq, void* dk, void* dv, void* dsink,
+                        int dsink_dtype, void* workspace, size_t workspace_bytes);
 
 /* The same attention of new tokens over a paged cache, forward only: sequence s holds kv_lens[s]
  * keys, of which its cu[s+1] - cu[s] tokens here are the last, token t at position
@@ -380,7 +380,8 @@ size_t alg_paged_attn_workspace_size(int N, int S, int H, int Hkv, int D, int wi
 int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                    const void* k_pages, long k_ps, long k_hs, long k_ts, const void* v_pages, long v_ps, long v_hs,
                    long v_ts, int pages, int page, const int* table, int width, const int* cu, const int* kv_lens,
-                   const float* sink, int sink_count, float c, int n, void* o, void* workspace, size_t workspace_bytes);
+                   const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, void* workspace,
+                   size_t workspace_bytes);
 
 /* What precedes it: the new tokens' QK RMS norm with gain and Cayley rotation at their positions
  * (model.py:170-174), y = rot((x tau) gain) in f32 rounded once; queries to q_out (N, H, D)
@@ -390,8 +391,8 @@ int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, con
 int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                      const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
                      long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, int pages, int page,
-                     const int* table, int width, const int* cu, const int* kv_lens, const float* q_gain,
-                     const float* k_gain, const float* cos, const float* sin, int table_rows, float eps, void* q_out);
+                     const int* table, int width, const int* cu, const int* kv_lens, const void* q_gain,
+                     const void* k_gain, int gain_dtype, const float* cos, const float* sin, int table_rows, float eps, void* q_out);
 
 /* Measurement hook (no counterpart in the reference; for benchmarks and profilers):
  * while enabled, every kernel launch of this library records a HIP event pair on its

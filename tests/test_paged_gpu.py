@@ -188,6 +188,10 @@ def test_storage_order_strides_and_shared_pages():
     wide = torch.full((3, 9), -1, dtype=torch.int32, device="cuda")
     wide[:, 2:2 + table.shape[1]] = table
     assert torch.equal(_ops()[1](proj[:, 1], kp, vp, wide[:, 2:2 + table.shape[1]], cu, kvl, sink, n=16, c=8.0), one)
+    # Heads before pages in storage.
+    kh, vh = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (kp, vp))
+    assert kh.stride(1) > kh.stride(0)
+    assert torch.equal(_ops()[1](q, kh, vh, table, cu, kvl, sink, n=16, c=8.0), one)
     # Two sequences over the same pages.
     o = _ops()[1](q[:2], kp, vp, table[[0, 0]], _i32([0, 1, 2]), _i32([100, 100]), sink, n=16, c=8.0)
     check({"o": o}, *_want(q[:2], [ks[0], ks[0]], [vs[0], vs[0]], [1, 1], sink, 16, 8.0))

@@ -122,10 +122,10 @@ def test_c_abi_refusals():
 
     INV, UNS = _lib.ALG_ERR_INVALID, _lib.ALG_ERR_UNSUPPORTED
 
-    def fwd(N=8, S=1, H=4, Hkv=2, D=64, q=P(16), q_ts=256, q_hs=64, k_ts=128, k_hs=64, cu=P(16), sink=None, ns=0, c=8.0,
+    def fwd(N=8, S=1, H=4, Hkv=2, D=64, q=P(16), q_ts=256, q_hs=64, k_ts=128, k_hs=64, cu=P(16), sink=None, sd=1, ns=0, c=8.0,
             n=16, o=P(16), stat=P(16)):
         return h.alg_packed_attn_fwd(None, N, S, H, Hkv, D, q, q_ts, q_hs, P(16), k_ts, k_hs, P(16), k_ts, k_hs, cu, sink,
-                                     ns, c, n, o, stat)
+                                     sd, ns, c, n, o, stat)
 
     fails(fwd(N=-1), INV, "negative")
     fails(fwd(S=-1), INV, "negative")
@@ -142,6 +142,7 @@ def test_c_abi_refusals():
     fails(fwd(c=1e-20), UNS, "2^-30")
     fails(fwd(cu=None), INV, "cu_seqlens")
     fails(fwd(sink=P(16), ns=3), INV, "sink_count")
+    fails(fwd(sink=P(16), ns=1, sd=2), INV, "bf16 or f32")
     fails(fwd(q=None), INV, "null")
     fails(fwd(stat=None), INV, "null")
     fails(fwd(q=P(24)), INV, "aligned")
@@ -153,8 +154,8 @@ def test_c_abi_refusals():
     assert fwd(N=0, q=None, o=None, stat=None) == _lib.ALG_OK
 
     def bwd(ws=P(16), bytes_=1 << 20, dsink=None, sink=None, dq=P(16), do_ts=256):
-        return h.alg_packed_attn_bwd(None, 8, 1, 4, 2, 64, P(16), 256, 64, P(16), 128, 64, P(16), 128, 64, P(16), sink, 1, 8.0,
-                                     16, P(16), P(16), P(16), do_ts, 64, dq, P(16), P(16), dsink, ws, bytes_)
+        return h.alg_packed_attn_bwd(None, 8, 1, 4, 2, 64, P(16), 256, 64, P(16), 128, 64, P(16), 128, 64, P(16), sink, 1, 1, 8.0,
+                                     16, P(16), P(16), P(16), do_ts, 64, dq, P(16), P(16), dsink, 1, ws, bytes_)
 
     need = h.alg_packed_attn_bwd_workspace_size(8, 1, 4, 2)
     assert need >= 8 * 4 * 4 and h.alg_packed_attn_bwd_workspace_size(8, 1, 5, 2) == 0
@@ -167,14 +168,14 @@ def test_c_abi_refusals():
 
     def paged(N=1, page=16, pages=4, width=2, k_ps=2048, table=P(16), kv=P(16), ws=None, bytes_=0, vp=P(16)):
         return h.alg_paged_attn(None, N, 1, 4, 2, 64, P(16), 256, 64, P(16), k_ps, 1024, 64, vp, 2048, 1024, 64, pages, page,
-                                table, width, P(16), kv, None, 0, 8.0, 16, P(16), ws, bytes_)
+                                table, width, P(16), kv, None, 1, 0, 8.0, 16, P(16), ws, bytes_)
 
     fails(paged(page=24), UNS, "multiple of 16")
     fails(paged(page=0), UNS, "multiple of 16")
     fails(paged(pages=0), INV, "positive")
     fails(paged(width=0), INV, "positive")
     fails(paged(width=1 << 28), UNS, "2^31")
-    fails(paged(k_ps=2044), INV, "page stride")
+    fails(paged(k_ps=2044), INV, "page and head strides")
     fails(paged(table=None), INV, "null")
     fails(paged(kv=None), INV, "null")
     fails(paged(vp=P(24)), INV, "aligned")
@@ -184,28 +185,30 @@ def test_c_abi_refusals():
     fails(paged(width=1000, ws=P(16), bytes_=need - 1), INV, "workspace too small")
     assert paged(N=0, table=None) == _lib.ALG_OK
 
-    def append(eps=1e-5, cos=None, sin=None, rows=0, gain=None, out=P(16), page=16):
+    def append(eps=1e-5, cos=None, sin=None, rows=0, gain=None, gd=1, out=P(16), page=16):
         return h.alg_paged_append(None, 2, 1, 4, 2, 64, P(16), 256, 64, P(16), 128, 64, P(16), 128, 64, P(16), 2048, 1024, 64,
-                                  P(16), 2048, 1024, 64, 4, page, P(16), 2, P(16), P(16), gain, None, cos, sin, rows, eps, out)
+                                  P(16), 2048, 1024, 64, 4, page, P(16), 2, P(16), P(16), gain, None, gd, cos, sin, rows, eps, out)
 
     fails(append(eps=0.0), INV, "eps")
     fails(append(cos=P(16)), INV, "together")
     fails(append(cos=P(16), sin=P(16), rows=31), INV, "rotation tables")
     fails(append(gain=P(20)), INV, "aligned")
+    fails(append(gain=P(16), gd=-1), INV, "bf16 or f32")
     fails(append(out=None), INV, "null")
     fails(append(page=8), UNS, "multiple of 16")
 
-    fails(h.alg_add_rms_norm_fwd(None, 0, 64, P(16), P(16), None, 1e-5, P(16), P(16), P(16)), INV, "positive")
-    fails(h.alg_add_rms_norm_fwd(None, 1, 60, P(16), P(16), None, 1e-5, P(16), P(16), P(16)), UNS, "% 8")
-    fails(h.alg_add_rms_norm_fwd(None, 1, 8192, P(16), P(16), None, 1e-5, P(16), P(16), P(16)), UNS, "at most")
-    fails(h.alg_add_rms_norm_fwd(None, 1, 64, P(16), None, None, 1e-5, P(16), P(16), P(16)), INV, "required")
-    fails(h.alg_add_rms_norm_fwd(None, 1, 64, P(16), P(24), None, 1e-5, P(16), P(16), P(16)), INV, "aligned")
-    fails(h.alg_add_rms_norm_fwd(None, 1, 64, P(16), P(16), P(20), 1e-5, P(16), P(16), P(16)), INV, "aligned")
-    fails(h.alg_add_rms_norm_fp8(None, 1, 64, P(16), P(16), None, 0.0, P(16), P(16), P(16)), INV, "eps")
-    fails(h.alg_add_rms_norm_fp8(None, 1, 64, P(16), P(16), None, 1e-5, P(16), P(16), None), INV, "required")
-    fails(h.alg_add_rms_norm_bwd(None, 1, 64, P(16), None, P(16), P(16), None, P(16), P(16), None, 0), INV, "gain gradient")
-    fails(h.alg_add_rms_norm_bwd(None, 1, 64, P(16), P(16), P(16), P(16), None, P(16), P(16), None, 0), INV, "workspace")
-    fails(h.alg_add_rms_norm_bwd(None, 1, 64, P(16), None, P(16), P(16), P(24), P(16), None, None, 0), INV, "aligned")
+    fails(h.alg_add_rms_norm_fwd(None, 0, 64, P(16), P(16), None, 1, 1e-5, P(16), P(16), P(16)), INV, "positive")
+    fails(h.alg_add_rms_norm_fwd(None, 1, 60, P(16), P(16), None, 1, 1e-5, P(16), P(16), P(16)), UNS, "% 8")
+    fails(h.alg_add_rms_norm_fwd(None, 1, 8192, P(16), P(16), None, 1, 1e-5, P(16), P(16), P(16)), UNS, "at most")
+    fails(h.alg_add_rms_norm_fwd(None, 1, 64, P(16), None, None, 1, 1e-5, P(16), P(16), P(16)), INV, "required")
+    fails(h.alg_add_rms_norm_fwd(None, 1, 64, P(16), P(24), None, 1, 1e-5, P(16), P(16), P(16)), INV, "aligned")
+    fails(h.alg_add_rms_norm_fwd(None, 1, 64, P(16), P(16), P(20), 1, 1e-5, P(16), P(16), P(16)), INV, "aligned")
+    fails(h.alg_add_rms_norm_fp8(None, 1, 64, P(16), P(16), P(16), 7, 1e-5, P(16), P(16), P(16)), INV, "bf16 or f32")
+    fails(h.alg_add_rms_norm_fp8(None, 1, 64, P(16), P(16), None, 1, 0.0, P(16), P(16), P(16)), INV, "eps")
+    fails(h.alg_add_rms_norm_fp8(None, 1, 64, P(16), P(16), None, 1, 1e-5, P(16), P(16), None), INV, "required")
+    fails(h.alg_add_rms_norm_bwd(None, 1, 64, P(16), None, 1, P(16), P(16), None, P(16), P(16), None, 0), INV, "gain gradient")
+    fails(h.alg_add_rms_norm_bwd(None, 1, 64, P(16), P(16), 1, P(16), P(16), None, P(16), P(16), None, 0), INV, "workspace")
+    fails(h.alg_add_rms_norm_bwd(None, 1, 64, P(16), None, 1, P(16), P(16), P(24), P(16), None, None, 0), INV, "aligned")
 
 
 @pytest.mark.parametrize("sink", [None, 0.7, -3.0])
