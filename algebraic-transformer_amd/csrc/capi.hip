@@ -1187,19 +1187,19 @@ int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, 
 
 // ---- packed sequences and paged caches --------------------------------------------------------
 
-// The arithmetic of one call's weights (packed_common.h): R = 4 holds |x| up to 1.875 in the plain
-// form, R = 2 up to 0.75 for n = 32; larger exponents would leave f32 and take the careful form.
+// The arithmetic of one call's weights (packed_common.h). Exponents above 32 would leave f32 in the
+// plain form and always take the careful one.
 static alg::AttnScale attn_scale(int n, float c, int D) {
   alg::AttnScale s;
   s.log2n = log2_pow2(n);
   const double alpha = 1.0 / (std::sqrt((double)D) * (double)c);
-  const double R = n <= 16 ? 4.0 : (n == 32 ? 2.0 : 1.0);
+  const double R = n <= 16 ? 4.0 : 2.0;
   const int e = (int)std::ceil(std::log2(R / alpha));
   const double a = std::ldexp(alpha, e);
   s.qmul = (float)std::ldexp(1.0, -e);
   s.a = (float)a;
   s.b = (float)(1.0 / (a * a));
-  s.bound = n <= 32 ? (float)(0.5 * (R - 1.0 / R) / a) : -1.0f;
+  s.low = n <= 32 ? (float)std::pow(R * a, -n) : INFINITY;
   return s;
 }
 
@@ -1258,7 +1258,7 @@ int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D
   return hip_status(alg::launch_packed_fwd(p, D, false, (hipStream_t)stream), "alg_packed_attn_fwd");
 }
 
-// Backward workspace: [di f32 N H][the slots' forms i32].
+// Backward workspace: [- di f32 N H][the slots' forms i32].
 struct PackedBwdWs {
   size_t care, total;
 };
@@ -1298,7 +1298,7 @@ int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D
   std::memset(&p, 0, sizeof p);
   p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
   p.o = static_cast<const bf16*>(o); p.dO = static_cast<const bf16*>(dO); p.stat = stat;
-  p.di = static_cast<float*>(workspace);
+  p.ndi = static_cast<float*>(workspace);
   p.care = reinterpret_cast<int*>(static_cast<char*>(workspace) + ws.care);
   p.sink = sink; p.sink_count = sink_count; p.sink_bf16 = sink_dtype == ALG_DTYPE_BF16; p.c = c; p.cu = cu;
   p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;

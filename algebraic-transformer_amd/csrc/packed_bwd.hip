@@ -26,14 +26,14 @@
 
 namespace alg {
 
-// Weight P (times the row's statistic) and dS = P (dP - di) r.
+// P and dS = P (dP - di) r; `dp` is dP - di.
 template <int L2N, bool CARE>
-__device__ __forceinline__ void packed_elem(float s, float dp, float rs, float di, float b, int log2n, bool dead,
-                                            float& pw, float& ds) {
+__device__ __forceinline__ void packed_elem(float s, float dp, float rs, float b, int log2n, bool dead, float& pw,
+                                            float& ds) {
   float r;
   const float t = CARE ? weight_t_careful(s, b, r) : weight_t(s, b, r);
   pw = pow2n<L2N>(t * __builtin_fabsf(rs), log2n);
-  ds = pw * (dp - di) * r;
+  ds = pw * dp * r;
   keep_here(pw, ds);
   if (dead) pw = ds = 0.0f;
 }
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
     const bf16x8 z = {};
     if (live) {
       for (int d = 8 * h; d < D; d += 16) *reinterpret_cast<bf16x8*>(p.dq + orow + d) = z;
-      if (h == 0) p.di[srow] = 0.0f;
+      if (h == 0) p.ndi[srow] = 0.0f;
     }
     return;
   }
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
     di += xor32(di);
   }
   const float rs = live ? p.stat[srow] : 0.0f;
-  if (live && h == 0) p.di[srow] = di;
+  if (live && h == 0) p.ndi[srow] = -di;
   const bool careful = __syncthreads_or(rs < 0.0f) != 0;
   if (threadIdx.x == 0) p.care[(size_t)packed_slot(f, G, PK_ROWS) * p.Hkv + kvh] = careful;
   const int log2n = p.sc.log2n;
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float pw, ds;
-          packed_elem<0, true>(s[i], dp[i], rs, di, b2, log2n, kb + 8 * (i >> 2) + 4 * h + (i & 3) > mytok, pw, ds);
+          packed_elem<0, true>(s[i], dp[i] - di, rs, b2, log2n, kb + 8 * (i >> 2) + 4 * h + (i & 3) > mytok, pw, ds);
           da[i >> 3][i & 7] = f2bf(ds);
         }
         const bf16* kl = Ks0 + blk * 32 * D;
@@ -334,14 +334,14 @@ __device__ __forceinline__ void packed_sink_grad(const PackedBwdParams& p, int k
 #pragma unroll 8
   for (int i = threadIdx.x; i < p.N; i += 256) {
     const size_t at = base + (size_t)i * p.G;
-    sum += pow2n<0>(t * __builtin_fabsf(p.stat[at]), p.sc.log2n) * p.di[at];
+    sum += pow2n<0>(t * __builtin_fabsf(p.stat[at]), p.sc.log2n) * p.ndi[at];
   }
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
-    const float d = -(red[0] + red[1] + red[2] + red[3]) * (float)(1 << p.sc.log2n) * (r / p.sc.a) / p.c;
+    const float d = (red[0] + red[1] + red[2] + red[3]) * (float)(1 << p.sc.log2n) * (r / p.sc.a) / p.c;
     if (p.dsink_bf16) static_cast<bf16*>(p.dsink)[head] = f2bf(d);
     else static_cast<float*>(p.dsink)[head] = d;
   }
@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
     const int left = min(max(t.left, 0), BQ);
     const size_t at = sbase + (left > 0 ? rows - t.left : 0);
     const __amdgpu_buffer_rsrc_t rst = __builtin_amdgcn_make_buffer_rsrc((void*)(p.stat + at), (short)0, left * 4, BUF_RSRC_WORD3);
-    const __amdgpu_buffer_rsrc_t rdi = __builtin_amdgcn_make_buffer_rsrc((void*)(p.di + at), (short)0, left * 4, BUF_RSRC_WORD3);
+    const __amdgpu_buffer_rsrc_t rdi = __builtin_amdgcn_make_buffer_rsrc((void*)(p.ndi + at), (short)0, left * 4, BUF_RSRC_WORD3);
     if (wave == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(rst, LDS_PTR(void, ls), 4, lane * 4, 0, 0, 0);
     if (wave == 1) __builtin_amdgcn_raw_ptr_buffer_load_lds(rdi, LDS_PTR(void, ld), 4, lane * 4, 0, 0, 0);
   };
@@ -526,7 +526,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
     const Tile next = source();
     const int row0 = (nq - 1 - qt) * BQ;  // the tile's first row
     floatx4 s[4], dp[4];
-    floatx4 sv[2], dvv[2];  // stat and di of a block's rows (slot = block & 1)
+    floatx4 sv[2];  // statistics of a block's rows (slot = block & 1); dP's sum starts from - di
     bf16x8 pa[2], da[2];
     float pw[4], dsx[4];
     bf16x8 cf[RING][2];     // transposed dO / Q fragments of the dV/dK steps, PF steps ahead
@@ -542,12 +542,12 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
     };
     auto load_stats = [&](int b) {
       sv[b & 1] = *reinterpret_cast<const floatx4*>(sts + 16 * b + qoff);
-      dvv[b & 1] = *reinterpret_cast<const floatx4*>(dis + 16 * b + qoff);
+      dp[b] = *reinterpret_cast<const floatx4*>(dis + 16 * b + qoff);
     };
     // P and dS of row 16 b + qoff + i of the tile.
     auto elem = [&](int b, int i) {
       const bool dead = MASKED && row0 + 16 * b + qoff + i < dead_below;
-      packed_elem<L2N, false>(s[b][i], dp[b][i], sv[b & 1][i], dvv[b & 1][i], b2, log2n, dead, pw[i], dsx[i]);
+      packed_elem<L2N, false>(s[b][i], dp[b][i], sv[b & 1][i], b2, log2n, dead, pw[i], dsx[i]);
       const int c = b >> 1, j0 = 4 * (b & 1);
       if (i & 1) {
         pa[c][j0 + i - 1] = f2bf(pw[i - 1]);
@@ -567,10 +567,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
       dk[db] = mfma16_bf16(da[c], cf[u % RING][1], dk[db]);
     };
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      s[b] = floatx4{};
-      dp[b] = floatx4{};
-    }
+    for (int b = 0; b < 4; ++b) s[b] = floatx4{};
     // S, dP steps: block b's carry the weights of block b - 1; block 0's the next tile's copy
     // (past the last tile nothing is read and zeros land in the unused buffer set).
     load_stats(0);
@@ -651,7 +648,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int b = 2 * c + u;
-          floatx4 s = {}, dp = {};
+          floatx4 s = {}, dp = *reinterpret_cast<const floatx4*>(di0 + 16 * b + qoff);
 #pragma unroll
           for (int st = 0; st < NS; ++st) {
             s = mfma16_bf16(ld8(Qs0 + b * 16 * D + a_off[st]), kf[st], s);
@@ -661,7 +658,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
           for (int i = 0; i < 4; ++i) {
             const int x = 16 * b + qoff + i;
             float pw, ds;
-            packed_elem<0, true>(s[i], dp[i], st0[x], di0[x], b2, log2n, (nq - 1 - qt) * BQ + x < dead_below, pw, ds);
+            packed_elem<0, true>(s[i], dp[i], st0[x], b2, log2n, (nq - 1 - qt) * BQ + x < dead_below, pw, ds);
             pa[4 * u + i] = f2bf(pw);
             da[4 * u + i] = f2bf(ds);
           }

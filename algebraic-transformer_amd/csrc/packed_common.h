@@ -6,12 +6,15 @@
 // key is rho(x)^n, rho(x) = x + sqrt(1 + x^2). The kernels form s = (q 2^-e).k (a power of two:
 // exact) and t = s + sqrt(s^2 + b), b = 1/a^2, a = alpha 2^e; then t = rho(x) / a, and the factor
 // a^-n, common to a row's weights and its sink, cancels in the normalisation. No rounding of a
-// scaled query and no multiplication per score is left. e makes a in [R, 2 R), R the rho of the
-// bound X on |x| (AttnScale): inside the bound t is at most 1, and t^n at least 2^-80 at n = 16
-// (2^-96 at n = 32), so plain f32 sums of t^n and of t^n v neither overflow nor vanish. A
-// workgroup keeps the largest |s| that it sees (half an instruction per score); if one lies
-// outside the bound, it does its rows again in the careful form: a running maximum per row, and
-// rho of a negative x as 1/rho(-x), which plain f32 would lose to cancellation.
+// scaled query and no multiplication per score is left. e makes a in [R, 2 R), R the rho of X =
+// 1.875 (n <= 16) or 0.75 (n = 32), so that t^n is at most 1 for x up to X.
+// The plain form sums t^n and t^n v in f32 as they are, which is exact enough for a row whose sum
+// lies in [low count, 2^30], low = (R a)^-n the weight at x = -X and count its keys. Above, a weight
+// may have overflowed, or its product with v. Below, the mean key lies under -X, where s + sqrt(s^2
+// + b) cancels: a key at x contributes at most (2/|x|)^n 4 n x^2 eps low of error, 32 eps low at the
+// least n, so that a sum above low count has lost no more than 2^-19 of itself. The sum is all that
+// is looked at, once a row, and nothing per score; if a row fails, its workgroup (or wave) does its
+// rows again in the careful form: a running maximum per row, and rho of a negative x as 1/rho(-x).
 // The row statistic is rs = (row's shift) Z^(-1/n), so that a normalised weight is (t rs)^n in
 // either form; its sign tells the backward pass which form the row took (negative: careful).
 //
@@ -42,7 +45,7 @@ struct AttnScale {
   float qmul;   // 2^-e, applied to the queries (exact in bf16 but for subnormals)
   float a;      // alpha 2^e: x = a s
   float b;      // 1 / a^2
-  float bound;  // largest |s| of the plain form; negative: every row takes the careful form
+  float low;    // least mean weight of the plain form; infinite: every row takes the careful form
 };
 
 struct PackedParams {
@@ -86,10 +89,15 @@ struct PagedAppendParams {
   int N, S, H, Hkv, D;
 };
 
+// Whether a row of `count` keys whose weights sum to `sum` needs the careful form (a NaN does).
+__device__ __forceinline__ bool needs_care(float sum, int count, float low) {
+  return count > 0 && !(sum >= low * (float)count && sum <= 0x1p30f);
+}
+
 struct PackedBwdParams {
   const bf16 *q, *k, *v, *o, *dO;
   const float* stat;  // (Hkv, N G)
-  float* di;          // (Hkv, N G), written by the dQ kernel
+  float* ndi;         // (Hkv, N G), - sum_d dO o, written by the dQ kernel
   int* care;          // (slots, Hkv): whether the slot's rows took the careful form, likewise
   const void* sink;
   int sink_count, sink_bf16;

@@ -155,7 +155,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   floatx16 oacc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) oacc[db] = floatx16{};
-  float lsum = 0.0f, smax = 0.0f;
+  float lsum = 0.0f;
 
   const int tr = (lane & 15) >> 2;
   int row_off[NF];  // row fragments of K: row l32, k chunk 2 st + h
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   __syncthreads();
   rk3[0] = ld8(Ks0 + row_off[0]);
   rk3[1] = ld8(Ks0 + row_off[1]);
-  constexpr int VE = 11;  // VALU instructions per weight (scheduling hint)
+  constexpr int VE = 10;  // VALU instructions per weight (scheduling hint)
 
   // One key tile in the plain form, software-pipelined over its two 32-key blocks:
   //   R1 S^T of keys 0..31 | the next tile's copy    R2 S^T of 32..63 | weights of 0..31
@@ -209,10 +209,8 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     };
     auto elem = [&](int blk, int i) {
       const bool dead = MASKED && kb0 + blk * 32 + 8 * (i >> 2) + 4 * h + (i & 3) > mypos;
-      const float x = dead ? 0.0f : s[blk][i];
-      smax = fmaxf(smax, __builtin_fabsf(x));
       float r;
-      float wi = pow2n<L2N>(weight_t(x, b2, r), log2n);
+      float wi = pow2n<L2N>(weight_t(s[blk][i], b2, r), log2n);
       if constexpr (MASKED) keep_here(wi);
       if (dead) wi = 0.0f;
       lsum += wi;
@@ -273,8 +271,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
 
   const bool has_sink = p.sink != nullptr && p.nsplit == 1;  // split: the sink joins in the combination
   const float ss = has_sink ? sink_score(p, head) : 0.0f;
-  const float bound = p.sc.bound;
-  bool careful = bound < 0.0f;
+  bool careful = isinf(p.sc.low);
   if (!careful) {
     // The tiles in pairs (buffer sets 0 and 1); the last pair may be half one, and a pair counts as
     // masked when one of its tiles does. No branch chooses a buffer set inside the loops: the
@@ -290,8 +287,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
       if (kt + 1 >= kt1) break;
       tile(std::integral_constant<int, 1>{}, std::true_type{}, kt + 1);
     }
-    // A score that is no number needs no other form: its row's results are NaN in either.
-    careful = __syncthreads_or(smax > bound || __builtin_fabsf(ss) > bound) != 0;
+    const int count = min(mypos + 1, kt1 * BK) - kt0 * BK;  // the row's keys in this range
+    float sink_w = 1.0f;
+    if (has_sink) {
+      float r;
+      sink_w = pow2n<L2N>(weight_t_careful(ss, b2, r), log2n);
+    }
+    careful = __syncthreads_or(live && (needs_care(lsum + xor32(lsum), count, p.sc.low) || !(sink_w <= 0x1p30f))) != 0;
   }
 
   float shift = 1.0f, tmax = 1.0f;  // the row's weights are (t shift)^n; tmax = 1 / shift
@@ -391,7 +393,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   }
   if (!careful && has_sink) {
     float r;
-    Z += pow2n<L2N>(weight_t(ss, b2, r), log2n);
+    Z += pow2n<L2N>(weight_t_careful(ss, b2, r), log2n);
   }
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;  // a row without keys and sink is zero
   bf16* O = p.o + orow;

@@ -17,8 +17,10 @@
 // scalar load, whose counter is not the vector loads', so that looking a page up never waits for
 // the keys and values in flight.
 // Keys past the range read as zeros (buffer descriptors end there) and have no weight.
-// The weights' two forms: packed_common.h. Here a wave changes to the careful form at the first
-// block that needs it and goes on from the sums it has, whose shift is 1.
+// The weights' two forms: packed_common.h; a wave whose rows need it goes over its blocks again in
+// the careful form.
+#include <type_traits>
+
 #include "launchers.h"
 #include "packed_common.h"
 
@@ -83,7 +85,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
   }
 
   const int log2n = p.sc.log2n;
-  const float b2 = p.sc.b, bound = p.sc.bound;
+  const float b2 = p.sc.b;
   const auto* trow = (const __attribute__((address_space(4))) int*)(p.table + (size_t)f.s * p.width);
   const bf16* kbase = p.k + (size_t)kvh * p.k_hs;
   const bf16* vbase = p.v + (size_t)kvh * p.v_hs;
@@ -98,7 +100,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
 
   bool bad = false;
   typedef bf16x8 KBlock[2][NS];
-  auto load = [&](int blk, KBlock& kf, bf16* vl) {
+  auto load = [&](int blk, KBlock& kf, bf16* vl) __attribute__((always_inline)) {
     auto ll = LDS_PTR(bf16, vl);
     asm volatile("" : "+s"(ll));
 #pragma unroll
@@ -137,65 +139,43 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
 
   floatx4 oacc[RT][NDB];
   float lsum[RT], T[RT], shift[RT];  // weights (t shift)^n, T = 1 / shift (0: no key yet)
+  int count[RT];                     // keys that the row saw
+  auto reset = [&](float t) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    lsum[rt] = 0.0f;
-    T[rt] = shift[rt] = 1.0f;
+    for (int rt = 0; rt < RT; ++rt) {
+      lsum[rt] = 0.0f;
+      T[rt] = shift[rt] = t;
+      count[rt] = 0;
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) oacc[rt][db] = floatx4{};
-  }
-  bool careful = false;
+      for (int db = 0; db < NDB; ++db) oacc[rt][db] = floatx4{};
+    }
+  };
 
-  auto compute = [&](int blk, const KBlock& kf, const bf16* vl) {
-    floatx4 s[RT][2];
-    float smax = 0.0f;
+  auto compute = [&](auto carec, int blk, const KBlock& kf, const bf16* vl) __attribute__((always_inline)) {
+    constexpr bool CARE = decltype(carec)::value;
+    bf16x8 pf[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int rt = 0; rt < RT; ++rt) {
+      floatx4 s[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        s[rt][u] = floatx4{};
+        s[u] = floatx4{};
 #pragma unroll
-        for (int st = 0; st < NS; ++st) s[rt][u] = mfma16_bf16(kf[u][st], qf[rt][st], s[rt][u]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          smax = fmaxf(smax, blk * BLK + 16 * u + 4 * g + i > mypos[rt] ? 0.0f : __builtin_fabsf(s[rt][u][i]));
+        for (int st = 0; st < NS; ++st) s[u] = mfma16_bf16(kf[u][st], qf[rt][st], s[u]);
       }
-    if (!careful && __any(smax > bound)) {
-      careful = true;
+      const int seen = mypos[rt] + 1 - blk * BLK;  // keys of the block up to the row's position
+      count[rt] += min(max(seen, 0), BLK);
+      float t[8], top = 0.0f;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {  // a row without a key yet takes its first key's shift
-        float z = lsum[rt];
-        z += __shfl_xor(z, 16, 64);
-        z += __shfl_xor(z, 32, 64);
-        if (z == 0.0f) T[rt] = shift[rt] = 0.0f;
+      for (int j = 0; j < 8; ++j) {
+        const int u = j >> 2, i = j & 3;
+        float r;
+        t[j] = CARE ? weight_t_careful(s[u][i], b2, r) : pow2n<L2N>(weight_t(s[u][i], b2, r), log2n);
+        keep_here(t[j]);
+        if (16 * u + 4 * g + i >= seen) t[j] = 0.0f;
+        if (CARE) top = fmaxf(top, t[j]);
       }
-    }
-    bf16x8 pf[RT];
-    if (!careful) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int u = j >> 2, i = j & 3;
-          float r;
-          float w = pow2n<L2N>(weight_t(s[rt][u][i], b2, r), log2n);
-          keep_here(w);
-          if (blk * BLK + 16 * u + 4 * g + i > mypos[rt]) w = 0.0f;
-          lsum[rt] += w;
-          pf[rt][j] = f2bf(w);
-        }
-    } else {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float t[8], top = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int u = j >> 2, i = j & 3;
-          float r;
-          const bool dead = blk * BLK + 16 * u + 4 * g + i > mypos[rt];
-          t[j] = dead ? 0.0f : weight_t_careful(s[rt][u][i], b2, r);
-          top = fmaxf(top, t[j]);
-        }
+      if constexpr (CARE) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         if (top > T[rt]) {
@@ -208,12 +188,12 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) oacc[rt][db][i] *= fall;
         }
+      }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float w = pow2n<0>(t[j] * shift[rt], log2n);
-          lsum[rt] += w;
-          pf[rt][j] = f2bf(w);
-        }
+      for (int j = 0; j < 8; ++j) {
+        const float w = CARE ? pow2n<0>(t[j] * shift[rt], log2n) : t[j];
+        lsum[rt] += w;
+        pf[rt][j] = f2bf(w);
       }
     }
 #pragma unroll
@@ -229,31 +209,47 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
 
   // Blocks b0 + wave, + WAVES, ...; a block past the range loads nothing (empty descriptors).
   KBlock ka, kb;
-  load(b0 + wave, ka, vbuf);
-  for (int blk = b0 + wave; blk < b1; blk += 2 * WAVES) {
-    load(blk + WAVES, kb, vbuf + BLK * D);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
+  auto sweep = [&](auto carec) __attribute__((always_inline)) {
+    load(b0 + wave, ka, vbuf);
+    for (int blk = b0 + wave; blk < b1; blk += 2 * WAVES) {
+      load(blk + WAVES, kb, vbuf + BLK * D);
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
+      __builtin_amdgcn_sched_barrier(0);
+      compute(carec, blk, ka, vbuf);
+      load(blk + 2 * WAVES, ka, vbuf);
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
+      __builtin_amdgcn_sched_barrier(0);
+      if (blk + WAVES < b1) compute(carec, blk + WAVES, kb, vbuf + BLK * D);
+    }
+    __builtin_amdgcn_s_waitcnt(VMCNT0);  // copies into the tiles that are written next
     __builtin_amdgcn_sched_barrier(0);
-    compute(blk, ka, vbuf);
-    load(blk + 2 * WAVES, ka, vbuf);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
-    __builtin_amdgcn_sched_barrier(0);
-    if (blk + WAVES < b1) compute(blk + WAVES, kb, vbuf + BLK * D);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {  // the row's sum over the lane groups
+      lsum[rt] += __shfl_xor(lsum[rt], 16, 64);
+      lsum[rt] += __shfl_xor(lsum[rt], 32, 64);
+    }
+  };
+  bool careful = isinf(p.sc.low);
+  reset(1.0f);
+  if (!careful) {
+    sweep(std::false_type{});
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) careful |= needs_care(lsum[rt], count[rt], p.sc.low);
+    careful = __any(careful);
   }
-  __builtin_amdgcn_s_waitcnt(VMCNT0);  // copies into the tiles that the join overwrites
+  if (careful) {
+    reset(0.0f);
+    sweep(std::true_type{});
+  }
 
   // The waves' states, joined in wave order.
   float* sO = reinterpret_cast<float*>(Vs);
   __syncthreads();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    float z = lsum[rt];
-    z += __shfl_xor(z, 16, 64);
-    z += __shfl_xor(z, 32, 64);
-    if (bad) z = __builtin_nanf("");
     if (g == 0) {
       jT[wave][16 * rt + l16] = T[rt];
-      jZ[wave][16 * rt + l16] = z;
+      jZ[wave][16 * rt + l16] = bad ? __builtin_nanf("") : lsum[rt];
     }
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
