@@ -84,7 +84,7 @@ class _AddRmsNormFn(torch.autograd.Function):
                 _lib.check(lib.alg_add_rms_norm_fwd(_lib.stream_of(x), rows, d, p(x), p(residual), p(g), gain_dtype, eps,
                                                     p(s), p(y), p(tau)), "add_rms_norm")
         ctx.save_for_backward(s, g, tau)
-        ctx.gain_meta = None if gain is None else (gain.shape, gain.dtype)
+        ctx.gain_meta = None if gain is None else (gain.dtype, gain.device)
         ctx.set_materialize_grads(False)
         return y, s
 
@@ -112,10 +112,9 @@ class _AddRmsNormFn(torch.autograd.Function):
                 _lib.check(lib.alg_add_rms_norm_bwd(_lib.stream_of(s), rows, d, p(s), p(g), gain_dtype, p(tau), p(dy),
                                                     p(ds), p(dx), p(dg), p(ws), nbytes), "add_rms_norm backward")
         if dg is not None:
-            shape, dtype = ctx.gain_meta
-            dg = dg.reshape(shape)
-            if dg.dtype is not dtype:
-                dg = dg.to(dtype)
+            dtype, where = ctx.gain_meta
+            if dg.dtype is not dtype or where != dg.device:
+                dg = dg.to(device=where, dtype=dtype)
         return dx, dx, dg, None
 
 
@@ -123,10 +122,10 @@ def _gain_vector(gain, device):
     """The gain, f32 or bf16, contiguous and aligned, and its type's code."""
     if gain is None:
         return None, 1
-    g = gain.detach()
+    g = gain
     if g.dtype not in _WEIGHTS or g.device != device:
-        g = g.to(device=device, dtype=_F32)
-    return _lib.aligned16(g.reshape(-1)), _WEIGHTS[g.dtype]
+        g = g.detach().to(device=device, dtype=_F32)
+    return _lib.aligned16(g), _WEIGHTS[g.dtype]
 
 
 def _check_add(x, residual, gain, eps, what):

@@ -70,12 +70,13 @@ def _sink_vector(sink_logit, H, device):
     (None, 0, 0) without."""
     if sink_logit is None:
         return None, 0, 0
-    s = sink_logit.detach()
-    if s.numel() not in (1, H):
+    count = sink_logit.numel()
+    if count != H and count != 1:
         raise ValueError(f"sink_logit must broadcast to ({H},)")
+    s = sink_logit
     if s.dtype not in _WEIGHTS or s.device != device:
-        s = s.to(device=device, dtype=_F32)
-    return s.reshape(-1).contiguous(), _WEIGHTS[s.dtype], s.numel()
+        s = s.detach().to(device=device, dtype=_F32)
+    return s if s.is_contiguous() else s.detach().contiguous(), _WEIGHTS[s.dtype], count
 
 
 _WEIGHTS = {_BF16: _lib.DTYPE_BF16, _F32: _lib.DTYPE_F32}
@@ -101,7 +102,7 @@ class _PackedFn(torch.autograd.Function):
                 count, c, n, p(o), p(stat)), "packed_flash_attention forward")
         ctx.save_for_backward(q, k, v, cu, sink, o, stat)
         ctx.scale = (n, c)
-        ctx.sink_meta = None if sink_logit is None else (sink_logit.shape, sink_logit.dtype)
+        ctx.sink_meta = None if sink_logit is None else (sink_logit.shape, sink_logit.dtype, sink_logit.device)
         return o
 
     @staticmethod
@@ -123,7 +124,7 @@ class _PackedFn(torch.autograd.Function):
         if sink is not None:
             sink_dtype = _WEIGHTS[sink.dtype]
         if wants_sink:  # per head in the sink's own type; a shared sink's are added up in f32
-            shape, dtype = ctx.sink_meta
+            shape, dtype, where = ctx.sink_meta
             dsink = torch.empty(H, dtype=dtype if dtype in _WEIGHTS and sink.numel() == H else _F32, device=dev)
         nbytes = lib.alg_packed_attn_bwd_workspace_size(N, S, H, Hkv)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -137,8 +138,8 @@ class _PackedFn(torch.autograd.Function):
             if sink.numel() != H:
                 dsink = dsink.sum()
             dsink = dsink.reshape(shape)
-            if dsink.dtype is not dtype:
-                dsink = dsink.to(dtype)
+            if dsink.dtype is not dtype or where != dev:
+                dsink = dsink.to(device=where, dtype=dtype)
         return dq, dk, dv, None, dsink, None, None, None
 
 

@@ -72,6 +72,9 @@ def _no_gradient(what, *tensors):
 
 def _gains(q_gain, k_gain, device):
     """Both gains in one of the types that the kernel reads, 16-byte aligned, and its code."""
+    if (q_gain is not None and k_gain is not None and q_gain.dtype is k_gain.dtype and q_gain.dtype in _WEIGHTS and
+            q_gain.device == device and k_gain.device == device):
+        return _lib.aligned16(q_gain), _lib.aligned16(k_gain), _WEIGHTS[q_gain.dtype]
     gains = [None if g is None else g.detach() for g in (q_gain, k_gain)]
     types = {g.dtype for g in gains if g is not None}
     same = types.pop() if len(types) == 1 else _F32

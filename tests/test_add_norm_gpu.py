@@ -78,6 +78,22 @@ def test_one_output_alone_and_a_bf16_gain():
     assert torch.equal(y, rms_norm(s, g))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_gains_of_other_types_and_places(dtype):
+    x, r, g, dy, ds = _inputs(20, 128, True, seed=9)
+    for gain in (g.to(dtype), g.to(dtype).cpu(), g.to(dtype).repeat_interleave(2)[::2], g.to(dtype)[None]):
+        gain = gain.detach().requires_grad_(True)
+        y, s = _ops()[0](x, r, gain)
+        want, rms = _ref(s.detach(), gain.cuda().reshape(-1))
+        _near(y.detach(), want, (U + F) * want.abs(), "y")
+        dg = torch.autograd.grad((y, s), gain, (dy, ds))[0]
+        assert dg.shape == gain.shape and dg.dtype == dtype and dg.device == gain.device
+        terms = dy.double() * s.detach().double() / rms
+        _near(dg.cuda().reshape(-1), terms.sum(0), F * terms.abs().sum(0) + torch.finfo(dtype).eps / 2 * terms.sum(0).abs(), "dgain")
+        y8, scale, _ = _ops()[1](x, r, gain.detach())
+        _near(y8.float() * scale, want, U8 * want.abs() + (2.0 ** -10) * scale.double() + F * want.abs(), "y8")
+
+
 def test_gradients_against_differences():
     """The bf16 gradient along a direction, against central differences of the float64 statement."""
     x, r, g, dy, ds = _inputs(7, 64, True, seed=5)

@@ -194,6 +194,25 @@ def test_one_captured_graph_serves_any_lengths():
                 assert torch.equal(a, b), (i, rep, name)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize("shape", [(4,), (1, 4, 1, 1), ()])
+def test_sinks_of_other_types_shapes_and_places(dtype, shape):
+    """The sink's gradient comes back in its type, shape and device; one more rounding, of that type."""
+    leaves, s, do, cu = _inputs([70, 33], 4, 2, 64, sink="heads" if shape else "one", seed=14)
+    for dev in ("cuda", "cpu"):
+        sink = s.detach().to(device=dev, dtype=dtype).reshape(shape).requires_grad_(True)
+        got = _run(leaves, sink, do, cu, 16, 8.0)
+        assert got["dsink"].shape == sink.shape and got["dsink"].dtype == dtype and got["dsink"].device == sink.device
+        val, tol = packed_ref(*leaves, cu, sink.detach().float().cuda().reshape(-1), do, n=16, c=8.0)
+        tol["dsink"] = tol["dsink"] + torch.finfo(dtype).eps / 2 * val["dsink"].abs()
+        got["dsink"] = got["dsink"].cuda()
+        check(got, val, tol)
+    if shape:  # every other entry of a longer vector
+        wide = s.detach().repeat_interleave(2)[::2].requires_grad_(True)
+        got = _run(leaves, wide, do, cu, 16, 8.0)
+        check(got, *packed_ref(*leaves, cu, wide, do, n=16, c=8.0))
+
+
 def test_no_tokens():
     q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
     k = torch.empty(0, 2, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
