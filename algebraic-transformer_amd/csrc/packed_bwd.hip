@@ -55,18 +55,16 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   if (f.tile < 0 || r0 >= R) return;
   const int myr = r0 + wave * 32 + l32;
   const bool live = myr < R;
-  const int tok = min(myr, R - 1) / G, head = kvh * G + (min(myr, R - 1) - tok * G);
-  const size_t orow = ((size_t)(f.start + tok) * p.H + head) * D;
-  const size_t srow = (size_t)kvh * p.N * G + (size_t)f.start * G + min(myr, R - 1);
+  const PackedRow at = packed_row<D>(p, f, kvh, min(myr, R - 1));
   if (f.s == p.S) {  // tokens behind the last sequence
     const bf16x8 z = {};
     if (live) {
-      for (int d = 8 * h; d < D; d += 16) *reinterpret_cast<bf16x8*>(p.dq + orow + d) = z;
-      if (h == 0) p.ndi[srow] = 0.0f;
+      for (int d = 8 * h; d < D; d += 16) *reinterpret_cast<bf16x8*>(p.dq + at.out + d) = z;
+      if (h == 0) p.ndi[at.stat] = 0.0f;
     }
     return;
   }
-  const int mytok = live ? tok : -1;
+  const int mytok = live ? at.tok : -1;
   const int posmax = (min(r0 + PK_ROWS, R) - 1) / G;
   const int wave_posmax = min(r0 + wave * 32 + 31, R - 1) / G;
   const int ntiles = posmax / BK + 1;
@@ -84,6 +82,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
     g.v = vbase + (size_t)k * p.v_ts;
     return g;
   };
+  // Instruction pair j of a copy: a lane's row and swizzled chunk, the same for every tile; the rest
+  // of the address is scalar.
+  const int lrow = lane / CPR;
+  const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
+  const int chunkb = 16 * ((lane % CPR) ^ swz_chunk<CPR>(lrow));
   auto dma = [&](bf16* la, bf16* lb, const KvGroup& g, int j) {
     const int kn = g.rows > 0 ? ((g.rows - 1) * (int)p.k_ts + D) * 2 : 0;
     const int vn = g.rows > 0 ? ((g.rows - 1) * (int)p.v_ts + D) * 2 : 0;
@@ -93,13 +96,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
     auto llb = LDS_PTR(bf16, lb);
     asm volatile("" : "+s"(lla), "+s"(llb));
     const int J = wave * PW + j;
-    int lrow = lane / CPR, chunkb = 16 * ((lane % CPR) ^ swz_chunk<CPR>(lane / CPR));
-    asm volatile("" : "+v"(lrow), "+v"(chunkb));  // computed here, not kept live
-    const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
-    const int col = chunkb ^ (16 * swz_chunk<CPR>(RPI * J));
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lla + J * 512, 16, RPI * j * (int)p.k_ts * 2 + k_row + col, 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, llb + J * 512, 16, RPI * j * (int)p.v_ts * 2 + v_row + col, 0, 0, 0);
+    const int col = chunkb ^ (16 * swz_chunk<CPR>(RPI * j));  // 16 rows a wave: the swizzle's period
+    const int ko = RPI * j * (int)p.k_ts * 2, vo = RPI * j * (int)p.v_ts * 2;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lla + J * 512, 16, k_row + col + ko, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, llb + J * 512, 16, v_row + col + vo, 0, 0, 0);
   };
+
   {
     const KvGroup g = group(0);
 #pragma unroll
@@ -110,9 +112,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   bf16x8 qf[NF], of[NF];
   float di = 0.0f;
   {
-    const bf16* Q = p.q + (size_t)(f.start + tok) * p.q_ts + (size_t)head * p.q_hs + 8 * h;
-    const bf16* dO = p.dO + (size_t)(f.start + tok) * p.do_ts + (size_t)head * p.do_hs + 8 * h;
-    const bf16* O = p.o + orow + 8 * h;
+    const bf16* Q = p.q + (size_t)(f.start + at.tok) * p.q_ts + (size_t)at.head * p.q_hs + 8 * h;
+    const bf16* dO = p.dO + (size_t)(f.start + at.tok) * p.do_ts + (size_t)at.head * p.do_hs + 8 * h;
+    const bf16* O = p.o + at.out + 8 * h;
     bf16x8 ov[NF];
 #pragma unroll
     for (int s = 0; s < NF; ++s) {
@@ -132,15 +134,16 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
       }
     di += xor32(di);
   }
-  const float rs = live ? p.stat[srow] : 0.0f;
-  if (live && h == 0) p.ndi[srow] = -di;
+  const float rs = live ? p.stat[at.stat] : 0.0f;
+  if (live && h == 0) p.ndi[at.stat] = -di;
   const bool careful = __syncthreads_or(rs < 0.0f) != 0;
   if (threadIdx.x == 0) p.care[(size_t)packed_slot(f, G, PK_ROWS) * p.Hkv + kvh] = careful;
   const int log2n = p.sc.log2n;
   const float b2 = p.sc.b;
   // Plain form: dS = (t^n r) fma(rs^n, dP, - rs^n di), one instruction less than P (dP - di) r.
-  const float pz = careful ? 0.0f : pow2n<0>(rs, log2n);
-  const float nzd = -pz * di;
+  // Careful form: the two registers hold the statistic and di themselves.
+  const float pz = careful ? rs : pow2n<0>(rs, log2n);
+  const float nzd = careful ? di : -pz * di;
   floatx16 dqa[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) dqa[db] = floatx16{};
@@ -149,12 +152,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   int row_off[NF];
 #pragma unroll
   for (int st = 0; st < NF; ++st) row_off[st] = swz_at<CPR>(l32, 16 * st + 8 * h);
-  int tk_lo[NDB], tk_hi[NDB];
+  int tk_lo[NDB];  // transposed K fragments: rows 4h + (0..3); the other half's lie eight rows on
 #pragma unroll
-  for (int db = 0; db < NDB; ++db) {
-    tk_lo[db] = swz_at<CPR>(4 * h + tr, tr_col(db * 32, lane));
-    tk_hi[db] = swz_at<CPR>(4 * h + 8 + tr, tr_col(db * 32, lane));
-  }
+  for (int db = 0; db < NDB; ++db) tk_lo[db] = swz_at<CPR>(4 * h + tr, tr_col(db * 32, lane));
+  const auto eight_on = [](int at) { return (again(at) ^ 16) + 8 * D; };  // the swizzle's next chunk pair
   bf16x8 rk2[2], rv2[2];  // row fragments of K / V, one step ahead
   __builtin_amdgcn_s_waitcnt(VMCNT0);
   __syncthreads();
@@ -213,8 +214,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
     bf16x8 ft[2][2];
     auto dq_load = [&](int blk, int db, bf16x8 (&fr)[2]) {
       const bf16* kb = Ks + blk * 32 * D;
-      fr[0] = tr_frag_at(kb, tk_lo[db], tk_hi[db]);
-      fr[1] = tr_frag_at(kb + 16 * D, tk_lo[db], tk_hi[db]);
+      // Formed here: held, four more addresses were spilled, and a reload waits for every copy
+      // before it (307 us instead of 293).
+      const int hi = eight_on(tk_lo[db]);
+      fr[0] = tr_frag_at(kb, tk_lo[db], hi);
+      fr[1] = tr_frag_at(kb + 16 * D, tk_lo[db], hi);
     };
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -295,22 +299,23 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float pw, ds;
-          packed_elem<0, true>(s[i], dp[i] - di, rs, b2, log2n, kb + 8 * (i >> 2) + 4 * h + (i & 3) > mytok, pw, ds);
+          packed_elem<0, true>(s[i], dp[i] - nzd, pz, b2, log2n, kb + 8 * (i >> 2) + 4 * h + (i & 3) > mytok, pw, ds);
           da[i >> 3][i & 7] = f2bf(ds);
         }
         const bf16* kl = Ks0 + blk * 32 * D;
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
-          dqa[db] = mfma_bf16(tr_frag_at(kl, tk_lo[db], tk_hi[db]), da[0], dqa[db]);
-          dqa[db] = mfma_bf16(tr_frag_at(kl + 16 * D, tk_lo[db], tk_hi[db]), da[1], dqa[db]);
+          const int hi = eight_on(tk_lo[db]);
+          dqa[db] = mfma_bf16(tr_frag_at(kl, tk_lo[db], hi), da[0], dqa[db]);
+          dqa[db] = mfma_bf16(tr_frag_at(kl + 16 * D, tk_lo[db], hi), da[1], dqa[db]);
         }
       }
     }
   }
 
-  if (live) {
+  if (mytok >= 0) {
     const float slope = (float)(1 << log2n) * p.sc.qmul;
-    bf16* DQ = p.dq + orow;
+    bf16* DQ = p.dq + packed_row<D>(p, f, kvh, again(r0 + wave * 32 + l32)).out;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -351,7 +356,10 @@ template <int D>
 constexpr int packed_dkdv_waves() { return D == 64 ? 3 : 2; }  // waves per SIMD
 constexpr int PK_KEYS = 64;  // keys per dK/dV workgroup
 
-template <int D, int L2N>
+// Whether a copy instruction's rows are whole tokens and tokens lie one behind another (ALIGNED, of a
+// group that divides the 8 or 4 rows; host: packed_aligned): a lane's address is then the same in
+// every tile but for a scalar, and rows past the sequence are past the descriptor's end.
+template <int D, int L2N, bool ALIGNED>
 __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kernel(PackedBwdParams p) {
   typedef Dkdv16Lay<D> Lay;
   constexpr int BQ = 64, CPR = D / 8, NS = D / 32, NDB = D / 16;
@@ -413,6 +421,8 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   const size_t sbase = (size_t)kvh * p.N * G + (size_t)(f.start + k0) * G;
   const int lrow = lane / CPR;
   const int chunkb = 16 * ((lane % CPR) ^ Lay::swz(lrow));
+  const int q_row = (lrow / G * (int)p.q_ts + lrow % G * (int)p.q_hs) * 2;
+  const int o_row = (lrow / G * (int)p.do_ts + lrow % G * (int)p.do_hs) * 2;
   struct Tile {
     const bf16 *q, *o;
     int rem, left;  // first row's head; rows left from the tile's first
@@ -437,18 +447,27 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
     return now;
   };
   auto dma_part = [&](bf16* la, bf16* lb, const Tile& t, int j) {
-    const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)t.q, (short)0, 0x7ffffff0, BUF_RSRC_WORD3);
-    const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc((void*)t.o, (short)0, 0x7ffffff0, BUF_RSRC_WORD3);
     auto lla = LDS_PTR(bf16, la);
     auto llb = LDS_PTR(bf16, lb);
     asm volatile("" : "+s"(lla), "+s"(llb));
     const int J = wave * PW + j;
-    const int x = RPI * J + lrow, y = t.rem + x;
-    const int dt = (y * inv_g) >> 16, gh = y - dt * G;
-    const int col = chunkb ^ (16 * Lay::swz(RPI * J));
-    const bool in = x < t.left;
-    const int qo = in ? (dt * (int)p.q_ts + gh * (int)p.q_hs) * 2 + col : -16;
-    const int oo = in ? (dt * (int)p.do_ts + gh * (int)p.do_hs) * 2 + col : -16;
+    const int col = chunkb ^ (16 * Lay::swz(RPI * j));  // 16 rows a wave: the swizzle's period
+    int qo, oo, qn = 0x7ffffff0, on = 0x7ffffff0;
+    if constexpr (ALIGNED) {
+      const int tok = RPI * J / G, left = min(t.left, BQ) / G;  // whole tokens either way
+      qo = q_row + col + tok * (int)p.q_ts * 2;
+      oo = o_row + col + tok * (int)p.do_ts * 2;
+      qn = left * (int)p.q_ts * 2;
+      on = left * (int)p.do_ts * 2;
+    } else {
+      const int x = RPI * J + lrow, y = t.rem + x;
+      const int dt = (y * inv_g) >> 16, gh = y - dt * G;
+      const bool in = x < t.left;
+      qo = in ? (dt * (int)p.q_ts + gh * (int)p.q_hs) * 2 + col : -16;
+      oo = in ? (dt * (int)p.do_ts + gh * (int)p.do_hs) * 2 + col : -16;
+    }
+    const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)t.q, (short)0, qn, BUF_RSRC_WORD3);
+    const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc((void*)t.o, (short)0, on, BUF_RSRC_WORD3);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, lla + J * 512, 16, qo, 0, 0, 0);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(ro, llb + J * 512, 16, oo, 0, 0, 0);
   };
@@ -688,6 +707,12 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   }
 }
 
+static bool packed_aligned(const PackedBwdParams& p, int D) {
+  const int rows = 512 / D;  // of a copy instruction
+  const auto behind = [&](long ts, long hs) { return (p.G - 1) * hs + D <= ts; };
+  return rows % p.G == 0 && behind(p.q_ts, p.q_hs) && behind(p.do_ts, p.do_hs);
+}
+
 template <int D, int L2N>
 static void launch_bwd(const PackedBwdParams& p, hipStream_t st) {
   {
@@ -695,8 +720,9 @@ static void launch_bwd(const PackedBwdParams& p, hipStream_t st) {
     hipLaunchKernelGGL((packed_dq_kernel<D, L2N>), dim3(p.Hkv * packed_slots(p.N, p.G, p.S, PK_ROWS)), dim3(256), 0, st, p);
   }
   KTimer t("packed_dkdv", st);
-  hipLaunchKernelGGL((packed_dkdv_kernel<D, L2N>),
-                     dim3(p.Hkv * (packed_slots(p.N, 1, p.S, PK_KEYS) + (p.dsink ? p.G : 0))), dim3(256), 0, st, p);
+  const dim3 grid(p.Hkv * (packed_slots(p.N, 1, p.S, PK_KEYS) + (p.dsink ? p.G : 0)));
+  if (packed_aligned(p, D)) hipLaunchKernelGGL((packed_dkdv_kernel<D, L2N, true>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((packed_dkdv_kernel<D, L2N, false>), grid, dim3(256), 0, st, p);
 }
 
 hipError_t launch_packed_bwd(const PackedBwdParams& p, int D, hipStream_t st) {

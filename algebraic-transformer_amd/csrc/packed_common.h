@@ -262,6 +262,26 @@ __device__ __forceinline__ PackedSeq packed_find_heavy(const int* cu, int N, int
   return r;
 }
 
+// Where row `r` of a sequence lies: its token, head, and elements in the outputs and statistics.
+struct PackedRow {
+  int tok, head;
+  size_t out, stat;
+};
+template <int D, typename P>
+__device__ __forceinline__ PackedRow packed_row(const P& p, const PackedSeq& f, int kvh, int r) {
+  PackedRow a;
+  a.tok = r / p.G;
+  a.head = kvh * p.G + r - a.tok * p.G;
+  a.out = ((size_t)(f.start + a.tok) * p.H + a.head) * D;
+  a.stat = (size_t)kvh * p.N * p.G + (size_t)f.start * p.G + r;
+  return a;
+}
+// A lane's row formed again where it is used (registers are short in the main loops).
+__device__ __forceinline__ int again(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // One 16-row group of a K / V tile: where its rows start, and how many of them exist.
 struct KvGroup {
   const bf16* k;

@@ -46,15 +46,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   if (f.tile < 0 || r0 >= R) return;
   const int myr = r0 + wave * 32 + l32;
   const bool live = myr < R;
-  const int tok = min(myr, R - 1) / G, head = kvh * G + (min(myr, R - 1) - tok * G);
-  const size_t orow = ((size_t)(f.start + tok) * p.H + head) * D;
-  const size_t srow = (size_t)kvh * p.N * G + (size_t)f.start * G + min(myr, R - 1);
+  const PackedRow at = packed_row<D>(p, f, kvh, min(myr, R - 1));
 
   if (f.s == p.S) {  // tokens behind the last sequence
     if (live && range == 0) {
       const bf16x8 z = {};
-      for (int d = 8 * h; d < D; d += 16) *reinterpret_cast<bf16x8*>(p.o + orow + d) = z;
-      if (p.stat && h == 0) p.stat[srow] = 0.0f;
+      for (int d = 8 * h; d < D; d += 16) *reinterpret_cast<bf16x8*>(p.o + at.out + d) = z;
+      if (p.stat && h == 0) p.stat[at.stat] = 0.0f;
     }
     return;
   }
@@ -62,7 +60,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   // Keys of the sequence, and the position of its first token among them.
   const int L = PAGED ? min(max(p.kv_lens[f.s], 0), p.width * p.page) : f.len;
   const int off = L - f.len;
-  const int mypos = live ? off + tok : -1;
+  const int mypos = live ? off + at.tok : -1;
   const int rlast = min(r0 + PK_ROWS, R) - 1;
   const int posmin = off + r0 / G, posmax = off + rlast / G;
   const int wave_posmax = off + min(r0 + wave * 32 + 31, R - 1) / G;
@@ -113,10 +111,12 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     }
     return g;
   };
+  // Instruction pair j of a copy: a lane's row and swizzled chunk, the same for every tile; the rest
+  // of the address is scalar.
+  const int lrow = lane / CPR;
+  const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
+  const int chunkb = 16 * ((lane % CPR) ^ swz_chunk<CPR>(lrow));
   auto dma = [&](bf16* la, bf16* lb, const KvGroup& g, int j) {
-    int lrow = lane / CPR, chunkb = 16 * ((lane % CPR) ^ swz_chunk<CPR>(lane / CPR));
-    asm volatile("" : "+v"(lrow), "+v"(chunkb));  // computed here, not kept live
-    const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
     const int kn = g.rows > 0 ? ((g.rows - 1) * (int)p.k_ts + D) * 2 : 0;
     const int vn = g.rows > 0 ? ((g.rows - 1) * (int)p.v_ts + D) * 2 : 0;
     const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)g.k, (short)0, kn, BUF_RSRC_WORD3);
@@ -125,9 +125,10 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     auto llb = LDS_PTR(bf16, lb);
     asm volatile("" : "+s"(lla), "+s"(llb));
     const int J = wave * PW + j;
-    const int col = chunkb ^ (16 * swz_chunk<CPR>(RPI * J));
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lla + J * 512, 16, RPI * j * (int)p.k_ts * 2 + k_row + col, 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, llb + J * 512, 16, RPI * j * (int)p.v_ts * 2 + v_row + col, 0, 0, 0);
+    const int col = chunkb ^ (16 * swz_chunk<CPR>(RPI * j));  // 16 rows a wave: the swizzle's period
+    const int ko = RPI * j * (int)p.k_ts * 2, vo = RPI * j * (int)p.v_ts * 2;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lla + J * 512, 16, k_row + col + ko, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, llb + J * 512, 16, v_row + col + vo, 0, 0, 0);
   };
 
   if constexpr (PAGED) {
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   // Query fragments (B operand of S^T = K Q^T), held for the whole kernel; dead rows are zero.
   bf16x8 qf[NF];
   {
-    const bf16* Q = p.q + (size_t)(f.start + tok) * p.q_ts + (size_t)head * p.q_hs;
+    const bf16* Q = p.q + (size_t)(f.start + at.tok) * p.q_ts + (size_t)at.head * p.q_hs;
 #pragma unroll
     for (int s = 0; s < NF; ++s) qf[s] = ld8(Q + 16 * s + 8 * h);
     keep_own_row<NF>(qf, live);
@@ -270,7 +271,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   };
 
   const bool has_sink = p.sink != nullptr && p.nsplit == 1;  // split: the sink joins in the combination
-  const float ss = has_sink ? sink_score(p, head) : 0.0f;
+  const float ss = has_sink ? sink_score(p, at.head) : 0.0f;
   bool careful = isinf(p.sc.low);
   if (!careful) {
     // The tiles in pairs (buffer sets 0 and 1); the last pair may be half one, and a pair counts as
@@ -373,8 +374,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     if (bad_page) Z = __builtin_nanf("");
   }
   if (!live) return;
+  const PackedRow my = packed_row<D>(p, f, kvh, again(r0 + wave * 32 + l32));
   if (p.nsplit > 1) {
-    const size_t part = (size_t)range * p.Hkv * p.N * G + srow;
+    const size_t part = (size_t)range * p.Hkv * p.N * G + my.stat;
     float* O = p.part_o + part * D;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
@@ -396,7 +398,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     Z += pow2n<L2N>(weight_t_careful(ss, b2, r), log2n);
   }
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;  // a row without keys and sink is zero
-  bf16* O = p.o + orow;
+  bf16* O = p.o + my.out;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     }
   if (p.stat && h == 0) {
     const float rs = Z == 0.0f ? 0.0f : shift * inv_root(Z, 1 << log2n);
-    p.stat[srow] = careful ? -rs : rs;
+    p.stat[my.stat] = careful ? -rs : rs;
   }
 }
 
