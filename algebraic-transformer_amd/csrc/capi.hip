@@ -1345,7 +1345,9 @@ static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int 
   const long groups = std::max(1L, std::max((rows + tile - 1) / tile, (long)std::min(S, N)) * Hkv);
   const long cap = (long)width * page, least = pl.row_tiles ? alg::DECODE_RANGE : 1024;
   const long most = pl.row_tiles ? std::min(256 / groups, (long)alg::MAX_RANGES) : (512 + groups - 1) / groups;
-  pl.nsplit = (int)std::max(1L, std::min(most, cap / least));
+  // Far more sequences than tokens: ranges of mostly empty slots would be a grid too large.
+  const long slots = (long)alg::packed_slots(N, (int)G, S, (int)tile) * Hkv;
+  pl.nsplit = (int)std::max(1L, std::min(std::min(most, cap / least), 65536 / slots));
   const size_t parts = pl.nsplit > 1 ? (size_t)pl.nsplit * N * H : 0;
   pl.zt = align256(parts * D * sizeof(float));
   pl.total = pl.zt + align256(parts * 2 * sizeof(float));

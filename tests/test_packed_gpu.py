@@ -57,6 +57,21 @@ def test_long_rows_and_large_groups(G, D, T):
     check(_run(leaves, sink, do, cu, 16, 8.0), *packed_ref(*leaves, cu, sink, do, n=16, c=8.0))
 
 
+@pytest.mark.parametrize("S", [64, 65, 200])
+def test_many_ragged_sequences(S):
+    """On both sides of 64 sequences, where the workgroups' order changes; empty ones among them."""
+    lens = [(37 * i) % 23 if i % 5 else 0 for i in range(S - 2)] + [150, 1]
+    print(f"[packed] {S} sequences", flush=True)
+    leaves, sink, do, cu = _inputs(lens, 6, 2, 64, tail=5, seed=S)
+    check(_run(leaves, sink, do, cu, 16, 8.0), *packed_ref(*leaves, cu, sink, do, n=16, c=8.0))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_long_sequence(D):
+    leaves, sink, do, cu = _inputs([2900, 130], 2, 1, D, seed=15)
+    check(_run(leaves, sink, do, cu, 16, 8.0), *packed_ref(*leaves, cu, sink, do, n=16, c=8.0))
+
+
 @pytest.mark.parametrize("n", [2, 4, 8, 32, 64, 1024])
 @pytest.mark.parametrize("sink", ["none", "one", "heads"])
 def test_exponents_and_sinks(n, sink):
@@ -124,8 +139,12 @@ def test_slices_of_one_projection_and_an_expanded_cotangent():
     val, tol = packed_ref(*leaves, cu, s, do1, n=16, c=8.0)
     parts = dict(zip(("dq", "dk", "dv"), (t.unflatten(1, (-1, D)) for t in dproj.split([H * D, Hkv * D, Hkv * D], 1))))
     check({"o": o, **parts, "dsink": ds}, val, tol)
-    head_major = [t.detach().transpose(0, 1).contiguous().transpose(0, 1) for t in leaves]
-    assert torch.equal(_op()(*head_major, cut, s, n=16, c=8.0), o)
+    head_major = [t.detach().transpose(0, 1).contiguous().transpose(0, 1).requires_grad_(True) for t in leaves]
+    o2 = _op()(*head_major, cut, s, n=16, c=8.0)
+    assert torch.equal(o2, o)
+    got = torch.autograd.grad(o2, [*head_major, s], do1.transpose(0, 1).contiguous().transpose(0, 1))
+    for a, b in zip(got, (*parts.values(), ds)):
+        assert torch.equal(a, b)
 
 
 def test_equal_lengths_match_flash_attention():

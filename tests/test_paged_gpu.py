@@ -235,6 +235,23 @@ def test_many_sequences():
             _check(case, [1] * S)
 
 
+def test_far_more_sequences_than_tokens():
+    """300000 sequences of which three have a new token."""
+    append, attend = _ops()
+    S, at = 300000, (5, 150000, 299999)
+    q, kp, vp, table, cu, kv, sink, ks, vs = _cache([700, 40, 1], [1, 1, 1], 2, 1, 64, 16, seed=16)
+    lens, wide, starts = torch.zeros(S, dtype=torch.int32), torch.zeros(S, table.shape[1], dtype=torch.int32), torch.zeros(S + 1, dtype=torch.int32)
+    for i, s in enumerate(at):
+        lens[s], wide[s] = kv[i], table[i].cpu()
+        starts[s + 1:] += 1
+    o = attend(q, kp, vp, wide.cuda(), starts.cuda(), lens.cuda(), sink, n=16, c=8.0)
+    check({"o": o}, *_want(q, ks, vs, [1, 1, 1], sink, 16, 8.0))
+    k, v = torch.ones(3, 1, 64, dtype=BF, device="cuda"), torch.ones(3, 1, 64, dtype=BF, device="cuda")
+    append(q, k, v, kp, vp, wide.cuda(), starts.cuda(), lens.cuda())
+    for i, n in enumerate((700, 40, 1)):
+        assert (vp[table[i, (n - 1) // 16], 0, (n - 1) % 16] == 1).all()
+
+
 def test_captured_steps_follow_the_lengths():
     """Append and attention captured once; replayed as the sequences grow by a token, between eager
     calls on other inputs."""
