@@ -72,8 +72,9 @@ _SIGNATURES = {
     "alg_add_rms_norm_fp8": (_I, [_P, _I, _I, _P, _P, _P, _I, _F, _P, _P, _P]),
     "alg_add_rms_norm_bwd": (_I, [_P, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _S]),
     "alg_packed_attn_fwd": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _F, _I,
-                                 _P, _P]),
-    "alg_packed_attn_bwd_workspace_size": (_S, [_I, _I, _I, _I]),
+                                 _P, _P, _P, _S]),
+    "alg_packed_attn_fwd_workspace_size": (_S, [_I, _I, _I, _I, _I]),
+    "alg_packed_attn_bwd_workspace_size": (_S, [_I, _I, _I, _I, _I]),
     "alg_packed_attn_bwd": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _F, _I,
                                  _P, _P, _P, _L, _L, _P, _P, _P, _P, _I, _P, _S]),
     "alg_paged_attn_workspace_size": (_S, [_I, _I, _I, _I, _I, _I, _I]),

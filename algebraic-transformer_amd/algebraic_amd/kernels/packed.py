@@ -95,11 +95,13 @@ class _PackedFn(torch.autograd.Function):
         # The statistic's sign says how a row was computed: its bits are kept as whole numbers, which
         # a hook that stores saved floating tensors in fewer bits leaves as they are.
         stat = torch.empty(N * H, dtype=_I32, device=dev)
+        nbytes = lib.alg_packed_attn_fwd_workspace_size(N, S, H, Hkv, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         p = _lib.ptr
         with _lib.device_of(q):
             _lib.check(lib.alg_packed_attn_fwd(
                 _lib.stream_of(q), N, S, H, Hkv, D, *_strided(q), *_strided(k), *_strided(v), p(cu), p(sink), sink_dtype,
-                count, c, n, p(o), p(stat)), "packed_flash_attention forward")
+                count, c, n, p(o), p(stat), p(ws), nbytes), "packed_flash_attention forward")
         ctx.save_for_backward(q, k, v, cu, sink, o, stat)
         ctx.scale = (n, c)
         ctx.sink_meta = None if sink_logit is None else (sink_logit.shape, sink_logit.dtype, sink_logit.device)
@@ -126,7 +128,7 @@ class _PackedFn(torch.autograd.Function):
         if wants_sink:  # per head in the sink's own type; a shared sink's are added up in f32
             shape, dtype, where = ctx.sink_meta
             dsink = torch.empty(H, dtype=dtype if dtype in _WEIGHTS and sink.numel() == H else _F32, device=dev)
-        nbytes = lib.alg_packed_attn_bwd_workspace_size(N, S, H, Hkv)
+        nbytes = lib.alg_packed_attn_bwd_workspace_size(N, S, H, Hkv, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         p = _lib.ptr
         with _lib.device_of(q):

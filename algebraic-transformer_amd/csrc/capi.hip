@@ -1234,9 +1234,58 @@ static int check_strides(const char* name, const void* base, long ts, long hs, i
   return ALG_OK;
 }
 
+static int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need && (!workspace || bytes < need)) return fail(ALG_ERR_INVALID, "workspace too small: need %zu bytes", need);
+  if (!aligned16({workspace})) return fail(ALG_ERR_INVALID, "workspace must be 16-byte aligned");
+  return ALG_OK;
+}
+
+// Workspace of keys in ranges: [partial sums f32][Z, T f32], `rows` of them over all ranges.
+struct SplitWs {
+  size_t zt, total;
+};
+static SplitWs split_ws(size_t rows, int D) {
+  SplitWs w;
+  w.zt = align256(rows * D * sizeof(float));
+  w.total = w.zt + align256(rows * 2 * sizeof(float));
+  return w;
+}
+
+// In how many ranges the forward and dQ take a row's keys, and dK/dV a key's rows. A causal row's
+// work grows with its position, and a launch ends with its longest item: ranges shorten that where
+// few items (tiles of 128 rows; of 64 keys) leave CUs without another one, as few key heads with
+// long sequences do. No range under six tiles of a sequence of average length. us unsplit, then split
+// as here, the joining launches included: 9000 tokens in 3 sequences, 4 heads over 1, D = 128: forward
+// 95, 82, dQ 141, 110, dK/dV 394, 115; 10025 tokens, 8 heads over 2, D = 64: dK/dV 594, 300; 1475
+// tokens, 3 heads over 1, D = 128: 35, 27 and 50, 32 and 106, 28. More items stay whole, the sooner the
+// shorter the sequences, for the sums' bytes go with the rows alone: forward and dQ of 11652 tokens in
+// 5 sequences, 4 heads, D = 128 (368 items): 70, 81 in two ranges and 97, 108; of 30000 in one, 2 heads
+// over 1 (469): 626, 534 and 875, 737; dK/dV of the former (732) 86, 115, of the latter (469) 1362, 1040.
+struct PackedPlan {
+  int fwd, dq, dkdv;
+};
+static PackedPlan packed_plan(int N, int S, int H, int Hkv) {
+  const auto parts = [](double items, double few, double many, double wanted, double tiles) {
+    const double n = items > (tiles >= 64 ? many : few) ? 1.0 : std::ceil(wanted / items);
+    return (int)std::max(1.0, std::min({n, std::floor(tiles / 6.0), (double)alg::MAX_RANGES}));
+  };
+  const double each = (double)N / std::max(S, 1), G = H / Hkv;
+  PackedPlan pl;
+  pl.fwd = pl.dq = parts(std::ceil(N * G / alg::PK_ROWS) * Hkv, 320, 480, 512, each / alg::PK_BK);
+  pl.dkdv = parts(std::ceil(N / 64.0) * Hkv, 512, 768, 1024, each * G / 64.0);
+  return pl;
+}
+
+size_t alg_packed_attn_fwd_workspace_size(int N, int S, int H, int Hkv, int D) {
+  if (N <= 0 || S < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0) return 0;
+  const int parts = packed_plan(N, S, H, Hkv).fwd;
+  return parts > 1 ? split_ws((size_t)parts * N * H, D).total : 0;
+}
+
 int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                         const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
-                        const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, float* stat) {
+                        const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, float* stat,
+                        void* workspace, size_t workspace_bytes) {
   int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_dtype, sink_count);
   if (rc) return rc;
   if (N == 0) return ALG_OK;
@@ -1246,6 +1295,9 @@ int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D
   if (!rc) rc = check_strides("v", v, v_ts, v_hs, Hkv, D);
   if (!rc) rc = check_strides("o", o, (long)H * D, D, H, D);
   if (rc) return rc;
+  const int parts = packed_plan(N, S, H, Hkv).fwd;
+  const SplitWs ws = parts > 1 ? split_ws((size_t)parts * N * H, D) : SplitWs{0, 0};
+  if ((rc = check_workspace(workspace, workspace_bytes, ws.total))) return rc;
   alg::PackedParams p;
   std::memset(&p, 0, sizeof p);
   p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
@@ -1254,24 +1306,34 @@ int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D
   p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
   p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
   p.sc = attn_scale(n, c, D);
-  p.nsplit = 1;
+  p.nsplit = parts;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_zt = ws.total ? reinterpret_cast<float*>(static_cast<char*>(workspace) + ws.zt) : nullptr;
   return hip_status(alg::launch_packed_fwd(p, D, false, (hipStream_t)stream), "alg_packed_attn_fwd");
 }
 
-// Backward workspace: [- di f32 N H][the slots' forms i32].
+// Backward workspace: [- di f32 N H][the slots' forms i32][the ranges' dQ, dK, dV f32].
 struct PackedBwdWs {
-  size_t care, total;
+  PackedPlan plan;
+  size_t care, dq, dk, dv, total;
 };
-static PackedBwdWs packed_bwd_ws(int N, int S, int H, int Hkv) {
+static PackedBwdWs packed_bwd_ws(int N, int S, int H, int Hkv, int D) {
   PackedBwdWs w;
+  w.plan = packed_plan(N, S, H, Hkv);
+  const auto sums = [&](int parts, int heads) {
+    return parts > 1 ? align256((size_t)parts * N * heads * D * sizeof(float)) : 0;
+  };
   w.care = align256((size_t)N * H * sizeof(float));
-  w.total = w.care + align256((size_t)alg::packed_slots(N, H / Hkv, S, alg::PK_ROWS) * Hkv * sizeof(int));
+  w.dq = w.care + align256((size_t)alg::packed_slots(N, H / Hkv, S, alg::PK_ROWS) * Hkv * sizeof(int));
+  w.dk = w.dq + sums(w.plan.dq, H);
+  w.dv = w.dk + sums(w.plan.dkdv, Hkv);
+  w.total = w.dv + sums(w.plan.dkdv, Hkv);
   return w;
 }
 
-size_t alg_packed_attn_bwd_workspace_size(int N, int S, int H, int Hkv) {
-  if (N <= 0 || S < 0 || H <= 0 || Hkv <= 0 || H % Hkv) return 0;
-  return packed_bwd_ws(N, S, H, Hkv).total;
+size_t alg_packed_attn_bwd_workspace_size(int N, int S, int H, int Hkv, int D) {
+  if (N <= 0 || S < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0) return 0;
+  return packed_bwd_ws(N, S, H, Hkv, D).total;
 }
 
 int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
@@ -1290,16 +1352,20 @@ int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D
   if (!rc) rc = check_strides("v", v, v_ts, v_hs, Hkv, D);
   if (!rc) rc = check_strides("dO", dO, do_ts, do_hs, H, D);
   if (rc) return rc;
-  if (!aligned16({o, dq, dk, dv, workspace})) return fail(ALG_ERR_INVALID, "o, dq, dk, dv and workspace must be 16-byte aligned");
-  const PackedBwdWs ws = packed_bwd_ws(N, S, H, Hkv);
-  if (!workspace || workspace_bytes < ws.total)
-    return fail(ALG_ERR_INVALID, "workspace too small: need %zu bytes", ws.total);
+  if (!aligned16({o, dq, dk, dv})) return fail(ALG_ERR_INVALID, "o, dq, dk and dv must be 16-byte aligned");
+  const PackedBwdWs ws = packed_bwd_ws(N, S, H, Hkv, D);
+  if ((rc = check_workspace(workspace, workspace_bytes, ws.total))) return rc;
   alg::PackedBwdParams p;
   std::memset(&p, 0, sizeof p);
   p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
   p.o = static_cast<const bf16*>(o); p.dO = static_cast<const bf16*>(dO); p.stat = stat;
-  p.ndi = static_cast<float*>(workspace);
-  p.care = reinterpret_cast<int*>(static_cast<char*>(workspace) + ws.care);
+  char* at = static_cast<char*>(workspace);
+  p.ndi = reinterpret_cast<float*>(at);
+  p.care = reinterpret_cast<int*>(at + ws.care);
+  p.dq_parts = ws.plan.dq; p.dkdv_parts = ws.plan.dkdv;
+  p.dq_sum = reinterpret_cast<float*>(at + ws.dq);
+  p.dk_sum = reinterpret_cast<float*>(at + ws.dk);
+  p.dv_sum = reinterpret_cast<float*>(at + ws.dv);
   p.sink = sink; p.sink_count = sink_count; p.sink_bf16 = sink_dtype == ALG_DTYPE_BF16; p.c = c; p.cu = cu;
   p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
   p.do_ts = do_ts; p.do_hs = do_hs;
@@ -1330,33 +1396,47 @@ static int check_table(int width, int page, int pages) {
 // Ranges, the former: at most one workgroup a CU, none under DECODE_RANGE keys of a sequence as long
 // as the table allows. One token over 131001 keys, 4 heads of 128: 64 workgroups 82 us, 128 to 256
 // 47 to 49, 320 60, 512 50; over 8000 keys, 8 heads: 64 20 us, 256 (250 keys each) 14, 512 17.
-// The latter, whose partial sums are 128 rows: two workgroups a CU, ranges of 1024 keys (2100 tokens
-// of 3 requests over 24000 keys, 16 heads over 4: 226 us whole, 2 ranges 200, 4 ranges 210).
+// The latter: the least of what n ranges take by rounds of one workgroup a CU (a second one on the CU
+// takes as much from the first), ceil(workgroups n / 256) / n times 17 ns a key and workgroup, of three
+// quarters of the keys that the table allows, and 6 us and 33 ns a workgroup and range for joining. Measured us of 1 to 6 and 8 ranges: 701 tokens
+// each over 12000, 8000 and 4000 keys, 16 heads over 4 (264 workgroups): 277 237 216 197 194 209 205,
+// takes 4; 645 over 9319, 32 over 4 (164): 182 155 127 144 146 135 152, 3; 300 over 30000, 16 over 4
+// (40): 562 299 209 162 136 119 135, 6; 459 over 12 x 2393, 8 over 1 (348): 84 87 98 99 105 116 134, 1.
 struct PagedPlan {
   int row_tiles;  // 1, 2: 16 or 32 rows (paged_decode); 0: 128 (packed_fwd)
   int nsplit;
-  size_t zt, total;  // workspace: [partial sums f32][Z, T f32]
+  SplitWs ws;
 };
 static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int page) {
   PagedPlan pl;
-  const long G = H / Hkv, rows = N * G, each = (rows + std::max(S, 1) - 1) / std::max(S, 1);
+  const long G = H / Hkv, rows = N * G, seqs = std::max(1, std::min(S, N)), each = (rows + seqs - 1) / seqs;
   pl.row_tiles = each <= 16 ? 1 : (each <= 32 ? 2 : 0);
   const long tile = pl.row_tiles ? 16 * pl.row_tiles : alg::PK_ROWS;
-  const long groups = std::max(1L, std::max((rows + tile - 1) / tile, (long)std::min(S, N)) * Hkv);
-  const long cap = (long)width * page, least = pl.row_tiles ? alg::DECODE_RANGE : 1024;
-  const long most = pl.row_tiles ? std::min(256 / groups, (long)alg::MAX_RANGES) : (512 + groups - 1) / groups;
+  const long groups = seqs * ((each + tile - 1) / tile) * Hkv;
+  const long cap = (long)width * page;
   // Far more sequences than tokens: ranges of mostly empty slots would be a grid too large.
   const long slots = (long)alg::packed_slots(N, (int)G, S, (int)tile) * Hkv;
-  pl.nsplit = (int)std::max(1L, std::min(std::min(most, cap / least), 65536 / slots));
-  const size_t parts = pl.nsplit > 1 ? (size_t)pl.nsplit * N * H : 0;
-  pl.zt = align256(parts * D * sizeof(float));
-  pl.total = pl.zt + align256(parts * 2 * sizeof(float));
+  const long most = std::min({cap / alg::DECODE_RANGE, 65536 / slots, (long)alg::MAX_RANGES});
+  pl.nsplit = 1;
+  if (pl.row_tiles) {
+    pl.nsplit = (int)std::max(1L, std::min(256 / groups, most));
+  } else {
+    double best = INFINITY;
+    for (int n = 1; n <= std::max(1L, std::min(most, 64L)); ++n) {
+      const double us = std::ceil((double)groups * n / 256.0) / n * cap * 0.013 + (n > 1 ? 6.0 + 0.033 * groups * n : 0.0);
+      if (us < best) {
+        best = us;
+        pl.nsplit = n;
+      }
+    }
+  }
+  pl.ws = pl.nsplit > 1 ? split_ws((size_t)pl.nsplit * N * H, D) : SplitWs{0, 0};
   return pl;
 }
 
 size_t alg_paged_attn_workspace_size(int N, int S, int H, int Hkv, int D, int width, int page) {
   if (N <= 0 || S < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || width <= 0 || page <= 0) return 0;
-  return paged_plan(N, S, H, Hkv, D, width, page).total;
+  return paged_plan(N, S, H, Hkv, D, width, page).ws.total;
 }
 
 int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
@@ -1375,9 +1455,7 @@ int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, con
   if (!rc) rc = check_strides("o", o, (long)H * D, D, H, D);
   if (rc) return rc;
   const PagedPlan pl = paged_plan(N, S, H, Hkv, D, width, page);
-  if (pl.total && (!workspace || workspace_bytes < pl.total))
-    return fail(ALG_ERR_INVALID, "workspace too small: need %zu bytes", pl.total);
-  if (!aligned16({workspace})) return fail(ALG_ERR_INVALID, "workspace must be 16-byte aligned");
+  if ((rc = check_workspace(workspace, workspace_bytes, pl.ws.total))) return rc;
   alg::PackedParams p;
   std::memset(&p, 0, sizeof p);
   p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k_pages); p.v = static_cast<const bf16*>(v_pages);
@@ -1390,7 +1468,7 @@ int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, con
   p.sc = attn_scale(n, c, D);
   p.nsplit = pl.nsplit;
   p.part_o = static_cast<float*>(workspace);
-  p.part_zt = pl.total ? reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.zt) : nullptr;
+  p.part_zt = pl.ws.total ? reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.ws.zt) : nullptr;
   return hip_status(pl.row_tiles ? alg::launch_paged_decode(p, D, pl.row_tiles, (hipStream_t)stream)
                                  : alg::launch_packed_fwd(p, D, true, (hipStream_t)stream),
                     "alg_paged_attn");

@@ -49,8 +49,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
 
   const int lane = threadIdx.x & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
-  const int kvh = blockIdx.x % p.Hkv;
-  const PackedSeq f = packed_find<true>(p.cu, p.N, p.S, p.G, PK_ROWS, blockIdx.x / p.Hkv, gridDim.x / p.Hkv);
+  // Workgroups: key head, range of keys, item.
+  const int kvh = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv, range = unit % p.dq_parts;
+  const PackedSeq f = packed_find<true>(p.cu, p.N, p.S, p.G, PK_ROWS, unit / p.dq_parts, gridDim.x / p.Hkv / p.dq_parts);
   const int G = p.G, R = f.len * G, r0 = f.tile * PK_ROWS;
   if (f.tile < 0 || r0 >= R) return;
   const int myr = r0 + wave * 32 + l32;
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   const PackedRow at = packed_row<D>(p, f, kvh, min(myr, R - 1));
   if (f.s == p.S) {  // tokens behind the last sequence
     const bf16x8 z = {};
-    if (live) {
+    if (live && range == 0) {
       for (int d = 8 * h; d < D; d += 16) *reinterpret_cast<bf16x8*>(p.dq + at.out + d) = z;
       if (h == 0) p.ndi[at.stat] = 0.0f;
     }
@@ -67,7 +68,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   const int mytok = live ? at.tok : -1;
   const int posmax = (min(r0 + PK_ROWS, R) - 1) / G;
   const int wave_posmax = min(r0 + wave * 32 + 31, R - 1) / G;
-  const int ntiles = posmax / BK + 1;
+  int kt0 = 0, kt1 = posmax / BK + 1;  // this workgroup's key tiles
+  if (p.dq_parts > 1) {
+    const int per = ceil_div(kt1, p.dq_parts);
+    kt0 = min(range * per, kt1);
+    kt1 = min(kt0 + per, kt1);
+  }
   const int nfull = (r0 / G + 1) / BK;  // tiles before every row's position
 
   const bf16* kbase = p.k + (size_t)kvh * p.k_hs + (size_t)f.start * p.k_ts;
@@ -76,7 +82,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   auto group = [&](int kt) {
     KvGroup g;
     const int key = kt * BK + 16 * wave;
-    g.rows = kt < ntiles ? min(max(f.len - key, 0), 16) : 0;
+    g.rows = kt < kt1 ? min(max(f.len - key, 0), 16) : 0;
     const int k = g.rows > 0 ? key : 0;
     g.k = kbase + (size_t)k * p.k_ts;
     g.v = vbase + (size_t)k * p.v_ts;
@@ -103,7 +109,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   };
 
   {
-    const KvGroup g = group(0);
+    const KvGroup g = group(kt0);
 #pragma unroll
     for (int j = 0; j < PW; ++j) dma(Ks0, Vs0, g, j);
   }
@@ -135,9 +141,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
     di += xor32(di);
   }
   const float rs = live ? p.stat[at.stat] : 0.0f;
-  if (live && h == 0) p.ndi[at.stat] = -di;
+  if (live && h == 0 && range == 0) p.ndi[at.stat] = -di;
   const bool careful = __syncthreads_or(rs < 0.0f) != 0;
-  if (threadIdx.x == 0) p.care[(size_t)packed_slot(f, G, PK_ROWS) * p.Hkv + kvh] = careful;
+  if (threadIdx.x == 0 && range == 0) p.care[(size_t)packed_slot(f, G, PK_ROWS) * p.Hkv + kvh] = careful;
   const int log2n = p.sc.log2n;
   const float b2 = p.sc.b;
   // Plain form: dS = (t^n r) fma(rs^n, dP, - rs^n di), one instruction less than P (dP - di) r.
@@ -267,19 +273,19 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   };
   if (!careful) {
     // In pairs of tiles, as in the forward.
-    const int full = min(nfull, ntiles) & ~1;
-    int kt = 0;
+    const int full = kt0 + (max(min(nfull, kt1) - kt0, 0) & ~1);
+    int kt = kt0;
     for (; kt < full; kt += 2) {
       tile(std::integral_constant<int, 0>{}, std::false_type{}, kt);
       tile(std::integral_constant<int, 1>{}, std::false_type{}, kt + 1);
     }
-    for (; kt < ntiles; kt += 2) {
+    for (; kt < kt1; kt += 2) {
       tile(std::integral_constant<int, 0>{}, std::true_type{}, kt);
-      if (kt + 1 >= ntiles) break;
+      if (kt + 1 >= kt1) break;
       tile(std::integral_constant<int, 1>{}, std::true_type{}, kt + 1);
     }
   } else {
-    for (int kt = 0; kt < ntiles; ++kt) {
+    for (int kt = kt0; kt < kt1; ++kt) {
       __syncthreads();  // every wave is done with the tile before
       const KvGroup g = group(kt);
 #pragma unroll
@@ -314,8 +320,22 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   }
 
   if (mytok >= 0) {
+    const size_t out = packed_row<D>(p, f, kvh, again(r0 + wave * 32 + l32)).out;
+    if (p.dq_parts > 1) {
+      float* DS = p.dq_sum + (size_t)range * p.N * p.H * D + out;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          floatx4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = dqa[db][4 * g + e];
+          *reinterpret_cast<floatx4*>(DS + db * 32 + 8 * g + 4 * h) = v;
+        }
+      return;
+    }
     const float slope = (float)(1 << log2n) * p.sc.qmul;
-    bf16* DQ = p.dq + packed_row<D>(p, f, kvh, again(r0 + wave * 32 + l32)).out;
+    bf16* DQ = p.dq + out;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -386,6 +406,8 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
     }
     item -= G;
   }
+  const int range = item % p.dkdv_parts;  // of the rows, in the order in which they are streamed
+  item /= p.dkdv_parts;
   const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
   // Keys: one row a token; the first keys of a sequence, which the most rows see, are its last tile.
@@ -395,7 +417,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   const size_t dk_base = ((size_t)f.start * p.Hkv + kvh) * D;
   if (f.s == p.S) {  // tokens behind the last sequence
     const bf16x8 z = {};
-    for (int i = threadIdx.x; i < min(PK_KEYS, f.len - k0) * CPR; i += 256) {
+    for (int i = threadIdx.x; range == 0 && i < min(PK_KEYS, f.len - k0) * CPR; i += 256) {
       const size_t at = dk_base + (size_t)(k0 + i / CPR) * p.Hkv * D + 8 * (i % CPR);
       *reinterpret_cast<bf16x8*>(p.dk + at) = z;
       *reinterpret_cast<bf16x8*>(p.dv + at) = z;
@@ -411,6 +433,12 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   const int nq = ceil_div(rows, BQ);
   const int nmask = min(ceil_div((PK_KEYS - 1) * G, BQ), nq);  // tiles with rows before the last key
   const int dead_below = key_in * G;              // rows before this lane's key
+  int q0 = 0, q1 = nq;                            // this workgroup's row tiles, counted from the last rows
+  if (p.dkdv_parts > 1) {
+    const int per = ceil_div(nq, p.dkdv_parts);
+    q0 = min(range * per, nq);
+    q1 = min(q0 + per, nq);
+  }
 
   // Copies of row tile j into LDS in this layout (lane l of an instruction writes 16 bytes at
   // base + 16 l). Row x of the tile is token tb + (rem + x) / G, head (rem + x) % G of the group;
@@ -432,7 +460,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   // 16384 tokens, 16 heads over 4, D = 128: 545 us from the first rows on, 418 us so). The next
   // tile's first token and head are kept up without a division.
   const int step_t = BQ / G, step_h = BQ - step_t * G;
-  int next_r = (nq - 1) * BQ, next_t = next_r / G, next_h = next_r - next_t * G;
+  int next_r = (nq - 1 - q0) * BQ, next_t = next_r / G, next_h = next_r - next_t * G;
   auto source = [&]() {
     const bool some = next_r >= 0;
     const size_t t = some ? next_t : 0;
@@ -639,22 +667,22 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   }
   if (!careful) {
     // In pairs of tiles, as in the forward.
-    const int full = (nq - nmask) & ~1;
-    int qt = 0;
+    const int full = q0 + (max(min(nq - nmask, q1) - q0, 0) & ~1);
+    int qt = q0;
     for (; qt < full; qt += 2) {
       tile(std::integral_constant<int, 0>{}, std::false_type{}, qt);
       tile(std::integral_constant<int, 1>{}, std::false_type{}, qt + 1);
     }
-    for (; qt < nq; qt += 2) {
+    for (; qt < q1; qt += 2) {
       tile(std::integral_constant<int, 0>{}, std::true_type{}, qt);
-      if (qt + 1 >= nq) break;
+      if (qt + 1 >= q1) break;
       tile(std::integral_constant<int, 1>{}, std::true_type{}, qt + 1);
     }
   } else {
-    next_r = (nq - 1) * BQ;
+    next_r = (nq - 1 - q0) * BQ;
     next_t = next_r / G;
     next_h = next_r - next_t * G;
-    for (int qt = 0; qt < nq; ++qt) {
+    for (int qt = q0; qt < q1; ++qt) {
       __syncthreads();  // every wave is done with the tile before
       const Tile now = source();
 #pragma unroll
@@ -692,6 +720,22 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   }
 
   // Register i of d block db holds key 16 wave + 4 g + i, column 16 db + l16.
+  if (p.dkdv_parts > 1) {
+    const size_t sum = (size_t)range * p.N * p.Hkv * D + dk_base;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = k0 + wave * 16 + 4 * g + i;
+      if (key < f.len) {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const size_t o = sum + (size_t)key * p.Hkv * D + 16 * db + l16;
+          p.dk_sum[o] = dk[db][i];
+          p.dv_sum[o] = dv[db][i];
+        }
+      }
+    }
+    return;
+  }
   const float slope = (float)(1 << log2n) * p.sc.qmul;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -707,6 +751,37 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   }
 }
 
+// The ranges' sums in their order, four columns a thread: dQ (dq_parts > 1), then dK and dV. The tokens
+// behind the last sequence have their zeros already.
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedBwdParams p, int D) {
+  const size_t nq = p.dq_parts > 1 ? (size_t)p.N * p.H * D : 0, nk = p.dkdv_parts > 1 ? (size_t)p.N * p.Hkv * D : 0;
+  size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const float* src = p.dq_sum;
+  bf16* out = p.dq;
+  size_t n = nq;
+  int parts = p.dq_parts, heads = p.H;
+  bool scaled = true;
+  if (i >= nq) {
+    i -= nq;
+    scaled = i < nk;
+    if (!scaled) i -= nk;
+    if (i >= nk) return;
+    src = scaled ? p.dk_sum : p.dv_sum;
+    out = scaled ? p.dk : p.dv;
+    n = nk;
+    parts = p.dkdv_parts;
+    heads = p.Hkv;
+  }
+  if ((int)(i / ((size_t)heads * D)) >= packed_start(p.cu, p.S, p.N)) return;
+  floatx4 sum = *reinterpret_cast<const floatx4*>(src + i);
+  for (int r = 1; r < parts; ++r) sum += *reinterpret_cast<const floatx4*>(src + r * n + i);
+  if (scaled) sum *= (float)(1 << p.sc.log2n) * p.sc.qmul;
+  bf16x4 b;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = f2bf(sum[e]);
+  *reinterpret_cast<bf16x4*>(out + i) = b;
+}
+
 static bool packed_aligned(const PackedBwdParams& p, int D) {
   const int rows = 512 / D;  // of a copy instruction
   const auto behind = [&](long ts, long hs) { return (p.G - 1) * hs + D <= ts; };
@@ -717,12 +792,19 @@ template <int D, int L2N>
 static void launch_bwd(const PackedBwdParams& p, hipStream_t st) {
   {
     KTimer t("packed_dq", st);
-    hipLaunchKernelGGL((packed_dq_kernel<D, L2N>), dim3(p.Hkv * packed_slots(p.N, p.G, p.S, PK_ROWS)), dim3(256), 0, st, p);
+    const dim3 grid(p.Hkv * p.dq_parts * packed_slots(p.N, p.G, p.S, PK_ROWS));
+    hipLaunchKernelGGL((packed_dq_kernel<D, L2N>), grid, dim3(256), 0, st, p);
   }
-  KTimer t("packed_dkdv", st);
-  const dim3 grid(p.Hkv * (packed_slots(p.N, 1, p.S, PK_KEYS) + (p.dsink ? p.G : 0)));
-  if (packed_aligned(p, D)) hipLaunchKernelGGL((packed_dkdv_kernel<D, L2N, true>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((packed_dkdv_kernel<D, L2N, false>), grid, dim3(256), 0, st, p);
+  {
+    KTimer t("packed_dkdv", st);
+    const dim3 grid(p.Hkv * (p.dkdv_parts * packed_slots(p.N, 1, p.S, PK_KEYS) + (p.dsink ? p.G : 0)));
+    if (packed_aligned(p, D)) hipLaunchKernelGGL((packed_dkdv_kernel<D, L2N, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((packed_dkdv_kernel<D, L2N, false>), grid, dim3(256), 0, st, p);
+  }
+  const size_t n = (size_t)p.N * D * ((p.dq_parts > 1 ? p.H : 0) + (p.dkdv_parts > 1 ? 2 * p.Hkv : 0));
+  if (n == 0) return;
+  KTimer t("packed_join", st);
+  hipLaunchKernelGGL(packed_join_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, p, D);
 }
 
 hipError_t launch_packed_bwd(const PackedBwdParams& p, int D, hipStream_t st) {

@@ -67,7 +67,7 @@ struct PackedParams {
   int N, S, H, Hkv, G;
   AttnScale sc;
   // Keys in `nsplit` ranges, each with its own partial row: f32 sums of t^n v, then per row Z and
-  // the shift's reciprocal.
+  // the shift's reciprocal (negative: the careful form).
   int nsplit;
   float* part_o;   // (nsplit, Hkv N G, D)
   float* part_zt;  // (nsplit, Hkv N G, 2)
@@ -109,6 +109,11 @@ struct PackedBwdParams {
   int dsink_bf16;
   int N, S, H, Hkv, G;
   AttnScale sc;
+  // dQ's keys and dK/dV's rows in ranges, of which each leaves its f32 sums (1: none; the gradients
+  // themselves are written); packed_join_kernel adds them up.
+  int dq_parts, dkdv_parts;
+  float* dq_sum;              // (dq_parts, N, H, D)
+  float *dk_sum, *dv_sum;     // (dkdv_parts, N, Hkv, D)
 };
 
 // Values formed here whatever is selected of them afterwards: without it the arithmetic of a masked

@@ -389,7 +389,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
       }
     if (h == 0) {
       p.part_zt[2 * part] = Z;
-      p.part_zt[2 * part + 1] = tmax;
+      p.part_zt[2 * part + 1] = careful ? -tmax : tmax;
     }
     return;
   }
@@ -417,91 +417,131 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
 // Rows whose keys were split: o = sum_i f_i O_i / (sum_i f_i Z_i + sink), f_i = (T_i / T)^n with
 // T_i the range's shift and T the largest of them and the sink's; a range without keys for the row
 // has Z_i = 0 and counts for nothing (its sums are not read: they may not be written). The order of
-// the sums is fixed. Latency is all of it, so every load that can be is issued before a result is
-// waited for. WIDE: a workgroup a row, thread i range i, its waves a quarter of the ranges' sums each
-// (16 rows of 64 ranges: 12.7 us by one wave a row, of which launches are about 5). Else, up to 8
-// ranges, a wave a row, every lane all of the ranges' factors.
-template <int D, bool WIDE>
+// the sums is fixed. Every load that can be is issued before a result is waited for.
+struct CombineRow {
+  size_t out, stat;
+  int head;
+  bool held;  // in a sequence: the tokens behind the last one are the first range's workgroups' to write
+};
+__device__ __forceinline__ CombineRow combine_row(const PackedParams& p, int row) {
+  const int tok = row / p.H, head = row - tok * p.H, kvh = head / p.G;
+  return CombineRow{(size_t)row, (size_t)kvh * p.N * p.G + (size_t)tok * p.G + (head - kvh * p.G), head,
+                    tok < packed_start(p.cu, p.S, p.N)};
+}
+__device__ __forceinline__ void combine_stat(const PackedParams& p, size_t at, float Z, float T, bool careful) {
+  const float rs = Z == 0.0f ? 0.0f : inv_root(Z, 1 << p.sc.log2n) / T;
+  p.stat[at] = careful ? -rs : rs;
+}
+
+// Up to RANGES ranges: D / 4 lanes a row, four columns each, every lane all of the ranges' factors.
+// Bytes bound it: 33648 rows of 128 in two ranges, 43 MB, 7 us beside the
+// launch's 5 (16 by a wave a row, whose loads are 8 bytes a lane).
+template <int D, int RANGES>
 __global__ __launch_bounds__(256) void packed_combine_kernel(PackedParams p) {
+  constexpr int LPR = D / 4;
+  const int row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
+  if (row >= p.N * p.H) return;
+  const CombineRow at = combine_row(p, row);
+  if (!at.held) return;
+  const size_t rows = (size_t)p.Hkv * p.N * p.G;
+  const float* O = p.part_o + at.stat * D + col;
+  const int log2n = p.sc.log2n;
+  float2 zt[RANGES];
+  floatx4 o[RANGES];
+#pragma unroll
+  for (int i = 0; i < RANGES; ++i) {
+    const size_t skip = (size_t)min(i, p.nsplit - 1) * rows;
+    zt[i] = *reinterpret_cast<const float2*>(p.part_zt + 2 * (skip + at.stat));
+    o[i] = *reinterpret_cast<const floatx4*>(O + skip * D);
+  }
+  float T = 0.0f, ts = 0.0f;
+  if (p.sink) {
+    float r;
+    T = ts = weight_t_careful(sink_score(p, at.head), p.sc.b, r);
+  }
+  bool careful = false;  // whether a range took that form
+#pragma unroll
+  for (int i = 0; i < RANGES; ++i) {
+    if (i >= p.nsplit) zt[i].x = 0.0f;
+    if (zt[i].x != 0.0f) {
+      T = fmaxf(T, __builtin_fabsf(zt[i].y));
+      careful |= zt[i].y < 0.0f;
+    }
+  }
+  float Z = 0.0f;
+  floatx4 acc = {};
+#pragma unroll
+  for (int i = 0; i < RANGES; ++i)
+    if (zt[i].x != 0.0f) {
+      const float f = pow2n<0>(__builtin_fabsf(zt[i].y) / T, log2n);
+      Z += f * zt[i].x;
+      acc += f * o[i];
+    }
+  if (p.sink) Z += pow2n<0>(ts / T, log2n);
+  if (p.stat && col == 0) combine_stat(p, at.stat, Z, T, careful);
+  const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
+  bf16x4 out;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = f2bf(acc[e] * inv);
+  *reinterpret_cast<bf16x4*>(p.o + at.out * D + col) = out;
+}
+
+// Over 16 ranges, few rows: latency is all of it. A workgroup a row, thread i range i, its waves a
+// quarter of the ranges' sums each (16 rows of 64 ranges: 12.7 us by one wave a row, of which launches
+// are about 5).
+template <int D>
+__global__ __launch_bounds__(256) void packed_combine_wide_kernel(PackedParams p) {
   constexpr int E = D / 64;  // columns a lane
   typedef float fvec __attribute__((ext_vector_type(E)));
   __shared__ float fs[MAX_RANGES], red[2][4];
-  __shared__ fvec part[WIDE ? 4 : 1][64];
+  __shared__ fvec part[4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = WIDE ? blockIdx.x : blockIdx.x * 4 + wave;  // token, head
-  if (row >= p.N * p.H) return;
-  const int tok = row / p.H, head = row - tok * p.H, kvh = head / p.G;
-  const int total = packed_start(p.cu, p.S, p.N);
-  if (tok >= total) return;  // behind the last sequence: zeros, written by the first range's workgroups
+  const CombineRow at = combine_row(p, blockIdx.x);
+  if (!at.held) return;
   const size_t rows = (size_t)p.Hkv * p.N * p.G;
-  const size_t srow = (size_t)kvh * p.N * p.G + (size_t)tok * p.G + (head - kvh * p.G);
-  const float* O = p.part_o + srow * D + lane * E;
+  const float* O = p.part_o + at.stat * D + lane * E;
   const int log2n = p.sc.log2n;
   float T = 0.0f, ts = 0.0f;
   if (p.sink) {
     float r;
-    T = ts = weight_t_careful(sink_score(p, head), p.sc.b, r);
+    T = ts = weight_t_careful(sink_score(p, at.head), p.sc.b, r);
   }
-  float Z;
+  const bool mine = (int)threadIdx.x < p.nsplit;
+  const float2 zt = mine ? *reinterpret_cast<const float2*>(p.part_zt + 2 * (threadIdx.x * rows + at.stat)) : make_float2(0.0f, 0.0f);
+  if (zt.x != 0.0f) T = fmaxf(T, __builtin_fabsf(zt.y));
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) T = fmaxf(T, __shfl_xor(T, m, 64));
+  if (lane == 0) red[0][wave] = T;
+  const bool careful = __syncthreads_or(zt.x != 0.0f && zt.y < 0.0f) != 0;
+  T = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  const float f = zt.x != 0.0f ? pow2n<0>(__builtin_fabsf(zt.y) / T, log2n) : 0.0f;
+  fs[threadIdx.x] = f;
+  float Z = f * zt.x;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) Z += __shfl_xor(Z, m, 64);
+  if (lane == 0) red[1][wave] = Z;
+  __syncthreads();
+  Z = red[1][0] + red[1][1] + red[1][2] + red[1][3];
   fvec acc = 0.0f;
-  if constexpr (WIDE) {
-    const bool mine = (int)threadIdx.x < p.nsplit;
-    const float2 zt = mine ? *reinterpret_cast<const float2*>(p.part_zt + 2 * (threadIdx.x * rows + srow)) : make_float2(0.0f, 0.0f);
-    if (zt.x != 0.0f) T = fmaxf(T, zt.y);
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) T = fmaxf(T, __shfl_xor(T, m, 64));
-    if (lane == 0) red[0][wave] = T;
-    __syncthreads();
-    T = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float f = zt.x != 0.0f ? pow2n<0>(zt.y / T, log2n) : 0.0f;
-    fs[threadIdx.x] = f;
-    Z = f * zt.x;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) Z += __shfl_xor(Z, m, 64);
-    if (lane == 0) red[1][wave] = Z;
-    __syncthreads();
-    Z = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-    for (int i0 = wave; i0 < p.nsplit; i0 += 32) {  // eight ranges' loads in flight
-      fvec o[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        o[k] = *reinterpret_cast<const fvec*>(O + min(i0 + 4 * k, p.nsplit - 1) * rows * D);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float fi = i0 + 4 * k < p.nsplit ? fs[i0 + 4 * k] : 0.0f;
-        if (fi != 0.0f) acc += fi * o[k];
-      }
-    }
-    part[wave][lane] = acc;
-    __syncthreads();
-    if (wave != 0) return;
-    acc = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-  } else {
-    float2 zt[8];
+  for (int i0 = wave; i0 < p.nsplit; i0 += 32) {  // eight ranges' loads in flight
     fvec o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const size_t at = (size_t)min(i, p.nsplit - 1) * rows;
-      zt[i] = *reinterpret_cast<const float2*>(p.part_zt + 2 * (at + srow));
-      o[i] = *reinterpret_cast<const fvec*>(O + at * D);
-    }
+    for (int k = 0; k < 8; ++k)
+      o[k] = *reinterpret_cast<const fvec*>(O + min(i0 + 4 * k, p.nsplit - 1) * rows * D);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= p.nsplit) zt[i].x = 0.0f;
-      if (zt[i].x != 0.0f) T = fmaxf(T, zt[i].y);
+    for (int k = 0; k < 8; ++k) {
+      const float fi = i0 + 4 * k < p.nsplit ? fs[i0 + 4 * k] : 0.0f;
+      if (fi != 0.0f) acc += fi * o[k];
     }
-    Z = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (zt[i].x != 0.0f) {
-        const float f = pow2n<0>(zt[i].y / T, log2n);
-        Z += f * zt[i].x;
-        acc += f * o[i];
-      }
   }
+  part[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0) return;
+  acc = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
   if (p.sink) Z += pow2n<0>(ts / T, log2n);
+  if (p.stat && lane == 0) combine_stat(p, at.stat, Z, T, careful);
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
-  bf16* out = p.o + (size_t)row * D + lane * E;
+  bf16* out = p.o + at.out * D + lane * E;
   if constexpr (E == 2) *reinterpret_cast<unsigned*>(out) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
   else out[0] = f2bf(acc[0] * inv);
 }
@@ -514,9 +554,12 @@ static void launch_fwd(const PackedParams& p, dim3 grid, hipStream_t st) {
 
 template <int D>
 static void launch_combine(const PackedParams& p, hipStream_t st) {
-  const long rows = (long)p.N * p.H;
-  if (p.nsplit > 8) hipLaunchKernelGGL((packed_combine_kernel<D, true>), dim3((unsigned)rows), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((packed_combine_kernel<D, false>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
+  const long rows = (long)p.N * p.H, each = 256 / (D / 4);
+  const dim3 grid((unsigned)((rows + each - 1) / each));
+  if (p.nsplit > 16) hipLaunchKernelGGL(packed_combine_wide_kernel<D>, dim3((unsigned)rows), dim3(256), 0, st, p);
+  else if (p.nsplit > 8) hipLaunchKernelGGL((packed_combine_kernel<D, 16>), grid, dim3(256), 0, st, p);
+  else if (p.nsplit > 2) hipLaunchKernelGGL((packed_combine_kernel<D, 8>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((packed_combine_kernel<D, 2>), grid, dim3(256), 0, st, p);
 }
 
 hipError_t launch_packed_combine(const PackedParams& p, int D, hipStream_t st) {

@@ -356,11 +356,15 @@ int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, 
  * contiguous, bases 16-byte aligned; o, dq, dk, dv are contiguous. sink: (sink_count = 1 or H)
  * logits, f32, or NULL. stat (Hkv N (H / Hkv)) f32: the rows' statistics for the backward pass,
  * which also takes o and dO; dsink (H) f32 = dL/dlogit per head, or NULL. Scores of any size:
- * |q.k| / (sqrt(D) c) up to 2^60 is exact to f32 rounding, without a guard ahead. */
+ * |q.k| / (sqrt(D) c) up to 2^60 is exact to f32 rounding, without a guard ahead. Few heads over
+ * long sequences are split over ranges of keys (dK, dV: of rows), whose f32 sums lie in the workspace
+ * (size 0: it may be NULL). */
+size_t alg_packed_attn_fwd_workspace_size(int N, int S, int H, int Hkv, int D);
 int alg_packed_attn_fwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                         const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
-                        const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, float* stat);
-size_t alg_packed_attn_bwd_workspace_size(int N, int S, int H, int Hkv);
+                        const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, float* stat,
+                        void* workspace, size_t workspace_bytes);
+size_t alg_packed_attn_bwd_workspace_size(int N, int S, int H, int Hkv, int D);
 int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                         const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const int* cu,
                         const void* sink, int sink_dtype, int sink_count, float c, int n, const void* o, const float* stat,

@@ -123,9 +123,9 @@ def test_c_abi_refusals():
     INV, UNS = _lib.ALG_ERR_INVALID, _lib.ALG_ERR_UNSUPPORTED
 
     def fwd(N=8, S=1, H=4, Hkv=2, D=64, q=P(16), q_ts=256, q_hs=64, k_ts=128, k_hs=64, cu=P(16), sink=None, sd=1, ns=0, c=8.0,
-            n=16, o=P(16), stat=P(16)):
+            n=16, o=P(16), stat=P(16), ws=None, bytes_=0):
         return h.alg_packed_attn_fwd(None, N, S, H, Hkv, D, q, q_ts, q_hs, P(16), k_ts, k_hs, P(16), k_ts, k_hs, cu, sink,
-                                     sd, ns, c, n, o, stat)
+                                     sd, ns, c, n, o, stat, ws, bytes_)
 
     fails(fwd(N=-1), INV, "negative")
     fails(fwd(S=-1), INV, "negative")
@@ -153,12 +153,19 @@ def test_c_abi_refusals():
     fails(fwd(q_hs=1 << 29), UNS, "32-bit")
     assert fwd(N=0, q=None, o=None, stat=None) == _lib.ALG_OK
 
+    long = dict(N=4096, H=1, Hkv=1, q_ts=64, k_ts=64)  # one head: its keys go in ranges
+    need = h.alg_packed_attn_fwd_workspace_size(4096, 1, 1, 1, 64)
+    assert need >= 2 * 4096 * 66 * 4 and h.alg_packed_attn_fwd_workspace_size(8, 1, 4, 2, 64) == 0
+    fails(fwd(**long), INV, "workspace too small")
+    fails(fwd(**long, ws=P(16), bytes_=need - 1), INV, "workspace too small")
+    fails(fwd(**long, ws=P(8), bytes_=need), INV, "aligned")
+
     def bwd(ws=P(16), bytes_=1 << 20, dsink=None, sink=None, dq=P(16), do_ts=256):
         return h.alg_packed_attn_bwd(None, 8, 1, 4, 2, 64, P(16), 256, 64, P(16), 128, 64, P(16), 128, 64, P(16), sink, 1, 1, 8.0,
                                      16, P(16), P(16), P(16), do_ts, 64, dq, P(16), P(16), dsink, 1, ws, bytes_)
 
-    need = h.alg_packed_attn_bwd_workspace_size(8, 1, 4, 2)
-    assert need >= 8 * 4 * 4 and h.alg_packed_attn_bwd_workspace_size(8, 1, 5, 2) == 0
+    need = h.alg_packed_attn_bwd_workspace_size(8, 1, 4, 2, 64)
+    assert need >= 8 * 4 * 4 and h.alg_packed_attn_bwd_workspace_size(8, 1, 5, 2, 64) == 0
     fails(bwd(bytes_=need - 1), INV, "workspace too small")
     fails(bwd(ws=None), INV, "workspace too small")
     fails(bwd(ws=P(8)), INV, "aligned")
