@@ -163,11 +163,11 @@ __device__ __forceinline__ int packed_start(const int* cu, int s, int N) {
 // leave the CUs unevenly filled: 8 requests of 8000 keys, 8 heads in 4 ranges, 58 us instead of 47).
 // The tokens behind the last sequence come last.
 struct PackedLanes {
-  int start, len, tiles;  // of the lane's sequence
+  int s, start, len, tiles;  // of the lane's sequence
 };
 __device__ __forceinline__ PackedLanes packed_lanes(const int* cu, int N, int S, int G, int rows) {
   const int lane = threadIdx.x & 63;
-  PackedLanes a{0, 0, 0};
+  PackedLanes a{lane, 0, 0, 0};
   if (lane < S) {
     a.start = packed_start(cu, lane, N);
     a.len = max(packed_start(cu, lane + 1, N) - a.start, 0);
@@ -184,12 +184,34 @@ __device__ __forceinline__ PackedSeq packed_tail(const int* cu, int N, int S, in
   f.tile = tile;
   return f;
 }
-// Item `item` of a launch of `slots` of them: sequence after sequence, or backwards.
+// The lanes' sequences by rising number of keys: over a cache, where a launch is a round or two of
+// workgroups and a sequence's work goes with the keys it holds, not with its tokens. (701 tokens each
+// over 12000, 8000 and 4000 keys, 16 heads over 4, two ranges: 230 us, 178 with the longest first; 459
+// each over 6000 and eleven of 2064 keys, 8 heads over 1: 106, 82. Packed sequences alone, of many more
+// workgroups, gained nothing: nine documents of 16384 tokens 203, 205.)
+__device__ __forceinline__ void packed_sort(PackedLanes& a, int S, const int* kv_lens) {
+  const int lane = threadIdx.x & 63;
+  const int key = lane < S ? kv_lens[lane] : 0;
+  int rank = 0;
+  for (int i = 0; i < S; ++i) {
+    const int k = __builtin_amdgcn_readlane(key, i);
+    rank += k < key || (k == key && i < lane);
+  }
+  if (lane >= S) rank = lane;
+  const int from = __builtin_amdgcn_ds_permute(4 * rank, lane);  // lane `rank` receives this lane
+  a.s = from;
+  a.start = __shfl(a.start, from, 64);
+  a.len = __shfl(a.len, from, 64);
+  a.tiles = __shfl(a.tiles, from, 64);
+}
+// Item `item` of a launch of `slots` of them: sequence after sequence (kv_lens: sorted), or backwards.
 template <bool BACKWARDS>
-__device__ __forceinline__ PackedSeq packed_find(const int* cu, int N, int S, int G, int rows, int item, int slots) {
+__device__ __forceinline__ PackedSeq packed_find(const int* cu, int N, int S, int G, int rows, int item, int slots,
+                                                 const int* kv_lens = nullptr) {
   const int lane = threadIdx.x & 63;
   if (S <= 64) {
-    const PackedLanes a = packed_lanes(cu, N, S, G, rows);
+    PackedLanes a = packed_lanes(cu, N, S, G, rows);
+    if (kv_lens && S > 1) packed_sort(a, S, kv_lens);
     int upto = a.tiles;  // tiles of the sequences up to the lane's
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -200,10 +222,11 @@ __device__ __forceinline__ PackedSeq packed_find(const int* cu, int N, int S, in
     if (item >= total) return packed_tail(cu, N, S, item - total);
     if (BACKWARDS) item = total - 1 - item;
     PackedSeq f;
-    f.s = __builtin_amdgcn_readfirstlane(__popcll(__ballot(upto <= item)));
-    f.start = lane_value(a.start, f.s);
-    f.len = lane_value(a.len, f.s);
-    f.tile = item - lane_value(upto - a.tiles, f.s);
+    const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(upto <= item)));
+    f.s = lane_value(a.s, at);
+    f.start = lane_value(a.start, at);
+    f.len = lane_value(a.len, at);
+    f.tile = item - lane_value(upto - a.tiles, at);
     return f;
   }
   const int slot = BACKWARDS ? slots - 1 - item : item;

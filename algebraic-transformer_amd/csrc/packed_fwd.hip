@@ -37,9 +37,11 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
 
   const int lane = threadIdx.x & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
-  // Workgroups: key head, range of keys, item; a sequence's longest rows first.
+  // Workgroups: key head, range of keys, item; a sequence's longest rows first (over a
+  // cache the longest sequence's).
   const int kvh = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv, range = unit % p.nsplit;
-  const PackedSeq f = packed_find<true>(p.cu, p.N, p.S, p.G, PK_ROWS, unit / p.nsplit, gridDim.x / p.Hkv / p.nsplit);
+  const PackedSeq f = packed_find<true>(p.cu, p.N, p.S, p.G, PK_ROWS, unit / p.nsplit, gridDim.x / p.Hkv / p.nsplit,
+                                        PAGED ? p.kv_lens : nullptr);
   const int G = p.G;
   const int R = f.len * G;           // rows of the sequence
   const int r0 = f.tile * PK_ROWS;   // this workgroup's first row
