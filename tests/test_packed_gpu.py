@@ -94,6 +94,64 @@ def test_scores_outside_the_plain_form(scale, shift, c, sink):
     check(_run(leaves, s, do, cu, 16, c), *packed_ref(*leaves, cu, s, do, n=16, c=c))
 
 
+def _ranges(N, S, H, Hkv, D):
+    """Whether the forward (and dQ), and whether dK/dV of these sizes run over ranges, by the sums
+    that their workspaces hold."""
+    from algebraic_amd import _lib
+    lib = _lib.load()
+    fwd, bwd = lib.alg_packed_attn_fwd_workspace_size(N, S, H, Hkv, D), lib.alg_packed_attn_bwd_workspace_size(N, S, H, Hkv, D)
+    base = lib.alg_packed_attn_bwd_workspace_size(8, 8, H, Hkv, D)
+    sums = max(bwd - base - N * H * 4 - 65536, 0)
+    return fwd > 0, sums >= (2 * N * H * D * 4 if fwd else 0) + 2 * 2 * N * Hkv * D * 4
+
+
+@pytest.mark.parametrize("lens,H,Hkv,D", [([1500], 3, 1, 128), ([1100, 300, 7], 4, 1, 64), ([2100, 1, 0, 900], 2, 2, 64),
+                                          ([2200, 1, 0, 1700], 2, 2, 64), ([400], 16, 1, 128), ([65, 900], 12, 1, 64)])
+@pytest.mark.parametrize("sink,n", [("heads", 16), ("none", 4), ("one", 64)])
+def test_few_heads_in_ranges(lens, H, Hkv, D, sink, n):
+    """Keys and rows split over workgroups, tokens behind the last sequence among them; one on the
+    other side of the rule."""
+    N = sum(lens) + 70
+    assert any(_ranges(N, len(lens), H, Hkv, D)) == (lens != [2100, 1, 0, 900])
+    print(f"[packed] ranges {lens} H{H}/{Hkv} D{D} sink {sink} n {n} {_ranges(N, len(lens), H, Hkv, D)}", flush=True)
+    leaves, s, do, cu = _inputs(lens, H, Hkv, D, tail=70, sink=sink, seed=N)
+    got = _run(leaves, s, do, cu, n, 8.0)
+    for name in ("o", "dq", "dk", "dv"):
+        assert not got[name][-70:].any(), name
+    check(got, *packed_ref(*leaves, cu, s, do, n=n, c=8.0))
+    again = _run(leaves, s, do, cu, n, 8.0)
+    for name in got:
+        assert torch.equal(got[name], again[name]), name
+
+
+@pytest.mark.parametrize("sink", ["none", "heads", "huge"])
+@pytest.mark.parametrize("late", [400.0, -400.0, -30.0])
+def test_ranges_of_both_forms(sink, late):
+    """A row whose first keys have ordinary scores and whose last ones lie outside the plain form (or
+    the other way round): ranges of different forms are joined, and the backward knows it."""
+    leaves, s, do, cu = _inputs([1500], 3, 1, 128, sink="none" if sink == "none" else "heads", seed=17)
+    assert all(_ranges(1500, 1, 3, 1, 128))
+    with torch.no_grad():
+        leaves[0][..., 0], leaves[1][..., 0] = 8.0, 0.0
+        leaves[1][700:1100, :, 0] = late
+        if sink == "huge":
+            s[0], s[1], s[2] = 1e3, -1e3, 300.0
+    print(f"[packed] ranges of both forms, late {late} sink {sink}", flush=True)
+    check(_run(leaves, s, do, cu, 16, 8.0), *packed_ref(*leaves, cu, s, do, n=16, c=8.0))
+
+
+def test_ranges_that_are_not_finite_stay_alone():
+    leaves, s, do, cu = _inputs([1300, 200], 3, 1, 64, seed=18)
+    val, tol = packed_ref(*leaves, cu, s, do, n=16, c=8.0)
+    with torch.no_grad():
+        leaves[1][600] = float("nan")
+        leaves[2][1290] = float("inf")
+    got = _run(leaves, s, do, cu, 16, 8.0)
+    assert not torch.isfinite(got["o"][600:1300]).any()
+    sel = lambda d: {m: d[m][1300:] for m in ("o", "dq", "dk", "dv")}  # noqa: E731
+    check(sel(got), sel(val), sel(tol))
+
+
 @pytest.mark.parametrize("D", [8, 40, 96, 120])
 def test_other_widths(D):
     leaves, s, do, cu = _inputs([70, 33], 4, 2, D, seed=D)
@@ -174,12 +232,13 @@ def test_repeats_are_bit_identical_and_other_streams_agree():
         assert torch.equal(first[name], again[name]) and torch.equal(first[name], third[name]), name
 
 
-def test_one_captured_graph_serves_any_lengths():
-    """Forward and backward captured once for 400 tokens and 5 sequences, replayed for other lengths
+@pytest.mark.parametrize("H,Hkv,N", [(4, 2, 400), (16, 1, 2200)], ids=["whole", "ranges"])
+def test_one_captured_graph_serves_any_lengths(H, Hkv, N):
+    """Forward and backward captured once for N tokens and 5 sequences, replayed for other lengths
     and inputs (one replay with scores outside the plain form) between eager calls."""
-    H, Hkv, D, N = 4, 2, 64, 400
+    D, f = 64, N // 400
     leaves, s, do, _ = _inputs([N], H, Hkv, D, seed=11)
-    cut = torch.tensor([0, 10, 150, 150, 290, 400], dtype=torch.int32, device="cuda")
+    cut = torch.tensor([0, 10, 150, 150, 290 * f, N], dtype=torch.int32, device="cuda")
     op = _op()
 
     def step():
@@ -196,7 +255,7 @@ def test_one_captured_graph_serves_any_lengths():
     with torch.cuda.graph(graph):
         static = step()
     torch.cuda.synchronize()
-    for i, (cu, scale) in enumerate([([0, 10, 150, 150, 290, 400], 1.0), ([0, 0, 0, 399, 400, 400], 30.0),
+    for i, (cu, scale) in enumerate([([0, 10, 150, 150, 290 * f, N], 1.0), ([0, 0, 0, N - 1, N, N], 30.0),
                                      ([0, 80, 160, 240, 320, 321], 1.0)]):
         new = _inputs([N], H, Hkv, D, scale=scale, seed=20 + i)
         with torch.no_grad():
