@@ -1396,12 +1396,15 @@ static int check_table(int width, int page, int pages) {
 // Ranges, the former: at most one workgroup a CU, none under DECODE_RANGE keys of a sequence as long
 // as the table allows. One token over 131001 keys, 4 heads of 128: 64 workgroups 82 us, 128 to 256
 // 47 to 49, 320 60, 512 50; over 8000 keys, 8 heads: 64 20 us, 256 (250 keys each) 14, 512 17.
-// The latter: the least of what n ranges take by rounds of one workgroup a CU (a second one on the CU
-// takes as much from the first), ceil(workgroups n / 256) / n times 17 ns a key and workgroup, of three
-// quarters of the keys that the table allows, and 6 us and 33 ns a workgroup and range for joining. Measured us of 1 to 6 and 8 ranges: 701 tokens
-// each over 12000, 8000 and 4000 keys, 16 heads over 4 (264 workgroups): 277 237 216 197 194 209 205,
-// takes 4; 645 over 9319, 32 over 4 (164): 182 155 127 144 146 135 152, 3; 300 over 30000, 16 over 4
-// (40): 562 299 209 162 136 119 135, 6; 459 over 12 x 2393, 8 over 1 (348): 84 87 98 99 105 116 134, 1.
+// The latter: the n ranges of the least estimate, 17 ns a key and workgroup (a second one on a CU takes as
+// much from the first), 6 us and 33 ns a workgroup and range for joining. One sequence: rounds of equal
+// workgroups, ceil(workgroups n / 256) / n. Several, the longest first: the longest range or the CUs'
+// average, the sequences taken for 0.6 of the table's reach, and a fifth of a range for the end. Three
+// rounds at most, for they may be far shorter. Measured us of 1 to 5 ranges: 701 tokens each over 12000,
+// 8000 and 4000 keys, 16 heads over 4 (264 workgroups): 271 189 199 192 194, takes 2; 300 each over 1000 to
+// 9000, 16 over 4 (240): 178 117 104 106 113, 2; 46 each over 12000 to 40000, 32 over 8 (112): 749 401 290
+// 234 210, 6; 459 each over 12 x 2393, 8 over 1 (348): 87 89 100 103 108, 1; 645 over 9319, 32 over 4 (164):
+// 187 158 129 144 147, 3; 300 over 30000, 16 over 4 (40): 562 300 210 163 137, 119 of 6, 135 of 8, takes 6.
 struct PagedPlan {
   int row_tiles;  // 1, 2: 16 or 32 rows (paged_decode); 0: 128 (packed_fwd)
   int nsplit;
@@ -1422,8 +1425,10 @@ static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int 
     pl.nsplit = (int)std::max(1L, std::min(256 / groups, most));
   } else {
     double best = INFINITY;
-    for (int n = 1; n <= std::max(1L, std::min(most, 64L)); ++n) {
-      const double us = std::ceil((double)groups * n / 256.0) / n * cap * 0.013 + (n > 1 ? 6.0 + 0.033 * groups * n : 0.0);
+    for (int n = 1; n <= std::min({768 / groups, most, 64L}) || n == 1; ++n) {
+      const double load = groups / 256.0;  // workgroups a CU, unsplit
+      const double ranges = seqs == 1 ? std::ceil(load * n) / n : std::max(1.0 / n, 0.6 * load) + 0.2 / n;
+      const double us = 0.017 * cap * ranges + (n > 1 ? 6.0 + 0.033 * groups * n : 0.0);
       if (us < best) {
         best = us;
         pl.nsplit = n;

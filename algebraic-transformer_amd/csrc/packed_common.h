@@ -36,7 +36,7 @@ namespace alg {
 
 constexpr int PK_ROWS = 128;  // rows (token, head of the group) per workgroup of the prompt kernels
 constexpr int PK_BK = 64;     // keys per LDS tile
-constexpr int DECODE_RANGE = 256;  // keys that a range of paged_decode's holds at least
+constexpr int DECODE_RANGE = 256;  // keys that a range holds at least, but for a sequence's last
 constexpr int MAX_RANGES = 256;    // ranges that packed_combine_kernel joins
 
 // How scores become weights for one call (host: attn_scale).

@@ -67,10 +67,18 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   const int posmin = off + r0 / G, posmax = off + rlast / G;
   const int wave_posmax = off + min(r0 + wave * 32 + 31, R - 1) / G;
   int kt0 = 0, kt1 = posmax < 0 ? 0 : posmax / BK + 1;  // this workgroup's key tiles
-  if (p.nsplit > 1) {
-    const int per = ceil_div(kt1, p.nsplit);
+  if (p.nsplit > 1) {  // an equal share, of at least DECODE_RANGE keys
+    const int per = max(ceil_div(kt1, p.nsplit), DECODE_RANGE / BK);
     kt0 = min(range * per, kt1);
     kt1 = min(kt0 + per, kt1);
+    if (kt0 == kt1) {  // no key: only that is written
+      if (live && h == 0) {
+        const size_t part = (size_t)range * p.Hkv * p.N * G + at.stat;
+        p.part_zt[2 * part] = 0.0f;
+        p.part_zt[2 * part + 1] = 1.0f;
+      }
+      return;
+    }
   }
   const int nfull = posmin < 0 ? 0 : (posmin + 1) / BK;  // tiles before every row's position
 
