@@ -3,7 +3,8 @@
 //
 // With P = (t rs)^n, dP = dO V^T, di = sum_d dO o and r = 1/sqrt(s^2 + b) the score gradient is
 // n alpha P (dP - di) / sqrt(1 + x^2) = n 2^-e P (dP - di) r, e the exponent that the queries are
-// scaled by; the factor n 2^-e is applied to the sums. Two launches, without atomics:
+// scaled by; the factor n 2^-e is applied to the sums. Two launches, without atomics (and
+// packed_join, where keys or rows are split over workgroups):
 //   packed_dq    one workgroup = the 128 rows of a forward workgroup: di, then dQ^T += K^T dS^T
 //                over the 64-key tiles up to the diagonal (S^T = K Q^T and dP^T = V dO^T formed
 //                again, dS in registers, K^T read transposed from LDS).
@@ -17,8 +18,15 @@
 // workgroups take the careful form where one of their rows does, and leave that in `care`, one
 // entry per slot and key head, by which a dK/dV workgroup knows whether one of its rows does; the
 // careful form serves either kind of row. Its loops are not pipelined: they are the rare case, and
-// in one loop with the plain form they cost that form registers (192 spilled against 4 in dQ at
+// in one loop with the plain form they cost that form registers (188 more spilled in dQ at
 // D = 128).
+// P and dS are rounded to bf16 for their products, and di is formed of the rounded o: dQ and dK are off by
+// these two and their own rounding, 0.003 of their size in all, dV by P's and its own. Sums are f32.
+// What bounds it: VALU and matrix issue beside waits for spilled registers and copies. Nine documents of
+// 16384 tokens, 16 heads over 4, D = 128: dQ 297 us, 0.81 PFLOP/s (VALU busy 57 % of cycles, matrix cores
+// 43 %), dK/dV 405, 0.79 (53, 48). 13 documents, 8161 tokens, 16 heads, D = 64: 50 and 55 us.
+// dK/dV with 8 waves, the columns of dK and dV split over them, was slower: 436 us (then 418), and 100 for
+// 55 at D = 64.
 #include <type_traits>
 
 #include "launchers.h"
@@ -378,7 +386,8 @@ constexpr int PK_KEYS = 64;  // keys per dK/dV workgroup
 
 // Whether a copy instruction's rows are whole tokens and tokens lie one behind another (ALIGNED, of a
 // group that divides the 8 or 4 rows; host: packed_aligned): a lane's address is then the same in
-// every tile but for a scalar, and rows past the sequence are past the descriptor's end.
+// every tile but for a scalar, and rows past the sequence are past the descriptor's end
+// (404 us at the size above; 424 with each lane's row divided by the group).
 template <int D, int L2N, bool ALIGNED>
 __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kernel(PackedBwdParams p) {
   typedef Dkdv16Lay<D> Lay;
@@ -457,7 +466,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   };
   // The tiles from the last rows to the first: workgroups of one sequence and head that run at the
   // same time then read the same rows, out of the L2, wherever their keys lie (packed documents of
-  // 16384 tokens, 16 heads over 4, D = 128: 545 us from the first rows on, 418 us so). The next
+  // 16384 tokens, 16 heads over 4, D = 128: 545 us from the first rows on, 418 us so then). The next
   // tile's first token and head are kept up without a division.
   const int step_t = BQ / G, step_h = BQ - step_t * G;
   int next_r = (nq - 1 - q0) * BQ, next_t = next_r / G, next_h = next_r - next_t * G;
@@ -751,7 +760,7 @@ __global__ __launch_bounds__(256, packed_dkdv_waves<D>()) void packed_dkdv_kerne
   }
 }
 
-// The ranges' sums in their order, four columns a thread: dQ (dq_parts > 1), then dK and dV. The tokens
+// dQ, dK and dV whose keys or rows were split: the ranges' sums in their order, four columns a thread: dQ (dq_parts > 1), then dK and dV. The tokens
 // behind the last sequence have their zeros already.
 __global__ __launch_bounds__(256) void packed_join_kernel(PackedBwdParams p, int D) {
   const size_t nq = p.dq_parts > 1 ? (size_t)p.N * p.H * D : 0, nk = p.dkdv_parts > 1 ? (size_t)p.N * p.Hkv * D : 0;

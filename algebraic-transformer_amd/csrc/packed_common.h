@@ -258,7 +258,7 @@ __device__ __forceinline__ int packed_slot(const PackedSeq& f, int G, int rows) 
 // sequences, so that the longest work starts first wherever its sequence lies. With f(l) the number
 // of tiles numbered l or more, item i has the largest l with f(l) > i, found by halving. From 65
 // sequences on, packed_find's order backwards. (dK/dV of nine documents, 16384 tokens, 16 heads over
-// 4, D = 128: 454 us, 486 us in packed_find's order; of 13 documents, 8161 tokens, 16 heads, D = 64,
+// 4, D = 128: 454 us then, 486 in packed_find's order; of 13 documents, 8161 tokens, 16 heads, D = 64,
 // which are more workgroups of more equal work: 63 and 60.)
 __device__ __forceinline__ PackedSeq packed_find_heavy(const int* cu, int N, int S, int G, int rows, int item, int slots) {
   if (S > 64) return packed_find<true>(cu, N, S, G, rows, item, slots);

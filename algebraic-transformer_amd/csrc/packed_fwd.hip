@@ -15,7 +15,18 @@
 //   * the rows of a tile end at different positions, so the number of masked tiles is not fixed;
 //   * nothing is known of the scores' range in advance: see the two forms in packed_common.h.
 // With nsplit > 1 the keys of a row are split over workgroups, whose sums are joined by
-// packed_combine_kernel.
+// packed_combine_kernel. The weights are rounded to bf16 for the second product (2^-8 of each, random),
+// sums and O in f32; o is rounded once.
+//
+// What bounds it: a weight takes 8.5 full-rate VALU instructions and one at a quarter of the rate, 50
+// cycles for a wave's 64 scores, of which the two products take 32 (D = 128) or 16 (D = 64) on the matrix
+// cores beside them. 16384 tokens in 3 sequences, 32 heads over 8, D = 128: 850 us, 0.93 PFLOP/s (VALU busy
+// 70 % of cycles, matrix cores 50 %, no LDS bank conflict); nine documents of 16384 tokens, 16 heads over 4:
+// 203 us, 0.79 PFLOP/s (65, 43: more of their tiles are at the diagonal); 13 documents, 8161 tokens, 16
+// heads, D = 64: 38 us. Over a cache, 701 tokens each of 3 requests over 24000 keys, 16 heads over 4: 172 us,
+// 0.77 PFLOP/s, and 12 for joining two ranges.
+// A key head's workgroups are neighbours in steps of Hkv: with 2, 4, 8 key heads each XCD's L2 holds the
+// keys of one, or of the same few, and K and V leave memory about once.
 #include <type_traits>
 
 #include "launchers.h"
