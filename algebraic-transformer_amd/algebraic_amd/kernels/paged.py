@@ -104,8 +104,9 @@ def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, q_g
     tokens; q and k become ``rot(x / rms(x) gain)`` in f32, rounded once, with the tables' row of that
     position (``cos``, ``sin`` (>= width page, D/2) float32, or both None: no rotation) and gains (D,)
     or None. Returns the queries (N, H, D); ``k_pages`` and ``v_pages`` are written in place, one
-    place a token. A token whose position or page number is out of range is not written; its query,
-    and those behind the last sequence, are zero. Two tokens in one place: either is kept.
+    place a token. A token whose position or page number is out of range is not written; queries at
+    such a position, and those behind the last sequence, are zero. Two tokens in one place: either is
+    kept.
     """
     _check_heads(q, k, v)
     (N, H, D), Hkv, dev = q.shape, k.shape[1], q.device
@@ -150,7 +151,7 @@ def paged_flash_attention(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, 
     head ``h // (H // Hkv)``. q's strides as in ``packed_flash_attention``; ``sink_logit`` broadcasts
     to (H,). Tokens behind the last sequence, or before position 0, get zeros. What pages hold behind
     a sequence's end is not read; a page number outside the cache makes the outputs that would have
-    read it NaN. The order of every sum is fixed by the shapes.
+    read it NaN (and may those of tokens before them in the call). The order of every sum is fixed by the shapes.
     """
     if k_pages.dim() != 4:
         raise ValueError("k_pages and v_pages must be (pages, Hkv, page, D)")

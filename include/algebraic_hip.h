@@ -353,9 +353,10 @@ int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, 
  * key head h / (H / Hkv); D in {64, 128}. cu (S + 1) int32 on the device: sequence s is the tokens
  * [cu[s], cu[s+1]), not decreasing, cu[0] = 0, cu[S] <= N; the tokens from cu[S] on get zeros.
  * Strides are in elements between tokens (_ts) and heads (_hs), multiples of 8, the last axis
- * contiguous, bases 16-byte aligned; o, dq, dk, dv are contiguous. sink: (sink_count = 1 or H)
- * logits, f32, or NULL. stat (Hkv N (H / Hkv)) f32: the rows' statistics for the backward pass,
- * which also takes o and dO; dsink (H) f32 = dL/dlogit per head, or NULL. Scores of any size:
+ * contiguous, bases 16-byte aligned; o, dq, dk, dv are contiguous. sink: sink_count = 1 or H
+ * logits of sink_dtype (ALG_DTYPE_F32 or _BF16), or NULL. stat (Hkv N (H / Hkv)) f32: the rows'
+ * statistics for the backward pass, which also takes o and dO; dsink (H) of dsink_dtype =
+ * dL/dlogit per head, or NULL. Scores of any size:
  * |q.k| / (sqrt(D) c) up to 2^60 is exact to f32 rounding, without a guard ahead. Few heads over
  * long sequences are split over ranges of keys (dK, dV: of rows), whose f32 sums lie in the workspace
  * (size 0: it may be NULL). */
@@ -377,8 +378,8 @@ int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D
  * i % page, of k_pages and v_pages (pages, Hkv, page, D) with strides between pages (_ps), heads
  * (_hs) and places (_ts) in any order; page a multiple of 16. What lies in a page behind a
  * sequence's end is not read. A token before position 0 gets zeros; a page number outside
- * [0, pages) is never followed, and makes the outputs that would have read it NaN. Split over
- * ranges of keys where few rows would leave CUs idle; workspace: alg_paged_attn_workspace_size
+ * [0, pages) is never followed, and makes the outputs that would have read it NaN (and may those of
+ * tokens before them in the call). Split over ranges of keys where few rows would leave CUs idle; workspace: alg_paged_attn_workspace_size
  * bytes (0: none). */
 size_t alg_paged_attn_workspace_size(int N, int S, int H, int Hkv, int D, int width, int page);
 int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
@@ -389,9 +390,9 @@ int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, con
 
 /* What precedes it: the new tokens' QK RMS norm with gain and Cayley rotation at their positions
  * (model.py:170-174), y = rot((x tau) gain) in f32 rounded once; queries to q_out (N, H, D)
- * contiguous, rotated keys and the values to their pages. Gains (D) f32 or NULL; cos, sin
+ * contiguous, rotated keys and the values to their pages. Gains (D) of gain_dtype or NULL; cos, sin
  * (table_rows >= width page, D / 2) f32, or both NULL. A token whose position or page number is
- * out of range is not written; behind the last sequence, or out of range, its query is zero. */
+ * out of range is not written; behind the last sequence, or at such a position, its query is zero. */
 int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                      const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
                      long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, int pages, int page,
