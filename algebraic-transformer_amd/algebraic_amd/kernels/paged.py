@@ -128,8 +128,8 @@ def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, q_g
     if not q.is_cuda:
         raise RuntimeError("paged_append needs GPU tensors (no CPU fallback)")
     out = torch.empty((N, H, D), dtype=_BF16, device=dev)
-    if N == 0:
-        return out
+    if N == 0 or S == 0:
+        return out.zero_()
     q, k, v = _rows(q), _rows(k), _rows(v)
     page_table, cu, kv = page_table.contiguous(), cu_seqlens.contiguous(), kv_lens.contiguous()
     gq, gk, gain_dtype = _gains(q_gain, k_gain, dev)
@@ -169,8 +169,8 @@ def paged_flash_attention(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, 
     if not q.is_cuda:
         raise RuntimeError("paged_flash_attention needs GPU tensors (no CPU fallback)")
     o = torch.empty((N, H, D), dtype=_BF16, device=dev)
-    if N == 0:
-        return o
+    if N == 0 or S == 0:
+        return o.zero_()
     lib = _lib.load()
     q = _rows(q)
     page_table, cu, kv = page_table.contiguous(), cu_seqlens.contiguous(), kv_lens.contiguous()

@@ -205,6 +205,24 @@ def test_slices_of_one_projection_and_an_expanded_cotangent():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("D,H,Hkv", [(64, 2, 1), (128, 4, 4)])
+def test_rows_past_32_bit_offsets(D, H, Hkv):
+    """q, k, v and the cotangent as slices of rows of 16 MB: the later tokens lie beyond 2^31 and 2^32
+    bytes."""
+    lens, row = [290, 1, 30], 8 * (1 << 20)
+    leaves, s, do, cu = _inputs(lens, H, Hkv, D, seed=19)
+    wide = torch.empty(sum(lens), row, dtype=torch.bfloat16, device="cuda")
+    views, at = [], row // 2
+    for t in (*leaves, do):
+        n = t[0].numel()
+        views.append(wide[:, at:at + n].unflatten(1, (-1, D)).copy_(t.detach()))
+        at += n
+    print(f"[packed] rows of {row} elements D{D}", flush=True)
+    far = [t.requires_grad_(True) for t in views[:3]]
+    assert far[0].stride(0) == row
+    check(_run(far, s, views[3], cu, 16, 8.0), *packed_ref(*leaves, cu, s, do, n=16, c=8.0))
+
+
 def test_equal_lengths_match_flash_attention():
     """Rows of one length with a key head a query head are flash_attention's, whose own bounds
     are two roundings of its scaled queries wider: both within the float64 statement's."""

@@ -163,6 +163,18 @@ def test_tokens_behind_the_last_sequence():
         assert not o[sum(new):].any()
 
 
+def test_no_sequences_and_no_tokens():
+    q, kp, vp, table, cu, kv, sink, ks, vs = _cache([20], [3], 2, 1, 64, 16, seed=15)
+    append, attend = _ops()
+    k = torch.randn(3, 1, 64, device="cuda").to(BF)
+    was = kp.clone()
+    none = (table[:0], _i32([0]), kv[:0])
+    assert not append(q, k, k, kp, vp, *none).any() and not attend(q, kp, vp, *none, sink).any()
+    assert append(q[:0], k[:0], k[:0], kp, vp, table, _i32([0, 0]), kv).shape == (0, 2, 64)
+    assert attend(q[:0], kp, vp, table, _i32([0, 0]), kv, sink).shape == (0, 2, 64)
+    assert torch.equal(kp.nan_to_num(9.0), was.nan_to_num(9.0))
+
+
 def test_bad_pages_are_not_followed():
     """A page number out of range where a sequence holds keys: its outputs are NaN, others' are not."""
     for new, kv in (([1, 1], [500, 70]), ([90, 1], [300, 300]), ([1, 1], [9000, 100])):
