@@ -153,9 +153,10 @@ def packed_flash_attention(q, k, v, cu_seqlens, sink_logit=None, *, n: int = 16,
     zeros, and zero gradients, so that a captured graph of N tokens serves any lengths. Query head h
     attends over key head ``h // (H // Hkv)``. bfloat16, D up to 128; any strides with a contiguous
     last axis (slices of one projection) are read in place where heads and tokens start on 16 bytes.
-    ``sink_logit`` broadcasts to (H,). Returns (N, H, D). The weights are exact for scores of any
-    size, as ``flash_attention(..., kind="asinh", range_guard=True)``'s are; a value that is not
-    finite reaches the outputs of its own sequence only.
+    ``sink_logit`` broadcasts to (H,). Returns (N, H, D). Scores may have any size, as
+    in ``flash_attention(..., kind="asinh", range_guard=True)``: a weight is right to f32 rounding, or to
+    2^-19 of the row's mean weight where that is more. A value that is not finite reaches the outputs
+    of its own sequence only.
     """
     _check_heads(q, k, v)
     _check_scale(n, c)

@@ -12,7 +12,8 @@
 // lies in [low count, 2^30], low = (R a)^-n the weight at x = -X and count its keys. Above, a weight
 // may have overflowed, or its product with v. Below, the mean key lies under -X, where s + sqrt(s^2
 // + b) cancels: a key at x contributes at most (2/|x|)^n 4 n x^2 eps low of error, 32 eps low at the
-// least n, so that a sum above low count has lost no more than 2^-19 of itself. The sum is all that
+// least n, so that a sum above low count has lost no more than 2^-19 of itself, and a weight no
+// more than 2^-19 of its row's mean one. The sum is all that
 // is looked at, once a row, and nothing per score; if a row fails, its workgroup (or wave) does its
 // rows again in the careful form: a running maximum per row, and rho of a negative x as 1/rho(-x).
 // The row statistic is rs = (row's shift) Z^(-1/n), so that a normalised weight is (t rs)^n in

@@ -357,7 +357,8 @@ int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, 
  * logits of sink_dtype (ALG_DTYPE_F32 or _BF16), or NULL. stat (Hkv N (H / Hkv)) f32: the rows'
  * statistics for the backward pass, which also takes o and dO; dsink (H) of dsink_dtype =
  * dL/dlogit per head, or NULL. Scores of any size:
- * |q.k| / (sqrt(D) c) up to 2^60 is exact to f32 rounding, without a guard ahead. Few heads over
+ * with |q.k| / (sqrt(D) c) up to 2^60 a weight is right to f32 rounding, or to 2^-19 of the row's mean
+ * weight where that is more, without a guard ahead. Few heads over
  * long sequences are split over ranges of keys (dK, dV: of rows), whose f32 sums lie in the workspace
  * (size 0: it may be NULL). */
 size_t alg_packed_attn_fwd_workspace_size(int N, int S, int H, int Hkv, int D);

@@ -5,6 +5,14 @@ The bounds count roundings: u = 2^-8 is the most by which one rounding to bf16 m
 relative to it. The kernels round the weights P, the score gradients dS, the output o (from which
 the backward takes di = sum_d dO o) and their results; everything else is f32, whose share is
 bounded by F32 times the sum of the magnitudes that a result adds up.
+
+Weights of scores far below zero, in a row that the plain form serves: t = s + sqrt(s^2 + b) cancels, so that
+t is off by 4 x^2 2^-24 of itself and w = t^n by n times that, which passes F32 / 2 where n x^2 > 209. There w <=
+a^-n (2 |x|)^-n, and the error is at most a^-n 4 n x^2 (2 |x|)^-n 2^-24: for n = 2 that is 2^-23 a^-2 = 2^-19 low
+(low = (4 a)^-n, the least mean weight of a row of that form); for n = 4, x^2 > 52 it is 256 / 52 2^-24 low, under
+2^-21 low; for larger n (2 |x| / 4)^-n falls faster still (n = 32, low = (2 a)^-n: |x|^-n 128 x^2 2^-24, x^2 > 6.5).
+FAR times the row's mean weight covers it: nothing to o, but to a gradient of a key whose every weight is
+so small it may be much of it.
 """
 
 import math
@@ -13,6 +21,7 @@ import torch
 
 U = 2.0 ** -8
 F32 = 1e-4
+FAR = 2.0 ** -19
 
 
 def rho_log(x):
@@ -39,7 +48,8 @@ def head_ref(q, k, v, sink, do=None, *, n, c, D=None, positions=None):
     p, pb = w / z, wb / z
     o = p @ v
     mag_o = p @ v.abs()
-    tol_o = U * (mag_o + o.abs()) + F32 * mag_o
+    far = torch.where(dead, 0.0, FAR * p.sum(-1, keepdim=True) / (~dead).sum(-1, keepdim=True).clamp(min=1))
+    tol_o = U * (mag_o + o.abs()) + F32 * mag_o + far @ v.abs()
     val, tol = {"o": o}, {"o": tol_o}
     if do is None:
         return val, tol
@@ -49,10 +59,10 @@ def head_ref(q, k, v, sink, do=None, *, n, c, D=None, positions=None):
     f = n * alpha * p * r                        # dS = f (dP - di)
     ds = f * (do @ v.T - di)
     mag_ds = f * (do.abs() @ v.abs().T + (do * o).abs().sum(-1, keepdim=True))
-    tol_ds = U * ds.abs() + f * tol_di + F32 * mag_ds
-    for name, value, far in (("dq", ds @ k, tol_ds @ k.abs()), ("dk", ds.T @ q, tol_ds.T @ q.abs()),
-                             ("dv", p.T @ do, (U + F32) * (p.T @ do.abs()))):
-        val[name], tol[name] = value, far + U * value.abs()
+    tol_ds = U * ds.abs() + f * tol_di + F32 * mag_ds + n * alpha * r * far * ((do @ v.T).abs() + di.abs())
+    for name, value, off in (("dq", ds @ k, tol_ds @ k.abs()), ("dk", ds.T @ q, tol_ds.T @ q.abs()),
+                             ("dv", p.T @ do, (U + F32) * (p.T @ do.abs()) + far.T @ do.abs())):
+        val[name], tol[name] = value, off + U * value.abs()
     if sink is not None:
         rb = n / torch.sqrt(1 + (sink / c) ** 2) / c
         val["dsink"] = -(pb * di).sum() * rb

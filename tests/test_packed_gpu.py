@@ -152,6 +152,15 @@ def test_ranges_that_are_not_finite_stay_alone():
     check(sel(got), sel(val), sel(tol))
 
 
+@pytest.mark.parametrize("n,c", [(2, 0.05), (2, 0.01), (4, 0.05), (8, 0.1), (32, 8.0)])
+def test_rows_of_large_scores_of_both_signs(n, c):
+    """Scores up to hundreds on either side of zero in one row, down to sequences of a few keys: the
+    smallest weights are far below the row's mean."""
+    leaves, s, do, cu = _inputs([1, 2, 3, 5, 8, 70, 200], 2, 2, 128, sink="none", scale=20.0, seed=21)
+    print(f"[packed] both signs n {n} c {c}", flush=True)
+    check(_run(leaves, None, do, cu, n, c), *packed_ref(*leaves, cu, None, do, n=n, c=c))
+
+
 @pytest.mark.parametrize("D", [8, 40, 96, 120])
 def test_other_widths(D):
     leaves, s, do, cu = _inputs([70, 33], 4, 2, D, seed=D)
