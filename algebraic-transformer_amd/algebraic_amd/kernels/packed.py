@@ -21,19 +21,17 @@ _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 def _rows(t):
     """(tokens, heads, D) with a contiguous last axis, strides of whole 16-byte chunks and rows that
-    do not overlap, as the kernels read it; a view of anything else is copied."""
-    ts, hs, one = t.stride()
+    do not overlap, as the kernels read it (a view of anything else is copied); with its pointer and
+    strides (tokens, heads), as the C entry points take them."""
     _, heads, D = t.shape
-    if (one == 1 and not (ts | hs) & 7 and ts >= D and (hs >= D or heads == 1) and not t.data_ptr() & 15 and
+    ts, hs, one = t.stride()
+    at = t.data_ptr()
+    if not (one == 1 and not (ts | hs) & 7 and ts >= D and (hs >= D or heads == 1) and not at & 15 and
             66 * ts + heads * hs + D < 1 << 30):
-        return t
-    return _lib.aligned16(t)
-
-
-def _strided(t):
-    """Pointer and strides (tokens, heads) of a rows tensor, as the C entry points take them."""
-    ts, hs, D = t.stride()[0], t.stride()[1], t.shape[2]
-    return t.data_ptr(), ts, hs if hs >= D else D  # one head: its stride is never used
+        t = _lib.aligned16(t)
+        ts, hs, one = t.stride()
+        at = t.data_ptr()
+    return t, (at, ts, hs if hs >= D else D)  # one head: its stride is never used
 
 
 def _check_scale(n, c):
@@ -88,10 +86,10 @@ class _PackedFn(torch.autograd.Function):
         lib = _lib.load()
         N, H, D = q.shape
         Hkv, S = k.shape[1], cu.shape[0] - 1
-        q, k, v, cu = _rows(q), _rows(k), _rows(v), cu.contiguous()
+        (q, q_at), (k, k_at), (v, v_at), cu = _rows(q), _rows(k), _rows(v), cu.contiguous()
         sink, sink_dtype, count = sink
         dev = q.device
-        o = torch.empty((N, H, D), dtype=_BF16, device=dev)
+        o = q.new_empty(N, H, D)
         # The statistic's sign says how a row was computed: its bits are kept as whole numbers, which
         # a hook that stores saved floating tensors in fewer bits leaves as they are.
         stat = torch.empty(N * H, dtype=_I32, device=dev)
@@ -100,7 +98,7 @@ class _PackedFn(torch.autograd.Function):
         p = _lib.ptr
         with _lib.device_of(q):
             _lib.check(lib.alg_packed_attn_fwd(
-                _lib.stream_of(q), N, S, H, Hkv, D, *_strided(q), *_strided(k), *_strided(v), p(cu), p(sink), sink_dtype,
+                _lib.stream_of(q), N, S, H, Hkv, D, *q_at, *k_at, *v_at, p(cu), p(sink), sink_dtype,
                 count, c, n, p(o), p(stat), p(ws), nbytes), "packed_flash_attention forward")
         ctx.save_for_backward(q, k, v, cu, sink, o, stat)
         ctx.scale = (n, c)
@@ -116,11 +114,9 @@ class _PackedFn(torch.autograd.Function):
         Hkv, S = k.shape[1], cu.shape[0] - 1
         if do.dtype is not _BF16:
             do = do.to(_BF16)
-        do = _rows(do)
+        (q, q_at), (k, k_at), (v, v_at), (do, do_at) = _rows(q), _rows(k), _rows(v), _rows(do)
         dev = q.device
-        dq = torch.empty((N, H, D), dtype=_BF16, device=dev)
-        dk = torch.empty((N, Hkv, D), dtype=_BF16, device=dev)
-        dv = torch.empty((N, Hkv, D), dtype=_BF16, device=dev)
+        dq, dk, dv = q.new_empty(N, H, D), q.new_empty(N, Hkv, D), q.new_empty(N, Hkv, D)
         wants_sink = ctx.sink_meta is not None and ctx.needs_input_grad[4]
         sink_dtype, dsink = 1, None
         if sink is not None:
@@ -133,8 +129,8 @@ class _PackedFn(torch.autograd.Function):
         p = _lib.ptr
         with _lib.device_of(q):
             _lib.check(lib.alg_packed_attn_bwd(
-                _lib.stream_of(q), N, S, H, Hkv, D, *_strided(q), *_strided(k), *_strided(v), p(cu), p(sink), sink_dtype,
-                0 if sink is None else sink.numel(), c, n, p(o), p(stat), *_strided(do), p(dq), p(dk), p(dv), p(dsink),
+                _lib.stream_of(q), N, S, H, Hkv, D, *q_at, *k_at, *v_at, p(cu), p(sink), sink_dtype,
+                0 if sink is None else sink.numel(), c, n, p(o), p(stat), *do_at, p(dq), p(dk), p(dv), p(dsink),
                 1 if dsink is None else _WEIGHTS[dsink.dtype], p(ws), nbytes), "packed_flash_attention backward")
         if wants_sink:
             if sink.numel() != H:

@@ -27,7 +27,19 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .packed import _BF16, _F32, _WEIGHTS, _check_heads, _check_index, _check_scale, _rows, _sink_vector, _strided
+from .packed import _BF16, _F32, _WEIGHTS, _check_heads, _check_index, _check_scale, _rows, _sink_vector
+
+
+def _pages(name, t, Hkv, D, device):
+    """Pointer and strides (pages, heads, places) of a cache's pages, as the C entry points take them."""
+    if t.dtype is not _BF16:
+        raise NotImplementedError(f"dtype {t.dtype}: the gfx950 cache kernels take bfloat16")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    (ps, hs, ts, one), at = t.stride(), t.data_ptr()
+    if one != 1 or (ps | hs | ts) & 7 or ps < D or ts < D or (hs < D and Hkv > 1) or at & 15:
+        raise ValueError(f"{name}: the last axis must be contiguous and the others start on 16 bytes")
+    return at, ps, hs if hs >= D else D, ts
 
 
 def _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv):
@@ -40,16 +52,7 @@ def _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv):
         raise NotImplementedError(f"head_dim {D}: the gfx950 cache kernels are built for 64 and 128")
     if pages == 0 or page == 0 or page % 16:
         raise NotImplementedError(f"{pages} pages of {page} positions: pages hold a positive multiple of 16")
-    args = []
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dtype is not _BF16:
-            raise NotImplementedError(f"dtype {t.dtype}: the gfx950 cache kernels take bfloat16")
-        if t.device != dev:
-            raise ValueError(f"{name} must be on {dev}")
-        (ps, hs, ts, one), at = t.stride(), t.data_ptr()
-        if one != 1 or (ps | hs | ts) & 7 or ps < D or ts < D or (hs < D and Hkv > 1) or at & 15:
-            raise ValueError(f"{name}: the last axis must be contiguous and the others start on 16 bytes")
-        args += (at, ps, hs if hs >= D else D, ts)
+    where = _pages("k_pages", k_pages, Hkv, D, dev) + _pages("v_pages", v_pages, Hkv, D, dev)
     if kv_lens.dim() != 1:
         raise ValueError("kv_lens must be (S,)")
     S = kv_lens.shape[0]
@@ -59,7 +62,7 @@ def _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv):
         raise ValueError(f"page_table must be ({S}, width)")
     width = page_table.shape[1]
     _check_index("page_table", page_table, (S, width), dev)
-    return pages, page, S, width, args
+    return pages, page, S, width, where
 
 
 def _no_gradient(what, *tensors):
@@ -127,17 +130,17 @@ def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, q_g
     _no_gradient("paged_append", q, k, v, k_pages, v_pages, q_gain, k_gain)
     if not q.is_cuda:
         raise RuntimeError("paged_append needs GPU tensors (no CPU fallback)")
-    out = torch.empty((N, H, D), dtype=_BF16, device=dev)
+    out = q.new_empty(N, H, D)
     if N == 0 or S == 0:
         return out.zero_()
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    (q, q_at), (k, k_at), (v, v_at) = _rows(q), _rows(k), _rows(v)
     page_table, cu, kv = page_table.contiguous(), cu_seqlens.contiguous(), kv_lens.contiguous()
     gq, gk, gain_dtype = _gains(q_gain, k_gain, dev)
     cs, sn = _table(cos, dev), _table(sin, dev)
     p = _lib.ptr
     with _lib.device_of(q):
         _lib.check(_lib.load().alg_paged_append(
-            _lib.stream_of(q), N, S, H, Hkv, D, *_strided(q), *_strided(k), *_strided(v), *where, pages, page,
+            _lib.stream_of(q), N, S, H, Hkv, D, *q_at, *k_at, *v_at, *where, pages, page,
             p(page_table), width, p(cu), p(kv), p(gq), p(gk), gain_dtype, p(cs), p(sn), rows, eps, p(out)),
             "paged_append")
     return out
@@ -168,17 +171,17 @@ def paged_flash_attention(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, 
     _no_gradient("paged_flash_attention", q, k_pages, v_pages, sink_logit)
     if not q.is_cuda:
         raise RuntimeError("paged_flash_attention needs GPU tensors (no CPU fallback)")
-    o = torch.empty((N, H, D), dtype=_BF16, device=dev)
+    o = q.new_empty(N, H, D)
     if N == 0 or S == 0:
         return o.zero_()
     lib = _lib.load()
-    q = _rows(q)
+    q, q_at = _rows(q)
     page_table, cu, kv = page_table.contiguous(), cu_seqlens.contiguous(), kv_lens.contiguous()
     nbytes = lib.alg_paged_attn_workspace_size(N, S, H, Hkv, D, width, page)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     p = _lib.ptr
     with _lib.device_of(q):
         _lib.check(lib.alg_paged_attn(
-            _lib.stream_of(q), N, S, H, Hkv, D, *_strided(q), *where, pages, page, p(page_table), width, p(cu), p(kv),
+            _lib.stream_of(q), N, S, H, Hkv, D, *q_at, *where, pages, page, p(page_table), width, p(cu), p(kv),
             p(sink), sink_dtype, count, float(c), int(n), p(o), p(ws), nbytes), "paged_flash_attention")
     return o
