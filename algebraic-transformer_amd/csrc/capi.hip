@@ -1392,7 +1392,10 @@ static int check_table(int width, int page, int pages) {
 
 // How a paged call runs: which kernel, on rows per workgroup, and over how many ranges of keys.
 // Rows: a sequence's average, since the lengths are on the device. Up to 16 or 32 of them take the
-// kernel whose waves split the keys; more, the one whose waves split 128 rows.
+// kernel whose waves split the keys; more, the one whose waves split 128 rows. 32 requests of 4000 keys, 32
+// heads over 4 of 128, us of tiles of 16, 32, 128 rows with their joins: 16 rows each 52 54 63, 32 rows 80 55
+// 63, 40 rows 94 82 64, 128 rows 153 98 73; 64 of 2000, 32 over 8: 16 rows 97 99 111, 32 rows 112 101 112,
+// 48 rows 147 121 114.
 // Ranges, the former: at most one workgroup a CU, none under DECODE_RANGE keys of a sequence as long
 // as the table allows. One token over 131001 keys, 4 heads of 128: 64 workgroups 82 us, 128 to 256
 // 47 to 49, 320 60, 512 50; over 8000 keys, 8 heads: 64 20 us, 256 (250 keys each) 14, 512 17.
