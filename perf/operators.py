@@ -191,19 +191,14 @@ def run(s):
     return _own(s) if own else _plain(s)
 
 
-_ops = []
-
-
 def _own(s):
-    if not _ops:  # a program imports its operators once
-        pkg = str(Path.cwd() / "algebraic-transformer_amd")
-        if pkg not in sys.path:
-            sys.path.insert(0, pkg)
-        from algebraic_amd.kernels.norm import add_rms_norm, add_rms_norm_fp8
-        from algebraic_amd.kernels.packed import packed_flash_attention
-        from algebraic_amd.kernels.paged import paged_append, paged_flash_attention
-        _ops.extend((add_rms_norm, add_rms_norm_fp8, packed_flash_attention, paged_append, paged_flash_attention))
-    add_rms_norm, add_rms_norm_fp8, packed_flash_attention, paged_append, paged_flash_attention = _ops
+    pkg = str(Path.cwd() / "algebraic-transformer_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from algebraic_amd.kernels.norm import add_rms_norm, add_rms_norm_fp8
+    from algebraic_amd.kernels.packed import packed_flash_attention
+    from algebraic_amd.kernels.paged import paged_append, paged_flash_attention
+
     case, kind = s["case"], s["case"]["kind"]
     if kind == "packed":
         o = packed_flash_attention(s["q"], s["k"], s["v"], s["cu"], s["sink"], n=N_EXP, c=C)
