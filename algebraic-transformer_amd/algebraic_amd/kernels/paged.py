@@ -18,7 +18,8 @@ last axis ((pages, page, Hkv, D) storage is a transposed view), page a multiple 
 ``page_table`` (S, width) int32: position i of sequence s lies in page ``page_table[s, i // page]``;
 entries behind a sequence's end are not read, sequences may share pages that are only read.
 ``cu_seqlens`` (S + 1) int32: sequence s's new tokens are ``cu_seqlens[s]:cu_seqlens[s + 1]``.
-``kv_lens`` (S) int32: the keys it holds, the new tokens (its last) among them.
+``kv_lens`` (S) int32: the keys it holds, the new tokens (its last) among them, as many as its row
+of the table reaches (``width page``).
 """
 
 import math
@@ -154,7 +155,9 @@ def paged_flash_attention(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, 
     head ``h // (H // Hkv)``. q's strides as in ``packed_flash_attention``; ``sink_logit`` broadcasts
     to (H,). Tokens behind the last sequence, or before position 0, get zeros. What pages hold behind
     a sequence's end is not read; a page number outside the cache makes the outputs that would have
-    read it NaN (and may those of tokens before them in the call). The order of every sum is fixed by the shapes.
+    read it NaN (and may those of tokens before them in the call). A sequence may outgrow its row of
+    the table: tokens at positions from ``width page`` on, which have no place in it, get NaN, those
+    before are what they would be. The order of every sum is fixed by the shapes.
     """
     if k_pages.dim() != 4:
         raise ValueError("k_pages and v_pages must be (pages, Hkv, page, D)")

@@ -70,14 +70,15 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     return;
   }
 
-  // Keys of the sequence, and the position of its first token among them.
-  const int L = PAGED ? min(max(p.kv_lens[f.s], 0), p.width * p.page) : f.len;
-  const int off = L - f.len;
+  // Keys of the sequence, those that the table reaches, and the position of its first token among them.
+  const int held = PAGED ? max(p.kv_lens[f.s], 0) : f.len;
+  const int L = PAGED ? min(held, p.width * p.page) : held;
+  const int off = held - f.len;
   const int mypos = live ? off + at.tok : -1;
   const int rlast = min(r0 + PK_ROWS, R) - 1;
   const int posmin = off + r0 / G, posmax = off + rlast / G;
   const int wave_posmax = off + min(r0 + wave * 32 + 31, R - 1) / G;
-  int kt0 = 0, kt1 = posmax < 0 ? 0 : posmax / BK + 1;  // this workgroup's key tiles
+  int kt0 = 0, kt1 = posmax < 0 ? 0 : min(posmax, L - 1) / BK + 1;  // this workgroup's key tiles
   if (p.nsplit > 1) {  // an equal share, of at least DECODE_RANGE keys
     const int per = max(ceil_div(kt1, p.nsplit), DECODE_RANGE / BK);
     kt0 = min(range * per, kt1);
@@ -392,7 +393,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   if constexpr (PAGED) {
     if (bad) bad_page = 1;
     __syncthreads();
-    if (bad_page) Z = __builtin_nanf("");
+    if (bad_page || mypos >= L) Z = __builtin_nanf("");  // a position behind the table's end holds no key of its own
   }
   if (!live) return;
   const PackedRow my = packed_row<D>(p, f, kvh, again(r0 + wave * 32 + l32));

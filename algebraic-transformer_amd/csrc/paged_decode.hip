@@ -61,9 +61,9 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
       }
     return;
   }
-  const int L = min(max(p.kv_lens[f.s], 0), p.width * p.page);
-  const int off = L - f.len;
-  const int kend = max(off + (r0 + nrow - 1) / G + 1, 0);  // keys that some row sees: [0, kend)
+  const int held = max(p.kv_lens[f.s], 0), L = min(held, p.width * p.page);  // keys; those that the table reaches
+  const int off = held - f.len;
+  const int kend = min(max(off + (r0 + nrow - 1) / G + 1, 0), L);  // keys that some row sees: [0, kend)
   // This workgroup's blocks of 32 keys: an equal share, of at least DECODE_RANGE keys.
   int b0 = 0, b1 = ceil_div(kend, BLK);
   if (p.nsplit > 1) {
@@ -259,7 +259,8 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
   for (int rt = 0; rt < RT; ++rt) {
     if (g == 0) {
       jT[wave][16 * rt + l16] = T[rt];
-      jZ[wave][16 * rt + l16] = bad ? __builtin_nanf("") : lsum[rt];
+      // A position behind the table's end holds no key of its own.
+      jZ[wave][16 * rt + l16] = bad || mypos[rt] >= L ? __builtin_nanf("") : lsum[rt];
     }
 #pragma unroll
     for (int db = 0; db < NDB; ++db)

@@ -378,10 +378,11 @@ int alg_packed_attn_bwd(alg_stream_t stream, int N, int S, int H, int Hkv, int D
  * kv_lens[s] - (cu[s+1] - cu[s]) + t; position i lies in page table[s width + i / page], place
  * i % page, of k_pages and v_pages (pages, Hkv, page, D) with strides between pages (_ps), heads
  * (_hs) and places (_ts) in any order; page a multiple of 16. What lies in a page behind a
- * sequence's end is not read. A token before position 0 gets zeros; a page number outside
- * [0, pages) is never followed, and makes the outputs that would have read it NaN (and may those of
- * tokens before them in the call). Split over ranges of keys where few rows would leave CUs idle; workspace: alg_paged_attn_workspace_size
- * bytes (0: none). */
+ * sequence's end is not read. A token before position 0 gets zeros; one at a position from
+ * width page on, which the table does not reach, NaN. A page number outside [0, pages) is never
+ * followed, and makes the outputs that would have read it NaN (and may those of tokens before them
+ * in the call). Split over ranges of keys where few rows would leave CUs idle; workspace:
+ * alg_paged_attn_workspace_size bytes (0: none). */
 size_t alg_paged_attn_workspace_size(int N, int S, int H, int Hkv, int D, int width, int page);
 int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                    const void* k_pages, long k_ps, long k_hs, long k_ts, const void* v_pages, long v_ps, long v_hs,

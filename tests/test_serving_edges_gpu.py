@@ -1,0 +1,87 @@
+"""GPU: calls of the packed, paged and residual-norm operators at the edges of what they take, against
+the float64 statement of tests/packed_ref.py."""
+
+import pytest
+
+from packed_ref import check, head_ref
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+def _ops():
+    from algebraic_amd.kernels.paged import paged_append, paged_flash_attention
+    return paged_append, paged_flash_attention
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _starts(new):
+    return [sum(new[:i]) for i in range(len(new) + 1)]
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return lambda *s: torch.randn(*s, device="cuda", generator=g)
+
+
+def _norm(t):
+    return t * (t.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+
+
+def _held(S, width, page, new, H, Hkv, D, seed):
+    """Queries, a cache whose every place is filled, its table, and each sequence's keys and values."""
+    rn = _gen(seed)
+    kp, vp = _norm(rn(S * width, Hkv, page, D)).to(BF), rn(S * width, Hkv, page, D).to(BF)
+    table = rn(S * width).argsort().to(torch.int32).view(S, width)
+    rows = lambda t, s: t[table[s].long()].transpose(1, 2).flatten(0, 1)  # noqa: E731
+    q = _norm(rn(sum(new), H, D)).to(BF)
+    return q, kp, vp, table, 0.3 * rn(H), [rows(kp, s) for s in range(S)], [rows(vp, s) for s in range(S)]
+
+
+def _row(q, k, v, sink, pos, n=16, c=8.0):
+    """One sequence's tokens at `pos` over its keys: value and bound."""
+    val, tol = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    G = q.shape[1] // k.shape[1]
+    for h in range(q.shape[1]):
+        s = None if sink is None else sink[h].double()
+        hv, ht = head_ref(q[:, h].double(), k[:, h // G].double(), v[:, h // G].double(), s, n=n, c=c, positions=pos)
+        val[:, h], tol[:, h] = hv["o"], ht["o"]
+    return {"o": val}, {"o": tol}
+
+
+# A sequence that outgrew its row of the table by `past` positions; another one beside it.
+@pytest.mark.parametrize("new,width,past,H,Hkv", [
+    ([2, 1], 2, 1, 4, 2), ([3, 1], 2, 2, 4, 4), ([1, 1], 3, 1, 4, 2), ([40, 1], 4, 39, 4, 1),
+    ([150, 3], 10, 40, 4, 2), ([150, 3], 11, 150, 4, 2), ([2], 562, 1, 4, 1), ([200], 375, 50, 2, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("sink", [False, True])
+def test_lengths_past_the_table(new, width, past, H, Hkv, D, sink):
+    """Tokens stand where kv_lens puts them: those that the table reaches see every key up to their
+    own, those behind it are NaN, and other sequences are as they were."""
+    page, reach = 16, 16 * width
+    print(f"[edges] {new} tokens, {past} past {reach} positions, H{H}/{Hkv} D{D} sink {sink}", flush=True)
+    q, kp, vp, table, s, ks, vs = _held(len(new), width, page, new, H, Hkv, D, seed=sum(new) + D)
+    s = s if sink else None
+    kv = [reach + past] + [reach - 1] * (len(new) - 1)
+    o = _ops()[1](q, kp, vp, table, _i32(_starts(new)), _i32(kv), s, n=16, c=8.0)
+    torch.cuda.synchronize()
+    inside = new[0] - past
+    assert torch.isnan(o[inside:new[0]]).all()
+    if inside:
+        check({"o": o[:inside]}, *_row(q[:inside], ks[0], vs[0], s, torch.arange(reach - inside, reach, device="cuda")), "inside")
+    for i in range(1, len(new)):
+        at = slice(_starts(new)[i], _starts(new)[i + 1])
+        check({"o": o[at]}, *_row(q[at], ks[i][:kv[i]], vs[i][:kv[i]], s, torch.arange(kv[i] - new[i], kv[i], device="cuda")), "beside")
+
+
+def test_lengths_at_the_largest_number():
+    for new in ([1, 1], [150, 3]):
+        q, kp, vp, table, s, ks, vs = _held(2, 12, 16, new, 4, 2, 64, seed=1)
+        o = _ops()[1](q, kp, vp, table, _i32(_starts(new)), _i32([(1 << 31) - 1, 20]), s, n=16, c=8.0)
+        assert torch.isnan(o[:new[0]]).all() and torch.isfinite(o[new[0]:]).all()
