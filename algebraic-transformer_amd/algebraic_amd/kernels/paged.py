@@ -153,11 +153,12 @@ def paged_flash_attention(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, 
 
     Token t of sequence s attends to positions up to ``kv_lens[s] - new + t``; query head h reads key
     head ``h // (H // Hkv)``. q's strides as in ``packed_flash_attention``; ``sink_logit`` broadcasts
-    to (H,). Tokens behind the last sequence, or before position 0, get zeros. What pages hold behind
-    a sequence's end is not read; a page number outside the cache makes the outputs that would have
-    read it NaN (and may those of tokens before them in the call). A sequence may outgrow its row of
-    the table: tokens at positions from ``width page`` on, which have no place in it, get NaN, those
-    before are what they would be. The order of every sum is fixed by the shapes.
+    to (H,), and -inf switches a head's off. Tokens behind the last sequence, or before position 0, get
+    zeros. What pages hold behind a sequence's end is not read; a page number outside the cache makes
+    the outputs that would have read it NaN (and may those of tokens before them in the call). A
+    sequence may outgrow its row of the table: tokens at positions from ``width page`` on, which have
+    no place in it, get NaN, those before are what they would be. The order of every sum is fixed by
+    the shapes.
     """
     if k_pages.dim() != 4:
         raise ValueError("k_pages and v_pages must be (pages, Hkv, page, D)")

@@ -146,6 +146,12 @@ __device__ __forceinline__ float weight_t_careful(float s, float b, float& r) {
   return s < 0.0f ? b * __builtin_amdgcn_rcpf(u) : u;
 }
 
+// A sink's weight beside the shift T >= ts, its own. A sink of -inf (ts = 0) has none, also where no
+// key gives T another value than 0.
+__device__ __forceinline__ float sink_weight(float ts, float T, int log2n) {
+  return ts == 0.0f ? 0.0f : pow2n<0>(ts / T, log2n);
+}
+
 // Slots of a launch, and the sequence of slot `slot` (S: the tokens behind the last sequence).
 __host__ __device__ inline int packed_slots(int N, int G, int S, int rows) { return (int)((long)N * G / rows) + S + 1; }
 

@@ -499,7 +499,7 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(PackedParams p) {
       Z += f * zt[i].x;
       acc += f * o[i];
     }
-  if (p.sink) Z += pow2n<0>(ts / T, log2n);
+  if (p.sink) Z += sink_weight(ts, T, log2n);
   if (p.stat && col == 0) combine_stat(p, at.stat, Z, T, careful);
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
   bf16x4 out;
@@ -560,7 +560,7 @@ __global__ __launch_bounds__(256) void packed_combine_wide_kernel(PackedParams p
   __syncthreads();
   if (wave != 0) return;
   acc = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-  if (p.sink) Z += pow2n<0>(ts / T, log2n);
+  if (p.sink) Z += sink_weight(ts, T, log2n);
   if (p.stat && lane == 0) combine_stat(p, at.stat, Z, T, careful);
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
   bf16* out = p.o + at.out * D + lane * E;

@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PackedParams p) {
 #pragma unroll
   for (int w = 0; w < WAVES; ++w)
     if (jZ[w][row] != 0.0f) Tm = fmaxf(Tm, jT[w][row]);
-  float Z = sink ? pow2n<0>(ts / Tm, log2n) : 0.0f;
+  float Z = sink ? sink_weight(ts, Tm, log2n) : 0.0f;
   fvec acc = 0.0f;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {

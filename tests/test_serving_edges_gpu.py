@@ -1,9 +1,11 @@
 """GPU: calls of the packed, paged and residual-norm operators at the edges of what they take, against
 the float64 statement of tests/packed_ref.py."""
 
+import math
+
 import pytest
 
-from packed_ref import check, head_ref
+from packed_ref import check, head_ref, packed_ref
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -85,3 +87,41 @@ def test_lengths_at_the_largest_number():
         q, kp, vp, table, s, ks, vs = _held(2, 12, 16, new, 4, 2, 64, seed=1)
         o = _ops()[1](q, kp, vp, table, _i32(_starts(new)), _i32([(1 << 31) - 1, 20]), s, n=16, c=8.0)
         assert torch.isnan(o[:new[0]]).all() and torch.isfinite(o[new[0]:]).all()
+
+
+@pytest.mark.parametrize("new,width", [([1, 1], 4), ([1, 1], 2000), ([1], 8192), ([2, 1], 40), ([60, 40], 4), ([150], 400)],
+                         ids=["whole", "ranges", "many-ranges", "two", "chunks", "chunk-in-ranges"])
+@pytest.mark.parametrize("G", [1, 4])
+def test_a_switched_off_sink_and_rows_without_keys(new, width, G):
+    """A head whose sink is -inf has none: a row that holds no key is zeros there as elsewhere, and
+    other rows are what they are without the sink."""
+    H, D = 2 * G, 64
+    q, kp, vp, table, s, ks, vs = _held(len(new), width, 16, new, H, 2, D, seed=width + G)
+    s[0] = s[-1] = -math.inf
+    cu = _i32(_starts(new))
+    o = _ops()[1](q, kp, vp, table, cu, _i32([0] * len(new)), s, n=16, c=8.0)
+    assert torch.equal(o, torch.zeros_like(o)), (new, width)
+    kv = [new[0] // 2] + [50] * (len(new) - 1)  # the first sequence's earlier tokens lie before position 0
+    o = _ops()[1](q, kp, vp, table, cu, _i32(kv), s, n=16, c=8.0)
+    gone = new[0] - kv[0]
+    assert torch.equal(o[:gone], torch.zeros_like(o[:gone]))
+    for i in range(len(new)):
+        a, b = _starts(new)[i] + (gone if i == 0 else 0), _starts(new)[i + 1]
+        if a < b:
+            pos = torch.arange(kv[i] - (b - a), kv[i], device="cuda")
+            check({"o": o[a:b]}, *_row(q[a:b], ks[i][:kv[i]], vs[i][:kv[i]], s, pos))
+
+
+@pytest.mark.parametrize("lens,H,Hkv,D", [([70, 1], 4, 2, 64), ([1500], 3, 1, 128)])
+def test_a_switched_off_sink_in_packed_rows(lens, H, Hkv, D):
+    from algebraic_amd.kernels.packed import packed_flash_attention
+    rn = _gen(H)
+    N, cu = sum(lens), _starts(lens)
+    for scale in (1.0, 40.0):  # both forms of the weights
+        leaves = [t.to(BF).requires_grad_(True) for t in (_norm(rn(N, H, D)) * scale, _norm(rn(N, Hkv, D)), rn(N, Hkv, D))]
+        do, s = rn(N, H, D).to(BF), 0.3 * rn(H)
+        s[0] = -math.inf
+        s.requires_grad_(True)
+        o = packed_flash_attention(*leaves, _i32(cu), s, n=16, c=8.0)
+        got = dict(zip(("o", "dq", "dk", "dv", "dsink"), (o, *torch.autograd.grad(o, [*leaves, s], do))))
+        check(got, *packed_ref(*leaves, cu, s, do, n=16, c=8.0))
