@@ -177,18 +177,22 @@ __global__ __launch_bounds__(256) void add_rms_norm_kernel(RmsNormParams p) {
       }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-    // Below 2^-100 the quotient would leave the normal numbers: such a row is zeros.
-    const float scale = top > 0x1p-100f ? top * (1.0f / 448.0f) : 1.0f;
-    const float mul = top > 0x1p-100f ? 448.0f / top : 1.0f;
+    // Below 2^-100 the quotients would leave the normal numbers: such a row is zeros.
+    const float scale = top > 0x1p-100f ? top / 448.0f : 1.0f, inv = 1.0f / scale;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int ch = lane + 64 * c;
       if (ch < nch) {
-        // The conversion saturates nothing: |y mul| passes 448 by a rounding at most, and is cut.
+        // y / scale of the scale as it is stored, rounded once before e4m3's own rounding: the product
+        // with the reciprocal, corrected by its exact remainder (Markstein 1990). The product alone put
+        // values next to the border of two e4m3 numbers on the other one (16384 rows of 4096: 107 us, 105
+        // by the product alone, 113 by the division instruction by instruction). The conversion
+        // saturates nothing: |y / scale| passes 448 by a rounding at most, and is cut.
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[e] = s[c][e] * mul;
+          const float q = s[c][e] * inv;
+          v[e] = __builtin_fmaf(__builtin_fmaf(-q, scale, s[c][e]), inv, q);
           v[e] = v[e] > 448.0f ? 448.0f : (v[e] < -448.0f ? -448.0f : v[e]);  // a NaN stays
         }
         int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);

@@ -125,3 +125,29 @@ def test_a_switched_off_sink_in_packed_rows(lens, H, Hkv, D):
         o = packed_flash_attention(*leaves, _i32(cu), s, n=16, c=8.0)
         got = dict(zip(("o", "dq", "dk", "dv", "dsink"), (o, *torch.autograd.grad(o, [*leaves, s], do))))
         check(got, *packed_ref(*leaves, cu, s, do, n=16, c=8.0))
+
+
+# --- the 8-bit norm --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 512, 4096])
+@pytest.mark.parametrize("gain", [False, True])
+def test_eight_bits_are_the_quotient_of_the_stored_scale(d, gain):
+    """y8 = e4m3(y / scale), scale = max|y| / 448, to the bit: whole numbers, whose squares add up
+    without a rounding in any order, and a power-of-two width leave the norm one value."""
+    from algebraic_amd.kernels.norm import add_rms_norm_fp8
+    rn = _gen(d)
+    x, r = ((3 * rn(700, d)).round().to(BF) for _ in range(2))
+    g = (1 + 0.2 * rn(d)) if gain else None
+    y8, scale, s = add_rms_norm_fp8(x, r, g)
+    h = s.cpu().double()
+    assert torch.equal(h, (x.double() + r.double()).cpu())
+    # f32 arithmetic, every step rounded once: the mean square is exact before eps.
+    f32 = lambda t: t.float().double()  # noqa: E731
+    ms = f32(f32((h * h).mean(-1, keepdim=True)) + float(torch.tensor(1e-5)))
+    tau = f32(1.0 / f32(ms.sqrt()))
+    y = f32(h * tau)
+    if gain:
+        y = f32(y * g.cpu().double())
+    want = f32(y.abs().amax(-1, keepdim=True) / 448.0)
+    assert torch.equal(scale.cpu().double(), want)
+    assert torch.equal(y8.cpu().float(), f32(y / want).float().clamp(-448.0, 448.0).to(torch.float8_e4m3fn).float())
