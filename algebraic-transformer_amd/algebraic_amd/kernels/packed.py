@@ -22,16 +22,20 @@ _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 def _rows(t):
     """(tokens, heads, D) with a contiguous last axis, strides of whole 16-byte chunks and rows that
     do not overlap, as the kernels read it (a view of anything else is copied); with its pointer and
-    strides (tokens, heads), as the C entry points take them."""
-    _, heads, D = t.shape
-    ts, hs, one = t.stride()
-    at = t.data_ptr()
-    if not (one == 1 and not (ts | hs) & 7 and ts >= D and (hs >= D or heads == 1) and not at & 15 and
-            66 * ts + heads * hs + D < 1 << 30):
-        t = _lib.aligned16(t)
+    strides (tokens, heads), as the C entry points take them. The stride of an axis of length one
+    says nothing, and contiguous() keeps it: D stands in its place."""
+    tokens, heads, D = t.shape
+    for copied in (False, True):
         ts, hs, one = t.stride()
+        if heads == 1:
+            hs = D
+        if tokens == 1:
+            ts = D
         at = t.data_ptr()
-    return t, (at, ts, hs if hs >= D else D)  # one head: its stride is never used
+        if copied or (one == 1 and not (ts | hs) & 7 and ts >= D and hs >= D and not at & 15 and
+                      66 * ts + heads * hs + D < 1 << 30):
+            return t, (at, ts, hs)
+        t = _lib.aligned16(t)
 
 
 def _check_scale(n, c):

@@ -38,9 +38,13 @@ def _pages(name, t, Hkv, D, device):
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
     (ps, hs, ts, one), at = t.stride(), t.data_ptr()
-    if one != 1 or (ps | hs | ts) & 7 or ps < D or ts < D or (hs < D and Hkv > 1) or at & 15:
+    if t.shape[0] == 1:  # an axis of length one: its stride says nothing
+        ps = D
+    if Hkv == 1:
+        hs = D
+    if one != 1 or (ps | hs | ts) & 7 or ps < D or ts < D or hs < D or at & 15:
         raise ValueError(f"{name}: the last axis must be contiguous and the others start on 16 bytes")
-    return at, ps, hs if hs >= D else D, ts
+    return at, ps, hs, ts
 
 
 def _check_cache(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, Hkv):

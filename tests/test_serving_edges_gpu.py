@@ -127,6 +127,61 @@ def test_a_switched_off_sink_in_packed_rows(lens, H, Hkv, D):
         check(got, *packed_ref(*leaves, cu, s, do, n=16, c=8.0))
 
 
+# --- single tokens ---------------------------------------------------------------------------
+
+def _awkward(t):
+    """(1, heads, D) views of `t`'s values whose token stride means nothing: one element, and more
+    than 32-bit offsets reach."""
+    _, h, D = t.shape
+    one = t.reshape(h, D, 1).permute(2, 0, 1)
+    wide = torch.as_strided(t.contiguous(), (1, h, D), (1 << 28, D, 1))
+    odd = torch.as_strided(t.contiguous(), (1, h, D), (h * D + 4, D, 1))
+    assert one.stride(0) == 1 and torch.equal(one, t)
+    return one, wide, odd
+
+
+def test_one_token_of_any_token_stride():
+    from algebraic_amd.kernels.packed import packed_flash_attention
+    rn = _gen(5)
+    H, Hkv, D = 4, 2, 64
+    q, k, v, do = (rn(1, h, D).to(BF) for h in (H, Hkv, Hkv, H))
+    cu = _i32([0, 1])
+
+    def run(q, k, v, do):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o = packed_flash_attention(*leaves, cu, n=16, c=8.0)
+        return [o, *torch.autograd.grad(o, leaves, do)]
+
+    kp, vp = (rn(4, Hkv, 16, D).to(BF) for _ in range(2))
+    table, kv = _i32([[2, 1]]), _i32([20])
+    want, rows = run(q, k, v, do), _ops()[1](q, kp, vp, table, cu, kv, n=16, c=8.0)
+    wk, wv = kp.clone(), vp.clone()
+    wq = _ops()[0](q, k, v, wk, wv, table, cu, kv)
+    for qa, ka, va, da in zip(*(_awkward(t) for t in (q, k, v, do))):
+        print(f"[edges] one token, strides {qa.stride()}", flush=True)
+        for a, b in zip(run(qa, ka, va, da), want):
+            assert torch.equal(a, b)
+        assert torch.equal(_ops()[1](qa, kp, vp, table, cu, kv, n=16, c=8.0), rows)
+        ck, cv = kp.clone(), vp.clone()
+        assert torch.equal(_ops()[0](qa, ka, va, ck, cv, table, cu, kv), wq)
+        assert torch.equal(ck, wk) and torch.equal(cv, wv)
+
+
+def test_one_page_and_one_head_of_any_stride():
+    """The strides of axes of length one are never used, and not looked at."""
+    rn = _gen(6)
+    q, k = rn(3, 2, 64).to(BF), rn(3, 1, 64).to(BF)
+    kp, vp = (rn(1, 1, 16, 64).to(BF) for _ in range(2))
+    args = (_i32([[0]]), _i32([0, 3]), _i32([13]))
+    want = _ops()[1](q, kp, vp, *args, n=16, c=8.0)
+    odd = [torch.as_strided(t, t.shape, (1, 4, 64, 1)) for t in (kp, vp)]
+    assert torch.equal(_ops()[1](q, *odd, *args, n=16, c=8.0), want)
+    other = [t.clone() for t in (kp, vp)]
+    _ops()[0](q, k, k, *other, *args)
+    _ops()[0](q, k, k, *odd, *args)
+    assert torch.equal(kp, other[0]) and torch.equal(vp, other[1])
+
+
 # --- the 8-bit norm --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("d", [64, 512, 4096])
