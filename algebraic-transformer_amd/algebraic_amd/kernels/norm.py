@@ -17,6 +17,7 @@ import math
 import torch
 
 from .. import _lib
+from .autograd import first_order
 
 
 class _RmsNormFn(torch.autograd.Function):
@@ -115,6 +116,7 @@ class _AddRmsNormFn(torch.autograd.Function):
             dtype, where = ctx.gain_meta
             if dg.dtype is not dtype or where != dg.device:
                 dg = dg.to(device=where, dtype=dtype)
+        dx, dg = first_order("add_rms_norm", s, dx, dg)
         return dx, dx, dg, None
 
 
@@ -150,7 +152,8 @@ def add_rms_norm(x, residual, gain=None, eps: float = 1e-5):
     """``(rms_norm(s, gain), s)`` with ``s = x + residual`` rounded to bfloat16, in one pass.
 
     bfloat16 rows of up to 4096 elements over the last axis; the norm is of the stored s.
-    Differentiable in x, residual (which have the one gradient) and the gain.
+    Differentiable in x, residual (which have the one gradient) and the gain, once: differentiating
+    the norm's gradients raises.
     """
     _check_add(x, residual, gain, eps, "add_rms_norm")
     return _AddRmsNormFn.apply(x, residual, gain, float(eps))

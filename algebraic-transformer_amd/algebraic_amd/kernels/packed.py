@@ -13,6 +13,7 @@ import math
 import torch
 
 from .. import _lib
+from .autograd import first_order
 from .flash import _BUILT_D
 
 
@@ -142,6 +143,7 @@ class _PackedFn(torch.autograd.Function):
             dsink = dsink.reshape(shape)
             if dsink.dtype is not dtype or where != dev:
                 dsink = dsink.to(device=where, dtype=dtype)
+        dq, dk, dv, dsink = first_order("packed_flash_attention", o, dq, dk, dv, dsink)
         return dq, dk, dv, None, dsink, None, None, None
 
 
@@ -156,7 +158,7 @@ def packed_flash_attention(q, k, v, cu_seqlens, sink_logit=None, *, n: int = 16,
     ``sink_logit`` broadcasts to (H,). Returns (N, H, D). Scores may have any size, as
     in ``flash_attention(..., kind="asinh", range_guard=True)``: a weight is right to f32 rounding, or to
     2^-19 of the row's mean weight where that is more. A value that is not finite reaches the outputs
-    of its own sequence only.
+    of its own sequence only. Differentiable once: differentiating the gradients raises.
     """
     _check_heads(q, k, v)
     _check_scale(n, c)

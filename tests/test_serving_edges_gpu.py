@@ -182,6 +182,33 @@ def test_one_page_and_one_head_of_any_stride():
     assert torch.equal(kp, other[0]) and torch.equal(vp, other[1])
 
 
+# --- gradients -------------------------------------------------------------------------------
+
+def test_second_derivatives_are_refused():
+    """The backward passes are kernels without one of their own: a penalty on their results raises,
+    and does not drop its terms, whether or not the cotangent has a gradient."""
+    from algebraic_amd.kernels.norm import add_rms_norm
+    from algebraic_amd.kernels.packed import packed_flash_attention
+    rn = _gen(7)
+    q, k, v = (rn(5, h, 64).to(BF).requires_grad_(True) for h in (2, 1, 1))
+    s, gain = rn(2).requires_grad_(True), rn(64).requires_grad_(True)
+    x, r = (rn(5, 64).to(BF).requires_grad_(True) for _ in range(2))
+    for call, leaves in ((lambda: packed_flash_attention(q, k, v, _i32([0, 5]), s), (q, k, v, s)),
+                         (lambda: add_rms_norm(x, r, gain)[0], (x, r, gain))):
+        for loss in (lambda o: o.float().square().sum(), lambda o: o.sum()):
+            once = torch.autograd.grad(loss(call()), leaves)
+            grads = torch.autograd.grad(loss(call()), leaves, create_graph=True)
+            for leaf, a, b in zip(leaves, once, grads):
+                assert torch.equal(a, b.detach())
+                with pytest.raises(RuntimeError, match="no second derivative"):
+                    torch.autograd.grad(b.float().square().sum() + leaf.float().square().sum(), leaf, retain_graph=True)
+    # The stream's own gradient is what came in, differentiable as ever.
+    y, h = add_rms_norm(x, r, gain)
+    (g,) = torch.autograd.grad(h.float().square().sum(), x, create_graph=True)
+    (gg,) = torch.autograd.grad(g.float().sum(), x)
+    assert torch.equal(gg, torch.full_like(gg, 2.0))
+
+
 # --- the 8-bit norm --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("d", [64, 512, 4096])
