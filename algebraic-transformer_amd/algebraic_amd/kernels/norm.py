@@ -144,6 +144,8 @@ def _check_add(x, residual, gain, eps, what):
         raise ValueError("eps must be positive and finite")
     if d == 0 or d % 8 or d > 4096:
         raise NotImplementedError(f"rows of {d}: the gfx950 norm takes multiples of 8 up to 4096")
+    if x.numel() // d > (1 << 26) - 4:
+        raise NotImplementedError(f"{x.numel() // d} rows: at most 2^26 - 4 in one launch")
     if not x.is_cuda:
         raise RuntimeError(f"{what} needs GPU tensors (no CPU fallback)")
 

@@ -1128,6 +1128,12 @@ int alg_head_bwd_streamed(alg_stream_t stream, int dtype, int N, int d, int V, c
 
 // ---- residual norm ----------------------------------------------------------------------------
 
+// One wave a row in workgroups of four, whose threads a launch counts in 32 bits.
+static int check_add_norm(int rows, int d, float eps) {
+  if (rows > (1 << 26) - 4) return fail(ALG_ERR_UNSUPPORTED, "%d rows: at most 2^26 - 4 in one launch", rows);
+  return check_rms_norm(rows, d, eps);
+}
+
 static alg::RmsNormParams add_norm_params(int rows, int d, const void* x, const void* res, const void* gain,
                                           int gain_dtype, float eps, void* sum) {
   alg::RmsNormParams p;
@@ -1141,7 +1147,7 @@ static alg::RmsNormParams add_norm_params(int rows, int d, const void* x, const 
 
 int alg_add_rms_norm_fwd(alg_stream_t stream, int rows, int d, const void* x, const void* res, const void* gain,
                          int gain_dtype, float eps, void* sum, void* y, float* tau) {
-  const int rc = check_rms_norm(rows, d, eps);
+  const int rc = check_add_norm(rows, d, eps);
   if (rc) return rc;
   if (!x || !res || !sum || !y || !tau) return fail(ALG_ERR_INVALID, "x, res, sum, y and tau are required");
   if (gain && !is_weight_dtype(gain_dtype)) return fail(ALG_ERR_INVALID, "gain must be bf16 or f32");
@@ -1153,7 +1159,7 @@ int alg_add_rms_norm_fwd(alg_stream_t stream, int rows, int d, const void* x, co
 
 int alg_add_rms_norm_fp8(alg_stream_t stream, int rows, int d, const void* x, const void* res, const void* gain,
                          int gain_dtype, float eps, void* sum, void* y8, float* scale) {
-  const int rc = check_rms_norm(rows, d, eps);
+  const int rc = check_add_norm(rows, d, eps);
   if (rc) return rc;
   if (!x || !res || !sum || !y8 || !scale) return fail(ALG_ERR_INVALID, "x, res, sum, y8 and scale are required");
   if (gain && !is_weight_dtype(gain_dtype)) return fail(ALG_ERR_INVALID, "gain must be bf16 or f32");
@@ -1209,11 +1215,10 @@ static int check_packed(int N, int S, int H, int Hkv, int D, float c, int n, con
   if (H <= 0 || Hkv <= 0 || H % Hkv) return fail(ALG_ERR_INVALID, "H = %d must be a positive multiple of Hkv = %d", H, Hkv);
   if (D != 64 && D != 128) return fail(ALG_ERR_UNSUPPORTED, "head_dim %d: gfx950 kernels are built for D in {64, 128}", D);
   if (H / Hkv > 128) return fail(ALG_ERR_UNSUPPORTED, "%d query heads to a key head: at most 128", H / Hkv);
-  // Rows are counted in 32 bits, and so are a grid's workgroups (a slot and key head each) and their
-  // threads.
-  if ((double)N * H >= 2147483648.0 - 1024.0) return fail(ALG_ERR_UNSUPPORTED, "N H = %d %d rows: at most 2^31 - 1024", N, H);
+  // A launch's threads are counted in 32 bits: workgroups of 256, one a slot of at least 16 rows and key
+  // head. Rows stay under 2^28 so.
   if (((double)N * H / 16.0 + (S + 1.0) * Hkv + H) * 256.0 >= 4294967296.0)
-    return fail(ALG_ERR_UNSUPPORTED, "too many rows and sequences for one launch");
+    return fail(ALG_ERR_UNSUPPORTED, "too many rows and sequences for one launch: N H / 16 + (S + 1) Hkv + H must stay under 2^24");
   if (const int rc = check_n(n)) return rc;
   if (!(c > 0.0f) || !std::isfinite(c)) return fail(ALG_ERR_INVALID, "asinh scale c must be positive and finite");
   if (c < 0x1p-30f || c > 0x1p30f) return fail(ALG_ERR_UNSUPPORTED, "asinh scale c = %g: built for 2^-30 to 2^30", (double)c);
@@ -1495,6 +1500,7 @@ int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, c
   if (!cos != !sin) return fail(ALG_ERR_INVALID, "cos and sin are given together");
   if (cos && (long)table_rows < (long)width * page)
     return fail(ALG_ERR_INVALID, "rotation tables of %d rows for %ld positions", table_rows, (long)width * page);
+  if (N >= 1 << 24) return fail(ALG_ERR_UNSUPPORTED, "%d tokens: a workgroup each, fewer than 2^24 in one launch", N);
   if (N == 0) return ALG_OK;
   if (!q || !k || !v || !k_pages || !v_pages || !q_out || !table || !kv_lens) return fail(ALG_ERR_INVALID, "null argument");
   rc = check_strides("q", q, q_ts, q_hs, H, D);

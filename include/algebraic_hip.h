@@ -337,8 +337,8 @@ int alg_head_bwd_streamed(alg_stream_t stream, int dtype, int N, int d, int V,
  * alg_rms_norm's y and tau of sum (bf16), or y in 8 bits: y8 = e4m3(y / scale) of the unrounded y,
  * scale (rows) f32 = max|y| / 448 (1 for rows without a value above 2^-100). Backward: dx, the
  * gradient of x and of res alike, = round(dx of the norm + dsum), dsum (the cotangent of sum) may
- * be NULL; dgain and workspace as in alg_rms_norm_bwd. Same sizes and alignment as alg_rms_norm;
- * gain 16-byte aligned. No counterpart in the reference, whose compiler fuses the addition
+ * be NULL; dgain and workspace as in alg_rms_norm_bwd. Same sizes (rows at most 2^26 - 4) and
+ * alignment as alg_rms_norm; gain 16-byte aligned. No counterpart in the reference, whose compiler fuses the addition
  * (src/algebraic/model.py:182-193). */
 int alg_add_rms_norm_fwd(alg_stream_t stream, int rows, int d, const void* x, const void* res, const void* gain,
                          int gain_dtype, float eps, void* sum, void* y, float* tau);

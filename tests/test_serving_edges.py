@@ -1,6 +1,8 @@
 """CPU: what the packed, paged and residual-norm entry points make of calls at the edges of what they
 take, before anything is launched."""
 
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -43,3 +45,28 @@ def test_one_page_and_one_head_have_any_stride():
         assert at == t.data_ptr() and all(x >= 64 and x % 8 == 0 for x in strides) and strides[2] == 64
     with pytest.raises(ValueError, match="contiguous"):
         _pages("k_pages", torch.as_strided(t, t.shape, (1024, 1024, 60, 1)), 1, 64, t.device)
+
+
+def test_sizes_past_one_launch_are_refused():
+    """A launch has fewer than 2^32 threads: said before anything runs, and no count wraps at 2^32."""
+    from algebraic_amd import _lib
+    from algebraic_amd.kernels.norm import add_rms_norm, add_rms_norm_fp8
+    h, P = _lib.load(), ctypes.c_void_p(16)
+
+    def unsupported(rc, text):
+        assert rc == _lib.ALG_ERR_UNSUPPORTED and text.encode() in h.alg_last_error(), (rc, h.alg_last_error())
+
+    def append(N):
+        return h.alg_paged_append(None, N, 1, 1, 1, 64, P, 64, 64, P, 64, 64, P, 64, 64, P, 1024, 1024, 64, P, 1024, 1024, 64,
+                                  4, 16, P, 2, P, P, None, None, 1, None, None, 0, 1e-5, P)
+
+    for N in (1 << 24, 1 << 27):
+        unsupported(append(N), "tokens")
+    for rows in ((1 << 26) - 3, 1 << 26, (1 << 31) - 1):
+        unsupported(h.alg_add_rms_norm_fwd(None, rows, 64, P, P, None, 1, 1e-5, P, P, P), "rows")
+        unsupported(h.alg_add_rms_norm_fp8(None, rows, 64, P, P, None, 1, 1e-5, P, P, P), "rows")
+    for rows in (1 << 26, (1 << 32) + 5):
+        x = torch.empty(rows, 8, dtype=BF, device="meta")
+        for op in (add_rms_norm, add_rms_norm_fp8):
+            with pytest.raises(NotImplementedError, match="rows"):
+                op(x, x)
