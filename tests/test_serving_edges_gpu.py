@@ -233,3 +233,102 @@ def test_eight_bits_are_the_quotient_of_the_stored_scale(d, gain):
     want = f32(y.abs().amax(-1, keepdim=True) / 448.0)
     assert torch.equal(scale.cpu().double(), want)
     assert torch.equal(y8.cpu().float(), f32(y / want).float().clamp(-448.0, 448.0).to(torch.float8_e4m3fn).float())
+
+
+# --- more than 64 sequences in ranges --------------------------------------------------------
+
+def _cached(kv, new, H, Hkv, D, seed):
+    """As _held, with kv_lens `kv`; and whether the call runs over ranges of keys."""
+    from algebraic_amd import _lib
+    width = -(-max(kv) // 16)
+    q, kp, vp, table, s, ks, vs = _held(len(kv), width, 16, new, H, Hkv, D, seed)
+    ranges = _lib.load().alg_paged_attn_workspace_size(sum(new), len(kv), H, Hkv, D, width, 16) > 0
+    want = {"o": torch.zeros(q.shape, dtype=torch.float64, device="cuda")}
+    tol = {"o": torch.zeros_like(want["o"])}
+    for i, m in enumerate(new):
+        at = slice(_starts(new)[i], _starts(new)[i + 1])
+        v, t = _row(q[at], ks[i][:kv[i]], vs[i][:kv[i]], s, torch.arange(kv[i] - m, kv[i], device="cuda"))
+        want["o"][at], tol["o"][at] = v["o"], t["o"]
+    return (q, kp, vp, table, _i32(_starts(new)), _i32(kv), s), ranges, want, tol
+
+
+@pytest.mark.parametrize("S", [65, 100])
+def test_single_tokens_of_many_sequences_in_ranges(S):
+    kv = [1000 + (811 * i) % 2000 for i in range(S)]
+    kv[3] = 1  # ranges without a key
+    args, ranges, want, tol = _cached(kv, [1] * S, 2, 1, 64, seed=S)
+    assert ranges
+    print(f"[edges] {S} single tokens in ranges", flush=True)
+    check({"o": _ops()[1](*args, n=16, c=8.0)}, want, tol)
+
+
+@pytest.mark.parametrize("S,H,Hkv,D", [(66, 2, 1, 64), (70, 2, 1, 128)])
+def test_chunks_of_many_sequences_in_ranges(S, H, Hkv, D):
+    new = [40 + i % 11 for i in range(S)]
+    kv = [300 + (277 * i) % 1200 for i in range(S)]
+    kv[5] = new[5]
+    args, ranges, want, tol = _cached(kv, new, H, Hkv, D, seed=S)
+    assert ranges
+    print(f"[edges] {S} chunks in ranges", flush=True)
+    check({"o": _ops()[1](*args, n=16, c=8.0)}, want, tol)
+
+
+@pytest.mark.parametrize("sink", [False, True])
+def test_packed_sequences_in_ranges_past_64(sink):
+    from algebraic_amd import _lib
+    from algebraic_amd.kernels.packed import packed_flash_attention
+    H, Hkv, D = 16, 1, 64
+    lens = [50 + (13 * i) % 21 for i in range(66)]
+    N, cu = sum(lens) + 9, _starts(lens)
+    base = _lib.load().alg_packed_attn_bwd_workspace_size(N, N, H, Hkv, D)  # short ones: no ranges, more slots
+    assert _lib.load().alg_packed_attn_bwd_workspace_size(N, 66, H, Hkv, D) >= base + 2 * N * Hkv * D * 4
+    rn = _gen(66)
+    leaves = [t.to(BF).requires_grad_(True) for t in (_norm(rn(N, H, D)), _norm(rn(N, Hkv, D)), rn(N, Hkv, D))]
+    do, s = rn(N, H, D).to(BF), (0.3 * rn(H)).requires_grad_(True) if sink else None
+    print("[edges] 66 packed sequences in ranges", flush=True)
+    o = packed_flash_attention(*leaves, _i32(cu), s, n=16, c=8.0)
+    wrt = [*leaves] + ([s] if sink else [])
+    got = dict(zip(("o", "dq", "dk", "dv", "dsink"), (o, *torch.autograd.grad(o, wrt, do))))
+    for name in ("o", "dq", "dk", "dv"):
+        assert not got[name][-9:].any(), name
+    check(got, *packed_ref(*leaves, cu, s, do, n=16, c=8.0))
+
+
+# --- captured steps --------------------------------------------------------------------------
+
+def test_captured_steps_write_the_cache_themselves():
+    """Append and attention captured once; before each replay the new tokens' places hold something
+    else than the eager step wrote there."""
+    append, attend = _ops()
+    rn = _gen(8)
+    table = rn(60).argsort().to(torch.int32).view(3, 20)
+    kp, vp = (rn(60, 2, 16, 64).to(BF) for _ in range(2))
+    q, k, v = rn(3, 4, 64).to(BF), rn(3, 2, 64).to(BF), rn(3, 2, 64).to(BF)
+    cu, kv, s = _i32([0, 1, 2, 3]), _i32([30, 200, 47]), 0.3 * rn(4)
+
+    def step():
+        return attend(append(q, k, v, kp, vp, table, cu, kv), kp, vp, table, cu, kv, s, n=16, c=8.0)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    torch.cuda.synchronize()
+    for i in range(4):
+        for t in (q, k, v):
+            t.copy_(rn(*t.shape))
+        kv += 1
+        before = kp.clone(), vp.clone()
+        want, wk, wv = step(), kp.clone(), vp.clone()
+        assert not torch.equal(wk, before[0]) and not torch.equal(wv, before[1])
+        kp.copy_(before[0]), vp.copy_(before[1])
+        torch.cuda.synchronize()
+        print(f"[edges] replay {i}", flush=True)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(kp, wk) and torch.equal(vp, wv), i
