@@ -20,8 +20,11 @@
 // careful form serves either kind of row. Its loops are not pipelined: they are the rare case, and
 // in one loop with the plain form they cost that form registers (188 more spilled in dQ at
 // D = 128).
-// P and dS are rounded to bf16 for their products, and di is formed of the rounded o: dQ and dK are off by
-// these two and their own rounding, 0.003 of their size in all, dV by P's and its own. Sums are f32.
+// P and dS are rounded to bf16 for their products. Plain form: di is formed of the rounded o, as the
+// (B, H, T, D) kernels do in range: dQ and dK are off by these two and their own rounding, 0.003 of their
+// size in all, dV by P's and its own. Careful form: di = sum_j P dP from a sweep over the keys of its
+// own, as those kernels do out of range, for there dS may be far smaller than dP and di (values near 3
+// whose differences are 0.1: dQ off by 0.42 of its size with the rounded o's di, 0.004 so). Sums are f32.
 // What bounds it: VALU and matrix issue beside waits for spilled registers and copies. Nine documents of
 // 16384 tokens, 16 heads over 4, D = 128: dQ 297 us, 0.81 PFLOP/s (VALU busy 57 % of cycles, matrix cores
 // 43 %), dK/dV 405, 0.79 (53, 48). 13 documents, 8161 tokens, 16 heads, D = 64: 50 and 55 us.
@@ -86,11 +89,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
 
   const bf16* kbase = p.k + (size_t)kvh * p.k_hs + (size_t)f.start * p.k_ts;
   const bf16* vbase = p.v + (size_t)kvh * p.v_hs + (size_t)f.start * p.v_ts;
-  // The 16 keys of tile kt that this wave copies; past the sequence they read as zeros.
-  auto group = [&](int kt) {
+  // The 16 keys of tile kt that this wave copies; past the sequence, and from tile `end` on, they read
+  // as zeros.
+  auto group = [&](int kt, int end) {
     KvGroup g;
     const int key = kt * BK + 16 * wave;
-    g.rows = kt < kt1 ? min(max(f.len - key, 0), 16) : 0;
+    g.rows = kt < end ? min(max(f.len - key, 0), 16) : 0;
     const int k = g.rows > 0 ? key : 0;
     g.k = kbase + (size_t)k * p.k_ts;
     g.v = vbase + (size_t)k * p.v_ts;
@@ -117,7 +121,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
   };
 
   {
-    const KvGroup g = group(kt0);
+    const KvGroup g = group(kt0, kt1);
 #pragma unroll
     for (int j = 0; j < PW; ++j) dma(Ks0, Vs0, g, j);
   }
@@ -149,15 +153,15 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
     di += xor32(di);
   }
   const float rs = live ? p.stat[at.stat] : 0.0f;
-  if (live && h == 0 && range == 0) p.ndi[at.stat] = -di;
   const bool careful = __syncthreads_or(rs < 0.0f) != 0;
+  if (!careful && live && h == 0 && range == 0) p.ndi[at.stat] = -di;
   if (threadIdx.x == 0 && range == 0) p.care[(size_t)packed_slot(f, G, PK_ROWS) * p.Hkv + kvh] = careful;
   const int log2n = p.sc.log2n;
   const float b2 = p.sc.b;
   // Plain form: dS = (t^n r) fma(rs^n, dP, - rs^n di), one instruction less than P (dP - di) r.
-  // Careful form: the two registers hold the statistic and di themselves.
+  // Careful form: the statistic itself, and di of its own (below).
   const float pz = careful ? rs : pow2n<0>(rs, log2n);
-  const float nzd = careful ? di : -pz * di;
+  const float nzd = -pz * di;
   floatx16 dqa[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) dqa[db] = floatx16{};
@@ -188,7 +192,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
     bf16* Kn = BUF ? Ks0 : Ks1;
     bf16* Vn = BUF ? Vs0 : Vs1;
     const int kb0 = kt * BK;
-    const KvGroup gn = group(kt + 1);
+    const KvGroup gn = group(kt + 1, kt1);
     if constexpr (MASKED) {
       if (kb0 > wave_posmax) {  // every key lies after this wave's rows
 #pragma unroll
@@ -293,27 +297,56 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedBwdParams p) {
       tile(std::integral_constant<int, 1>{}, std::true_type{}, kt + 1);
     }
   } else {
-    for (int kt = kt0; kt < kt1; ++kt) {
+    // Key tile kt (past the sequence it reads as zeros), and S and dP of one of its blocks.
+    auto load = [&](int kt) {
       __syncthreads();  // every wave is done with the tile before
-      const KvGroup g = group(kt);
+      const KvGroup g = group(kt, posmax / BK + 1);
 #pragma unroll
       for (int j = 0; j < PW; ++j) dma(Ks0, Vs0, g, j);
       __builtin_amdgcn_s_waitcnt(VMCNT0);
       __syncthreads();
+    };
+    auto scores = [&](int blk, floatx16& s, floatx16& dp) {
+      s = floatx16{};
+      dp = floatx16{};
+#pragma unroll
+      for (int st = 0; st < NF; ++st) {
+        s = mfma_bf16(ld8(Ks0 + blk * 32 * D + row_off[st]), qf[st], s);
+        dp = mfma_bf16(ld8(Vs0 + blk * 32 * D + row_off[st]), of[st], dp);
+      }
+    };
+    // di = sum_j P dP over all of the row's keys, whatever range of them is this workgroup's.
+    float dw = 0.0f;
+    for (int kt = 0; kt <= posmax / BK; ++kt) {
+      load(kt);
       for (int blk = 0; blk < 2; ++blk) {
         const int kb = kt * BK + 32 * blk;
         if (kb > wave_posmax) continue;
-        floatx16 s = {}, dp = {};
+        floatx16 s, dp;
+        scores(blk, s, dp);
 #pragma unroll
-        for (int st = 0; st < NF; ++st) {
-          s = mfma_bf16(ld8(Ks0 + blk * 32 * D + row_off[st]), qf[st], s);
-          dp = mfma_bf16(ld8(Vs0 + blk * 32 * D + row_off[st]), of[st], dp);
+        for (int i = 0; i < 16; ++i) {
+          const bool dead = kb + 8 * (i >> 2) + 4 * h + (i & 3) > mytok;
+          float pw, ds;
+          packed_elem<0, true>(s[i], dp[i], pz, b2, log2n, dead, pw, ds);
+          dw += dead ? 0.0f : pw * dp[i];
         }
+      }
+    }
+    dw += xor32(dw);
+    if (mytok >= 0 && h == 0 && range == 0) p.ndi[packed_row<D>(p, f, kvh, again(r0 + wave * 32 + l32)).stat] = -dw;
+    for (int kt = kt0; kt < kt1; ++kt) {
+      load(kt);
+      for (int blk = 0; blk < 2; ++blk) {
+        const int kb = kt * BK + 32 * blk;
+        if (kb > wave_posmax) continue;
+        floatx16 s, dp;
+        scores(blk, s, dp);
         bf16x8 da[2];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float pw, ds;
-          packed_elem<0, true>(s[i], dp[i] - nzd, pz, b2, log2n, kb + 8 * (i >> 2) + 4 * h + (i & 3) > mytok, pw, ds);
+          packed_elem<0, true>(s[i], dp[i] - dw, pz, b2, log2n, kb + 8 * (i >> 2) + 4 * h + (i & 3) > mytok, pw, ds);
           da[i >> 3][i & 7] = f2bf(ds);
         }
         const bf16* kl = Ks0 + blk * 32 * D;

@@ -209,6 +209,65 @@ def test_second_derivatives_are_refused():
     assert torch.equal(gg, torch.full_like(gg, 2.0))
 
 
+# --- gradients of scores out of range --------------------------------------------------------
+
+def _backward_of_weights(q, k, v, sink, do, n, c):
+    """One head in float64 (all rows of one sequence) and bounds that hold no rounding of o: P and dS are
+    rounded to bf16 for their products and the results to bf16, u = 2^-8 each; di = sum_j P dP, like
+    every other sum, is f32, whose share is 1e-4 of the magnitudes added up (16 times a weight's few
+    2^-24, and up to 1500 terms' 2^-24 each)."""
+    U, F = 2.0 ** -8, 1e-4
+    alpha = 1.0 / (math.sqrt(q.shape[1]) * c)
+    x = (q @ k.T) * alpha
+    dead = torch.ones_like(x, dtype=torch.bool).triu(1)
+    a = (n * torch.asinh(x)).masked_fill(dead, -math.inf)
+    ab = torch.full_like(a[:, :1], -math.inf) if sink is None else (n * torch.asinh(sink / c)).expand(a.shape[0], 1)
+    both = torch.softmax(torch.cat([a, ab], 1), 1)
+    p, pb = both[:, :-1], both[:, -1:]
+    dp, mag_dp = do @ v.T, do.abs() @ v.abs().T
+    di, mag_di = (p * dp).sum(1, keepdim=True), (p * mag_dp).sum(1, keepdim=True)
+    f = n * alpha * p / torch.sqrt(1 + x * x)
+    ds = f * (dp - di)
+    off = U * ds.abs() + F * f * (mag_dp + mag_di)
+    val = {"dq": ds @ k, "dk": ds.T @ q, "dv": p.T @ do}
+    tol = {"dq": off @ k.abs(), "dk": off.T @ q.abs(), "dv": (U + F) * (p.T @ do.abs())}
+    tol = {m: t + U * val[m].abs() for m, t in tol.items()}
+    if sink is not None:
+        rb = n / torch.sqrt(1 + (sink / c) ** 2) / c
+        val["dsink"], tol["dsink"] = -(pb * di).sum() * rb, F * (pb * mag_di).sum() * rb
+    return val, tol
+
+
+@pytest.mark.parametrize("lens,H,Hkv,D", [([300, 70], 2, 2, 64), ([513, 1, 40], 4, 1, 128), ([1500], 3, 1, 128)],
+                         ids=["heads", "group", "ranges"])
+@pytest.mark.parametrize("sink", [False, True])
+@pytest.mark.parametrize("n", [16, 64])
+def test_gradients_of_scores_out_of_range_do_not_see_the_output_rounded(lens, H, Hkv, D, sink, n):
+    """Values that share a large part: dP and di are far larger than their difference, and a di of the
+    rounded output would be off by more than that. As flash_attention's range guard computes it."""
+    from algebraic_amd.kernels.packed import packed_flash_attention
+    rn = _gen(D + H)
+    N, cu, G = sum(lens), _starts(lens), H // Hkv
+    q, k = _norm(rn(N, H, D)), _norm(rn(N, Hkv, D))
+    q[..., 0], k[..., 0] = 1600.0, 8.0  # every score near 200 (141 at D = 128)
+    leaves = [t.to(BF).requires_grad_(True) for t in (q, k, 3 + 0.1 * rn(N, Hkv, D))]
+    do, s = (1 + rn(N, H, D)).to(BF), (1600.0 + 30 * rn(H)).requires_grad_(True) if sink else None
+    print(f"[edges] far scores {lens} H{H}/{Hkv} D{D} sink {sink} n {n}", flush=True)
+    o = packed_flash_attention(*leaves, _i32(cu), s, n=n, c=8.0)
+    got = dict(zip(("dq", "dk", "dv", "dsink"), torch.autograd.grad(o, [*leaves] + ([s] if sink else []), do)))
+    val = {m: torch.zeros(t.shape, dtype=torch.float64, device="cuda") for m, t in got.items()}
+    tol = {m: torch.zeros_like(t) for m, t in val.items()}
+    for a, b in zip(cu, cu[1:]):
+        for h in range(H):
+            hv, ht = _backward_of_weights(*(t[a:b, i].detach().double() for t, i in zip(leaves, (h, h // G, h // G))),
+                                          s[h].detach().double() if sink else None, do[a:b, h].double(), n, 8.0)
+            for m in hv:
+                at = (h,) if m == "dsink" else (slice(a, b), h if m == "dq" else h // G)
+                val[m][at] += hv[m]
+                tol[m][at] += ht[m]
+    check(got, val, tol)
+
+
 # --- the 8-bit norm --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("d", [64, 512, 4096])
