@@ -391,3 +391,31 @@ def test_captured_steps_write_the_cache_themselves():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(kp, wk) and torch.equal(vp, wv), i
+
+
+def test_a_captured_call_over_ranges_follows_the_lengths():
+    """One captured call over ranges of keys, replayed with other lengths between eager ones: ranges
+    that were written become empty and the other way round."""
+    attend = _ops()[1]
+    rn = _gen(9)
+    q, kp, vp, table, s, _, _ = _held(2, 400, 16, [1, 1], 8, 2, 128, seed=9)
+    cu, kv = _i32([0, 1, 2]), _i32([6400, 6400])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attend(q, kp, vp, table, cu, kv, s, n=16, c=8.0)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend(q, kp, vp, table, cu, kv, s, n=16, c=8.0)
+    torch.cuda.synchronize()
+    for lens in ([6400, 6400], [1, 6000], [700, 0], [6399, 257], [0, 0]):
+        q.copy_(_norm(rn(*q.shape)))
+        kv.copy_(torch.tensor(lens, dtype=torch.int32))
+        want = attend(q, kp, vp, table, cu, kv, s, n=16, c=8.0)
+        torch.cuda.synchronize()
+        print(f"[edges] replay of {lens}", flush=True)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.isfinite(out).all(), lens
