@@ -113,8 +113,8 @@ def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, q_g
     position (``cos``, ``sin`` (>= width page, D/2) float32, or both None: no rotation) and gains (D,)
     or None. Returns the queries (N, H, D); ``k_pages`` and ``v_pages`` are written in place, one
     place a token. A token whose position or page number is out of range is not written; queries at
-    such a position, and those behind the last sequence, are zero. Two tokens in one place: either is
-    kept.
+    such a position, and those behind the last sequence, are zero. A place given to two tokens of a
+    call (a page that two sequences write) may end up with parts of both.
     """
     _check_heads(q, k, v)
     (N, H, D), Hkv, dev = q.shape, k.shape[1], q.device
@@ -162,7 +162,8 @@ def paged_flash_attention(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, 
     the outputs that would have read it NaN (and may those of tokens before them in the call). A
     sequence may outgrow its row of the table: tokens at positions from ``width page`` on, which have
     no place in it, get NaN, those before are what they would be. The order of every sum is fixed by
-    the shapes.
+    the shapes, and so is a weight's form in the second product, by the call's average rows (tokens
+    times H / Hkv) a sequence: two bfloat16 numbers up to 32 of them, one above.
     """
     if k_pages.dim() != 4:
         raise ValueError("k_pages and v_pages must be (pages, Hkv, page, D)")

@@ -1403,14 +1403,15 @@ static int check_table(int width, int page, int pages) {
 // 48 rows 147 121 114.
 // Ranges, the former: at most one workgroup a CU, none under DECODE_RANGE keys of a sequence as long
 // as the table allows. One token over 131001 keys, 4 heads of 128: 64 workgroups 82 us, 128 to 256
-// 47 to 49, 320 60, 512 50; over 8000 keys, 8 heads: 64 20 us, 256 (250 keys each) 14, 512 17.
+// 47 to 49, 320 60, 512 50; over 8000 keys, 8 heads: 64 20 us, 256 (250 keys each) 14, 512 17. (All of
+// D = 128; D = 64 takes the same. From 129 workgroups on nothing is split, whatever the lengths.)
 // The latter: the n ranges of the least estimate, 17 ns a key and workgroup (a second one on a CU takes as
 // much from the first), 6 us and 33 ns a workgroup and range for joining. One sequence: rounds of equal
 // workgroups, ceil(workgroups n / 256) / n. Several, the longest first: the longest range or the CUs'
 // average, the sequences taken for 0.6 of the table's reach, and a fifth of a range for the end. Three
 // rounds at most, for they may be far shorter. Measured us of 1 to 5 ranges: 701 tokens each over 12000,
 // 8000 and 4000 keys, 16 heads over 4 (264 workgroups): 271 189 199 192 194, takes 2; 300 each over 1000 to
-// 9000, 16 over 4 (240): 178 117 104 106 113, 2; 46 each over 12000 to 40000, 32 over 8 (112): 749 401 290
+// 9000, 16 over 4 (240): 178 117 104 106 113, 2, a tenth over the best; 46 each over 12000 to 40000, 32 over 8 (112): 749 401 290
 // 234 210, 6; 459 each over 12 x 2393, 8 over 1 (348): 87 89 100 103 108, 1; 645 over 9319, 32 over 4 (164):
 // 187 158 129 144 147, 3; 300 over 30000, 16 over 4 (40): 562 300 210 163 137, 119 of 6, 135 of 8, takes 6.
 struct PagedPlan {

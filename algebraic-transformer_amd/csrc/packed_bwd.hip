@@ -26,8 +26,9 @@
 // own, as those kernels do out of range, for there dS may be far smaller than dP and di (values near 3
 // whose differences are 0.1: dQ off by 0.42 of its size with the rounded o's di, 0.004 so). Sums are f32.
 // What bounds it: VALU and matrix issue beside waits for spilled registers and copies. Nine documents of
-// 16384 tokens, 16 heads over 4, D = 128: dQ 297 us, 0.81 PFLOP/s (VALU busy 57 % of cycles, matrix cores
-// 43 %), dK/dV 405, 0.79 (53, 48). 13 documents, 8161 tokens, 16 heads, D = 64: 50 and 55 us.
+// 16384 tokens, 16 heads over 4, D = 128: dQ 302 us, 0.80 PFLOP/s (VALU busy 56 % of cycles, matrix cores
+// 42 %), dK/dV 408, 0.79 (52, 48); every row careful 980 and 877. 13 documents, 8161 tokens, 16 heads,
+// D = 64: 50 and 55 us (64, 23; 66, 26).
 // dK/dV with 8 waves, the columns of dK and dV split over them, was slower: 436 us (then 418), and 100 for
 // 55 at D = 64.
 #include <type_traits>

@@ -23,7 +23,7 @@
 // cores beside them. 16384 tokens in 3 sequences, 32 heads over 8, D = 128: 850 us, 0.93 PFLOP/s (VALU busy
 // 70 % of cycles, matrix cores 50 %, no LDS bank conflict); nine documents of 16384 tokens, 16 heads over 4:
 // 203 us, 0.79 PFLOP/s (65, 43: more of their tiles are at the diagonal); 13 documents, 8161 tokens, 16
-// heads, D = 64: 38 us. Over a cache, 701 tokens each of 3 requests over 24000 keys, 16 heads over 4: 172 us,
+// heads, D = 64: 38 us (73, 22). Over a cache, 701 tokens each of 3 requests over 24000 keys, 16 heads over 4: 172 us,
 // 0.77 PFLOP/s, and 12 for joining two ranges.
 // A key head's workgroups are neighbours in steps of Hkv: with 2, 4, 8 key heads each XCD's L2 holds the
 // keys of one, or of the same few, and K and V leave memory about once.

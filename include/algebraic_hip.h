@@ -394,7 +394,8 @@ int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, con
  * (model.py:170-174), y = rot((x tau) gain) in f32 rounded once; queries to q_out (N, H, D)
  * contiguous, rotated keys and the values to their pages. Gains (D) of gain_dtype or NULL; cos, sin
  * (table_rows >= width page, D / 2) f32, or both NULL. A token whose position or page number is
- * out of range is not written; behind the last sequence, or at such a position, its query is zero. */
+ * out of range is not written; behind the last sequence, or at such a position, its query is zero.
+ * A place given to two tokens may end up with parts of both. */
 int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                      const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
                      long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, int pages, int page,
