@@ -11,10 +11,10 @@ from pathlib import Path
 _HERE = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("ALGEBRAIC_HIP_LIB", _HERE / "libalgebraic_hip.so"))
 
-ABI_VERSION = 4  # ALG_ABI_VERSION of include/algebraic_hip.h these signatures follow
+ABI_VERSION = 5  # ALG_ABI_VERSION of include/algebraic_hip.h these signatures follow
 
 ALG_OK, ALG_ERR_INVALID, ALG_ERR_UNSUPPORTED, ALG_ERR_HIP = 0, 1, 2, 3
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_F64, DTYPE_I32, DTYPE_I64 = 0, 1, 2, 3, 4
 FFN_GEMM, FFN_GATE_UP, FFN_DY = 0, 1, 2
 HEAD_LOGITS, HEAD_DH, HEAD_DE = 0, 1, 2
 ATTN_INRANGE, ATTN_CLIPPED, ATTN_SHIFTED, ATTN_GUARDED = 0, 1, 2, 3
@@ -82,6 +82,18 @@ _SIGNATURES = {
                             _P, _P, _I, _I, _F, _I, _P, _P, _S]),
     "alg_paged_append": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _L, _P, _L, _L,
                               _L, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P, _P, _I, _F, _P]),
+    "alg_paged_append_fp8": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _L, _P, _L, _L,
+                                  _L, _P, _L, _L, _P, _L, _L, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P, _P, _I, _F, _P]),
+    "alg_paged_read_fp8": (_I, [_P, _I, _I, _I, _I, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _P,
+                                _I, _P, _P, _P, _P]),
+    "alg_paged_attn_fp8_workspace_size": (_S, [_I, _I, _I, _I, _I, _I, _I]),
+    "alg_paged_attn_fp8": (_I, [_P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _P, _L,
+                                _L, _I, _I, _P, _I, _P, _P, _P, _I, _I, _F, _I, _P, _P, _S]),
+    "alg_embedding_fwd": (_I, [_P, _I, _I, _I, _P, _I, _P, _I, _F, _P, _I]),
+    "alg_embedding_bwd_workspace_size": (_S, [_I, _I, _I]),
+    "alg_embedding_bwd": (_I, [_P, _I, _I, _I, _P, _I, _P, _I, _F, _P, _I, _P, _S]),
+    "alg_head_logits": (_I, [_P, _I, _I, _I, _I, _P, _P, _P]),
+    "alg_head_sample": (_I, [_P, _I, _I, _P, _I, _L, _P, _I, _I, _F, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P]),
     "alg_timer_enable": (None, [_I]),
     "alg_timer_report": (_S, [ctypes.c_char_p, _S]),
 }

@@ -311,7 +311,7 @@ int noalloc_scratch(void** out) {
 extern "C" {
 
 const char* alg_last_error(void) { return g_err.c_str(); }
-const char* alg_version(void) { return "algebraic_hip 0.4 gfx950 (ABI 4)"; }
+const char* alg_version(void) { return "algebraic_hip 0.5 gfx950 (ABI 5)"; }
 int alg_abi_version(void) { return ALG_ABI_VERSION; }
 
 size_t alg_attn_workspace_size(int dtype, int B, int H, int T, int D) {
@@ -1191,6 +1191,132 @@ int alg_add_rms_norm_bwd(alg_stream_t stream, int rows, int d, const void* sum, 
   return hip_status(alg::launch_rms_norm_bwd(p, dgain, (hipStream_t)stream), "alg_add_rms_norm_bwd");
 }
 
+// ---- from one token to the next ----------------------------------------------------------------
+
+static int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need && (!workspace || bytes < need)) return fail(ALG_ERR_INVALID, "workspace too small: need %zu bytes", need);
+  if (!aligned16({workspace})) return fail(ALG_ERR_INVALID, "workspace must be 16-byte aligned");
+  return ALG_OK;
+}
+
+static int check_embedding(int N, int d, int V, int token_dtype, int table_dtype, int y_dtype) {
+  if (N < 0 || V <= 0 || d <= 0) return fail(ALG_ERR_INVALID, "N must not be negative, V and d positive (got %d, %d, %d)", N, V, d);
+  if (d % 8) return fail(ALG_ERR_UNSUPPORTED, "rows of %d: the embedding takes multiples of 8", d);
+  if (N >= 1 << 24 || V >= 1 << 24 || d > 1 << 16) return fail(ALG_ERR_UNSUPPORTED, "built for N and V under 2^24 and d up to 2^16");
+  if ((double)N * d / 8 >= 4294967040.0) return fail(ALG_ERR_UNSUPPORTED, "N d = %.0f: at most 2^35 in one launch", (double)N * d);
+  if (token_dtype != ALG_DTYPE_I32 && token_dtype != ALG_DTYPE_I64) return fail(ALG_ERR_INVALID, "tokens must be int32 or int64");
+  if (!is_weight_dtype(table_dtype) || !is_weight_dtype(y_dtype)) return fail(ALG_ERR_INVALID, "table and rows must be bf16 or f32");
+  return ALG_OK;
+}
+
+int alg_embedding_fwd(alg_stream_t stream, int N, int d, int V, const void* tokens, int token_dtype, const void* table,
+                      int table_dtype, float scale, void* y, int y_dtype) {
+  if (const int rc = check_embedding(N, d, V, token_dtype, table_dtype, y_dtype)) return rc;
+  if (N == 0) return ALG_OK;
+  if (!tokens || !table || !y) return fail(ALG_ERR_INVALID, "null argument");
+  if (!aligned16({table, y})) return fail(ALG_ERR_INVALID, "table and rows must be 16-byte aligned");
+  alg::EmbeddingParams p;
+  std::memset(&p, 0, sizeof p);
+  p.tokens = tokens; p.tokens64 = token_dtype == ALG_DTYPE_I64;
+  p.table = table; p.table_bf16 = table_dtype == ALG_DTYPE_BF16; p.y = y; p.y_bf16 = y_dtype == ALG_DTYPE_BF16;
+  p.scale = scale; p.N = N; p.d = d; p.V = V;
+  return hip_status(alg::launch_embedding_fwd(p, (hipStream_t)stream), "alg_embedding_fwd");
+}
+
+// Workspace of the embedding's gradient: two buffers of sorted tokens and where they stood, the counts of a
+// pass, and the sums at the chunks' borders. Chunks of 32 tokens, longer ones from 32768 tokens on, so
+// that a run over all of them is joined from 1024 parts at most.
+struct EmbeddingWs {
+  int blocks, passes, chunk, chunks;
+  size_t pos, hist, part, total;
+};
+static EmbeddingWs embedding_ws(int N, int d, int V) {
+  EmbeddingWs w;
+  w.blocks = alg::embedding_sort_blocks(N);
+  w.passes = 1;
+  while (w.passes < 3 && V >> (8 * w.passes)) ++w.passes;
+  w.chunk = std::max(32, (N + 1023) / 1024);
+  w.chunks = (N + w.chunk - 1) / w.chunk;
+  const size_t each = align256((size_t)N * sizeof(int));
+  w.pos = 2 * each;
+  w.hist = 4 * each;
+  w.part = w.hist + align256((size_t)256 * w.blocks * sizeof(int));
+  w.total = w.part + (size_t)2 * w.chunks * d * sizeof(float);
+  return w;
+}
+
+size_t alg_embedding_bwd_workspace_size(int N, int d, int V) { return N <= 0 || d <= 0 || V <= 0 ? 0 : embedding_ws(N, d, V).total; }
+
+int alg_embedding_bwd(alg_stream_t stream, int N, int d, int V, const void* tokens, int token_dtype, const void* dy,
+                      int dy_dtype, float scale, void* dtable, int table_dtype, void* workspace, size_t workspace_bytes) {
+  int rc = check_embedding(N, d, V, token_dtype, table_dtype, dy_dtype);
+  if (rc) return rc;
+  if (!dtable || (N && (!tokens || !dy))) return fail(ALG_ERR_INVALID, "null argument");
+  if (!aligned16({dy, dtable})) return fail(ALG_ERR_INVALID, "dy and dtable must be 16-byte aligned");
+  const EmbeddingWs w = embedding_ws(N, d, V);
+  if ((rc = check_workspace(workspace, workspace_bytes, N ? w.total : 0))) return rc;
+  alg::EmbeddingParams p;
+  std::memset(&p, 0, sizeof p);
+  p.tokens = tokens; p.tokens64 = token_dtype == ALG_DTYPE_I64;
+  p.table_bf16 = table_dtype == ALG_DTYPE_BF16; p.y = const_cast<void*>(dy); p.y_bf16 = dy_dtype == ALG_DTYPE_BF16;
+  p.scale = scale; p.N = N; p.d = d; p.V = V; p.grad = dtable;
+  char* ws = static_cast<char*>(workspace);
+  for (int i = 0; N && i < 2; ++i) {
+    p.keys[i] = reinterpret_cast<int*>(ws + i * (w.pos / 2));
+    p.pos[i] = reinterpret_cast<int*>(ws + w.pos + i * (w.pos / 2));
+  }
+  p.hist = reinterpret_cast<int*>(ws + w.hist);
+  p.part = reinterpret_cast<float*>(ws + w.part);
+  p.blocks = w.blocks; p.passes = w.passes; p.chunk = w.chunk; p.chunks = w.chunks;
+  return hip_status(alg::launch_embedding_bwd(p, (hipStream_t)stream), "alg_embedding_bwd");
+}
+
+int alg_head_logits(alg_stream_t stream, int dtype, int N, int d, int V, const void* h, const void* E, float* z) {
+  if (!is_weight_dtype(dtype)) return fail(ALG_ERR_INVALID, "dtype must be bf16 or f32");
+  if (N < 0 || d <= 0 || V <= 0) return fail(ALG_ERR_INVALID, "N must not be negative, d and V positive (got %d, %d, %d)", N, d, V);
+  if (d % 8) return fail(ALG_ERR_UNSUPPORTED, "d = %d: the head takes multiples of 8", d);
+  if (N > 1 << 20 || V > 1 << 24 || d > 1 << 20) return fail(ALG_ERR_UNSUPPORTED, "built for N and d up to 2^20 and V up to 2^24");
+  if (N == 0) return ALG_OK;
+  if (!h || !E || !z) return fail(ALG_ERR_INVALID, "null argument");
+  if (!aligned16({h, E, z})) return fail(ALG_ERR_INVALID, "h, E and z must be 16-byte aligned");
+  alg::HeadLogitsParams p;
+  p.h = h; p.e = E; p.z = z; p.bf16_in = dtype == ALG_DTYPE_BF16; p.N = N; p.d = d; p.V = V;
+  return hip_status(alg::launch_head_logits(p, (hipStream_t)stream), "alg_head_logits");
+}
+
+int alg_head_sample(alg_stream_t stream, int N, int V, const void* z, int z_dtype, long z_stride, const void* u, int u_dtype,
+                    int n, float c, const float* temperature, float temperature_all, const int* top_k, int top_k_all,
+                    const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* token, float* logprob) {
+  if (N < 0 || V <= 0) return fail(ALG_ERR_INVALID, "N must not be negative and V positive (got %d, %d)", N, V);
+  if (V > 1 << 20) return fail(ALG_ERR_UNSUPPORTED, "V = %d: the sampler is built for vocabularies of up to 2^20", V);
+  if (N >= 1 << 22) return fail(ALG_ERR_UNSUPPORTED, "%d rows: a workgroup of 1024 threads each, fewer than 2^22 in one launch", N);
+  const int log2n = log2_pow2(n);
+  if (log2n < 0 || log2n > MAX_LOG2N) return fail(ALG_ERR_INVALID, "n must be a power of two up to 2^%d (got %d)", MAX_LOG2N, n);
+  if (!(c > 0.0f) || !std::isfinite(c)) return fail(ALG_ERR_INVALID, "scale c must be positive and finite");
+  if (!is_weight_dtype(z_dtype)) return fail(ALG_ERR_INVALID, "logits must be bf16 or f32");
+  if (u_dtype != ALG_DTYPE_F32 && u_dtype != ALG_DTYPE_F64) return fail(ALG_ERR_INVALID, "uniform numbers must be f32 or f64");
+  if (z_stride < V && N > 1) return fail(ALG_ERR_INVALID, "rows of %d logits, %ld apart", V, z_stride);
+  if (!temperature && !(temperature_all >= 0.0f)) return fail(ALG_ERR_INVALID, "temperature must not be negative");
+  if (N == 0) return ALG_OK;
+  if (!z || !u || !token || !logprob) return fail(ALG_ERR_INVALID, "null argument");
+  alg::HeadSampleParams p;
+  std::memset(&p, 0, sizeof p);
+  const int size = z_dtype == ALG_DTYPE_BF16 ? 2 : 4;
+  p.z = z; p.stride = z_stride; p.z_bf16 = size == 2; p.vec = ((uintptr_t)z | (N > 1 ? z_stride * size : 0)) % (4 * size) == 0;
+  p.N = N; p.V = V; p.u = u; p.u_f64 = u_dtype == ALG_DTYPE_F64;
+  p.temperature = temperature; p.top_p = top_p; p.min_p = min_p; p.top_k = top_k;
+  p.temperature_all = temperature_all; p.top_p_all = top_p_all; p.min_p_all = min_p_all; p.top_k_all = top_k_all;
+  p.n = n; p.inv_c = 1.0 / (double)c;
+  p.clamp = 0.25 * std::pow(1e38 / (double)V, 1.0 / n);  // fused_head.py:273
+  const double border = (double)c * p.clamp;
+  p.z_clamp = border >= 3.4e38 ? INFINITY : (float)border;
+  if ((double)p.z_clamp < border) p.z_clamp = std::nextafterf(p.z_clamp, INFINITY);
+  p.bits = 62;
+  while (V > 1 << (62 - p.bits)) --p.bits;
+  p.token = token; p.logprob = logprob;
+  return hip_status(alg::launch_head_sample(p, (hipStream_t)stream), "alg_head_sample");
+}
+
 // ---- packed sequences and paged caches --------------------------------------------------------
 
 // The arithmetic of one call's weights (packed_common.h). Exponents above 32 would leave f32 in the
@@ -1236,12 +1362,6 @@ static int check_strides(const char* name, const void* base, long ts, long hs, i
     return fail(ALG_ERR_INVALID, "%s: strides (%ld, %ld) must be multiples of 8 and at least %d", name, ts, hs, D);
   if (66.0 * (double)ts + (double)heads * (double)hs + D >= 1073741824.0)
     return fail(ALG_ERR_UNSUPPORTED, "%s: strides (%ld, %ld) pass 32-bit offsets", name, ts, hs);
-  return ALG_OK;
-}
-
-static int check_workspace(const void* workspace, size_t bytes, size_t need) {
-  if (need && (!workspace || bytes < need)) return fail(ALG_ERR_INVALID, "workspace too small: need %zu bytes", need);
-  if (!aligned16({workspace})) return fail(ALG_ERR_INVALID, "workspace must be 16-byte aligned");
   return ALG_OK;
 }
 
@@ -1389,6 +1509,22 @@ static int check_pages(const char* name, const void* base, long ps, long hs, lon
   if (!rc && (page <= 0 || page % 16)) rc = fail(ALG_ERR_UNSUPPORTED, "pages of %d positions: a positive multiple of 16", page);
   return rc;
 }
+// The same of e4m3 pages, whose elements are bytes read 16 a lane, and of their rows' scales, read four
+// or 16 places at once.
+static int check_pages8(const char* name, const void* base, long ps, long hs, long ts, int Hkv, int page, int D) {
+  if (!aligned16({base})) return fail(ALG_ERR_INVALID, "%s must be 16-byte aligned", name);
+  if (ts % 16 || ts < D || ps % 16 || ps < D || (Hkv > 1 && (hs % 16 || hs < D)))
+    return fail(ALG_ERR_INVALID, "%s: strides (%ld, %ld, %ld) must be multiples of 16 and at least %d", name, ps, hs, ts, D);
+  if (66.0 * (double)ts + D >= 1073741824.0) return fail(ALG_ERR_UNSUPPORTED, "%s: a place stride of %ld passes 32-bit offsets", name, ts);
+  if (page <= 0 || page % 16) return fail(ALG_ERR_UNSUPPORTED, "pages of %d positions: a positive multiple of 16", page);
+  return ALG_OK;
+}
+static int check_scales(const char* name, const void* base, long ps, long hs, int Hkv, int page) {
+  if (!aligned16({base})) return fail(ALG_ERR_INVALID, "%s must be 16-byte aligned", name);
+  if (ps % 16 || ps < page || (Hkv > 1 && (hs % 16 || hs < page)))
+    return fail(ALG_ERR_INVALID, "%s: strides (%ld, %ld) must be multiples of 16 and at least %d", name, ps, hs, page);
+  return ALG_OK;
+}
 static int check_table(int width, int page, int pages) {
   if (width <= 0 || pages <= 0) return fail(ALG_ERR_INVALID, "the page table's width and the pages must be positive");
   if ((double)width * page > 2147483647.0 - 256.0) return fail(ALG_ERR_UNSUPPORTED, "%d pages of %d positions a sequence: at most 2^31", width, page);
@@ -1419,10 +1555,10 @@ struct PagedPlan {
   int nsplit;
   SplitWs ws;
 };
-static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int page) {
+static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int page, bool fp8 = false) {
   PagedPlan pl;
   const long G = H / Hkv, rows = N * G, seqs = std::max(1, std::min(S, N)), each = (rows + seqs - 1) / seqs;
-  pl.row_tiles = each <= 16 ? 1 : (each <= 32 ? 2 : 0);
+  pl.row_tiles = each <= 16 ? 1 : (each <= 32 || fp8 ? 2 : 0);
   const long tile = pl.row_tiles ? 16 * pl.row_tiles : alg::PK_ROWS;
   const long groups = seqs * ((each + tile - 1) / tile) * Hkv;
   const long cap = (long)width * page;
@@ -1452,63 +1588,114 @@ size_t alg_paged_attn_workspace_size(int N, int S, int H, int Hkv, int D, int wi
   if (N <= 0 || S < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || width <= 0 || page <= 0) return 0;
   return paged_plan(N, S, H, Hkv, D, width, page).ws.total;
 }
+size_t alg_paged_attn_fp8_workspace_size(int N, int S, int H, int Hkv, int D, int width, int page) {
+  if (N <= 0 || S < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || width <= 0 || page <= 0) return 0;
+  return paged_plan(N, S, H, Hkv, D, width, page, true).ws.total;
+}
+
+// A cache as the paged calls take it; bytes and scales (ks, vs) for one of 8 bits.
+struct PagedCache {
+  const void *k, *v;
+  long k_ps, k_hs, k_ts, v_ps, v_hs, v_ts;
+  const void *ks, *vs;
+  long ks_ps, ks_hs, vs_ps, vs_hs;
+  int pages, page;
+  const int* table;
+  int width;
+  const int *cu, *kv_lens;
+};
+static int check_cache(const PagedCache& c, bool fp8, int Hkv, int D) {
+  int rc;
+  if (!fp8) {
+    rc = check_pages("k_pages", c.k, c.k_ps, c.k_hs, c.k_ts, Hkv, c.page, D);
+    if (!rc) rc = check_pages("v_pages", c.v, c.v_ps, c.v_hs, c.v_ts, Hkv, c.page, D);
+    return rc;
+  }
+  rc = check_pages8("k_pages", c.k, c.k_ps, c.k_hs, c.k_ts, Hkv, c.page, D);
+  if (!rc) rc = check_pages8("v_pages", c.v, c.v_ps, c.v_hs, c.v_ts, Hkv, c.page, D);
+  if (!rc) rc = check_scales("k_scales", c.ks, c.ks_ps, c.ks_hs, Hkv, c.page);
+  if (!rc) rc = check_scales("v_scales", c.vs, c.vs_ps, c.vs_hs, Hkv, c.page);
+  return rc;
+}
+
+static int paged_attn(alg_stream_t stream, const char* name, bool fp8, int N, int S, int H, int Hkv, int D, const void* q,
+                      long q_ts, long q_hs, const PagedCache& c, const void* sink, int sink_dtype, int sink_count,
+                      float scale, int n, void* o, void* workspace, size_t workspace_bytes) {
+  int rc = check_packed(N, S, H, Hkv, D, scale, n, c.cu, sink, sink_dtype, sink_count);
+  if (!rc) rc = check_table(c.width, c.page, c.pages);
+  if (rc) return rc;
+  if (N == 0) return ALG_OK;
+  if (!q || !c.k || !c.v || !o || !c.table || !c.kv_lens || (fp8 && (!c.ks || !c.vs))) return fail(ALG_ERR_INVALID, "null argument");
+  rc = check_strides("q", q, q_ts, q_hs, H, D);
+  if (!rc) rc = check_cache(c, fp8, Hkv, D);
+  if (!rc) rc = check_strides("o", o, (long)H * D, D, H, D);
+  if (rc) return rc;
+  const PagedPlan pl = paged_plan(N, S, H, Hkv, D, c.width, c.page, fp8);
+  if ((rc = check_workspace(workspace, workspace_bytes, pl.ws.total))) return rc;
+  alg::PackedParams p;
+  std::memset(&p, 0, sizeof p);
+  p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(c.k); p.v = static_cast<const bf16*>(c.v);
+  p.o = static_cast<bf16*>(o);
+  p.sink = sink; p.sink_count = sink_count; p.sink_bf16 = sink_dtype == ALG_DTYPE_BF16; p.c = scale; p.cu = c.cu; p.kv_lens = c.kv_lens;
+  p.table = c.table; p.width = c.width; p.page = c.page; p.pages = c.pages;
+  p.q_ts = q_ts; p.q_hs = q_hs;
+  p.k_ts = c.k_ts; p.k_hs = c.k_hs; p.k_ps = c.k_ps; p.v_ts = c.v_ts; p.v_hs = c.v_hs; p.v_ps = c.v_ps;
+  p.ks = static_cast<const uint8_t*>(c.ks); p.vs = static_cast<const uint8_t*>(c.vs);
+  p.ks_hs = c.ks_hs; p.ks_ps = c.ks_ps; p.vs_hs = c.vs_hs; p.vs_ps = c.vs_ps;
+  p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
+  p.sc = attn_scale(n, scale, D);
+  p.nsplit = pl.nsplit;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_zt = pl.ws.total ? reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.ws.zt) : nullptr;
+  const hipStream_t st = (hipStream_t)stream;
+  return hip_status(fp8 ? alg::launch_paged_decode_fp8(p, D, pl.row_tiles, st)
+                        : pl.row_tiles ? alg::launch_paged_decode(p, D, pl.row_tiles, st) : alg::launch_packed_fwd(p, D, true, st),
+                    name);
+}
 
 int alg_paged_attn(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                    const void* k_pages, long k_ps, long k_hs, long k_ts, const void* v_pages, long v_ps, long v_hs,
                    long v_ts, int pages, int page, const int* table, int width, const int* cu, const int* kv_lens,
                    const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, void* workspace,
                    size_t workspace_bytes) {
-  int rc = check_packed(N, S, H, Hkv, D, c, n, cu, sink, sink_dtype, sink_count);
-  if (!rc) rc = check_table(width, page, pages);
-  if (rc) return rc;
-  if (N == 0) return ALG_OK;
-  if (!q || !k_pages || !v_pages || !o || !table || !kv_lens) return fail(ALG_ERR_INVALID, "null argument");
-  rc = check_strides("q", q, q_ts, q_hs, H, D);
-  if (!rc) rc = check_pages("k_pages", k_pages, k_ps, k_hs, k_ts, Hkv, page, D);
-  if (!rc) rc = check_pages("v_pages", v_pages, v_ps, v_hs, v_ts, Hkv, page, D);
-  if (!rc) rc = check_strides("o", o, (long)H * D, D, H, D);
-  if (rc) return rc;
-  const PagedPlan pl = paged_plan(N, S, H, Hkv, D, width, page);
-  if ((rc = check_workspace(workspace, workspace_bytes, pl.ws.total))) return rc;
-  alg::PackedParams p;
-  std::memset(&p, 0, sizeof p);
-  p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k_pages); p.v = static_cast<const bf16*>(v_pages);
-  p.o = static_cast<bf16*>(o);
-  p.sink = sink; p.sink_count = sink_count; p.sink_bf16 = sink_dtype == ALG_DTYPE_BF16; p.c = c; p.cu = cu; p.kv_lens = kv_lens;
-  p.table = table; p.width = width; p.page = page; p.pages = pages;
-  p.q_ts = q_ts; p.q_hs = q_hs;
-  p.k_ts = k_ts; p.k_hs = k_hs; p.k_ps = k_ps; p.v_ts = v_ts; p.v_hs = v_hs; p.v_ps = v_ps;
-  p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
-  p.sc = attn_scale(n, c, D);
-  p.nsplit = pl.nsplit;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_zt = pl.ws.total ? reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.ws.zt) : nullptr;
-  return hip_status(pl.row_tiles ? alg::launch_paged_decode(p, D, pl.row_tiles, (hipStream_t)stream)
-                                 : alg::launch_packed_fwd(p, D, true, (hipStream_t)stream),
-                    "alg_paged_attn");
+  const PagedCache cache{k_pages, v_pages, k_ps, k_hs, k_ts, v_ps, v_hs, v_ts, nullptr, nullptr, 0, 0, 0, 0,
+                         pages, page, table, width, cu, kv_lens};
+  return paged_attn(stream, "alg_paged_attn", false, N, S, H, Hkv, D, q, q_ts, q_hs, cache, sink, sink_dtype, sink_count, c, n,
+                    o, workspace, workspace_bytes);
 }
 
-int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
-                     const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
-                     long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, int pages, int page,
-                     const int* table, int width, const int* cu, const int* kv_lens, const void* q_gain,
-                     const void* k_gain, int gain_dtype, const float* cos, const float* sin, int table_rows, float eps, void* q_out) {
-  int rc = check_packed(N, S, H, Hkv, D, 1.0f, 2, cu, nullptr, 0, 0);
-  if (!rc) rc = check_table(width, page, pages);
+int alg_paged_attn_fp8(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                       const void* k_pages, long k_ps, long k_hs, long k_ts, const void* v_pages, long v_ps, long v_hs,
+                       long v_ts, const void* k_scales, long ks_ps, long ks_hs, const void* v_scales, long vs_ps,
+                       long vs_hs, int pages, int page, const int* table, int width, const int* cu, const int* kv_lens,
+                       const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, void* workspace,
+                       size_t workspace_bytes) {
+  const PagedCache cache{k_pages, v_pages, k_ps, k_hs, k_ts, v_ps, v_hs, v_ts, k_scales, v_scales, ks_ps, ks_hs, vs_ps, vs_hs,
+                         pages, page, table, width, cu, kv_lens};
+  return paged_attn(stream, "alg_paged_attn_fp8", true, N, S, H, Hkv, D, q, q_ts, q_hs, cache, sink, sink_dtype, sink_count, c,
+                    n, o, workspace, workspace_bytes);
+}
+
+static int paged_append(alg_stream_t stream, const char* name, bool fp8, int N, int S, int H, int Hkv, int D, const void* q,
+                        long q_ts, long q_hs, const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs,
+                        const PagedCache& c, const void* q_gain, const void* k_gain, int gain_dtype, const float* cos,
+                        const float* sin, int table_rows, float eps, void* q_out) {
+  int rc = check_packed(N, S, H, Hkv, D, 1.0f, 2, c.cu, nullptr, 0, 0);
+  if (!rc) rc = check_table(c.width, c.page, c.pages);
   if (rc) return rc;
   if (!(eps > 0.0f) || !std::isfinite(eps)) return fail(ALG_ERR_INVALID, "eps must be positive and finite");
   if ((q_gain || k_gain) && !is_weight_dtype(gain_dtype)) return fail(ALG_ERR_INVALID, "gains must be bf16 or f32");
   if (!cos != !sin) return fail(ALG_ERR_INVALID, "cos and sin are given together");
-  if (cos && (long)table_rows < (long)width * page)
-    return fail(ALG_ERR_INVALID, "rotation tables of %d rows for %ld positions", table_rows, (long)width * page);
+  if (cos && (long)table_rows < (long)c.width * c.page)
+    return fail(ALG_ERR_INVALID, "rotation tables of %d rows for %ld positions", table_rows, (long)c.width * c.page);
   if (N >= 1 << 24) return fail(ALG_ERR_UNSUPPORTED, "%d tokens: a workgroup each, fewer than 2^24 in one launch", N);
   if (N == 0) return ALG_OK;
-  if (!q || !k || !v || !k_pages || !v_pages || !q_out || !table || !kv_lens) return fail(ALG_ERR_INVALID, "null argument");
+  if (!q || !k || !v || !c.k || !c.v || !q_out || !c.table || !c.kv_lens || (fp8 && (!c.ks || !c.vs)))
+    return fail(ALG_ERR_INVALID, "null argument");
   rc = check_strides("q", q, q_ts, q_hs, H, D);
   if (!rc) rc = check_strides("k", k, k_ts, k_hs, Hkv, D);
   if (!rc) rc = check_strides("v", v, v_ts, v_hs, Hkv, D);
-  if (!rc) rc = check_pages("k_pages", k_pages, k_ps, kp_hs, kp_ts, Hkv, page, D);
-  if (!rc) rc = check_pages("v_pages", v_pages, v_ps, vp_hs, vp_ts, Hkv, page, D);
+  if (!rc) rc = check_cache(c, fp8, Hkv, D);
   if (rc) return rc;
   if (!aligned16({q_out, q_gain, k_gain, cos, sin}))
     return fail(ALG_ERR_INVALID, "q_out, gains and tables must be 16-byte aligned");
@@ -1516,13 +1703,65 @@ int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, c
   std::memset(&p, 0, sizeof p);
   p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
   p.q_ts = q_ts; p.q_hs = q_hs; p.k_ts = k_ts; p.k_hs = k_hs; p.v_ts = v_ts; p.v_hs = v_hs;
-  p.kp = static_cast<bf16*>(k_pages); p.vp = static_cast<bf16*>(v_pages);
-  p.kp_ps = k_ps; p.kp_hs = kp_hs; p.kp_ts = kp_ts; p.vp_ps = v_ps; p.vp_hs = vp_hs; p.vp_ts = vp_ts;
+  p.kp = const_cast<void*>(c.k); p.vp = const_cast<void*>(c.v);
+  p.kp_ps = c.k_ps; p.kp_hs = c.k_hs; p.kp_ts = c.k_ts; p.vp_ps = c.v_ps; p.vp_hs = c.v_hs; p.vp_ts = c.v_ts;
+  p.ks = static_cast<uint8_t*>(const_cast<void*>(c.ks)); p.vs = static_cast<uint8_t*>(const_cast<void*>(c.vs));
+  p.ks_ps = c.ks_ps; p.ks_hs = c.ks_hs; p.vs_ps = c.vs_ps; p.vs_hs = c.vs_hs;
   p.qo = static_cast<bf16*>(q_out);
-  p.cu = cu; p.kv_lens = kv_lens; p.table = table; p.width = width; p.page = page; p.pages = pages;
+  p.cu = c.cu; p.kv_lens = c.kv_lens; p.table = c.table; p.width = c.width; p.page = c.page; p.pages = c.pages;
   p.q_gain = q_gain; p.k_gain = k_gain; p.gain_bf16 = gain_dtype == ALG_DTYPE_BF16; p.cos = cos; p.sin = sin; p.eps = eps;
   p.N = N; p.S = S; p.H = H; p.Hkv = Hkv; p.D = D;
-  return hip_status(alg::launch_paged_append(p, (hipStream_t)stream), "alg_paged_append");
+  return hip_status(alg::launch_paged_append(p, (hipStream_t)stream), name);
+}
+
+int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                     const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
+                     long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, int pages, int page,
+                     const int* table, int width, const int* cu, const int* kv_lens, const void* q_gain,
+                     const void* k_gain, int gain_dtype, const float* cos, const float* sin, int table_rows, float eps, void* q_out) {
+  const PagedCache cache{k_pages, v_pages, k_ps, kp_hs, kp_ts, v_ps, vp_hs, vp_ts, nullptr, nullptr, 0, 0, 0, 0,
+                         pages, page, table, width, cu, kv_lens};
+  return paged_append(stream, "alg_paged_append", false, N, S, H, Hkv, D, q, q_ts, q_hs, k, k_ts, k_hs, v, v_ts, v_hs, cache,
+                      q_gain, k_gain, gain_dtype, cos, sin, table_rows, eps, q_out);
+}
+
+int alg_paged_append_fp8(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                         const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
+                         long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, void* k_scales, long ks_ps,
+                         long ks_hs, void* v_scales, long vs_ps, long vs_hs, int pages, int page, const int* table, int width,
+                         const int* cu, const int* kv_lens, const void* q_gain, const void* k_gain, int gain_dtype,
+                         const float* cos, const float* sin, int table_rows, float eps, void* q_out) {
+  const PagedCache cache{k_pages, v_pages, k_ps, kp_hs, kp_ts, v_ps, vp_hs, vp_ts, k_scales, v_scales, ks_ps, ks_hs, vs_ps, vs_hs,
+                         pages, page, table, width, cu, kv_lens};
+  return paged_append(stream, "alg_paged_append_fp8", true, N, S, H, Hkv, D, q, q_ts, q_hs, k, k_ts, k_hs, v, v_ts, v_hs, cache,
+                      q_gain, k_gain, gain_dtype, cos, sin, table_rows, eps, q_out);
+}
+
+int alg_paged_read_fp8(alg_stream_t stream, int N, int S, int Hkv, int D, const void* k_pages, long k_ps, long k_hs, long k_ts,
+                       const void* v_pages, long v_ps, long v_hs, long v_ts, const void* k_scales, long ks_ps, long ks_hs,
+                       const void* v_scales, long vs_ps, long vs_hs, int pages, int page, const int* table, int width,
+                       const int* cu, const int* kv_lens, void* k_out, void* v_out) {
+  const PagedCache c{k_pages, v_pages, k_ps, k_hs, k_ts, v_ps, v_hs, v_ts, k_scales, v_scales, ks_ps, ks_hs, vs_ps, vs_hs,
+                     pages, page, table, width, cu, kv_lens};
+  int rc = check_packed(N, S, Hkv, Hkv, D, 1.0f, 2, cu, nullptr, 0, 0);
+  if (!rc) rc = check_table(width, page, pages);
+  if (rc) return rc;
+  if (N >= 1 << 24) return fail(ALG_ERR_UNSUPPORTED, "%d tokens: a workgroup each, fewer than 2^24 in one launch", N);
+  if (N == 0) return ALG_OK;
+  if (!k_pages || !v_pages || !k_scales || !v_scales || !table || !kv_lens || !k_out || !v_out)
+    return fail(ALG_ERR_INVALID, "null argument");
+  if ((rc = check_cache(c, true, Hkv, D))) return rc;
+  if (!aligned16({k_out, v_out})) return fail(ALG_ERR_INVALID, "k_out and v_out must be 16-byte aligned");
+  alg::PagedReadParams p;
+  std::memset(&p, 0, sizeof p);
+  p.kp = static_cast<const uint8_t*>(k_pages); p.vp = static_cast<const uint8_t*>(v_pages);
+  p.ks = static_cast<const uint8_t*>(k_scales); p.vs = static_cast<const uint8_t*>(v_scales);
+  p.kp_ps = k_ps; p.kp_hs = k_hs; p.kp_ts = k_ts; p.vp_ps = v_ps; p.vp_hs = v_hs; p.vp_ts = v_ts;
+  p.ks_ps = ks_ps; p.ks_hs = ks_hs; p.vs_ps = vs_ps; p.vs_hs = vs_hs;
+  p.ko = static_cast<bf16*>(k_out); p.vo = static_cast<bf16*>(v_out);
+  p.cu = cu; p.kv_lens = kv_lens; p.table = table; p.width = width; p.page = page; p.pages = pages;
+  p.N = N; p.S = S; p.Hkv = Hkv; p.D = D;
+  return hip_status(alg::launch_paged_read(p, (hipStream_t)stream), "alg_paged_read_fp8");
 }
 
 }  // extern "C"

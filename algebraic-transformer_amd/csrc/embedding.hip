@@ -1,0 +1,302 @@
+// The token embedding y_t = s E[token_t] and its gradient dE_v = s sum of dy_t over the tokens equal v
+// (src/algebraic/model.py: the table that the head reads as well).
+//
+// A token outside [0, V) has no row: below 0 (padding) it gets zeros, from V on NaN, and no gradient.
+//
+// The gradient's sums run in the order of the tokens, whatever runs when, so that a step gives the same bits
+// each time; atomic adds would not, and would read and write the f32 table again for every token. So the
+// tokens are sorted (stably, 8 bits a pass, in whole numbers), which makes equal ones neighbours, and one
+// launch reads each dy row once, adds up runs of equal tokens in f32, and writes every row of dE once, zeros
+// included. A run may be of any length (a few tokens make up much of a text), so the work is cut into chunks
+// of sorted tokens, not into runs: a chunk writes the runs that lie within it, and leaves the sums of those
+// that reach over its borders for a second launch, which adds them in order.
+#include <type_traits>
+
+#include "common.h"
+#include "embedding.h"
+#include "launchers.h"
+
+namespace alg {
+
+namespace {
+
+constexpr int EMB_THREADS = 256;
+constexpr int SORT_BLOCK = 2048;  // tokens a workgroup of a pass takes
+constexpr int SORT_WAVES = EMB_THREADS / 64, SORT_EACH = SORT_BLOCK / SORT_WAVES;
+constexpr int ZERO_ROWS = 16;     // rows of the table that a workgroup looks after for zeros
+constexpr int EMB_COLS = 512;     // columns a wave takes: 8 a lane
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
+  } else {
+    const bf16x8 v = *reinterpret_cast<const bf16x8*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(x);
+    *reinterpret_cast<float4*>(p + 4) = *reinterpret_cast<const float4*>(x + 4);
+  } else {
+    bf16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = f2bf(x[e]);
+    *reinterpret_cast<bf16x8*>(p) = v;
+  }
+}
+
+__device__ __forceinline__ long token_at(const EmbeddingParams& p, int i) {
+  return p.tokens64 ? (long)static_cast<const int64_t*>(p.tokens)[i] : (long)static_cast<const int*>(p.tokens)[i];
+}
+// The key that a token is sorted by: V where it has no row.
+__device__ __forceinline__ int token_key(const EmbeddingParams& p, int i) {
+  const long t = token_at(p, i);
+  return t >= 0 && t < p.V ? (int)t : p.V;
+}
+
+}  // namespace
+
+// Eight elements a lane, rows one after the other.
+template <typename E, typename Y>
+__global__ __launch_bounds__(EMB_THREADS) void embedding_fwd_kernel(EmbeddingParams p) {
+  const int each = p.d / 8;
+  const size_t id = (size_t)blockIdx.x * EMB_THREADS + threadIdx.x;
+  const size_t row = id / each;
+  if (row >= (size_t)p.N) return;
+  const int col = 8 * (int)(id - row * each);
+  const long t = token_at(p, (int)row);
+  float x[8];
+  if (t >= 0 && t < p.V) {
+    load8(static_cast<const E*>(p.table) + (size_t)t * p.d + col, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= p.scale;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = t < 0 ? 0.0f : __builtin_nanf("");
+  }
+  store8(static_cast<Y*>(p.y) + row * p.d + col, x);
+}
+
+// How often each value of 8 bits of the key occurs in each block of tokens.
+__global__ __launch_bounds__(EMB_THREADS) void embedding_hist_kernel(EmbeddingParams p, int pass) {
+  __shared__ int count[256];
+  count[threadIdx.x] = 0;
+  __syncthreads();
+  const int end = min(p.N, (int)(blockIdx.x + 1) * SORT_BLOCK);
+  for (int i = blockIdx.x * SORT_BLOCK + threadIdx.x; i < end; i += EMB_THREADS) {
+    const int key = pass ? p.keys[(pass - 1) & 1][i] : token_key(p, i);
+    atomicAdd(&count[(key >> (8 * pass)) & 255], 1);
+  }
+  __syncthreads();
+  p.hist[threadIdx.x * p.blocks + blockIdx.x] = count[threadIdx.x];
+}
+
+// Each token to its place in the order of these 8 bits, equal ones as they stand. A wave takes a stretch of the
+// block's tokens, 64 at a time; lanes of equal bits find each other by ballots.
+__global__ __launch_bounds__(EMB_THREADS) void embedding_scatter_kernel(EmbeddingParams p, int pass) {
+  __shared__ int base[SORT_WAVES][256], sums[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // Where the block's tokens of value `tid` begin: after the lower values and the earlier blocks.
+  int total = 0, earlier = 0;
+  for (int b = 0; b < p.blocks; ++b) {
+    const int c = p.hist[tid * p.blocks + b];
+    if (b < (int)blockIdx.x) earlier += c;
+    total += c;
+  }
+  sums[tid] = total;
+#pragma unroll
+  for (int w = 0; w < SORT_WAVES; ++w) base[w][tid] = 0;
+  __syncthreads();
+  for (int m = 1; m < 256; m <<= 1) {
+    const int below = tid >= m ? sums[tid - m] : 0;
+    __syncthreads();
+    sums[tid] += below;
+    __syncthreads();
+  }
+  const int begin = blockIdx.x * SORT_BLOCK + wave * SORT_EACH, end = min(p.N, begin + SORT_EACH);
+  const auto same = [&](int bits, bool live) {  // the lanes with these bits
+    unsigned long long m = __ballot(live);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const unsigned long long set = __ballot((bits >> k) & 1);
+      m &= (bits >> k) & 1 ? set : ~set;
+    }
+    return m;
+  };
+  for (int i0 = begin; i0 < end; i0 += 64) {
+    const int i = i0 + lane;
+    const bool live = i < end;
+    const int key = live ? (pass ? p.keys[(pass - 1) & 1][i] : token_key(p, i)) : 0, bits = (key >> (8 * pass)) & 255;
+    const unsigned long long m = same(bits, live);
+    if (live && lane == __builtin_ctzll(m)) base[wave][bits] += __popcll(m);
+  }
+  __syncthreads();
+  int at = sums[tid] - total + earlier;
+#pragma unroll
+  for (int w = 0; w < SORT_WAVES; ++w) {
+    const int c = base[w][tid];
+    base[w][tid] = at;
+    at += c;
+  }
+  __syncthreads();
+  for (int i0 = begin; i0 < end; i0 += 64) {
+    const int i = i0 + lane;
+    const bool live = i < end;
+    const int key = live ? (pass ? p.keys[(pass - 1) & 1][i] : token_key(p, i)) : 0, bits = (key >> (8 * pass)) & 255;
+    const unsigned long long m = same(bits, live);
+    if (live) {
+      const int to = base[wave][bits] + __popcll(m & ((1ull << lane) - 1));
+      p.keys[pass & 1][to] = key;
+      p.pos[pass & 1][to] = pass ? p.pos[(pass - 1) & 1][i] : i;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (live && lane == __builtin_ctzll(m)) base[wave][bits] += __popcll(m);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Runs of equal tokens: a wave one chunk of sorted tokens and EMB_COLS columns; the workgroups behind those the
+// rows without a token.
+template <typename E, typename Y>
+__global__ __launch_bounds__(EMB_THREADS) void embedding_bwd_kernel(EmbeddingParams p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int* keys = p.keys[(p.passes - 1) & 1];
+  const int* pos = p.pos[(p.passes - 1) & 1];
+  const int strips = (p.d + EMB_COLS - 1) / EMB_COLS, units = p.chunks * strips;
+  const int work = (units + EMB_THREADS / 64 - 1) / (EMB_THREADS / 64);
+  E* grad = static_cast<E*>(p.grad);
+  if ((int)blockIdx.x >= work) {
+    // The first sorted token of each of these rows, by halving; a row is empty if the next one's is the same.
+    __shared__ int first[ZERO_ROWS + 1];
+    const int v0 = (blockIdx.x - work) * ZERO_ROWS;
+    if (threadIdx.x <= ZERO_ROWS) {
+      int lo = 0, hi = p.N;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (keys[mid] < v0 + (int)threadIdx.x) lo = mid + 1;
+        else hi = mid;
+      }
+      first[threadIdx.x] = lo;
+    }
+    __syncthreads();
+    const float zero[8] = {};
+    for (int r = 0; r < min(ZERO_ROWS, p.V - v0); ++r)
+      if (first[r] == first[r + 1])
+        for (int c = 8 * threadIdx.x; c < p.d; c += 8 * EMB_THREADS) store8(grad + (size_t)(v0 + r) * p.d + c, zero);
+    return;
+  }
+  const int unit = blockIdx.x * (EMB_THREADS / 64) + wave;
+  if (unit >= units) return;
+  const int j = unit / strips, col = (unit - j * strips) * EMB_COLS + 8 * lane;
+  const bool live = col < p.d;
+  const int begin = j * p.chunk, end = min(p.N, begin + p.chunk);
+  const Y* dy = static_cast<const Y*>(p.y) + (live ? col : 0);
+  float sum[8] = {};
+  int run = keys[begin];
+  bool head = begin > 0 && keys[begin - 1] == run;  // the run began before the chunk
+  const auto leave = [&](bool tail) {
+    if (run < p.V && live) {
+      if (head || tail) {
+        store8(p.part + ((size_t)2 * j + (head ? 0 : 1)) * p.d + col, sum);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] *= p.scale;
+        store8(grad + (size_t)run * p.d + col, sum);
+      }
+    }
+    head = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
+  };
+  for (int i = begin; i < end; ++i) {
+    const int key = keys[i];
+    if (key != run) {
+      leave(false);
+      run = key;
+    }
+    if (key >= p.V) break;  // tokens without a row are the last
+    float x[8];
+    load8(dy + (size_t)pos[i] * p.d, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += x[e];
+  }
+  leave(end < p.N && keys[end] == run);
+}
+
+// Runs over several chunks: the wave of the chunk where one begins adds up its parts.
+template <typename E>
+__global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(EmbeddingParams p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int* keys = p.keys[(p.passes - 1) & 1];
+  const int strips = (p.d + EMB_COLS - 1) / EMB_COLS;
+  const int unit = blockIdx.x * (EMB_THREADS / 64) + wave;
+  const int j = unit / strips, col = (unit - j * strips) * EMB_COLS + 8 * lane;
+  const int end = (j + 1) * p.chunk;
+  if (j >= p.chunks || end >= p.N) return;
+  const int run = keys[end - 1];
+  if (run >= p.V || keys[end] != run || (j > 0 && keys[j * p.chunk - 1] == run)) return;
+  if (col >= p.d) return;
+  float sum[8], x[8];
+  load8(p.part + ((size_t)2 * j + 1) * p.d + col, sum);
+  for (int i = j + 1; i < p.chunks && keys[i * p.chunk] == run; ++i) {
+    load8(p.part + (size_t)2 * i * p.d + col, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += x[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[e] *= p.scale;
+  store8(static_cast<E*>(p.grad) + (size_t)run * p.d + col, sum);
+}
+
+namespace {
+
+template <typename F>
+void by_types(const EmbeddingParams& p, F f) {
+  if (p.table_bf16) p.y_bf16 ? f(bf16{}, bf16{}) : f(bf16{}, float{});
+  else p.y_bf16 ? f(float{}, bf16{}) : f(float{}, float{});
+}
+
+}  // namespace
+
+int embedding_sort_blocks(int N) { return (N + SORT_BLOCK - 1) / SORT_BLOCK; }
+
+hipError_t launch_embedding_fwd(const EmbeddingParams& p, hipStream_t st) {
+  KTimer t("embedding_fwd", st);
+  const size_t lanes = (size_t)p.N * (p.d / 8);
+  const dim3 grid((unsigned)((lanes + EMB_THREADS - 1) / EMB_THREADS));
+  by_types(p, [&](auto e, auto y) {
+    hipLaunchKernelGGL((embedding_fwd_kernel<decltype(e), decltype(y)>), grid, dim3(EMB_THREADS), 0, st, p);
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_embedding_bwd(const EmbeddingParams& p, hipStream_t st) {
+  if (p.N) {
+    KTimer t("embedding_sort", st);
+    for (int pass = 0; pass < p.passes; ++pass) {
+      hipLaunchKernelGGL(embedding_hist_kernel, dim3(p.blocks), dim3(EMB_THREADS), 0, st, p, pass);
+      hipLaunchKernelGGL(embedding_scatter_kernel, dim3(p.blocks), dim3(EMB_THREADS), 0, st, p, pass);
+    }
+  }
+  const long strips = (p.d + EMB_COLS - 1) / EMB_COLS, work = (p.chunks * strips + 3) / 4;
+  {
+    KTimer t("embedding_bwd", st);
+    by_types(p, [&](auto e, auto y) {
+      hipLaunchKernelGGL((embedding_bwd_kernel<decltype(e), decltype(y)>), dim3((unsigned)(work + (p.V + ZERO_ROWS - 1) / ZERO_ROWS)),
+                         dim3(EMB_THREADS), 0, st, p);
+    });
+  }
+  if (p.chunks > 1) {
+    KTimer t("embedding_join", st);
+    if (p.table_bf16) hipLaunchKernelGGL(embedding_join_kernel<bf16>, dim3((unsigned)work), dim3(EMB_THREADS), 0, st, p);
+    else hipLaunchKernelGGL(embedding_join_kernel<float>, dim3((unsigned)work), dim3(EMB_THREADS), 0, st, p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace alg

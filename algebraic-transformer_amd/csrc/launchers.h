@@ -6,7 +6,10 @@
 
 #include "attn_common.h"
 #include "attn_prep.h"
+#include "embedding.h"
+#include "head_logits.h"
 #include "head_params.h"
+#include "head_sample.h"
 #include "packed_common.h"
 
 namespace alg {
@@ -73,6 +76,11 @@ hipError_t launch_head_bwd(const HeadParams& p, hipStream_t st);
 HeadParams head_vocab_chunk(const HeadParams& p, int v0, int vc);
 hipError_t launch_head_bwd_streamed(const HeadParams& p, int chunk, hipStream_t st);
 hipError_t launch_head_eval(const HeadParams& p, hipStream_t st);
+hipError_t launch_head_logits(const HeadLogitsParams& p, hipStream_t st);
+int embedding_sort_blocks(int N);
+hipError_t launch_embedding_fwd(const EmbeddingParams& p, hipStream_t st);
+hipError_t launch_embedding_bwd(const EmbeddingParams& p, hipStream_t st);
+hipError_t launch_head_sample(const HeadSampleParams& p, hipStream_t st);
 hipError_t launch_head_stats(const HeadParams& p, int vocab_tiles, hipStream_t st);
 hipError_t launch_head_eval_stats(const HeadParams& p, int vocab_tiles, hipStream_t st);
 int head_f32_vocab_tiles(int V);
@@ -103,9 +111,11 @@ hipError_t launch_ffn_gemm(const FfnGemmParams& g, int a_mode, int b_mode, hipSt
 hipError_t launch_rms_norm_bwd(const RmsNormParams& p, void* dgain, hipStream_t st);
 hipError_t launch_add_rms_norm(const RmsNormParams& p, hipStream_t st);
 hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t st);
+hipError_t launch_paged_read(const PagedReadParams& p, hipStream_t st);
 hipError_t launch_packed_bwd(const PackedBwdParams& p, int D, hipStream_t st);
 hipError_t launch_packed_fwd(const PackedParams& p, int D, bool paged, hipStream_t st);
 hipError_t launch_packed_combine(const PackedParams& p, int D, hipStream_t st);
 hipError_t launch_paged_decode(const PackedParams& p, int D, int row_tiles, hipStream_t st);
+hipError_t launch_paged_decode_fp8(const PackedParams& p, int D, int row_tiles, hipStream_t st);
 
 }  // namespace alg

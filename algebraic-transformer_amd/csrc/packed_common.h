@@ -65,6 +65,9 @@ struct PackedParams {
   long q_ts, q_hs;             // elements between tokens, between heads
   long k_ts, k_hs, k_ps;       // tokens, heads, pages
   long v_ts, v_hs, v_ps;
+  // A cache of 8 bits: k, v hold bytes, and these the rows' scales, (pages, Hkv, page).
+  const uint8_t *ks, *vs;
+  long ks_hs, ks_ps, vs_hs, vs_ps;
   int N, S, H, Hkv, G;
   AttnScale sc;
   // Keys in `nsplit` ranges, each with its own partial row: f32 sums of t^n v, then per row Z and
@@ -78,8 +81,10 @@ struct PackedParams {
 struct PagedAppendParams {
   const bf16 *q, *k, *v;  // raw projections (N, H or Hkv, D)
   long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
-  bf16 *kp, *vp;          // pages of (Hkv, page, D)
+  void *kp, *vp;          // pages of (Hkv, page, D), bf16 or e4m3
   long kp_ps, kp_hs, kp_ts, vp_ps, vp_hs, vp_ts;
+  uint8_t *ks, *vs;       // e4m3: the rows' scales (pages, Hkv, page), e8m0
+  long ks_ps, ks_hs, vs_ps, vs_hs;
   bf16* qo;               // (N, H, D) contiguous
   const int *cu, *kv_lens, *table;
   int width, page, pages;
@@ -88,6 +93,16 @@ struct PagedAppendParams {
   const float *cos, *sin;        // (>= width page, D / 2) or nullptr
   float eps;
   int N, S, H, Hkv, D;
+};
+
+// The tokens at the new tokens' places of an 8-bit cache, read back (paged_append.hip).
+struct PagedReadParams {
+  const uint8_t *kp, *vp, *ks, *vs;
+  long kp_ps, kp_hs, kp_ts, vp_ps, vp_hs, vp_ts, ks_ps, ks_hs, vs_ps, vs_hs;
+  bf16 *ko, *vo;  // (N, Hkv, D) contiguous
+  const int *cu, *kv_lens, *table;
+  int width, page, pages;
+  int N, S, Hkv, D;
 };
 
 // Whether a row of `count` keys whose weights sum to `sum` needs the careful form (a NaN does).
@@ -315,6 +330,28 @@ __device__ __forceinline__ PackedRow packed_row(const P& p, const PackedSeq& f, 
 __device__ __forceinline__ int again(int v) {
   asm volatile("" : "+v"(v));
   return v;
+}
+
+// A row of an 8-bit cache is e4m3(x 2^-e) of its values and one scale 2^e, kept as the byte e + 127
+// (e8m0). A power of two costs the values nothing, for e4m3 rounds relatively: only what lies 2^14 and
+// more under the row's largest value loses bits. And the stored values are bf16 numbers exactly, so that
+// reading them is one conversion, and they can go into the products as they are. e is the least
+// for which max |x| 2^-e <= 448, the type's largest. `top`: the largest |x|, as bits (a NaN's and
+// infinity's bits pass every number's). 255: a row that held such a value.
+__device__ __forceinline__ int scale_byte(unsigned top) {
+  if (top >= 0x7F800000u) return 255;
+  if (top == 0) return 127;
+  return max((int)(top >> 23) - 8 + ((top & 0x7FFFFFu) > 0x600000u), 1);
+}
+__device__ __forceinline__ float scale_value(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }
+// Eight e4m3 values times a power of two, exact in bf16 (below 2^-126: zero).
+__device__ __forceinline__ bf16x8 values8(int lo, int hi, float scale) {
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // One 16-row group of a K / V tile: where its rows start, and how many of them exist.

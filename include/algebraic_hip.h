@@ -45,7 +45,7 @@ enum {
   ALG_ERR_HIP = 3           /* a HIP launch error */
 };
 
-enum { ALG_DTYPE_BF16 = 0, ALG_DTYPE_F32 = 1 };
+enum { ALG_DTYPE_BF16 = 0, ALG_DTYPE_F32 = 1, ALG_DTYPE_F64 = 2, ALG_DTYPE_I32 = 3, ALG_DTYPE_I64 = 4 };
 
 /* Storage of the (B, ., ., D) tensors of an attention call (q, k, v, o, dO, dq, dk, dv and the
  * prologue's outputs): (B, H, T, D), the reference's layout, or the projection layout
@@ -66,7 +66,7 @@ enum { ALG_ATTN_INRANGE = 0, ALG_ATTN_CLIPPED = 1, ALG_ATTN_SHIFTED = 2, ALG_ATT
  * and alg_ffn_plan; nothing else changed.
  * Version 4: adds alg_add_rms_norm_*, alg_packed_attn_*, alg_paged_attn* and alg_paged_append;
  * nothing else changed. */
-#define ALG_ABI_VERSION 4
+#define ALG_ABI_VERSION 5
 
 const char* alg_last_error(void);
 const char* alg_version(void);
@@ -401,6 +401,70 @@ int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, c
                      long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, int pages, int page,
                      const int* table, int width, const int* cu, const int* kv_lens, const void* q_gain,
                      const void* k_gain, int gain_dtype, const float* cos, const float* sin, int table_rows, float eps, void* q_out);
+
+/* A cache of 8 bits. A row (the D values of a token at a key head) is stored as x8 = e4m3(x 2^-e),
+ * rounded to nearest even, and a scale 2^e, kept as the byte e + 127 (e8m0), e the least whole number
+ * from -126 on with max |x| 2^-e <= 448 (rows of zeros: 127). The values x8 2^e are bf16 numbers
+ * exactly (but those under 2^-126, which read as zeros). A row with a value that is not finite has
+ * the scale 255 and reads as NaN, where it is seen and nowhere else. k_pages, v_pages (pages, Hkv,
+ * page, D) bytes, strides in bytes, multiples of 16; k_scales, v_scales (pages, Hkv, page) bytes,
+ * places contiguous, strides between pages (_ps) and heads (_hs) multiples of 16; bases 16-byte
+ * aligned. Everything else as in the calls without _fp8: alg_paged_append_fp8 forms y in f32 and
+ * rounds it once, to 8 bits; alg_paged_attn_fp8 is the attention over the stored values, with their
+ * products and sums as over a bf16 cache that held them. alg_paged_read_fp8 reads the N tokens'
+ * places back into k_out, v_out (N, Hkv, D) bf16, contiguous: behind the last sequence and before
+ * position 0 zeros, at a page number outside [0, pages) or a position that the table does not reach
+ * NaN. */
+int alg_paged_append_fp8(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                         const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
+                         long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, void* k_scales, long ks_ps,
+                         long ks_hs, void* v_scales, long vs_ps, long vs_hs, int pages, int page, const int* table, int width,
+                         const int* cu, const int* kv_lens, const void* q_gain, const void* k_gain, int gain_dtype,
+                         const float* cos, const float* sin, int table_rows, float eps, void* q_out);
+int alg_paged_read_fp8(alg_stream_t stream, int N, int S, int Hkv, int D, const void* k_pages, long k_ps, long k_hs, long k_ts,
+                       const void* v_pages, long v_ps, long v_hs, long v_ts, const void* k_scales, long ks_ps, long ks_hs,
+                       const void* v_scales, long vs_ps, long vs_hs, int pages, int page, const int* table, int width,
+                       const int* cu, const int* kv_lens, void* k_out, void* v_out);
+size_t alg_paged_attn_fp8_workspace_size(int N, int S, int H, int Hkv, int D, int width, int page);
+int alg_paged_attn_fp8(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
+                       const void* k_pages, long k_ps, long k_hs, long k_ts, const void* v_pages, long v_ps, long v_hs,
+                       long v_ts, const void* k_scales, long ks_ps, long ks_hs, const void* v_scales, long vs_ps,
+                       long vs_hs, int pages, int page, const int* table, int width, const int* cu, const int* kv_lens,
+                       const void* sink, int sink_dtype, int sink_count, float c, int n, void* o, void* workspace,
+                       size_t workspace_bytes);
+
+/* The token embedding: y (N, d) = scale table[tokens], rounded once to y_dtype; tokens (N) of
+ * ALG_DTYPE_I32 or _I64, table (V, d) and y of ALG_DTYPE_BF16 or _F32, contiguous, 16-byte aligned, d
+ * a multiple of 8. A token below 0 (padding) has a row of zeros, one from V on a row of NaN. Backward:
+ * dtable (V, d) of table_dtype, every row written, = scale times the sum of the tokens' dy, added in
+ * f32 in a fixed order (the tokens', in groups that N alone sets); tokens outside [0, V) give
+ * nothing. */
+int alg_embedding_fwd(alg_stream_t stream, int N, int d, int V, const void* tokens, int token_dtype, const void* table,
+                      int table_dtype, float scale, void* y, int y_dtype);
+size_t alg_embedding_bwd_workspace_size(int N, int d, int V);
+int alg_embedding_bwd(alg_stream_t stream, int N, int d, int V, const void* tokens, int token_dtype, const void* dy,
+                      int dy_dtype, float scale, void* dtable, int table_dtype, void* workspace, size_t workspace_bytes);
+
+/* The head's logits z (N, V) f32 = h E^T, f32 sums (model.py:225-230's logits): h (N, d) and E (V, d)
+ * of one dtype, contiguous, 16-byte aligned, d a multiple of 8. */
+int alg_head_logits(alg_stream_t stream, int dtype, int N, int d, int V, const void* h, const void* E, float* z);
+
+/* One token a row drawn from the algebraic likelihood (algebraic.py:223-265) of logits z (N, V), f32 or
+ * bf16, rows z_stride elements apart: weights rho(x)^(n / temperature), x = min(z / c, X), X =
+ * (1e38 / V)^(1 / n) / 4. Of the tokens by falling logit, equal ones by their index, are kept the
+ * first top_k (all if that is below 1 or not below V), of those the fewest that have top_p of their
+ * weight (all if that is 1 or more; one at least), of those the ones of min_p times the largest weight
+ * or more. token = the first kept one, by index, at which the running sum of the kept weights passes
+ * u times their sum; logprob = the log of the probability that it was drawn with. temperature 0: the first
+ * of the largest. Weights are f64 relative to the row's largest and summed as whole multiples of
+ * 2^-62 V (rounded up to a power of two), so that results depend on nothing but the row. Each setting
+ * is an array (N) or, where the array is NULL, one value for all. u (N) f32 or f64 in [0, 1); below or
+ * NaN counts as 0, 1 or more as the largest number below 1. Logits of -infinity are never drawn; a row
+ * without another, with a NaN, or whose temperature is negative or NaN gets token -1 and
+ * logprob NaN. V up to 2^20. */
+int alg_head_sample(alg_stream_t stream, int N, int V, const void* z, int z_dtype, long z_stride, const void* u, int u_dtype,
+                    int n, float c, const float* temperature, float temperature_all, const int* top_k, int top_k_all,
+                    const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* token, float* logprob);
 
 /* Measurement hook (no counterpart in the reference; for benchmarks and profilers):
  * while enabled, every kernel launch of this library records a HIP event pair on its
