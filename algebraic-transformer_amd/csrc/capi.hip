@@ -1301,8 +1301,7 @@ int alg_head_sample(alg_stream_t stream, int N, int V, const void* z, int z_dtyp
   if (!z || !u || !token || !logprob) return fail(ALG_ERR_INVALID, "null argument");
   alg::HeadSampleParams p;
   std::memset(&p, 0, sizeof p);
-  const int size = z_dtype == ALG_DTYPE_BF16 ? 2 : 4;
-  p.z = z; p.stride = z_stride; p.z_bf16 = size == 2; p.vec = ((uintptr_t)z | (N > 1 ? z_stride * size : 0)) % (4 * size) == 0;
+  p.z = z; p.stride = z_stride; p.z_bf16 = z_dtype == ALG_DTYPE_BF16;
   p.N = N; p.V = V; p.u = u; p.u_f64 = u_dtype == ALG_DTYPE_F64;
   p.temperature = temperature; p.top_p = top_p; p.min_p = min_p; p.top_k = top_k;
   p.temperature_all = temperature_all; p.top_p_all = top_p_all; p.min_p_all = min_p_all; p.top_k_all = top_k_all;

@@ -8,7 +8,7 @@ namespace alg {
 struct HeadSampleParams {
   const void* z;  // (N, V) logits, f32 or bf16, rows `stride` elements apart
   long stride;
-  int z_bf16, vec;  // vec: rows start on 16 bytes (bf16: 8)
+  int z_bf16;
   int N, V;
   const void* u;    // (N) uniform numbers, f32 or f64
   int u_f64;

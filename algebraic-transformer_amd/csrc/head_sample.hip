@@ -4,17 +4,18 @@
 //
 // Which token a number selects depends on sums over the vocabulary to their last bits wherever the number lies
 // next to a border, and V = 32000 borders lie everywhere. So the weights are f64, relative to the
-// row's largest, and are summed as whole numbers of 2^-bits (2^62 / V): such sums are equal in any order,
-// among any number of lanes and atomics, and a row's token depends on its inputs alone.
+// row's largest (to 2^-40 or better), and are summed as whole numbers of 2^-bits (2^62 / V): such sums are
+// equal in any order, among any number of lanes and atomics, and a row's token depends on the row alone.
 //
-// Order: logits falling, equal ones by their index. The kept tokens are a prefix of it, so that a pair (key, last
-// index of that key) says which: `Prefix`. Top-k and top-p ask for the shortest prefix that sums to something (a
-// count, a mass). select() finds it without sorting: a histogram over 2048 ranges of the logits, the
-// range where the sum is reached, and if that holds few tokens their exact ranks, else a histogram of its
-// keys' bits (at most three more); tokens of one single logit are counted.
+// Order: logits falling, equal ones by their index. The kept tokens are a prefix of it. Where a
+// histogram over 2048 ranges of the logits (by count for top-k, by weight for top-p) says that no more than
+// 1024 tokens can be in it, those are sorted in LDS and everything else happens among them. Otherwise
+// the prefix is a pair (key, last index of that key), found without sorting: the exact ranks within the range
+// where the sum is reached, or if that is crowded too, histograms of its keys' bits (at most three more);
+// tokens of one single logit are counted.
 //
 // One workgroup a row, 16 waves. A lane takes four neighbouring tokens of a tile of 4096, so that a wave's
-// tokens are neighbours and the draw needs the sums of waves, then of one wave's lanes.
+// tokens are neighbours and a draw among all tokens needs the sums of waves, then of one wave's lanes.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
@@ -44,12 +45,6 @@ __device__ __forceinline__ float key_logit(unsigned k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
-  return v;
-}
-
 struct Prefix {
   unsigned key;
   int last;
@@ -60,12 +55,15 @@ __device__ __forceinline__ bool in_prefix(const Prefix& p, unsigned key, int i) 
 
 struct SampleShared {
   u64 bins[SAMPLE_BINS];
+  int counts[SAMPLE_BINS];
   u64 list[SAMPLE_LIST];  // key, and the index's complement: falling order
   u64 value[SAMPLE_LIST];
   u64 tile[SAMPLE_TILES][SAMPLE_WAVES];
+  double2 logs[128];  // 1 / m and -log2 of that, m the middles of [1, 2)'s 128 parts
+  double exps[64];    // 2^(i / 64)
   u64 wave[SAMPLE_WAVES];
   unsigned lo, hi, count;
-  int bin;
+  int bin, upto;
   u64 above;
   Prefix found;
 };
@@ -76,66 +74,100 @@ struct Sampler {
   SampleShared& s;
   const T* row;
   int tid, lane, wave, tiles;
-  unsigned top;          // the largest logit's key
-  double power, log_top;  // n / T, log2 rho of the largest
+  unsigned top;             // the largest logit's key
+  double power, log_top;    // n / temperature, log2 rho of the largest
+  double unit;              // 2^bits
 
   __device__ Sampler(const HeadSampleParams& p_, SampleShared& s_)
       : p(p_), s(s_), row(static_cast<const T*>(p_.z) + (size_t)blockIdx.x * p_.stride), tid(threadIdx.x),
         lane(threadIdx.x & 63), wave(threadIdx.x >> 6), tiles((p_.V + SAMPLE_TILE - 1) / SAMPLE_TILE) {}
 
   __device__ __forceinline__ int first(int t) const { return t * SAMPLE_TILE + 4 * tid; }
-  __device__ __forceinline__ void logits(int t, float (&z)[4]) const {
+  // A lane's four tokens of a tile; none past the row's end. Rows start anywhere.
+  __device__ __forceinline__ void logits(int t, T (&z)[4]) const {
     const int i = first(t);
-    if (p.vec && i + 4 <= p.V) {
-      if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(z) = *reinterpret_cast<const float4*>(row + i);
-      } else {
-        const bf16x4 v = *reinterpret_cast<const bf16x4*>(row + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] = (float)v[e];
-      }
+    if (i + 4 <= p.V) {
+      __builtin_memcpy(z, row + i, sizeof z);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = i + e < p.V ? (float)row[i + e] : -INFINITY;
+      for (int e = 0; e < 4; ++e) z[e] = i + e < p.V ? row[i + e] : (T)-INFINITY;
     }
   }
-  __device__ __forceinline__ void keys(int t, unsigned (&k)[4]) const {
-    float z[4];
-    logits(t, z);
+  // f(logit, token) for every token, the next tiles' loads under way.
+  template <typename F>
+  __device__ __forceinline__ void sweep(F f) const {
+    T z[2][4];
+    logits(0, z[0]);
+    if (tiles > 1) logits(1, z[1]);
+    for (int t = 0; t < tiles; ++t) {
+      T now[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) k[e] = logit_key(z[e], p.z_clamp);
+      for (int e = 0; e < 4; ++e) {
+        now[e] = z[0][e];
+        z[0][e] = z[1][e];
+      }
+      if (t + 2 < tiles) logits(t + 2, z[1]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f((float)now[e], first(t) + e);
+    }
   }
   // f(key, token) for every token that the prefix holds.
   template <typename F>
   __device__ __forceinline__ void each(const Prefix& in, F f) const {
-    for (int t = 0; t < tiles; ++t) {
-      unsigned k[4];
-      keys(t, k);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (k[e] != 0 && in_prefix(in, k[e], first(t) + e)) f(k[e], first(t) + e);
+    sweep([&](float z, int i) {
+      const unsigned k = logit_key(z, p.z_clamp);
+      if (k != 0 && in_prefix(in, k, i)) f(k, i);
+    });
+  }
+
+  // log2 rho(x), to 2^-43: |x| + sqrt(1 + x^2) = 2^e m, log2 m from the middle of m's 128th part and five
+  // terms of the series. The root is s rsqrt(s), the hardware's with one step of Newton's method.
+  __device__ __forceinline__ double log2_rho(unsigned key) const {
+    const double x = key == KEY_CLAMPED ? p.clamp : (double)key_logit(key) * p.inv_c, a = __builtin_fabs(x);
+    const double q = __builtin_fma(a, a, 1.0), y = __builtin_amdgcn_rsq(q), h = q * y;
+    const double r = a + __builtin_fma(0.5 * h, __builtin_fma(-h, y, 1.0), h);
+    const u64 b = __builtin_bit_cast(u64, r);
+    const int high = (int)(b >> 32);
+    const double m = __builtin_bit_cast(double, (b & 0x000FFFFFFFFFFFFFull) | 0x3FF0000000000000ull);
+    const double2 part = s.logs[(high >> 13) & 127];
+    const double t = __builtin_fma(m, part.x, -1.0);
+    constexpr double C = 1.4426950408889634;  // 1 / ln 2
+    double poly = __builtin_fma(t, C / 5, -C / 4);
+    poly = __builtin_fma(t, poly, C / 3);
+    poly = __builtin_fma(t, poly, -C / 2);
+    poly = __builtin_fma(t, poly, C);
+    const double l = __builtin_fma(t, poly, part.y + (double)((high >> 20) - 1023));
+    return x < 0.0 ? -l : l;
+  }
+  // The weight times 2^bits: 2^d of the nearest 64th below a table's and five terms of the series.
+  __device__ __forceinline__ double scaled(unsigned key) const {
+    const double d = fmax(power * (log2_rho(key) - log_top), -1000.0), j = __builtin_rint(d * 64.0);
+    const double f = __builtin_fma(j, -0.015625, d);
+    const int ji = (int)j;
+    constexpr double L = 0.6931471805599453;
+    double poly = __builtin_fma(f, L * L * L * L * L / 120, L * L * L * L / 24);
+    poly = __builtin_fma(f, poly, L * L * L / 6);
+    poly = __builtin_fma(f, poly, L * L / 2);
+    poly = __builtin_fma(f, poly, L);
+    poly = __builtin_fma(f, poly, 1.0);
+    return __builtin_amdgcn_ldexp(s.exps[ji & 63] * poly, (ji >> 6) + p.bits);
+  }
+  static __device__ __forceinline__ u64 whole_part(double v) {
+    const unsigned high = (unsigned)(v * 0x1p-32);
+    return (u64)high << 32 | (unsigned)__builtin_fma((double)high, -0x1p32, v);
+  }
+  __device__ __forceinline__ u64 mass(unsigned key) const { return whole_part(scaled(key)); }
+  __device__ void tables() {
+    if (tid < 128) {
+      const double inv = 1.0 / (1.0 + (tid + 0.5) / 128.0);
+      s.logs[tid] = make_double2(inv, -log2(inv));
+    } else if (tid < 192) {
+      s.exps[tid - 128] = exp2((tid - 128) / 64.0);
     }
   }
 
-  __device__ __forceinline__ double log2_rho(unsigned key) const {
-    const double x = key == KEY_CLAMPED ? p.clamp : (double)key_logit(key) * p.inv_c, a = fabs(x);
-    return copysign(log2(a + sqrt(1.0 + a * a)), x);
-  }
-  __device__ __forceinline__ double weight(unsigned key) const { return exp2(power * (log2_rho(key) - log_top)); }
-  __device__ __forceinline__ u64 mass(unsigned key) const { return (u64)rint(ldexp(weight(key), p.bits)); }
-
-  // The workgroup's sum.
-  __device__ u64 total(u64 v) {
-    v = wave_sum(v);
-    __syncthreads();
-    if (lane == 0) s.wave[wave] = v;
-    __syncthreads();
-    u64 sum = 0;
-    for (int w = 0; w < SAMPLE_WAVES; ++w) sum += s.wave[w];
-    return sum;
-  }
-  // The sum over the lanes up to this one's.
-  __device__ u64 scan(u64 v) {
+  // The sum over the lanes up to this one's, and over all.
+  __device__ u64 scan(u64 v, u64& total) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
       const u64 below = __shfl_up(v, m, 64);
@@ -144,30 +176,68 @@ struct Sampler {
     __syncthreads();
     if (lane == 63) s.wave[wave] = v;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) v += s.wave[w];
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < SAMPLE_WAVES; ++w) {
+      if (w == wave) v += total;
+      total += s.wave[w];
+    }
     return v;
   }
 
-  // The token at which the running sum of value(key, i), over tokens by their index, first passes `target`
-  // (less than the whole sum).
+  // The lanes' numbers in falling order, a lane each; `size` a power of two, the lanes from there on hold 0.
+  template <typename K>
+  __device__ K sorted(K v, int size) {
+    K* buf = reinterpret_cast<K*>(s.bins);
+    for (int block = 2; block <= size; block <<= 1)
+      for (int step = block >> 1; step > 0; step >>= 1) {
+        K o;
+        if (step < 64) {
+          o = __shfl_xor(v, step, 64);
+        } else {
+          __syncthreads();
+          buf[tid] = v;
+          __syncthreads();
+          o = buf[tid ^ step];
+        }
+        v = ((tid & step) == 0) == ((tid & block) == 0) ? max(v, o) : min(v, o);
+      }
+    return v;
+  }
+
+  // The sum of value(key, i) over all tokens, which pick() then draws from.
   template <typename F>
-  __device__ int draw(u64 target, F value) {
+  __device__ u64 sums(F value) {
+    T z[4];
+    logits(0, z);
     for (int t = 0; t < tiles; ++t) {
-      unsigned k[4];
-      keys(t, k);
+      T now[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) now[e] = z[e];
+      if (t + 1 < tiles) logits(t + 1, z);
       u64 v = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v += value(k[e], first(t) + e);
-      v = wave_sum(v);
+      for (int e = 0; e < 4; ++e) v += value(logit_key((float)now[e], p.z_clamp), first(t) + e);
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
       if (lane == 0) s.tile[t][wave] = v;
     }
     __syncthreads();
+    u64 v = 0, total;
+    for (int i = tid; i < tiles * SAMPLE_WAVES; i += SAMPLE_THREADS) v += (&s.tile[0][0])[i];
+    scan(v, total);
+    return total;
+  }
+  // The token at which the running sum, over tokens by their index, first passes `target` (less than the sum).
+  template <typename F>
+  __device__ int pick(u64 target, F value) {
     int t = 0, w = 0;
     u64 below = 0;
-    for (; t < tiles; ++t) {
+    for (; t < tiles - 1; ++t) {
       u64 sum = 0;
+#pragma unroll
       for (int i = 0; i < SAMPLE_WAVES; ++i) sum += s.tile[t][i];
-      if (below + sum > target || t == tiles - 1) break;
+      if (below + sum > target) break;
       below += sum;
     }
     for (; w < SAMPLE_WAVES - 1; ++w) {
@@ -175,11 +245,11 @@ struct Sampler {
       below += s.tile[t][w];
     }
     if (wave == w) {
-      unsigned k[4];
-      keys(t, k);
+      T z[4];
+      logits(t, z);
       u64 v[4], sum = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum += v[e] = value(k[e], first(t) + e);
+      for (int e = 0; e < 4; ++e) sum += v[e] = value(logit_key((float)z[e], p.z_clamp), first(t) + e);
       u64 upto = sum;
 #pragma unroll
       for (int m = 1; m < 64; m <<= 1) {
@@ -188,9 +258,13 @@ struct Sampler {
       }
       below += upto - sum;  // up to this lane's tokens
       if (below <= target && below + sum > target) {
-        int e = 0;
-        while (below + v[e] <= target) below += v[e++];
-        s.found.last = first(t) + e;
+        int last = first(t);
+#pragma unroll
+        for (int e = 0; e < 3; ++e) {
+          below += v[e];
+          last += below <= target;
+        }
+        s.found.last = last;
       }
     }
     __syncthreads();
@@ -199,13 +273,15 @@ struct Sampler {
     return got;
   }
 
-  // The shortest prefix, within `in`, whose values sum to `need` (at least 1, at most their sum).
-  template <typename F>
-  __device__ Prefix select(const Prefix& in, u64 need, F value) {
+  // The shortest prefix, within `in`, of whose tokens' values the sum reaches want(their sum) (at least 1, at most
+  // the sum; 0: all of `in`). Either a list of no more than SAMPLE_LIST tokens, sorted, with that prefix among its
+  // first (`listed` says how many it has), or `in` itself made shorter (`listed` = 0).
+  template <typename F, typename W>
+  __device__ void select(Prefix& in, int& listed, u64& need, F value, W want) {
     unsigned lo = 0, hi = top;
     u64 above = 0;
     // First by ranges of the logits themselves (a monotone function of the key, whatever it rounds), of 1/64 of
-    // the scale or as wide as 2048 of them have to be.
+    // the scale.
     const float z_top = top == KEY_CLAMPED ? p.z_clamp : key_logit(top);
     const float z_step = (float)(64.0 * p.inv_c);
     for (int round = 0;; ++round) {
@@ -215,62 +291,93 @@ struct Sampler {
         return (int)((hi - k) >> shift);
       };
       __syncthreads();
-      for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_THREADS) s.bins[i] = 0;
+      for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_THREADS) {
+        s.bins[i] = 0;
+        s.counts[i] = 0;
+      }
       if (tid == 0) {
         s.lo = 0xFFFFFFFFu;
         s.hi = s.count = 0;
       }
       __syncthreads();
       each(in, [&](unsigned k, int i) {
-        if (k >= lo && k <= hi) atomicAdd(&s.bins[bin(k)], value(k, i));
+        if (k < lo || k > hi) return;
+        const int b = bin(k);
+        atomicAdd(&s.bins[b], value(k, i));
+        atomicAdd(&s.counts[b], 1);
       });
       __syncthreads();
       const u64 a = s.bins[2 * tid], b = s.bins[2 * tid + 1];
-      const u64 upto = above + scan(a + b);
+      const int ca = s.counts[2 * tid], cb = s.counts[2 * tid + 1];
+      u64 total, tokens;
+      const u64 upto = above + scan(a + b, total);
+      const int held = (int)scan((u64)(ca + cb), tokens);
+      if (round == 0) need = want(total);
+      if (need == 0) return;
       const u64 before = upto - a - b;
       if (before < need && before + a >= need) {
         s.bin = 2 * tid;
         s.above = before;
+        s.upto = held - cb;
       } else if (before + a < need && upto >= need) {
         s.bin = 2 * tid + 1;
         s.above = before + a;
+        s.upto = held;
       }
       __syncthreads();
-      const int at = s.bin;
+      const int at = s.bin, count = s.counts[at];
+      const bool all = round == 0 && s.upto <= SAMPLE_LIST;  // that range's tokens and all above fit the list
       above = s.above;
-      // The tokens of that range: into the list, as many as it holds, with their extremes.
       each(in, [&](unsigned k, int i) {
-        if (k < lo || k > hi || bin(k) != at) return;
-        const unsigned n = atomicAdd(&s.count, 1u);
-        atomicMin(&s.lo, k);
-        atomicMax(&s.hi, k);
-        if (n < SAMPLE_LIST) {
-          s.list[n] = (u64)k << 32 | (unsigned)~i;
-          s.value[n] = value(k, i);
+        if (k < lo || k > hi) return;
+        const int b = bin(k);
+        if (b > at || (b < at && !all)) return;
+        if (!all) {
+          atomicMin(&s.lo, k);
+          atomicMax(&s.hi, k);
         }
+        const unsigned n = atomicAdd(&s.count, 1u);
+        if (n < SAMPLE_LIST) s.list[n] = (u64)k << 32 | (unsigned)~i;
       });
       __syncthreads();
-      const int count = (int)s.count;
       lo = s.lo;
       hi = s.hi;
-      if (count <= SAMPLE_LIST) {
-        if (tid < count) {
-          const u64 mine = s.list[tid];
-          u64 sum = above;
-          for (int i = 0; i < count; ++i)
-            if (s.list[i] > mine) sum += s.value[i];
-          if (sum < need && sum + s.value[tid] >= need) s.found = Prefix{(unsigned)(mine >> 32), (int)~(unsigned)mine};
+      if (all || count <= SAMPLE_LIST) {
+        const int n = all ? s.upto : count;
+        int size = 64;
+        while (size < n) size <<= 1;
+        const u64 mine = sorted(tid < n ? s.list[tid] : 0, size);
+        __syncthreads();
+        s.list[tid] = mine;
+        if (all) {
+          listed = n;
+          __syncthreads();
+          return;
         }
+        u64 ignored;
+        const u64 v = tid < n ? value((unsigned)(mine >> 32), (int)~(unsigned)mine) : 0;
+        const u64 sum = above + scan(v, ignored);
+        if (sum - v < need && sum >= need) s.found = Prefix{(unsigned)(mine >> 32), (int)~(unsigned)mine};
         __syncthreads();
-        const Prefix got = s.found;
+        in = s.found;
         __syncthreads();
-        return got;
+        return;
       }
       if (lo == hi) {  // one logit: as many of its tokens as it takes
         const u64 each_one = value(lo, 0), wanted = (need - above + each_one - 1) / each_one;
-        const int last = draw(wanted - 1, [&](unsigned k, int i) { return (u64)(k == lo && in_prefix(in, k, i)); });
-        return Prefix{lo, last};
+        const Prefix from = in;
+        const auto it = [&](unsigned k, int i) { return (u64)(k == lo && in_prefix(from, k, i)); };
+        sums(it);
+        in = Prefix{lo, pick(wanted - 1, it)};
+        return;
       }
+    }
+  }
+
+  __device__ void answer(int token, double logprob) {
+    if (tid == 0) {
+      p.token[blockIdx.x] = token;
+      p.logprob[blockIdx.x] = (float)logprob;
     }
   }
 
@@ -281,76 +388,84 @@ struct Sampler {
     const float least = p.min_p ? p.min_p[r] : p.min_p_all;
     const double min_p = least > 0.0f ? fminf(least, 1.0f) : 0.0f;  // the likeliest token stays
     const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
+    const double u = p.u_f64 ? static_cast<const double*>(p.u)[r] : (double)static_cast<const float*>(p.u)[r];
+    tables();
     // The largest logit, its first token, and whether one is NaN.
-    u64 best = 0;
+    unsigned best = 0;
+    int best_at = 0;
     bool nan = false;
-    for (int t = 0; t < tiles; ++t) {
-      float z[4];
-      logits(t, z);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        nan |= z[e] != z[e];
-        const u64 c = (u64)logit_key(z[e], p.z_clamp) << 32 | (unsigned)~(first(t) + e);
-        if (c > best) best = c;
+    sweep([&](float z, int i) {
+      nan |= z != z;
+      const unsigned k = logit_key(z, p.z_clamp);
+      if (k > best) {  // a lane meets its tokens by their index
+        best = k;
+        best_at = i;
       }
-    }
+    });
+    u64 c = (u64)best << 32 | (unsigned)~best_at;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const u64 o = __shfl_xor(best, m, 64);
-      if (o > best) best = o;
-    }
-    if (lane == 0) s.wave[wave] = best;
+    for (int m = 1; m < 64; m <<= 1) c = max(c, (u64)__shfl_xor(c, m, 64));
+    if (lane == 0) s.wave[wave] = c;
     nan = __syncthreads_or(nan) != 0;
-    for (int w = 0; w < SAMPLE_WAVES; ++w)
-      if (s.wave[w] > best) best = s.wave[w];
-    __syncthreads();
-    top = (unsigned)(best >> 32);
-    if (nan || top == 0 || !(temperature >= 0.0f)) {
-      if (tid == 0) {
-        p.token[r] = -1;
-        p.logprob[r] = __builtin_nanf("");
-      }
-      return;
-    }
-    if (temperature == 0.0f) {
-      if (tid == 0) {
-        p.token[r] = (int)~(unsigned)best;
-        p.logprob[r] = 0.0f;
-      }
-      return;
-    }
+#pragma unroll
+    for (int w = 0; w < SAMPLE_WAVES; ++w) c = max(c, s.wave[w]);
+    top = (unsigned)(c >> 32);
+    if (nan || top == 0 || !(temperature >= 0.0f)) return answer(-1, __builtin_nan(""));
+    if (temperature == 0.0f) return answer((int)~(unsigned)c, 0.0);
     power = p.n / (double)temperature;
     log_top = log2_rho(top);
+    unit = __builtin_amdgcn_ldexp(1.0, p.bits);
+
     Prefix in{0, p.V};
-    if (top_k > 0 && top_k < p.V) {
-      u64 tokens = 0;
-      each(in, [&](unsigned, int) { ++tokens; });
-      if ((u64)top_k < total(tokens)) in = select(in, top_k, [](unsigned, int) { return (u64)1; });
-    }
-    if (top_p < 1.0f) {
-      u64 m = 0;
-      each(in, [&](unsigned k, int) { m += mass(k); });
-      const double want = ceil((double)top_p * (double)total(m));
-      in = select(in, want >= 1.0 ? (u64)want : 1, [&](unsigned k, int) { return mass(k); });
+    int listed = 0;
+    u64 need = 0;
+    const bool cut_k = top_k > 0 && top_k < p.V, cut_p = top_p < 1.0f;
+    if (cut_k)
+      select(in, listed, need, [](unsigned, int) { return (u64)1; },
+             [&](u64 tokens) { return (u64)top_k < tokens ? (u64)top_k : (u64)0; });
+    const auto wanted = [&](u64 total) { return max((u64)ceil((double)top_p * (double)total), (u64)1); };
+    const int first_k = listed ? top_k : 0;  // of the list
+    if (cut_p && !listed) select(in, listed, need, [&](unsigned k, int) { return mass(k); }, wanted);
+
+    const double floor_v = min_p * unit;
+    // u as a share of `total`, and the tokens that it passes; below 0 or NaN as 0, 1 or more as the largest below.
+    const auto target = [&](u64 total) {
+      const double at = floor((u >= 0.0 ? u : 0.0) * (double)total);
+      return at < (double)total ? min((u64)at, total - 1) : total - 1;
+    };
+    if (listed) {
+      // The list's tokens, a lane each, by falling logit; then the kept ones by their index.
+      const u64 mine = s.list[tid];
+      const bool is = tid < (first_k ? first_k : listed);
+      const double v = is ? scaled((unsigned)(mine >> 32)) : 0.0;
+      const u64 m = is ? whole_part(v) : 0;
+      u64 total, kept_total;
+      const u64 upto = scan(m, total);
+      if (first_k) need = cut_p ? wanted(total) : total;
+      const bool keep = is && v >= floor_v && (tid == 0 || upto - m < need);
+      s.value[tid] = m;
+      int size = 64;
+      while (size < listed) size <<= 1;
+      const unsigned index = ~(unsigned)mine;
+      const unsigned by_index = sorted(keep ? ~(index << 10 | (unsigned)tid) : 0u, size);
+      __syncthreads();
+      const unsigned slot = ~by_index & 1023;
+      const u64 w = by_index ? s.value[slot] : 0;
+      const u64 sum = scan(w, kept_total), t = target(kept_total);
+      if (by_index && sum - w <= t && sum > t) {
+        p.token[r] = (int)(~by_index >> 10);
+        p.logprob[r] = (float)log((double)w / (double)kept_total);
+      }
+      return;
     }
     const auto kept = [&](unsigned k, int i) {
       if (k == 0 || !in_prefix(in, k, i)) return (u64)0;
-      const double w = weight(k);
-      return w >= min_p ? (u64)rint(ldexp(w, p.bits)) : (u64)0;
+      const double v = scaled(k);
+      return v >= floor_v ? whole_part(v) : (u64)0;
     };
-    u64 m = 0;
-    each(in, [&](unsigned k, int i) { m += kept(k, i); });
-    const u64 whole = total(m);
-    double u = p.u_f64 ? static_cast<const double*>(p.u)[r] : (double)static_cast<const float*>(p.u)[r];
-    u = u >= 0.0 ? u : 0.0;  // NaN too
-    const double at = floor(u * (double)whole);
-    const u64 target = at < (double)whole ? min((u64)at, whole - 1) : whole - 1;
-    const int token = draw(target, kept);
-    if (tid == 0) {
-      p.token[r] = token;
-      const unsigned k = logit_key((float)row[token], p.z_clamp);
-      p.logprob[r] = (float)log((double)kept(k, token) / (double)whole);
-    }
+    const u64 total = sums(kept);
+    const int token = pick(target(total), kept);
+    answer(token, tid == 0 ? log((double)kept(logit_key((float)row[token], p.z_clamp), token) / (double)total) : 0.0);
   }
 };
 
