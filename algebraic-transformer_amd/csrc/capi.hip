@@ -1557,7 +1557,7 @@ struct PagedPlan {
 static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int page, bool fp8 = false) {
   PagedPlan pl;
   const long G = H / Hkv, rows = N * G, seqs = std::max(1, std::min(S, N)), each = (rows + seqs - 1) / seqs;
-  pl.row_tiles = each <= 16 ? 1 : (each <= 32 || fp8 ? 2 : 0);
+  pl.row_tiles = each <= 16 ? 1 : (each <= 32 ? 2 : 0);
   const long tile = pl.row_tiles ? 16 * pl.row_tiles : alg::PK_ROWS;
   const long groups = seqs * ((each + tile - 1) / tile) * Hkv;
   const long cap = (long)width * page;
@@ -1647,8 +1647,8 @@ static int paged_attn(alg_stream_t stream, const char* name, bool fp8, int N, in
   p.part_o = static_cast<float*>(workspace);
   p.part_zt = pl.ws.total ? reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.ws.zt) : nullptr;
   const hipStream_t st = (hipStream_t)stream;
-  return hip_status(fp8 ? alg::launch_paged_decode_fp8(p, D, pl.row_tiles, st)
-                        : pl.row_tiles ? alg::launch_paged_decode(p, D, pl.row_tiles, st) : alg::launch_packed_fwd(p, D, true, st),
+  return hip_status(!pl.row_tiles ? alg::launch_packed_fwd(p, D, true, st)
+                    : fp8 ? alg::launch_paged_decode_fp8(p, D, pl.row_tiles, st) : alg::launch_paged_decode(p, D, pl.row_tiles, st),
                     name);
 }
 

@@ -355,10 +355,13 @@ __device__ __forceinline__ bf16x8 values8(int lo, int hi, float scale) {
 }
 
 // One 16-row group of a K / V tile: where its rows start, and how many of them exist.
-struct KvGroup {
-  const bf16* k;
-  const bf16* v;
+template <typename Stored>
+struct KvGroupOf {
+  const Stored* k;
+  const Stored* v;
+  const uint8_t *ks, *vs;  // 8 bits: their scales
   int rows;
 };
+typedef KvGroupOf<bf16> KvGroup;
 
 }  // namespace alg

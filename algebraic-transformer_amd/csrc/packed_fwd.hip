@@ -34,7 +34,7 @@
 
 namespace alg {
 
-template <int D, int L2N, bool PAGED>
+template <int D, int L2N, bool PAGED, bool KV8 = false>
 __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   static_assert(D == 64 || D == 128, "head_dim");
   constexpr int BK = PK_BK, CPR = D / 8, NDB = D / 32, NF = D / 16;
@@ -95,8 +95,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   const int nfull = posmin < 0 ? 0 : (posmin + 1) / BK;  // tiles before every row's position
 
   // The 16 keys of tile kt that this wave copies. Pages: one table entry, read a tile ahead.
-  const bf16* kbase = p.k + (size_t)kvh * p.k_hs + (PAGED ? 0 : (size_t)f.start * p.k_ts);
-  const bf16* vbase = p.v + (size_t)kvh * p.v_hs + (PAGED ? 0 : (size_t)f.start * p.v_ts);
+  typedef std::conditional_t<KV8, uint8_t, bf16> Stored;
+  const Stored* kbase = reinterpret_cast<const Stored*>(p.k) + (size_t)kvh * p.k_hs + (PAGED ? 0 : (size_t)f.start * p.k_ts);
+  const Stored* vbase = reinterpret_cast<const Stored*>(p.v) + (size_t)kvh * p.v_hs + (PAGED ? 0 : (size_t)f.start * p.v_ts);
   int pidx = 0, prow = 0;  // page of the group within the sequence, and row in the page
   if constexpr (PAGED) {
     const int key = kt0 * BK + 16 * wave;
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   int next_id = PAGED && pidx < p.width && kt0 < kt1 ? trow[pidx] : 0;
   bool bad = false;
   auto group = [&](int kt) {
-    KvGroup g;
+    KvGroupOf<Stored> g;
     const int key = kt * BK + 16 * wave;
     g.rows = kt < kt1 ? min(max(L - key, 0), 16) : 0;
     if constexpr (PAGED) {
@@ -120,6 +121,10 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
       id = g.rows > 0 ? id : 0;
       g.k = kbase + (size_t)id * p.k_ps + (size_t)prow * p.k_ts;
       g.v = vbase + (size_t)id * p.v_ps + (size_t)prow * p.v_ts;
+      if constexpr (KV8) {
+        g.ks = p.ks + (size_t)kvh * p.ks_hs + (size_t)id * p.ks_ps + prow;
+        g.vs = p.vs + (size_t)kvh * p.vs_hs + (size_t)id * p.vs_ps + prow;
+      }
       prow += BK;
       while (prow >= p.page) {
         prow -= p.page;
@@ -138,7 +143,8 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   const int lrow = lane / CPR;
   const int k_row = lrow * (int)p.k_ts * 2, v_row = lrow * (int)p.v_ts * 2;
   const int chunkb = 16 * ((lane % CPR) ^ swz_chunk<CPR>(lrow));
-  auto dma = [&](bf16* la, bf16* lb, const KvGroup& g, int j) {
+  auto dma = [&](bf16* la, bf16* lb, const KvGroupOf<Stored>& g, int j) {
+    if constexpr (!KV8) {
     const int kn = g.rows > 0 ? ((g.rows - 1) * (int)p.k_ts + D) * 2 : 0;
     const int vn = g.rows > 0 ? ((g.rows - 1) * (int)p.v_ts + D) * 2 : 0;
     const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)g.k, (short)0, kn, BUF_RSRC_WORD3);
@@ -151,15 +157,74 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     const int ko = RPI * j * (int)p.k_ts * 2, vo = RPI * j * (int)p.v_ts * 2;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lla + J * 512, 16, k_row + col + ko, 0, 0, 0);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, llb + J * 512, 16, v_row + col + vo, 0, 0, 0);
+    }
+  };
+  // A cache of 8 bits goes through registers: a lane a quarter of a key's row, D / 4 bytes each of K and V, fetched
+  // while a tile is computed, made bf16 (exactly, packed_common.h) and written into the tiles one 16-byte
+  // chunk after the other.
+  constexpr int NC = D / 32;  // chunks a lane
+  struct Fetched {
+    int k[D / 16], v[D / 16];
+    float ks, vs;
+  };
+  Fetched next8;
+  auto fetch = [&](const KvGroupOf<Stored>& g) {
+    if constexpr (KV8) {
+      const int row = lane >> 2, col = (lane & 3) * (D / 4);
+      const int kn = g.rows > 0 ? (g.rows - 1) * (int)p.k_ts + D : 0, vn = g.rows > 0 ? (g.rows - 1) * (int)p.v_ts + D : 0;
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)g.k, (short)0, kn, BUF_RSRC_WORD3);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)g.v, (short)0, vn, BUF_RSRC_WORD3);
+      const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc((void*)g.ks, (short)0, g.rows, BUF_RSRC_WORD3);
+      const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc((void*)g.vs, (short)0, g.rows, BUF_RSRC_WORD3);
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const auto a = __builtin_amdgcn_raw_buffer_load_b128(rk, row * (int)p.k_ts + col + 16 * i, 0, 0);
+        const auto b = __builtin_amdgcn_raw_buffer_load_b128(rv, row * (int)p.v_ts + col + 16 * i, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          next8.k[4 * i + e] = a[e];
+          next8.v[4 * i + e] = b[e];
+        }
+      }
+      next8.ks = scale_value(__builtin_amdgcn_raw_buffer_load_b8(rks, row, 0, 0));
+      next8.vs = scale_value(__builtin_amdgcn_raw_buffer_load_b8(rvs, row, 0, 0));
+    }
+  };
+  // A key whose value was not finite (its bytes are zeros, its scale 255) becomes a NaN key: the rows that
+  // see it are NaN, and the others do not meet it as a factor of their zero weights.
+  auto mark = [&]() {
+    if constexpr (KV8) {
+      const bool lost = isinf(next8.vs);
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) next8.k[e] = lost ? 0x7F7F7F7F : next8.k[e];
+      next8.vs = lost ? 1.0f : next8.vs;
+      next8.ks = isinf(next8.ks) ? 1.0f : next8.ks;
+    }
+  };
+  auto put = [&](bf16* la, bf16* lb, int c) {
+    if constexpr (KV8) {
+      const int row = 16 * wave + (lane >> 2), at = row * D + (((NC * (lane & 3) + c) ^ swz_chunk<CPR>(row)) << 3);
+      *reinterpret_cast<bf16x8*>(la + at) = values8(next8.k[2 * c], next8.k[2 * c + 1], next8.ks);
+      *reinterpret_cast<bf16x8*>(lb + at) = values8(next8.v[2 * c], next8.v[2 * c + 1], next8.vs);
+    }
+  };
+  auto put_all = [&](bf16* la, bf16* lb) {
+    if constexpr (KV8) {
+      mark();
+#pragma unroll
+      for (int c = 0; c < NC; ++c) put(la, lb, c);
+    }
   };
 
   if constexpr (PAGED) {
     if (threadIdx.x == 0) bad_page = 0;
   }
   {
-    const KvGroup g = group(kt0);
+    const KvGroupOf<Stored> g = group(kt0);
+    fetch(g);
 #pragma unroll
     for (int j = 0; j < PW; ++j) dma(Ks0, Vs0, g, j);
+    put_all(Ks0, Vs0);
   }
   // Query fragments (B operand of S^T = K Q^T), held for the whole kernel; dead rows are zero.
   bf16x8 qf[NF];
@@ -209,11 +274,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     bf16* Kn = BUF ? Ks0 : Ks1;
     bf16* Vn = BUF ? Vs0 : Vs1;
     const int kb0 = kt * BK;
-    const KvGroup gn = group(kt + 1);
+    const KvGroupOf<Stored> gn = group(kt + 1);
+    fetch(gn);
     if constexpr (MASKED) {
       if (kb0 > wave_posmax) {  // every key lies after this wave's rows
 #pragma unroll
         for (int j = 0; j < PW; ++j) dma(Kn, Vn, gn, j);
+        put_all(Kn, Vn);
         __builtin_amdgcn_s_waitcnt(VMCNT0);
         __syncthreads();
         rk3[0] = ld8(Kn + row_off[0]);
@@ -278,13 +345,16 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
       for (int k = 0; k < E3; ++k) elem(1, E3 * db + k);
       step_order<2, VE * E3, 4, 0>();
     }
+    mark();
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
       const int c = (db + NDB) & 1;
       if (db + 1 < NDB) pv_load(1, db + 1, ft[c ^ 1]);
       oacc[db] = mfma_bf16(ft[c][0], pf[1][0], oacc[db]);
       oacc[db] = mfma_bf16(ft[c][1], pf[1][1], oacc[db]);
-      step_order<2, 0, 4, 0>();
+      put(Kn, Vn, db);
+      if constexpr (KV8) step_order<2, 8, 4, 2>();
+      else step_order<2, 0, 4, 0>();
     }
     __builtin_amdgcn_s_waitcnt(VMCNT0);  // this wave's copies of the next tile have landed
     __syncthreads();                     // the next tile is complete; this buffer set is free
@@ -339,9 +409,11 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
     }
     for (int kt = kt0; kt < kt1; ++kt) {
       __syncthreads();  // every wave is done with the tile before
-      const KvGroup g = group(kt);
+      const KvGroupOf<Stored> g = group(kt);
+      fetch(g);
 #pragma unroll
       for (int j = 0; j < PW; ++j) dma(Ks0, Vs0, g, j);
+      put_all(Ks0, Vs0);
       __builtin_amdgcn_s_waitcnt(VMCNT0);
       __syncthreads();
       for (int blk = 0; blk < 2; ++blk) {
@@ -568,10 +640,10 @@ __global__ __launch_bounds__(256) void packed_combine_wide_kernel(PackedParams p
   else out[0] = f2bf(acc[0] * inv);
 }
 
-template <int D, bool PAGED>
+template <int D, bool PAGED, bool KV8 = false>
 static void launch_fwd(const PackedParams& p, dim3 grid, hipStream_t st) {
-  if (p.sc.log2n == 4) hipLaunchKernelGGL((packed_fwd_kernel<D, 4, PAGED>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((packed_fwd_kernel<D, 0, PAGED>), grid, dim3(256), 0, st, p);
+  if (p.sc.log2n == 4) hipLaunchKernelGGL((packed_fwd_kernel<D, 4, PAGED, KV8>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((packed_fwd_kernel<D, 0, PAGED, KV8>), grid, dim3(256), 0, st, p);
 }
 
 template <int D>
@@ -594,8 +666,9 @@ hipError_t launch_packed_combine(const PackedParams& p, int D, hipStream_t st) {
 hipError_t launch_packed_fwd(const PackedParams& p, int D, bool paged, hipStream_t st) {
   const dim3 grid(p.Hkv * p.nsplit * packed_slots(p.N, p.G, p.S, PK_ROWS));
   {
-    KTimer t(paged ? "paged_fwd" : "packed_fwd", st);
-    if (D == 64) paged ? launch_fwd<64, true>(p, grid, st) : launch_fwd<64, false>(p, grid, st);
+    KTimer t(p.ks ? "paged_fwd_fp8" : paged ? "paged_fwd" : "packed_fwd", st);
+    if (p.ks) D == 64 ? launch_fwd<64, true, true>(p, grid, st) : launch_fwd<128, true, true>(p, grid, st);
+    else if (D == 64) paged ? launch_fwd<64, true>(p, grid, st) : launch_fwd<64, false>(p, grid, st);
     else paged ? launch_fwd<128, true>(p, grid, st) : launch_fwd<128, false>(p, grid, st);
   }
   const hipError_t e = hipGetLastError();
