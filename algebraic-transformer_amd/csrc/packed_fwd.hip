@@ -161,58 +161,64 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
   };
   // A cache of 8 bits goes through registers: a lane a quarter of a key's row, D / 4 bytes each of K and V, fetched
   // while a tile is computed, made bf16 (exactly, packed_common.h) and written into the tiles one 16-byte
-  // chunk after the other.
+  // chunk after the other, beside the last products, which leave the VALU free. 16 neighbouring lanes hold 16
+  // rows, whose chunks the swizzle keeps in 16 parts of the banks (four rows of four lanes each: 217 us, 200
+  // so). Descriptors and byte scales stay scalar and unshifted until used: a wait for them here would be one
+  // for the whole fetch.
   constexpr int NC = D / 32;  // chunks a lane
   struct Fetched {
     int k[D / 16], v[D / 16];
-    float ks, vs;
+    int ks, vs;  // bytes; from mark() on the scales' bits
   };
   Fetched next8;
   auto fetch = [&](const KvGroupOf<Stored>& g) {
     if constexpr (KV8) {
-      const int row = lane >> 2, col = (lane & 3) * (D / 4);
+      const int l = again(lane), row = l & 15, col = (l >> 4) * (D / 4);
       const int kn = g.rows > 0 ? (g.rows - 1) * (int)p.k_ts + D : 0, vn = g.rows > 0 ? (g.rows - 1) * (int)p.v_ts + D : 0;
+      const int sn = g.rows > 0 ? 16 : 0;  // a page holds all 16 places
       const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)g.k, (short)0, kn, BUF_RSRC_WORD3);
       const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)g.v, (short)0, vn, BUF_RSRC_WORD3);
-      const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc((void*)g.ks, (short)0, g.rows, BUF_RSRC_WORD3);
-      const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc((void*)g.vs, (short)0, g.rows, BUF_RSRC_WORD3);
+      const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc((void*)g.ks, (short)0, sn, BUF_RSRC_WORD3);
+      const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc((void*)g.vs, (short)0, sn, BUF_RSRC_WORD3);
+      const int ko = __umul24(row, (int)p.k_ts) + col, vo = __umul24(row, (int)p.v_ts) + col;  // strides are under 2^24
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
-        const auto a = __builtin_amdgcn_raw_buffer_load_b128(rk, row * (int)p.k_ts + col + 16 * i, 0, 0);
-        const auto b = __builtin_amdgcn_raw_buffer_load_b128(rv, row * (int)p.v_ts + col + 16 * i, 0, 0);
+        const auto a = __builtin_amdgcn_raw_buffer_load_b128(rk, ko, 16 * i, 0);
+        const auto b = __builtin_amdgcn_raw_buffer_load_b128(rv, vo, 16 * i, 0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           next8.k[4 * i + e] = a[e];
           next8.v[4 * i + e] = b[e];
         }
       }
-      next8.ks = scale_value(__builtin_amdgcn_raw_buffer_load_b8(rks, row, 0, 0));
-      next8.vs = scale_value(__builtin_amdgcn_raw_buffer_load_b8(rvs, row, 0, 0));
+      next8.ks = __builtin_amdgcn_raw_buffer_load_b8(rks, row, 0, 0);
+      next8.vs = __builtin_amdgcn_raw_buffer_load_b8(rvs, row, 0, 0);
     }
   };
   // A key whose value was not finite (its bytes are zeros, its scale 255) becomes a NaN key: the rows that
   // see it are NaN, and the others do not meet it as a factor of their zero weights.
   auto mark = [&]() {
+    int at = 0;  // where the lane's first chunk goes
     if constexpr (KV8) {
-      const bool lost = isinf(next8.vs);
-#pragma unroll
-      for (int e = 0; e < D / 16; ++e) next8.k[e] = lost ? 0x7F7F7F7F : next8.k[e];
-      next8.vs = lost ? 1.0f : next8.vs;
-      next8.ks = isinf(next8.ks) ? 1.0f : next8.ks;
+      next8.k[0] |= next8.vs == 255 ? 0x7F7F7F7F : 0;  // one element is enough
+      next8.vs = min(next8.vs, 254) << 23;
+      next8.ks <<= 23;
+      const int l = again(lane), row = 16 * wave + (l & 15);
+      at = row * D + (((NC * (l >> 4)) ^ swz_chunk<CPR>(row)) << 3);
     }
+    return at;
   };
-  auto put = [&](bf16* la, bf16* lb, int c) {
+  auto put = [&](bf16* la, bf16* lb, int at, int c) {
     if constexpr (KV8) {
-      const int row = 16 * wave + (lane >> 2), at = row * D + (((NC * (lane & 3) + c) ^ swz_chunk<CPR>(row)) << 3);
-      *reinterpret_cast<bf16x8*>(la + at) = values8(next8.k[2 * c], next8.k[2 * c + 1], next8.ks);
-      *reinterpret_cast<bf16x8*>(lb + at) = values8(next8.v[2 * c], next8.v[2 * c + 1], next8.vs);
+      *reinterpret_cast<bf16x8*>(la + (at ^ (8 * c))) = values8(next8.k[2 * c], next8.k[2 * c + 1], __builtin_bit_cast(float, next8.ks));
+      *reinterpret_cast<bf16x8*>(lb + (at ^ (8 * c))) = values8(next8.v[2 * c], next8.v[2 * c + 1], __builtin_bit_cast(float, next8.vs));
     }
   };
   auto put_all = [&](bf16* la, bf16* lb) {
     if constexpr (KV8) {
-      mark();
+      const int at = mark();
 #pragma unroll
-      for (int c = 0; c < NC; ++c) put(la, lb, c);
+      for (int c = 0; c < NC; ++c) put(la, lb, at, c);
     }
   };
 
@@ -345,14 +351,14 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedParams p) {
       for (int k = 0; k < E3; ++k) elem(1, E3 * db + k);
       step_order<2, VE * E3, 4, 0>();
     }
-    mark();
+    const int put_at = mark();
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
       const int c = (db + NDB) & 1;
       if (db + 1 < NDB) pv_load(1, db + 1, ft[c ^ 1]);
       oacc[db] = mfma_bf16(ft[c][0], pf[1][0], oacc[db]);
       oacc[db] = mfma_bf16(ft[c][1], pf[1][1], oacc[db]);
-      put(Kn, Vn, db);
+      put(Kn, Vn, put_at, db);
       if constexpr (KV8) step_order<2, 8, 4, 2>();
       else step_order<2, 0, 4, 0>();
     }
