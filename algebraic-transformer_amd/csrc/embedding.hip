@@ -21,9 +21,10 @@ namespace alg {
 namespace {
 
 constexpr int EMB_THREADS = 256;
-constexpr int SORT_BLOCK = 2048;  // tokens a workgroup of a pass takes
-constexpr int SORT_WAVES = EMB_THREADS / 64, SORT_EACH = SORT_BLOCK / SORT_WAVES;
-constexpr int ZERO_ROWS = 16;     // rows of the table that a workgroup looks after for zeros
+constexpr int SORT_BLOCK = 1024;  // tokens a workgroup of a pass takes, one a lane
+constexpr int SORT_WAVES = SORT_BLOCK / 64;
+constexpr int SORT_COUNT = 32;    // blocks up to which each counts all tokens
+constexpr int ZERO_ROWS = 32;     // rows of the table that a workgroup looks after for zeros
 constexpr int EMB_COLS = 512;     // columns a wave takes: 8 a lane
 
 template <typename T>
@@ -58,6 +59,9 @@ __device__ __forceinline__ int token_key(const EmbeddingParams& p, int i) {
   const long t = token_at(p, i);
   return t >= 0 && t < p.V ? (int)t : p.V;
 }
+__device__ __forceinline__ int sort_key(const EmbeddingParams& p, int pass, int i) {
+  return pass ? p.keys[(pass - 1) & 1][i] : token_key(p, i);
+}
 
 }  // namespace
 
@@ -83,87 +87,114 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_fwd_kernel(EmbeddingPar
 }
 
 // How often each value of 8 bits of the key occurs in each block of tokens.
-__global__ __launch_bounds__(EMB_THREADS) void embedding_hist_kernel(EmbeddingParams p, int pass) {
+__global__ __launch_bounds__(SORT_BLOCK) void embedding_hist_kernel(EmbeddingParams p, int pass) {
   __shared__ int count[256];
-  count[threadIdx.x] = 0;
+  const int i = blockIdx.x * SORT_BLOCK + threadIdx.x;
+  if (threadIdx.x < 256) count[threadIdx.x] = 0;
   __syncthreads();
-  const int end = min(p.N, (int)(blockIdx.x + 1) * SORT_BLOCK);
-  for (int i = blockIdx.x * SORT_BLOCK + threadIdx.x; i < end; i += EMB_THREADS) {
-    const int key = pass ? p.keys[(pass - 1) & 1][i] : token_key(p, i);
-    atomicAdd(&count[(key >> (8 * pass)) & 255], 1);
-  }
+  if (i < p.N) atomicAdd(&count[(sort_key(p, pass, i) >> (8 * pass)) & 255], 1);
   __syncthreads();
-  p.hist[threadIdx.x * p.blocks + blockIdx.x] = count[threadIdx.x];
+  if (threadIdx.x < 256) p.hist[threadIdx.x * p.blocks + blockIdx.x] = count[threadIdx.x];
 }
 
-// Each token to its place in the order of these 8 bits, equal ones as they stand. A wave takes a stretch of the
-// block's tokens, 64 at a time; lanes of equal bits find each other by ballots.
-__global__ __launch_bounds__(EMB_THREADS) void embedding_scatter_kernel(EmbeddingParams p, int pass) {
-  __shared__ int base[SORT_WAVES][256], sums[256];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // Where the block's tokens of value `tid` begin: after the lower values and the earlier blocks.
+// Each token to its place in the order of these 8 bits, equal ones as they stand: a workgroup 1024 tokens, a wave
+// 64, whose lanes of equal bits find each other by ballots. With few tokens every workgroup counts them all
+// itself, which takes as long as a launch that counts them, and saves it (16384 tokens, two passes: 18 us so, 25).
+template <bool COUNT>
+__global__ __launch_bounds__(SORT_BLOCK) void embedding_scatter_kernel(EmbeddingParams p, int pass) {
+  __shared__ int base[SORT_WAVES][256], sums[256], before[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, begin = blockIdx.x * SORT_BLOCK;
+  const int i = begin + tid;
+  const bool live = i < p.N;
+  const int key = live ? sort_key(p, pass, i) : 0, bits = (key >> (8 * pass)) & 255;
+  const int where = live && pass ? p.pos[(pass - 1) & 1][i] : i;
+  // How many tokens of value `tid` there are, and how many in the blocks before this one.
   int total = 0, earlier = 0;
-  for (int b = 0; b < p.blocks; ++b) {
-    const int c = p.hist[tid * p.blocks + b];
-    if (b < (int)blockIdx.x) earlier += c;
-    total += c;
-  }
-  sums[tid] = total;
-#pragma unroll
-  for (int w = 0; w < SORT_WAVES; ++w) base[w][tid] = 0;
-  __syncthreads();
-  for (int m = 1; m < 256; m <<= 1) {
-    const int below = tid >= m ? sums[tid - m] : 0;
+  if constexpr (COUNT) {
+    if (tid < 256) sums[tid] = before[tid] = 0;
     __syncthreads();
-    sums[tid] += below;
+    for (int k0 = tid; k0 < p.N; k0 += 8 * SORT_BLOCK) {
+      int k[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int at = k0 + e * SORT_BLOCK;
+        k[e] = at < p.N ? (sort_key(p, pass, at) >> (8 * pass)) & 255 : -1;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k[e] >= 0) atomicAdd(k0 + e * SORT_BLOCK < begin ? &before[k[e]] : &sums[k[e]], 1);
+    }
     __syncthreads();
-  }
-  const int begin = blockIdx.x * SORT_BLOCK + wave * SORT_EACH, end = min(p.N, begin + SORT_EACH);
-  const auto same = [&](int bits, bool live) {  // the lanes with these bits
-    unsigned long long m = __ballot(live);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const unsigned long long set = __ballot((bits >> k) & 1);
-      m &= (bits >> k) & 1 ? set : ~set;
+    if (tid < 256) {
+      earlier = before[tid];
+      total = earlier + sums[tid];
     }
-    return m;
-  };
-  for (int i0 = begin; i0 < end; i0 += 64) {
-    const int i = i0 + lane;
-    const bool live = i < end;
-    const int key = live ? (pass ? p.keys[(pass - 1) & 1][i] : token_key(p, i)) : 0, bits = (key >> (8 * pass)) & 255;
-    const unsigned long long m = same(bits, live);
-    if (live && lane == __builtin_ctzll(m)) base[wave][bits] += __popcll(m);
+    __syncthreads();
+  } else if (tid < 256) {
+    for (int b = 0; b < p.blocks; ++b) {
+      const int c = p.hist[tid * p.blocks + b];
+      if (b < (int)blockIdx.x) earlier += c;
+      total += c;
+    }
+  }
+  // The tokens of lower values: a sum over 256 lanes, four waves.
+  int upto = total;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int below = __shfl_up(upto, m, 64);
+    if (lane >= m) upto += below;
+  }
+  if (tid < 256 && lane == 63) sums[wave] = upto;
+  // The wave's lanes of the same bits.
+  unsigned long long same = __ballot(live);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const unsigned long long set = __ballot((bits >> k) & 1);
+    same &= (bits >> k) & 1 ? set : ~set;
+  }
+  for (int w = tid; w < SORT_WAVES * 256; w += SORT_BLOCK) (&base[0][0])[w] = 0;
+  __syncthreads();
+  const int rank = __popcll(same & ((1ull << lane) - 1));
+  if (live && rank == 0) base[wave][bits] = __popcll(same);
+  if (tid < 256)
+    for (int w = 0; w < wave; ++w) upto += sums[w];
+  __syncthreads();
+  if (tid < 256) {
+    int at = upto - total + earlier;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      const int c = base[w][tid];
+      base[w][tid] = at;
+      at += c;
+    }
   }
   __syncthreads();
-  int at = sums[tid] - total + earlier;
-#pragma unroll
-  for (int w = 0; w < SORT_WAVES; ++w) {
-    const int c = base[w][tid];
-    base[w][tid] = at;
-    at += c;
-  }
-  __syncthreads();
-  for (int i0 = begin; i0 < end; i0 += 64) {
-    const int i = i0 + lane;
-    const bool live = i < end;
-    const int key = live ? (pass ? p.keys[(pass - 1) & 1][i] : token_key(p, i)) : 0, bits = (key >> (8 * pass)) & 255;
-    const unsigned long long m = same(bits, live);
-    if (live) {
-      const int to = base[wave][bits] + __popcll(m & ((1ull << lane) - 1));
-      p.keys[pass & 1][to] = key;
-      p.pos[pass & 1][to] = pass ? p.pos[(pass - 1) & 1][i] : i;
-    }
-    __builtin_amdgcn_wave_barrier();
-    if (live && lane == __builtin_ctzll(m)) base[wave][bits] += __popcll(m);
-    __builtin_amdgcn_wave_barrier();
+  if (live) {
+    const int to = base[wave][bits] + rank;
+    p.keys[pass & 1][to] = key;
+    p.pos[pass & 1][to] = where;
   }
 }
 
-// Runs of equal tokens: a wave one chunk of sorted tokens and EMB_COLS columns; the workgroups behind those the
-// rows without a token.
+// The first of n sorted keys that is not below v: 64 of them looked at each time.
+__device__ __forceinline__ int lower_bound(const int* keys, int n, int v) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  while (n > 0) {
+    const int step = (n + 63) / 64, at = lane * step;
+    const int c = __popcll(__ballot(at < n && keys[lo + at] < v));
+    if (c == 0) break;
+    lo += (c - 1) * step + 1;
+    n = min(step, n - (c - 1) * step) - 1;
+  }
+  return lo;
+}
+
+// Runs of equal tokens: a wave one chunk of sorted tokens and EMB_COLS columns, BATCH rows' loads under way at a
+// time; the workgroups behind those the rows without a token.
 template <typename E, typename Y>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_bwd_kernel(EmbeddingParams p) {
+  constexpr int BATCH = sizeof(Y) == 2 ? 16 : 8;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int* keys = p.keys[(p.passes - 1) & 1];
   const int* pos = p.pos[(p.passes - 1) & 1];
@@ -171,22 +202,21 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_bwd_kernel(EmbeddingPar
   const int work = (units + EMB_THREADS / 64 - 1) / (EMB_THREADS / 64);
   E* grad = static_cast<E*>(p.grad);
   if ((int)blockIdx.x >= work) {
-    // The first sorted token of each of these rows, by halving; a row is empty if the next one's is the same.
-    __shared__ int first[ZERO_ROWS + 1];
+    __shared__ int ends[2];
+    __shared__ int held[ZERO_ROWS];
     const int v0 = (blockIdx.x - work) * ZERO_ROWS;
-    if (threadIdx.x <= ZERO_ROWS) {
-      int lo = 0, hi = p.N;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (keys[mid] < v0 + (int)threadIdx.x) lo = mid + 1;
-        else hi = mid;
-      }
-      first[threadIdx.x] = lo;
+    if (threadIdx.x < ZERO_ROWS) held[threadIdx.x] = 0;
+    if (wave < 2) {
+      const int at = lower_bound(keys, p.N, v0 + wave * ZERO_ROWS);
+      if (lane == 0) ends[wave] = at;
     }
+    __syncthreads();
+    for (int i = ends[0] + threadIdx.x; i < ends[1]; i += EMB_THREADS)
+      if (keys[i] < p.V) held[keys[i] - v0] = 1;
     __syncthreads();
     const float zero[8] = {};
     for (int r = 0; r < min(ZERO_ROWS, p.V - v0); ++r)
-      if (first[r] == first[r + 1])
+      if (!held[r])
         for (int c = 8 * threadIdx.x; c < p.d; c += 8 * EMB_THREADS) store8(grad + (size_t)(v0 + r) * p.d + c, zero);
     return;
   }
@@ -197,8 +227,9 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_bwd_kernel(EmbeddingPar
   const int begin = j * p.chunk, end = min(p.N, begin + p.chunk);
   const Y* dy = static_cast<const Y*>(p.y) + (live ? col : 0);
   float sum[8] = {};
-  int run = keys[begin];
+  int run = __builtin_amdgcn_readfirstlane(keys[begin]);
   bool head = begin > 0 && keys[begin - 1] == run;  // the run began before the chunk
+  const bool tail = end < p.N && keys[end] == keys[end - 1];
   const auto leave = [&](bool tail) {
     if (run < p.V && live) {
       if (head || tail) {
@@ -213,24 +244,36 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_bwd_kernel(EmbeddingPar
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
   };
-  for (int i = begin; i < end; ++i) {
-    const int key = keys[i];
-    if (key != run) {
-      leave(false);
-      run = key;
-    }
-    if (key >= p.V) break;  // tokens without a row are the last
-    float x[8];
-    load8(dy + (size_t)pos[i] * p.d, x);
+  for (int i0 = begin; i0 < end; i0 += 64) {
+    const int n = min(64, end - i0);
+    const int at = i0 + min(lane, n - 1), my_key = keys[at], my_pos = pos[at];
+    for (int b = 0; b < n; b += BATCH) {
+      Y x[BATCH][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] += x[e];
+      for (int e = 0; e < BATCH; ++e) {  // rows past the end again the last one
+        const int row = __builtin_amdgcn_readlane(my_pos, min(b + e, n - 1));
+        __builtin_memcpy(x[e], __builtin_assume_aligned(dy + (size_t)row * p.d, 16), sizeof x[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        if (b + e >= n) break;
+        const int key = __builtin_amdgcn_readlane(my_key, b + e);
+        if (key != run) {
+          leave(false);
+          run = key;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) sum[c] += (float)x[e][c];
+      }
+    }
   }
-  leave(end < p.N && keys[end] == run);
+  leave(tail);
 }
 
-// Runs over several chunks: the wave of the chunk where one begins adds up its parts.
+// Runs over several chunks: the wave of the chunk where one begins adds up its parts, in order.
 template <typename E>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(EmbeddingParams p) {
+  constexpr int BATCH = 8;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int* keys = p.keys[(p.passes - 1) & 1];
   const int strips = (p.d + EMB_COLS - 1) / EMB_COLS;
@@ -238,16 +281,31 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(EmbeddingPa
   const int j = unit / strips, col = (unit - j * strips) * EMB_COLS + 8 * lane;
   const int end = (j + 1) * p.chunk;
   if (j >= p.chunks || end >= p.N) return;
-  const int run = keys[end - 1];
-  if (run >= p.V || keys[end] != run || (j > 0 && keys[j * p.chunk - 1] == run)) return;
-  if (col >= p.d) return;
-  float sum[8], x[8];
-  load8(p.part + ((size_t)2 * j + 1) * p.d + col, sum);
-  for (int i = j + 1; i < p.chunks && keys[i * p.chunk] == run; ++i) {
-    load8(p.part + (size_t)2 * i * p.d + col, x);
+  const int run = keys[end - 1], next = keys[end], last = j > 0 ? keys[j * p.chunk - 1] : -1;
+  if (run >= p.V || next != run || last == run) return;
+  const bool live = col < p.d;
+  float sum[8] = {};
+  if (live) load8(p.part + ((size_t)2 * j + 1) * p.d + col, sum);
+  for (int i0 = j + 1; i0 < p.chunks; i0 += 64) {
+    // How many of these chunks begin with the run.
+    const int i = i0 + lane;
+    const unsigned long long more = __ballot(i < p.chunks && keys[min(i, p.chunks - 1) * p.chunk] == run);
+    const int n = more == ~0ull ? 64 : __builtin_ctzll(~more);
+    for (int b = 0; b < n; b += BATCH) {
+      float x[BATCH][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] += x[e];
+      for (int e = 0; e < BATCH; ++e)
+        load8(p.part + (size_t)2 * (i0 + min(b + e, n - 1)) * p.d + (live ? col : 0), x[e]);
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        if (b + e >= n) break;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) sum[c] += x[e][c];
+      }
+    }
+    if (n < 64) break;
   }
+  if (!live) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[e] *= p.scale;
   store8(static_cast<E*>(p.grad) + (size_t)run * p.d + col, sum);
@@ -279,8 +337,12 @@ hipError_t launch_embedding_bwd(const EmbeddingParams& p, hipStream_t st) {
   if (p.N) {
     KTimer t("embedding_sort", st);
     for (int pass = 0; pass < p.passes; ++pass) {
-      hipLaunchKernelGGL(embedding_hist_kernel, dim3(p.blocks), dim3(EMB_THREADS), 0, st, p, pass);
-      hipLaunchKernelGGL(embedding_scatter_kernel, dim3(p.blocks), dim3(EMB_THREADS), 0, st, p, pass);
+      if (p.blocks <= SORT_COUNT) {
+        hipLaunchKernelGGL(embedding_scatter_kernel<true>, dim3(p.blocks), dim3(SORT_BLOCK), 0, st, p, pass);
+      } else {
+        hipLaunchKernelGGL(embedding_hist_kernel, dim3(p.blocks), dim3(SORT_BLOCK), 0, st, p, pass);
+        hipLaunchKernelGGL(embedding_scatter_kernel<false>, dim3(p.blocks), dim3(SORT_BLOCK), 0, st, p, pass);
+      }
     }
   }
   const long strips = (p.d + EMB_COLS - 1) / EMB_COLS, work = (p.chunks * strips + 3) / 4;
