@@ -28,15 +28,16 @@ class _EmbeddingFn(torch.autograd.Function):
             _lib.check(_lib.load().alg_embedding_fwd(
                 _lib.stream_of(embed), N, d, V, p(tokens), _INTS[tokens.dtype], p(table), _FLOATS[table.dtype], scale,
                 p(y), _FLOATS[dtype]), "token_embedding")
-        ctx.save_for_backward(tokens, y)
+        ctx.save_for_backward(tokens)
         ctx.meta = (V, d, scale, embed.dtype)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        tokens, y = ctx.saved_tensors
+        tokens, = ctx.saved_tensors
         V, d, scale, dtype = ctx.meta
         lib = _lib.load()
+        cotangent = dy  # all that the gradient depends on: differentiating it by that raises
         dy = _lib.aligned16(dy if dy.dtype in _FLOATS else dy.float())
         N = tokens.numel()
         grad = torch.empty(V, d, dtype=dtype, device=dy.device)
@@ -47,7 +48,7 @@ class _EmbeddingFn(torch.autograd.Function):
             _lib.check(lib.alg_embedding_bwd(
                 _lib.stream_of(dy), N, d, V, p(tokens), _INTS[tokens.dtype], p(dy), _FLOATS[dy.dtype], scale, p(grad),
                 _FLOATS[dtype], p(ws), nbytes), "token_embedding backward")
-        return None, *first_order("token_embedding", y, grad), None, None
+        return None, *first_order("token_embedding", cotangent, grad), None, None
 
 
 def token_embedding(tokens, embed, *, scale: float = 1.0, dtype: Optional[torch.dtype] = None):
