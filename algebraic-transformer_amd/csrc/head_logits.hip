@@ -1,13 +1,14 @@
 // Logits of the tied head, z = h E^T (src/algebraic/model.py:225-230 without the likelihood), summed and written in
-// f32, for the tokens of a serving step: E is read once and bounds it.
+// f32. For the tokens of a serving step reading E bounds it, for many the products of gemm_core.h.
 //
-// A wave takes 16 rows of E and up to 64 tokens: E goes from memory to registers in its own order, 128 bytes
-// of each row at a time (16x16 MFMA, A = E; lane group g holds 16-byte pieces g and g + 4 of the 128, and h
-// is laid out alike), h through LDS, which the workgroup's waves share. Lane l then holds four neighbouring
-// logits of token l % 16.
+// Few tokens (and f32): a wave takes 16 rows of E and up to 64 tokens. E goes from memory to registers in
+// its own order, 128 bytes of each row at a time (16x16 MFMA, A = E; lane group g holds 16-byte pieces g and
+// g + 4 of the 128, and h is laid out alike), h through LDS, which the workgroup's waves share. Lane l then
+// holds four neighbouring logits of token l % 16. 5 tokens, d 2048, V 32000, the table from memory: 27 us, 4.9
+// TB/s. f32, 64 tokens: 110 us, of which the matrix cores' rate for f32 makes 54.
 #include <type_traits>
 
-#include "common.h"
+#include "gemm_core.h"
 #include "head_logits.h"
 #include "launchers.h"
 
@@ -16,6 +17,7 @@ namespace alg {
 namespace {
 
 constexpr int LG_WAVES = 8, LG_THREADS = 64 * LG_WAVES;
+constexpr int DEPTH = 4;  // steps of 128 bytes a row
 constexpr int LG_LDS = 64 * 1024;  // bytes of h in LDS, beside the rows' padding
 
 template <typename T, int NT>
@@ -26,15 +28,19 @@ struct LogitsShape {
   static constexpr int PITCH = KC * (int)sizeof(T) + 16;      // bytes; 16 rows at one place lie in 16 parts of the banks
 };
 
-template <typename T>
-__device__ __forceinline__ floatx4 logits_mfma(const u32x4& a, const u32x4& b, floatx4 c) {
+// One 16-byte piece of 16 rows of E with the same of each token (f32: four products of K = 4 each).
+template <typename T, int NT>
+__device__ __forceinline__ void logits_mfma(const u32x4& a, const u32x4 (&b)[NT], floatx4 (&c)[NT]) {
   if constexpr (sizeof(T) == 2) {
-    return mfma16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
-  } else {
-    const floatx4 x = __builtin_bit_cast(floatx4, a), y = __builtin_bit_cast(floatx4, b);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-    return c;
+    for (int nt = 0; nt < NT; ++nt) c[nt] = mfma16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b[nt]), c[nt]);
+  } else {
+    const floatx4 x = __builtin_bit_cast(floatx4, a);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        c[nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], __builtin_bit_cast(floatx4, b[nt])[j], c[nt], 0, 0, 0);
   }
 }
 
@@ -53,9 +59,19 @@ __global__ __launch_bounds__(LG_THREADS) void head_logits_kernel(HeadLogitsParam
   floatx4 acc[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) acc[nt] = floatx4{};
-  for (int k0 = 0; k0 < row_bytes; k0 += S::KC * (int)sizeof(T)) {
-    const int len = min(S::KC * (int)sizeof(T), row_bytes - k0);
-    const int steps = (len + 127) / 128;
+  constexpr int PIECE = S::KC * (int)sizeof(T);  // bytes of a row of h in LDS
+  for (int k0 = 0; k0 < row_bytes; k0 += PIECE) {
+    const int len = min(PIECE, row_bytes - k0), full = len / 128, steps = (len + 127) / 128;
+    const char* from = row + k0;
+    // DEPTH steps of E are always under way, from before h's piece is there.
+    u32x4 a[DEPTH][2];
+    const auto load = [&](int s, u32x4 (&x)[2]) {
+      x[0] = *reinterpret_cast<const u32x4*>(from + 128 * s);
+      x[1] = *reinterpret_cast<const u32x4*>(from + 128 * s + 64);
+    };
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+      if (i < full) load(i, a[i]);
     if (k0) __syncthreads();
     // h's piece, zeros past its end and past the last token.
     for (int i = threadIdx.x; i < S::TOK * 8 * steps; i += LG_THREADS) {
@@ -67,16 +83,37 @@ __global__ __launch_bounds__(LG_THREADS) void head_logits_kernel(HeadLogitsParam
     }
     __syncthreads();
     const char* B = hs + l16 * S::PITCH + 16 * g;
-    for (int s = 0; s < steps; ++s) {
-      u32x4 a[2] = {};
+    const auto multiply = [&](int s, const u32x4 (&x)[2]) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        u32x4 b[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) b[nt] = *reinterpret_cast<const u32x4*>(B + 16 * nt * S::PITCH + 128 * s + 64 * i);
+        logits_mfma<T, NT>(x[i], b, acc);
+      }
+    };
+    int s = 0;
+    for (; s + 2 * DEPTH <= full; s += DEPTH) {
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) {
+        multiply(s + i, a[i]);
+        load(s + DEPTH + i, a[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+      if (s + i < full) multiply(s + i, a[i]);
+    for (s += DEPTH; s < full; ++s) {
+      u32x4 x[2];
+      load(s, x);
+      multiply(s, x);
+    }
+    if (full < steps) {  // the end of a row
+      u32x4 x[2] = {};
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (128 * s + 64 * i + 16 * g < len) a[i] = *reinterpret_cast<const u32x4*>(row + k0 + 128 * s + 64 * i);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          acc[nt] = logits_mfma<T>(a[i], *reinterpret_cast<const u32x4*>(B + 16 * nt * S::PITCH + 128 * s + 64 * i), acc[nt]);
+        if (128 * full + 64 * i + 16 * g < len) x[i] = *reinterpret_cast<const u32x4*>(from + 128 * full + 64 * i);
+      multiply(full, x);
     }
   }
 #pragma unroll
@@ -84,25 +121,76 @@ __global__ __launch_bounds__(LG_THREADS) void head_logits_kernel(HeadLogitsParam
     const int n = n0 + 16 * nt + l16, v = v0 + 4 * g;
     if (n >= p.N) continue;
     float* z = p.z + (size_t)n * p.V + v;
+    if (v + 4 <= p.V) {
+      __builtin_memcpy(z, &acc[nt], 16);  // rows start anywhere
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (v + i < p.V) z[i] = acc[nt][i];
+      for (int i = 0; i < 4; ++i)
+        if (v + i < p.V) z[i] = acc[nt][i];
+    }
   }
 }
 
-template <typename T>
-static void launch_logits(const HeadLogitsParams& p, hipStream_t st) {
-  const int rows = LG_WAVES * 16;
-  const auto grid = [&](int tokens) { return dim3((p.V + rows - 1) / rows, (p.N + tokens - 1) / tokens); };
-  if (p.N <= 16) hipLaunchKernelGGL((head_logits_kernel<T, 1>), grid(16), dim3(LG_THREADS), 0, st, p);
-  else if (p.N <= 32) hipLaunchKernelGGL((head_logits_kernel<T, 2>), grid(32), dim3(LG_THREADS), 0, st, p);
-  else hipLaunchKernelGGL((head_logits_kernel<T, 4>), grid(64), dim3(LG_THREADS), 0, st, p);
+// Many tokens, bf16: the products of gemm_core.h, rows of C tokens, columns the vocabulary, so that a store
+// instruction writes two rows' 128 bytes. Each XCD's share of the tiles is compact.
+template <class C>
+__global__ __launch_bounds__(C::THREADS, 2) void head_logits_gemm_kernel(HeadLogitsParams p) {
+  int tv, tn;
+  xcd_tile(blockIdx.x, (p.V + C::TN - 1) / C::TN, (p.N + C::TM - 1) / C::TM, tv, tn);
+  const int m0 = tn * C::TM, n0 = tv * C::TN;  // tokens, vocabulary
+  const GemmOperand A{static_cast<const bf16*>(p.h), p.d, p.N, p.d, (long)p.N * p.d};
+  const GemmOperand B{static_cast<const bf16*>(p.e), p.d, p.V, p.d, (long)p.V * p.d};
+  floatx16 acc[C::MB][C::NB];
+  gemm_tile<KMAJOR, KMAJOR, C>(A, B, m0, n0, 0, p.d, acc);
+  const int lane = threadIdx.x & 63, h = lane >> 5, l32 = lane & 31;
+  int wm, wn;
+  wave_coords<C>(wm, wn);
+  const int mw = m0 + wm * C::WTM, nw = n0 + wn * C::WTN + l32;
+  float* z = p.z + (size_t)mw * p.V + nw;
+#pragma unroll
+  for (int mb = 0; mb < C::MB; ++mb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = mb * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+#pragma unroll
+      for (int nb = 0; nb < C::NB; ++nb)
+        if (mw + row < p.N && nw + nb * 32 < p.V) z[(size_t)row * p.V + nb * 32] = acc[mb][nb][i];
+    }
 }
 
+template <typename T, int NT>
+static void launch_logits(const HeadLogitsParams& p, hipStream_t st) {
+  const int rows = LG_WAVES * 16, tokens = 16 * NT;
+  const dim3 grid((p.V + rows - 1) / rows, (p.N + tokens - 1) / tokens);
+  hipLaunchKernelGGL((head_logits_kernel<T, NT>), grid, dim3(LG_THREADS), 0, st, p);
+}
+template <class C>
+static void launch_logits_gemm(const HeadLogitsParams& p, hipStream_t st) {
+  const dim3 grid(((p.V + C::TN - 1) / C::TN) * ((p.N + C::TM - 1) / C::TM));
+  hipLaunchKernelGGL(head_logits_gemm_kernel<C>, grid, dim3(C::THREADS), 0, st, p);
+}
+
+// bf16: up to 16 tokens a wave's rows of E, then the tiles of the least gemm_tile_time (launchers.h). us for
+// rows of E / tiles of 64 / 128 / 256, the table not in a cache: d 2048, V 32000: 5 tokens 28 28 34 56, 64 tokens 42
+// 30 35 57, 128 tokens 55 43 37 58, 509 tokens 197 132 125 68; d 768, V 50257: 5 tokens 17 19 28 26, 64 tokens
+// 23 22 28 28, 509 tokens 135 96 90 63; d 1024, V 8000: 5 tokens 10 10 18 28, 128 tokens 18 8 18 28.
 hipError_t launch_head_logits(const HeadLogitsParams& p, hipStream_t st) {
   KTimer t("head_logits", st);
-  if (p.bf16_in) launch_logits<bf16>(p, st);
-  else launch_logits<float>(p, st);
+  if (!p.bf16_in) {
+    if (p.N <= 16) launch_logits<float, 1>(p, st);
+    else if (p.N <= 32) launch_logits<float, 2>(p, st);
+    else launch_logits<float, 4>(p, st);
+  } else if (p.N <= 16) {
+    launch_logits<bf16, 1>(p, st);
+  } else {
+    const auto time = [&](int tile) {
+      return gemm_tile_time(tile, ((p.V + tile - 1) / tile) * ((p.N + tile - 1) / tile), p.d, p.N, p.V);
+    };
+    const double t64 = time(64), t128 = time(128), t256 = time(256);
+    if (t64 <= t128 && t64 <= t256) launch_logits_gemm<GemmCfg<64, 64, 2, 2>>(p, st);
+    else if (t128 <= t256) launch_logits_gemm<GemmCfg<128, 128, 2, 2>>(p, st);
+    else launch_logits_gemm<HeadGemm>(p, st);
+  }
   return hipGetLastError();
 }
 
