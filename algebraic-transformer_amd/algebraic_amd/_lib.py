@@ -93,7 +93,8 @@ _SIGNATURES = {
     "alg_embedding_bwd_workspace_size": (_S, [_I, _I, _I]),
     "alg_embedding_bwd": (_I, [_P, _I, _I, _I, _P, _I, _P, _I, _F, _P, _I, _P, _S]),
     "alg_head_logits": (_I, [_P, _I, _I, _I, _I, _P, _P, _P]),
-    "alg_head_sample": (_I, [_P, _I, _I, _P, _I, _L, _P, _I, _I, _F, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P]),
+    "alg_head_sample_workspace_size": (_S, [_I, _I]),
+    "alg_head_sample": (_I, [_P, _I, _I, _P, _I, _L, _P, _I, _I, _F, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P, _S]),
     "alg_timer_enable": (None, [_I]),
     "alg_timer_report": (_S, [ctypes.c_char_p, _S]),
 }

@@ -110,11 +110,13 @@ def head_sample(logits, uniforms, *, n: int = 8, c: float = 2.0, temperature=1.0
     if V > 1 and logits.stride(1) != 1 or N > 1 and logits.stride(0) < V:
         logits = logits.contiguous()
     uniforms = uniforms.contiguous()
-    p = _lib.ptr
+    lib, p = _lib.load(), _lib.ptr
+    nbytes = lib.alg_head_sample_workspace_size(N, V)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _lib.device_of(logits):
-        _lib.check(_lib.load().alg_head_sample(
+        _lib.check(lib.alg_head_sample(
             _lib.stream_of(logits), N, V, p(logits), _DTYPES[logits.dtype], max(logits.stride(0), V), p(uniforms),
             _DTYPES[uniforms.dtype], int(n), float(c), p(temperature), float(temperature_all), p(top_k),
-            min(int(top_k_all), 2 ** 31 - 1), p(top_p), float(top_p_all), p(min_p), float(min_p_all), p(token), p(logprob)),
-            "head_sample")
+            min(int(top_k_all), 2 ** 31 - 1), p(top_p), float(top_p_all), p(min_p), float(min_p_all), p(token), p(logprob),
+            p(ws), nbytes), "head_sample")
     return token, logprob

@@ -1284,9 +1284,27 @@ int alg_head_logits(alg_stream_t stream, int dtype, int N, int d, int V, const v
   return hip_status(alg::launch_head_logits(p, (hipStream_t)stream), "alg_head_logits");
 }
 
+// Few rows are spread over their tiles (head_sample.hip): [best][bins][counts][sums].
+struct SampleWs {
+  size_t bins, counts, sums, total;
+};
+static SampleWs sample_ws(int N, int V) {
+  SampleWs w{0, 0, 0, 0};
+  const size_t tiles = alg::sample_tiles(V);
+  if (tiles < 2 || N > 256) return w;
+  w.bins = align256(N * tiles * 8);
+  w.counts = w.bins + (size_t)N * alg::SAMPLE_BINS * 8;
+  w.sums = w.counts + (size_t)N * alg::SAMPLE_BINS * 4;
+  w.total = w.sums + N * tiles * alg::SAMPLE_WAVES * 8;
+  return w;
+}
+
+size_t alg_head_sample_workspace_size(int N, int V) { return N <= 0 || V <= 0 ? 0 : sample_ws(N, V).total; }
+
 int alg_head_sample(alg_stream_t stream, int N, int V, const void* z, int z_dtype, long z_stride, const void* u, int u_dtype,
                     int n, float c, const float* temperature, float temperature_all, const int* top_k, int top_k_all,
-                    const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* token, float* logprob) {
+                    const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* token, float* logprob,
+                    void* workspace, size_t workspace_bytes) {
   if (N < 0 || V <= 0) return fail(ALG_ERR_INVALID, "N must not be negative and V positive (got %d, %d)", N, V);
   if (V > 1 << 20) return fail(ALG_ERR_UNSUPPORTED, "V = %d: the sampler is built for vocabularies of up to 2^20", V);
   if (N >= 1 << 22) return fail(ALG_ERR_UNSUPPORTED, "%d rows: a workgroup of 1024 threads each, fewer than 2^22 in one launch", N);
@@ -1313,6 +1331,15 @@ int alg_head_sample(alg_stream_t stream, int N, int V, const void* z, int z_dtyp
   p.bits = 62;
   while (V > 1 << (62 - p.bits)) --p.bits;
   p.token = token; p.logprob = logprob;
+  const SampleWs w = sample_ws(N, V);
+  if (const int rc = check_workspace(workspace, workspace_bytes, w.total)) return rc;
+  if (w.total) {
+    char* ws = static_cast<char*>(workspace);
+    p.best = reinterpret_cast<unsigned long long*>(ws);
+    p.bins = reinterpret_cast<unsigned long long*>(ws + w.bins);
+    p.counts = reinterpret_cast<int*>(ws + w.counts);
+    p.sums = reinterpret_cast<unsigned long long*>(ws + w.sums);
+  }
   return hip_status(alg::launch_head_sample(p, (hipStream_t)stream), "alg_head_sample");
 }
 

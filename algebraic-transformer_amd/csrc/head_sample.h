@@ -22,6 +22,17 @@ struct HeadSampleParams {
   int bits;                // a weight of 1 counts 2^bits: V of them stay under 2^62
   int64_t* token;
   float* logprob;
+  // Few rows: what the tiles of each row found before (nullptr: nothing).
+  unsigned long long* best;  // (N, tiles): the largest key, and the complement of its first token; all ones: a NaN
+  unsigned long long* bins;  // (N, SAMPLE_BINS) the first histogram's sums, and its counts
+  int* counts;
+  unsigned long long* sums;  // (N, tiles, SAMPLE_WAVES) kept weights, of rows without top-k and top-p
 };
+
+constexpr int SAMPLE_THREADS = 1024, SAMPLE_WAVES = SAMPLE_THREADS / 64;
+constexpr int SAMPLE_TILE = 4 * SAMPLE_THREADS;  // tokens of a tile
+constexpr int SAMPLE_TILES = 256;                // tiles of the largest vocabulary
+constexpr int SAMPLE_BINS = 2048;
+inline int sample_tiles(int V) { return (V + SAMPLE_TILE - 1) / SAMPLE_TILE; }
 
 }  // namespace alg

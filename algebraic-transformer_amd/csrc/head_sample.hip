@@ -27,10 +27,6 @@ namespace alg {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int SAMPLE_THREADS = 1024, SAMPLE_WAVES = SAMPLE_THREADS / 64;
-constexpr int SAMPLE_TILE = 4 * SAMPLE_THREADS;  // tokens of a tile
-constexpr int SAMPLE_TILES = 256;                // tiles of the largest vocabulary
-constexpr int SAMPLE_BINS = 2048;
 constexpr int SAMPLE_LIST = 1024;                // tokens that are ranked one against the other
 constexpr unsigned KEY_CLAMPED = 0xFF800000u;    // +infinity's: a logit at the clamp or above
 
@@ -68,19 +64,34 @@ struct SampleShared {
   Prefix found;
 };
 
-template <typename T>
+// READY: the row's best, and the histogram or sums that it needs first, are there.
+template <typename T, bool READY>
 struct Sampler {
   const HeadSampleParams& p;
   SampleShared& s;
+  const int r;  // the row
   const T* row;
   int tid, lane, wave, tiles;
   unsigned top;             // the largest logit's key
   double power, log_top;    // n / temperature, log2 rho of the largest
-  double unit;              // 2^bits
 
-  __device__ Sampler(const HeadSampleParams& p_, SampleShared& s_)
-      : p(p_), s(s_), row(static_cast<const T*>(p_.z) + (size_t)blockIdx.x * p_.stride), tid(threadIdx.x),
-        lane(threadIdx.x & 63), wave(threadIdx.x >> 6), tiles((p_.V + SAMPLE_TILE - 1) / SAMPLE_TILE) {}
+  // The row's settings.
+  float temperature, top_p;
+  double floor_v;  // the least weight kept, times 2^bits
+  int top_k;
+  bool cut_k, cut_p;
+
+  __device__ Sampler(const HeadSampleParams& p_, SampleShared& s_, int r_)
+      : p(p_), s(s_), r(r_), row(static_cast<const T*>(p_.z) + (size_t)r_ * p_.stride), tid(threadIdx.x),
+        lane(threadIdx.x & 63), wave(threadIdx.x >> 6), tiles((p_.V + SAMPLE_TILE - 1) / SAMPLE_TILE) {
+    temperature = p.temperature ? p.temperature[r] : p.temperature_all;
+    top_p = p.top_p ? p.top_p[r] : p.top_p_all;
+    top_k = p.top_k ? p.top_k[r] : p.top_k_all;
+    const float least = p.min_p ? p.min_p[r] : p.min_p_all;
+    floor_v = __builtin_amdgcn_ldexp(least > 0.0f ? (double)fminf(least, 1.0f) : 0.0, p.bits);  // the likeliest token stays
+    cut_k = top_k > 0 && top_k < p.V;
+    cut_p = top_p < 1.0f;
+  }
 
   __device__ __forceinline__ int first(int t) const { return t * SAMPLE_TILE + 4 * tid; }
   // A lane's four tokens of a tile; none past the row's end. Rows start anywhere.
@@ -273,40 +284,43 @@ struct Sampler {
     return got;
   }
 
+  // The first histogram's ranges, of the logits themselves, of 1/64 of the scale: a monotone function of the key,
+  // whatever it rounds.
+  __device__ __forceinline__ int first_bin(unsigned k) const {
+    const float z_top = top == KEY_CLAMPED ? p.z_clamp : key_logit(top), z = k == KEY_CLAMPED ? p.z_clamp : key_logit(k);
+    return (int)fminf((z_top - z) * (float)(64.0 * p.inv_c), SAMPLE_BINS - 1.0f);
+  }
+
   // The shortest prefix, within `in`, of whose tokens' values the sum reaches want(their sum) (at least 1, at most
   // the sum; 0: all of `in`). Either a list of no more than SAMPLE_LIST tokens, sorted, with that prefix among its
   // first (`listed` says how many it has), or `in` itself made shorter (`listed` = 0).
   template <typename F, typename W>
-  __device__ void select(Prefix& in, int& listed, u64& need, F value, W want) {
+  __device__ void select(Prefix& in, int& listed, u64& need, bool ready, F value, W want) {
     unsigned lo = 0, hi = top;
     u64 above = 0;
-    // First by ranges of the logits themselves (a monotone function of the key, whatever it rounds), of 1/64 of
-    // the scale.
-    const float z_top = top == KEY_CLAMPED ? p.z_clamp : key_logit(top);
-    const float z_step = (float)(64.0 * p.inv_c);
     for (int round = 0;; ++round) {
       const int shift = max(0, 21 - (int)__builtin_clz((hi - lo) | 1u));  // (hi - lo) >> shift < 2048
-      const auto bin = [&](unsigned k) {
-        if (round == 0) return (int)fminf((z_top - (k == KEY_CLAMPED ? p.z_clamp : key_logit(k))) * z_step, SAMPLE_BINS - 1.0f);
-        return (int)((hi - k) >> shift);
-      };
+      const auto bin = [&](unsigned k) { return round == 0 ? first_bin(k) : (int)((hi - k) >> shift); };
+      const bool have = READY && ready && round == 0;
       __syncthreads();
       for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_THREADS) {
-        s.bins[i] = 0;
-        s.counts[i] = 0;
+        s.bins[i] = have ? p.bins[(size_t)r * SAMPLE_BINS + i] : 0;
+        s.counts[i] = have ? p.counts[(size_t)r * SAMPLE_BINS + i] : 0;
       }
       if (tid == 0) {
         s.lo = 0xFFFFFFFFu;
         s.hi = s.count = 0;
       }
       __syncthreads();
-      each(in, [&](unsigned k, int i) {
-        if (k < lo || k > hi) return;
-        const int b = bin(k);
-        atomicAdd(&s.bins[b], value(k, i));
-        atomicAdd(&s.counts[b], 1);
-      });
-      __syncthreads();
+      if (!have) {
+        each(in, [&](unsigned k, int i) {
+          if (k < lo || k > hi) return;
+          const int b = bin(k);
+          atomicAdd(&s.bins[b], value(k, i));
+          atomicAdd(&s.counts[b], 1);
+        });
+        __syncthreads();
+      }
       const u64 a = s.bins[2 * tid], b = s.bins[2 * tid + 1];
       const int ca = s.counts[2 * tid], cb = s.counts[2 * tid + 1];
       u64 total, tokens;
@@ -376,58 +390,103 @@ struct Sampler {
 
   __device__ void answer(int token, double logprob) {
     if (tid == 0) {
-      p.token[blockIdx.x] = token;
-      p.logprob[blockIdx.x] = (float)logprob;
+      p.token[r] = token;
+      p.logprob[r] = (float)logprob;
     }
   }
 
-  __device__ void run() {
-    const int r = blockIdx.x;
-    const float temperature = p.temperature ? p.temperature[r] : p.temperature_all;
-    const float top_p = p.top_p ? p.top_p[r] : p.top_p_all;
-    const float least = p.min_p ? p.min_p[r] : p.min_p_all;
-    const double min_p = least > 0.0f ? fminf(least, 1.0f) : 0.0f;  // the likeliest token stays
-    const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
-    const double u = p.u_f64 ? static_cast<const double*>(p.u)[r] : (double)static_cast<const float*>(p.u)[r];
-    tables();
-    // The largest logit, its first token, and whether one is NaN.
-    unsigned best = 0;
-    int best_at = 0;
-    bool nan = false;
-    sweep([&](float z, int i) {
-      nan |= z != z;
-      const unsigned k = logit_key(z, p.z_clamp);
-      if (k > best) {  // a lane meets its tokens by their index
-        best = k;
-        best_at = i;
-      }
-    });
-    u64 c = (u64)best << 32 | (unsigned)~best_at;
+  // The workgroup's largest of the lanes' numbers.
+  __device__ u64 largest(u64 c) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) c = max(c, (u64)__shfl_xor(c, m, 64));
+    __syncthreads();
     if (lane == 0) s.wave[wave] = c;
-    nan = __syncthreads_or(nan) != 0;
+    __syncthreads();
 #pragma unroll
     for (int w = 0; w < SAMPLE_WAVES; ++w) c = max(c, s.wave[w]);
+    return c;
+  }
+  // The largest logit's key and the complement of its first token, of tiles [begin, end); all ones with a NaN.
+  __device__ u64 best(int begin, int end) {
+    u64 c = 0;
+    for (int t = begin; t < end; ++t) {
+      T z[4];
+      logits(t, z);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float f = (float)z[e];
+        c = max(c, f != f ? ~0ull : (u64)logit_key(f, p.z_clamp) << 32 | (unsigned)~(first(t) + e));
+      }
+    }
+    return largest(c);
+  }
+  // Takes the row's best; false: it has its answer, or none.
+  __device__ bool begin(u64 c) {
     top = (unsigned)(c >> 32);
-    if (nan || top == 0 || !(temperature >= 0.0f)) return answer(-1, __builtin_nan(""));
-    if (temperature == 0.0f) return answer((int)~(unsigned)c, 0.0);
+    if (c == ~0ull || top == 0 || !(temperature >= 0.0f)) {
+      answer(-1, __builtin_nan(""));
+      return false;
+    }
+    if (temperature == 0.0f) {
+      answer((int)~(unsigned)c, 0.0);
+      return false;
+    }
     power = p.n / (double)temperature;
     log_top = log2_rho(top);
-    unit = __builtin_amdgcn_ldexp(1.0, p.bits);
+    return true;
+  }
+  __device__ __forceinline__ u64 kept(const Prefix& in, unsigned k, int i) const {
+    if (k == 0 || !in_prefix(in, k, i)) return 0;
+    const double v = scaled(k);
+    return v >= floor_v ? whole_part(v) : 0;
+  }
 
+  // One tile's share of what the row needs first: the histogram of its cut, or its waves' sums. `s` is clear.
+  __device__ void share(int t) {
+    T z[4];
+    logits(t, z);
+    unsigned k[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) k[e] = logit_key((float)z[e], p.z_clamp);
+    if (!cut_k && !cut_p) {
+      u64 v = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v += kept(Prefix{0, p.V}, k[e], first(t) + e);
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
+      if (lane == 0) p.sums[((size_t)r * tiles + t) * SAMPLE_WAVES + wave] = v;
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k[e] != 0) {
+        const int b = first_bin(k[e]);
+        atomicAdd(&s.bins[b], cut_k ? (u64)1 : mass(k[e]));
+        atomicAdd(&s.counts[b], 1);
+      }
+    __syncthreads();
+    for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_THREADS)
+      if (s.counts[i]) {
+        atomicAdd(p.bins + (size_t)r * SAMPLE_BINS + i, s.bins[i]);
+        atomicAdd(p.counts + (size_t)r * SAMPLE_BINS + i, s.counts[i]);
+      }
+  }
+
+  __device__ void run() {
+    const double u = p.u_f64 ? static_cast<const double*>(p.u)[r] : (double)static_cast<const float*>(p.u)[r];
+    tables();
+    const u64 c = READY ? largest(tid < tiles ? p.best[(size_t)r * tiles + tid] : 0) : best(0, tiles);
+    if (!begin(c)) return;
     Prefix in{0, p.V};
     int listed = 0;
     u64 need = 0;
-    const bool cut_k = top_k > 0 && top_k < p.V, cut_p = top_p < 1.0f;
     if (cut_k)
-      select(in, listed, need, [](unsigned, int) { return (u64)1; },
+      select(in, listed, need, true, [](unsigned, int) { return (u64)1; },
              [&](u64 tokens) { return (u64)top_k < tokens ? (u64)top_k : (u64)0; });
     const auto wanted = [&](u64 total) { return max((u64)ceil((double)top_p * (double)total), (u64)1); };
     const int first_k = listed ? top_k : 0;  // of the list
-    if (cut_p && !listed) select(in, listed, need, [&](unsigned k, int) { return mass(k); }, wanted);
+    if (cut_p && !listed) select(in, listed, need, !cut_k, [&](unsigned k, int) { return mass(k); }, wanted);
 
-    const double floor_v = min_p * unit;
     // u as a share of `total`, and the tokens that it passes; below 0 or NaN as 0, 1 or more as the largest below.
     const auto target = [&](u64 total) {
       const double at = floor((u >= 0.0 ? u : 0.0) * (double)total);
@@ -458,29 +517,74 @@ struct Sampler {
       }
       return;
     }
-    const auto kept = [&](unsigned k, int i) {
-      if (k == 0 || !in_prefix(in, k, i)) return (u64)0;
-      const double v = scaled(k);
-      return v >= floor_v ? whole_part(v) : (u64)0;
-    };
-    const u64 total = sums(kept);
-    const int token = pick(target(total), kept);
-    answer(token, tid == 0 ? log((double)kept(logit_key((float)row[token], p.z_clamp), token) / (double)total) : 0.0);
+    const auto value = [&](unsigned k, int i) { return kept(in, k, i); };
+    u64 total;
+    if (READY && !cut_k && !cut_p) {
+      u64 v = 0;
+      for (int i = tid; i < tiles * SAMPLE_WAVES; i += SAMPLE_THREADS)
+        v += (&s.tile[0][0])[i] = p.sums[(size_t)r * tiles * SAMPLE_WAVES + i];
+      scan(v, total);
+    } else {
+      total = sums(value);
+    }
+    const int token = pick(target(total), value);
+    answer(token, tid == 0 ? log((double)value(logit_key((float)row[token], p.z_clamp), token) / (double)total) : 0.0);
   }
 };
 
 }  // namespace
 
-template <typename T>
+template <typename T, bool READY>
 __global__ __launch_bounds__(SAMPLE_THREADS) void head_sample_kernel(HeadSampleParams p) {
   __shared__ SampleShared s;
-  Sampler<T>(p, s).run();
+  Sampler<T, READY>(p, s, blockIdx.x).run();
+}
+
+// Few rows leave most CUs without one, so the passes over a whole row are spread over its tiles, a workgroup each:
+// first the largest logit (which clears the row's histogram too), then what share() says. The sums are
+// whole numbers: the results are those of one workgroup.
+template <typename T>
+__global__ __launch_bounds__(SAMPLE_THREADS) void head_sample_best_kernel(HeadSampleParams p) {
+  __shared__ SampleShared s;
+  Sampler<T, false> row(p, s, blockIdx.y);
+  const u64 c = row.best(blockIdx.x, blockIdx.x + 1);
+  if (threadIdx.x == 0) p.best[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = c;
+  for (int i = blockIdx.x * SAMPLE_THREADS + threadIdx.x; i < SAMPLE_BINS; i += gridDim.x * SAMPLE_THREADS) {
+    p.bins[(size_t)blockIdx.y * SAMPLE_BINS + i] = 0;
+    p.counts[(size_t)blockIdx.y * SAMPLE_BINS + i] = 0;
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(SAMPLE_THREADS) void head_sample_share_kernel(HeadSampleParams p) {
+  __shared__ SampleShared s;
+  Sampler<T, true> row(p, s, blockIdx.y);
+  row.tables();
+  for (int i = threadIdx.x; i < SAMPLE_BINS; i += SAMPLE_THREADS) s.bins[i] = s.counts[i] = 0;
+  const int tiles = gridDim.x;
+  const u64 c = row.largest((int)threadIdx.x < tiles ? p.best[(size_t)blockIdx.y * tiles + threadIdx.x] : 0);
+  if (c != ~0ull && c >> 32 && row.temperature > 0.0f) {
+    row.begin(c);
+    row.share(blockIdx.x);
+  }
+}
+
+template <typename T>
+static void launch_sample(const HeadSampleParams& p, hipStream_t st) {
+  const dim3 threads(SAMPLE_THREADS);
+  if (!p.best) {
+    hipLaunchKernelGGL((head_sample_kernel<T, false>), dim3(p.N), threads, 0, st, p);
+    return;
+  }
+  const dim3 grid(sample_tiles(p.V), p.N);
+  hipLaunchKernelGGL(head_sample_best_kernel<T>, grid, threads, 0, st, p);
+  hipLaunchKernelGGL(head_sample_share_kernel<T>, grid, threads, 0, st, p);
+  hipLaunchKernelGGL((head_sample_kernel<T, true>), dim3(p.N), threads, 0, st, p);
 }
 
 hipError_t launch_head_sample(const HeadSampleParams& p, hipStream_t st) {
   KTimer t("head_sample", st);
-  if (p.z_bf16) hipLaunchKernelGGL(head_sample_kernel<bf16>, dim3(p.N), dim3(SAMPLE_THREADS), 0, st, p);
-  else hipLaunchKernelGGL(head_sample_kernel<float>, dim3(p.N), dim3(SAMPLE_THREADS), 0, st, p);
+  if (p.z_bf16) launch_sample<bf16>(p, st);
+  else launch_sample<float>(p, st);
   return hipGetLastError();
 }
 

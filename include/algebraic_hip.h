@@ -461,10 +461,13 @@ int alg_head_logits(alg_stream_t stream, int dtype, int N, int d, int V, const v
  * is an array (N) or, where the array is NULL, one value for all. u (N) f32 or f64 in [0, 1); below or
  * NaN counts as 0, 1 or more as the largest number below 1. Logits of -infinity are never drawn; a row
  * without another, with a NaN, or whose temperature is negative or NaN gets token -1 and
- * logprob NaN. V up to 2^20. */
+ * logprob NaN. V up to 2^20. Workspace: alg_head_sample_workspace_size bytes (0: none), in which few
+ * rows are spread over the CUs, with the same results. */
+size_t alg_head_sample_workspace_size(int N, int V);
 int alg_head_sample(alg_stream_t stream, int N, int V, const void* z, int z_dtype, long z_stride, const void* u, int u_dtype,
                     int n, float c, const float* temperature, float temperature_all, const int* top_k, int top_k_all,
-                    const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* token, float* logprob);
+                    const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* token, float* logprob,
+                    void* workspace, size_t workspace_bytes);
 
 /* Measurement hook (no counterpart in the reference; for benchmarks and profilers):
  * while enabled, every kernel launch of this library records a HIP event pair on its

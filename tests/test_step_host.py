@@ -199,9 +199,9 @@ def test_step_c_abi_refusals():
     _fails(h.alg_head_logits(None, bf, 3, 64, 10, None, A, A), bad, "null argument")
     _fails(h.alg_head_logits(None, bf, (1 << 20) + 1, 64, 10, A, A, A), no, "2^20")
 
-    def sample(code, text, N=3, V=50, z=A, dtype=f32, stride=50, u=A, u_dtype=f32, n=8, c=2.0, T=1.0, token=A):
+    def sample(code, text, N=3, V=50, z=A, dtype=f32, stride=50, u=A, u_dtype=f32, n=8, c=2.0, T=1.0, token=A, ws=0):
         _fails(h.alg_head_sample(None, N, V, z, dtype, stride, u, u_dtype, n, f(c), None, f(T), None, 0, None, f(1.0), None, f(0.0),
-                                 token, A), code, text)
+                                 token, A, A, ws), code, text)
 
     sample(bad, "must not be negative", N=-1)
     sample(no, "2^20", V=(1 << 20) + 1)
@@ -213,3 +213,6 @@ def test_step_c_abi_refusals():
     sample(bad, "apart", stride=49)
     sample(bad, "temperature", T=-1.0)
     sample(bad, "null argument", token=None)
+    need = h.alg_head_sample_workspace_size(3, 50000)
+    assert need > 0 and h.alg_head_sample_workspace_size(3, 50) == h.alg_head_sample_workspace_size(0, 50000) == 0
+    sample(bad, "workspace too small", V=50000, stride=50000, ws=need - 1)
