@@ -1284,17 +1284,16 @@ int alg_head_logits(alg_stream_t stream, int dtype, int N, int d, int V, const v
   return hip_status(alg::launch_head_logits(p, (hipStream_t)stream), "alg_head_logits");
 }
 
-// Few rows are spread over their tiles (head_sample.hip): [best][bins][counts][sums].
+// Few rows are spread over their tiles (head_sample.hip): [best][bins][sums].
 struct SampleWs {
-  size_t bins, counts, sums, total;
+  size_t bins, sums, total;
 };
 static SampleWs sample_ws(int N, int V) {
-  SampleWs w{0, 0, 0, 0};
+  SampleWs w{0, 0, 0};
   const size_t tiles = alg::sample_tiles(V);
   if (tiles < 2 || N > 256) return w;
   w.bins = align256(N * tiles * 8);
-  w.counts = w.bins + (size_t)N * alg::SAMPLE_BINS * 8;
-  w.sums = w.counts + (size_t)N * alg::SAMPLE_BINS * 4;
+  w.sums = w.bins + (size_t)N * alg::SAMPLE_BINS * 8;
   w.total = w.sums + N * tiles * alg::SAMPLE_WAVES * 8;
   return w;
 }
@@ -1337,7 +1336,6 @@ int alg_head_sample(alg_stream_t stream, int N, int V, const void* z, int z_dtyp
     char* ws = static_cast<char*>(workspace);
     p.best = reinterpret_cast<unsigned long long*>(ws);
     p.bins = reinterpret_cast<unsigned long long*>(ws + w.bins);
-    p.counts = reinterpret_cast<int*>(ws + w.counts);
     p.sums = reinterpret_cast<unsigned long long*>(ws + w.sums);
   }
   return hip_status(alg::launch_head_sample(p, (hipStream_t)stream), "alg_head_sample");

@@ -24,8 +24,7 @@ struct HeadSampleParams {
   float* logprob;
   // Few rows: what the tiles of each row found before (nullptr: nothing).
   unsigned long long* best;  // (N, tiles): the largest key, and the complement of its first token; all ones: a NaN
-  unsigned long long* bins;  // (N, SAMPLE_BINS) the first histogram's sums, and its counts
-  int* counts;
+  unsigned long long* bins;  // (N, SAMPLE_BINS) the first histogram
   unsigned long long* sums;  // (N, tiles, SAMPLE_WAVES) kept weights, of rows without top-k and top-p
 };
 

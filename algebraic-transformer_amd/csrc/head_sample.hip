@@ -27,7 +27,8 @@ namespace alg {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int SAMPLE_LIST = 1024;                // tokens that are ranked one against the other
+constexpr int SAMPLE_LIST = 1024;                // tokens that are sorted
+constexpr int SAMPLE_RANKED = 192;               // so many by counting, for each, those before it
 constexpr unsigned KEY_CLAMPED = 0xFF800000u;    // +infinity's: a logit at the clamp or above
 
 // Logits as whole numbers of the same order; 0: no token (a logit of -infinity, or none).
@@ -41,6 +42,38 @@ __device__ __forceinline__ float key_logit(unsigned k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
+// The lanes' numbers combined up to each lane (`op` with 0 leaves a number as it is), without a trip through LDS: the
+// lanes before it in a row of 16, then the rows before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 lanes_before(u64 v) {
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xF, true);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xF, true);
+  return (u64)hi << 32 | lo;
+}
+template <typename Op>
+__device__ __forceinline__ u64 row_scan(u64 v, Op op) {
+  v = op(v, lanes_before<0x111, 0xF>(v));
+  v = op(v, lanes_before<0x112, 0xF>(v));
+  v = op(v, lanes_before<0x114, 0xF>(v));
+  return op(v, lanes_before<0x118, 0xF>(v));
+}
+template <typename Op>
+__device__ __forceinline__ u64 wave_scan(u64 v, Op op) {
+  v = row_scan(v, op);
+  v = op(v, lanes_before<0x142, 0xA>(v));
+  return op(v, lanes_before<0x143, 0xC>(v));
+}
+__device__ __forceinline__ u64 lane_of(u64 v, int lane) {
+  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), lane) << 32 |
+         (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, lane);
+}
+struct Add {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a + b; }
+};
+struct Max {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return max(a, b); }
+};
+
 struct Prefix {
   unsigned key;
   int last;
@@ -49,39 +82,82 @@ __device__ __forceinline__ bool in_prefix(const Prefix& p, unsigned key, int i) 
   return key > p.key || (key == p.key && i <= p.last);
 }
 
+// Tables of log2 and 2^x: 1 / m and log2 m for the middles m of [1, 2)'s 128 parts, and 2^(i / 64). Formed by the
+// compiler, from log((1 + y) / (1 - y)) = 2 (y + y^3 / 3 + ...) and the exponential's series.
+struct SampleTables {
+  double logs[128][2];
+  double exps[64];
+};
+constexpr double LN2 = 0.69314718055994530942;
+constexpr SampleTables sample_tables() {
+  SampleTables t{};
+  for (int i = 0; i < 128; ++i) {
+    const double m = 1.0 + (i + 0.5) / 128.0, y = (m - 1.0) / (m + 1.0);
+    double sum = 0.0, power = y;
+    for (int k = 1; k < 60; k += 2, power *= y * y) sum += power / k;
+    t.logs[i][0] = 1.0 / m;
+    t.logs[i][1] = 2.0 * sum / LN2;
+  }
+  for (int i = 0; i < 64; ++i) {
+    double sum = 1.0, term = 1.0;
+    for (int k = 1; k < 30; ++k) {
+      term *= i / 64.0 * LN2 / k;
+      sum += term;
+    }
+    t.exps[i] = sum;
+  }
+  return t;
+}
+__device__ constexpr SampleTables SAMPLE_TABLES = sample_tables();
+
 struct SampleShared {
+  SampleTables tables;
   u64 bins[SAMPLE_BINS];
-  int counts[SAMPLE_BINS];
   u64 list[SAMPLE_LIST];  // key, and the index's complement: falling order
   u64 value[SAMPLE_LIST];
   u64 tile[SAMPLE_TILES][SAMPLE_WAVES];
-  double2 logs[128];  // 1 / m and -log2 of that, m the middles of [1, 2)'s 128 parts
-  double exps[64];    // 2^(i / 64)
   u64 wave[SAMPLE_WAVES];
   unsigned lo, hi, count;
-  int bin, upto;
+  int bin, token;
   u64 above;
   Prefix found;
 };
 
-// READY: the row's best, and the histogram or sums that it needs first, are there.
-template <typename T, bool READY>
+// log2 of a normal number, to 2^-50: its exponent, and log2 m from the middle of m's 128th part and five terms of
+// the series.
+typedef __attribute__((address_space(3))) const SampleTables* TablesPtr;
+__device__ __noinline__ double log2_of(double v, TablesPtr tables) {
+  const u64 b = __builtin_bit_cast(u64, v);
+  const int high = (int)(b >> 32), part = (high >> 13) & 127;
+  const double m = __builtin_bit_cast(double, (b & 0x000FFFFFFFFFFFFFull) | 0x3FF0000000000000ull);
+  const double t = __builtin_fma(m, tables->logs[part][0], -1.0);
+  constexpr double C = 1.0 / LN2;
+  double poly = __builtin_fma(t, C / 5, -C / 4);
+  poly = __builtin_fma(t, poly, C / 3);
+  poly = __builtin_fma(t, poly, -C / 2);
+  poly = __builtin_fma(t, poly, C);
+  return __builtin_fma(t, poly, tables->logs[part][1] + (double)((high >> 20) - 1023));
+}
+
+// One row, by one workgroup. What is done to a token stands once in the code and every loop is kept a loop: a
+// workgroup goes through it once, and instructions that are fetched for it alone cost more than those that
+// are executed (unrolled, 150 KB of them took three times as long).
+template <typename T>
 struct Sampler {
   const HeadSampleParams& p;
   SampleShared& s;
   const int r;  // the row
   const T* row;
   int tid, lane, wave, tiles;
-  unsigned top;             // the largest logit's key
-  double power, log_top;    // n / temperature, log2 rho of the largest
-
+  unsigned top;           // the largest logit's key
+  double power, log_top;  // n / temperature, log2 rho of the largest
   // The row's settings.
   float temperature, top_p;
   double floor_v;  // the least weight kept, times 2^bits
   int top_k;
   bool cut_k, cut_p;
 
-  __device__ Sampler(const HeadSampleParams& p_, SampleShared& s_, int r_)
+  __device__ __forceinline__ Sampler(const HeadSampleParams& p_, SampleShared& s_, int r_)
       : p(p_), s(s_), r(r_), row(static_cast<const T*>(p_.z) + (size_t)r_ * p_.stride), tid(threadIdx.x),
         lane(threadIdx.x & 63), wave(threadIdx.x >> 6), tiles((p_.V + SAMPLE_TILE - 1) / SAMPLE_TILE) {
     temperature = p.temperature ? p.temperature[r] : p.temperature_all;
@@ -92,117 +168,107 @@ struct Sampler {
     cut_k = top_k > 0 && top_k < p.V;
     cut_p = top_p < 1.0f;
   }
+  __device__ __forceinline__ void tables() {
+    constexpr int N = sizeof(SampleTables) / sizeof(double);
+    const double* from = reinterpret_cast<const double*>(&SAMPLE_TABLES);
+    if (tid < N) reinterpret_cast<double*>(&s.tables)[tid] = from[tid];
+  }
 
   __device__ __forceinline__ int first(int t) const { return t * SAMPLE_TILE + 4 * tid; }
   // A lane's four tokens of a tile; none past the row's end. Rows start anywhere.
-  __device__ __forceinline__ void logits(int t, T (&z)[4]) const {
+  struct Four {
+    T z[4];
+  };
+  __device__ __forceinline__ Four logits(int t) const {
     const int i = first(t);
+    Four f;
     if (i + 4 <= p.V) {
-      __builtin_memcpy(z, row + i, sizeof z);
+      __builtin_memcpy(f.z, row + i, sizeof f.z);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = i + e < p.V ? row[i + e] : (T)-INFINITY;
+      for (int e = 0; e < 4; ++e) f.z[e] = i + e < p.V ? row[i + e] : (T)-INFINITY;
     }
+    return f;
   }
-  // f(logit, token) for every token, the next tiles' loads under way.
-  template <typename F>
-  __device__ __forceinline__ void sweep(F f) const {
-    T z[2][4];
-    logits(0, z[0]);
-    if (tiles > 1) logits(1, z[1]);
-    for (int t = 0; t < tiles; ++t) {
-      T now[4];
-#pragma unroll
+  // f(logit, token) for every token of tiles [begin, end), and g(t) after each tile; four tiles' loads are under way.
+  template <typename F, typename G>
+  __device__ __forceinline__ void sweep(int begin, int end, F f, G g) const {
+    const auto load = [&](int t) { return logits(min(t, end - 1)); };
+    Four a = load(begin), b = load(begin + 1), c = load(begin + 2), d = load(begin + 3);
+#pragma unroll 1
+    for (int t = begin; t < end; ++t) {
+      Four now = a;
+      a = b;
+      b = c;
+      c = d;
+      if (t + 4 < end) d = logits(t + 4);
+#pragma unroll 1
       for (int e = 0; e < 4; ++e) {
-        now[e] = z[0][e];
-        z[0][e] = z[1][e];
+        f((float)now.z[0], first(t) + e);
+        now.z[0] = now.z[1];
+        now.z[1] = now.z[2];
+        now.z[2] = now.z[3];
       }
-      if (t + 2 < tiles) logits(t + 2, z[1]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f((float)now[e], first(t) + e);
+      g(t);
     }
   }
-  // f(key, token) for every token that the prefix holds.
-  template <typename F>
-  __device__ __forceinline__ void each(const Prefix& in, F f) const {
-    sweep([&](float z, int i) {
-      const unsigned k = logit_key(z, p.z_clamp);
-      if (k != 0 && in_prefix(in, k, i)) f(k, i);
-    });
-  }
+  struct Nothing {
+    __device__ __forceinline__ void operator()(int) const {}
+  };
 
-  // log2 rho(x), to 2^-43: |x| + sqrt(1 + x^2) = 2^e m, log2 m from the middle of m's 128th part and five
-  // terms of the series. The root is s rsqrt(s), the hardware's with one step of Newton's method.
+  // log2 rho(x) = log2(|x| + sqrt(1 + x^2)), to 2^-43: the root is q rsqrt(q), the hardware's with one step of
+  // Newton's method.
   __device__ __forceinline__ double log2_rho(unsigned key) const {
     const double x = key == KEY_CLAMPED ? p.clamp : (double)key_logit(key) * p.inv_c, a = __builtin_fabs(x);
     const double q = __builtin_fma(a, a, 1.0), y = __builtin_amdgcn_rsq(q), h = q * y;
-    const double r = a + __builtin_fma(0.5 * h, __builtin_fma(-h, y, 1.0), h);
-    const u64 b = __builtin_bit_cast(u64, r);
-    const int high = (int)(b >> 32);
-    const double m = __builtin_bit_cast(double, (b & 0x000FFFFFFFFFFFFFull) | 0x3FF0000000000000ull);
-    const double2 part = s.logs[(high >> 13) & 127];
-    const double t = __builtin_fma(m, part.x, -1.0);
-    constexpr double C = 1.4426950408889634;  // 1 / ln 2
-    double poly = __builtin_fma(t, C / 5, -C / 4);
-    poly = __builtin_fma(t, poly, C / 3);
-    poly = __builtin_fma(t, poly, -C / 2);
-    poly = __builtin_fma(t, poly, C);
-    const double l = __builtin_fma(t, poly, part.y + (double)((high >> 20) - 1023));
+    const double l = log2_of(a + __builtin_fma(0.5 * h, __builtin_fma(-h, y, 1.0), h), (TablesPtr)&s.tables);
     return x < 0.0 ? -l : l;
   }
-  // The weight times 2^bits: 2^d of the nearest 64th below a table's and five terms of the series.
+  // The weight times 2^bits: 2^d by the table's nearest 64th and five terms of the series.
   __device__ __forceinline__ double scaled(unsigned key) const {
     const double d = fmax(power * (log2_rho(key) - log_top), -1000.0), j = __builtin_rint(d * 64.0);
     const double f = __builtin_fma(j, -0.015625, d);
     const int ji = (int)j;
-    constexpr double L = 0.6931471805599453;
-    double poly = __builtin_fma(f, L * L * L * L * L / 120, L * L * L * L / 24);
-    poly = __builtin_fma(f, poly, L * L * L / 6);
-    poly = __builtin_fma(f, poly, L * L / 2);
-    poly = __builtin_fma(f, poly, L);
+    double poly = __builtin_fma(f, LN2 * LN2 * LN2 * LN2 * LN2 / 120, LN2 * LN2 * LN2 * LN2 / 24);
+    poly = __builtin_fma(f, poly, LN2 * LN2 * LN2 / 6);
+    poly = __builtin_fma(f, poly, LN2 * LN2 / 2);
+    poly = __builtin_fma(f, poly, LN2);
     poly = __builtin_fma(f, poly, 1.0);
-    return __builtin_amdgcn_ldexp(s.exps[ji & 63] * poly, (ji >> 6) + p.bits);
+    return __builtin_amdgcn_ldexp(s.tables.exps[ji & 63] * poly, (ji >> 6) + p.bits);
   }
   static __device__ __forceinline__ u64 whole_part(double v) {
     const unsigned high = (unsigned)(v * 0x1p-32);
     return (u64)high << 32 | (unsigned)__builtin_fma((double)high, -0x1p32, v);
   }
-  __device__ __forceinline__ u64 mass(unsigned key) const { return whole_part(scaled(key)); }
-  __device__ void tables() {
-    if (tid < 128) {
-      const double inv = 1.0 / (1.0 + (tid + 0.5) / 128.0);
-      s.logs[tid] = make_double2(inv, -log2(inv));
-    } else if (tid < 192) {
-      s.exps[tid - 128] = exp2((tid - 128) / 64.0);
-    }
+  __device__ __forceinline__ u64 kept(unsigned k) const {
+    const double v = scaled(k);
+    return v >= floor_v ? whole_part(v) : 0;
   }
 
-  // The sum over the lanes up to this one's, and over all.
-  __device__ u64 scan(u64 v, u64& total) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const u64 below = __shfl_up(v, m, 64);
-      if (lane >= m) v += below;
-    }
+  // op over the lanes up to this one, and over all: wave by wave, then a row of 16 lanes over the waves' results.
+  template <typename Op>
+  __device__ __forceinline__ u64 scan(u64 v, u64& total, Op op) {
+    static_assert(SAMPLE_WAVES == 16, "a row of lanes");
+    v = wave_scan(v, op);
     __syncthreads();
     if (lane == 63) s.wave[wave] = v;
     __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < SAMPLE_WAVES; ++w) {
-      if (w == wave) v += total;
-      total += s.wave[w];
-    }
-    return v;
+    const u64 upto = row_scan(s.wave[lane & 15], op);
+    total = lane_of(upto, 15);
+    return wave > 0 ? op(v, lane_of(upto, max(wave - 1, 0))) : v;
   }
-
+  __device__ __forceinline__ u64 largest(u64 c) {
+    scan(c, c, Max());
+    return c;
+  }
   // The lanes' numbers in falling order, a lane each; `size` a power of two, the lanes from there on hold 0.
-  template <typename K>
-  __device__ K sorted(K v, int size) {
-    K* buf = reinterpret_cast<K*>(s.bins);
+  __device__ __forceinline__ u64 sorted(u64 v, int size) {
+    u64* buf = s.bins;
+#pragma unroll 1
     for (int block = 2; block <= size; block <<= 1)
+#pragma unroll 1
       for (int step = block >> 1; step > 0; step >>= 1) {
-        K o;
+        u64 o;
         if (step < 64) {
           o = __shfl_xor(v, step, 64);
         } else {
@@ -216,74 +282,6 @@ struct Sampler {
     return v;
   }
 
-  // The sum of value(key, i) over all tokens, which pick() then draws from.
-  template <typename F>
-  __device__ u64 sums(F value) {
-    T z[4];
-    logits(0, z);
-    for (int t = 0; t < tiles; ++t) {
-      T now[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) now[e] = z[e];
-      if (t + 1 < tiles) logits(t + 1, z);
-      u64 v = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v += value(logit_key((float)now[e], p.z_clamp), first(t) + e);
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
-      if (lane == 0) s.tile[t][wave] = v;
-    }
-    __syncthreads();
-    u64 v = 0, total;
-    for (int i = tid; i < tiles * SAMPLE_WAVES; i += SAMPLE_THREADS) v += (&s.tile[0][0])[i];
-    scan(v, total);
-    return total;
-  }
-  // The token at which the running sum, over tokens by their index, first passes `target` (less than the sum).
-  template <typename F>
-  __device__ int pick(u64 target, F value) {
-    int t = 0, w = 0;
-    u64 below = 0;
-    for (; t < tiles - 1; ++t) {
-      u64 sum = 0;
-#pragma unroll
-      for (int i = 0; i < SAMPLE_WAVES; ++i) sum += s.tile[t][i];
-      if (below + sum > target) break;
-      below += sum;
-    }
-    for (; w < SAMPLE_WAVES - 1; ++w) {
-      if (below + s.tile[t][w] > target) break;
-      below += s.tile[t][w];
-    }
-    if (wave == w) {
-      T z[4];
-      logits(t, z);
-      u64 v[4], sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += v[e] = value(logit_key((float)z[e], p.z_clamp), first(t) + e);
-      u64 upto = sum;
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) {
-        const u64 x = __shfl_up(upto, m, 64);
-        if (lane >= m) upto += x;
-      }
-      below += upto - sum;  // up to this lane's tokens
-      if (below <= target && below + sum > target) {
-        int last = first(t);
-#pragma unroll
-        for (int e = 0; e < 3; ++e) {
-          below += v[e];
-          last += below <= target;
-        }
-        s.found.last = last;
-      }
-    }
-    __syncthreads();
-    const int got = s.found.last;
-    __syncthreads();
-    return got;
-  }
-
   // The first histogram's ranges, of the logits themselves, of 1/64 of the scale: a monotone function of the key,
   // whatever it rounds.
   __device__ __forceinline__ int first_bin(unsigned k) const {
@@ -291,253 +289,321 @@ struct Sampler {
     return (int)fminf((z_top - z) * (float)(64.0 * p.inv_c), SAMPLE_BINS - 1.0f);
   }
 
-  // The shortest prefix, within `in`, of whose tokens' values the sum reaches want(their sum) (at least 1, at most
-  // the sum; 0: all of `in`). Either a list of no more than SAMPLE_LIST tokens, sorted, with that prefix among its
-  // first (`listed` says how many it has), or `in` itself made shorter (`listed` = 0).
-  template <typename F, typename W>
-  __device__ void select(Prefix& in, int& listed, u64& need, bool ready, F value, W want) {
-    unsigned lo = 0, hi = top;
-    u64 above = 0;
-    for (int round = 0;; ++round) {
-      const int shift = max(0, 21 - (int)__builtin_clz((hi - lo) | 1u));  // (hi - lo) >> shift < 2048
-      const auto bin = [&](unsigned k) { return round == 0 ? first_bin(k) : (int)((hi - k) >> shift); };
-      const bool have = READY && ready && round == 0;
-      __syncthreads();
-      for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_THREADS) {
-        s.bins[i] = have ? p.bins[(size_t)r * SAMPLE_BINS + i] : 0;
-        s.counts[i] = have ? p.counts[(size_t)r * SAMPLE_BINS + i] : 0;
-      }
-      if (tid == 0) {
-        s.lo = 0xFFFFFFFFu;
-        s.hi = s.count = 0;
-      }
-      __syncthreads();
-      if (!have) {
-        each(in, [&](unsigned k, int i) {
-          if (k < lo || k > hi) return;
-          const int b = bin(k);
-          atomicAdd(&s.bins[b], value(k, i));
-          atomicAdd(&s.counts[b], 1);
-        });
-        __syncthreads();
-      }
-      const u64 a = s.bins[2 * tid], b = s.bins[2 * tid + 1];
-      const int ca = s.counts[2 * tid], cb = s.counts[2 * tid + 1];
-      u64 total, tokens;
-      const u64 upto = above + scan(a + b, total);
-      const int held = (int)scan((u64)(ca + cb), tokens);
-      if (round == 0) need = want(total);
-      if (need == 0) return;
-      const u64 before = upto - a - b;
-      if (before < need && before + a >= need) {
-        s.bin = 2 * tid;
-        s.above = before;
-        s.upto = held - cb;
-      } else if (before + a < need && upto >= need) {
-        s.bin = 2 * tid + 1;
-        s.above = before + a;
-        s.upto = held;
-      }
-      __syncthreads();
-      const int at = s.bin, count = s.counts[at];
-      const bool all = round == 0 && s.upto <= SAMPLE_LIST;  // that range's tokens and all above fit the list
-      above = s.above;
-      each(in, [&](unsigned k, int i) {
-        if (k < lo || k > hi) return;
-        const int b = bin(k);
-        if (b > at || (b < at && !all)) return;
-        if (!all) {
-          atomicMin(&s.lo, k);
-          atomicMax(&s.hi, k);
-        }
-        const unsigned n = atomicAdd(&s.count, 1u);
-        if (n < SAMPLE_LIST) s.list[n] = (u64)k << 32 | (unsigned)~i;
-      });
-      __syncthreads();
-      lo = s.lo;
-      hi = s.hi;
-      if (all || count <= SAMPLE_LIST) {
-        const int n = all ? s.upto : count;
-        int size = 64;
-        while (size < n) size <<= 1;
-        const u64 mine = sorted(tid < n ? s.list[tid] : 0, size);
-        __syncthreads();
-        s.list[tid] = mine;
-        if (all) {
-          listed = n;
-          __syncthreads();
-          return;
-        }
-        u64 ignored;
-        const u64 v = tid < n ? value((unsigned)(mine >> 32), (int)~(unsigned)mine) : 0;
-        const u64 sum = above + scan(v, ignored);
-        if (sum - v < need && sum >= need) s.found = Prefix{(unsigned)(mine >> 32), (int)~(unsigned)mine};
-        __syncthreads();
-        in = s.found;
-        __syncthreads();
-        return;
-      }
-      if (lo == hi) {  // one logit: as many of its tokens as it takes
-        const u64 each_one = value(lo, 0), wanted = (need - above + each_one - 1) / each_one;
-        const Prefix from = in;
-        const auto it = [&](unsigned k, int i) { return (u64)(k == lo && in_prefix(from, k, i)); };
-        sums(it);
-        in = Prefix{lo, pick(wanted - 1, it)};
-        return;
-      }
-    }
+  __device__ __forceinline__ void answer(int token, double logprob) {
+    p.token[r] = token;
+    p.logprob[r] = (float)logprob;
   }
-
-  __device__ void answer(int token, double logprob) {
-    if (tid == 0) {
-      p.token[r] = token;
-      p.logprob[r] = (float)logprob;
-    }
-  }
-
-  // The workgroup's largest of the lanes' numbers.
-  __device__ u64 largest(u64 c) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) c = max(c, (u64)__shfl_xor(c, m, 64));
-    __syncthreads();
-    if (lane == 0) s.wave[wave] = c;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < SAMPLE_WAVES; ++w) c = max(c, s.wave[w]);
-    return c;
+  __device__ __forceinline__ double log_share(u64 part, u64 whole) const {
+    return part == whole ? 0.0 : LN2 * log2_of((double)part / (double)whole, (TablesPtr)&s.tables);
   }
   // The largest logit's key and the complement of its first token, of tiles [begin, end); all ones with a NaN.
-  __device__ u64 best(int begin, int end) {
+  __device__ __forceinline__ u64 best(int begin, int end) {
     u64 c = 0;
-    for (int t = begin; t < end; ++t) {
-      T z[4];
-      logits(t, z);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float f = (float)z[e];
-        c = max(c, f != f ? ~0ull : (u64)logit_key(f, p.z_clamp) << 32 | (unsigned)~(first(t) + e));
-      }
-    }
+    sweep(begin, end, [&](float z, int i) {
+      c = max(c, z != z ? ~0ull : (u64)logit_key(z, p.z_clamp) << 32 | (unsigned)~i);
+    }, Nothing());
     return largest(c);
   }
   // Takes the row's best; false: it has its answer, or none.
-  __device__ bool begin(u64 c) {
+  __device__ __forceinline__ bool begin(u64 c) {
     top = (unsigned)(c >> 32);
-    if (c == ~0ull || top == 0 || !(temperature >= 0.0f)) {
-      answer(-1, __builtin_nan(""));
-      return false;
-    }
-    if (temperature == 0.0f) {
-      answer((int)~(unsigned)c, 0.0);
+    const bool none = c == ~0ull || top == 0 || !(temperature >= 0.0f);
+    if (none || temperature == 0.0f) {
+      if (tid == 0) answer(none ? -1 : (int)~(unsigned)c, none ? __builtin_nan("") : 0.0);
       return false;
     }
     power = p.n / (double)temperature;
     log_top = log2_rho(top);
     return true;
   }
-  __device__ __forceinline__ u64 kept(const Prefix& in, unsigned k, int i) const {
-    if (k == 0 || !in_prefix(in, k, i)) return 0;
-    const double v = scaled(k);
-    return v >= floor_v ? whole_part(v) : 0;
-  }
 
-  // One tile's share of what the row needs first: the histogram of its cut, or its waves' sums. `s` is clear.
-  __device__ void share(int t) {
-    T z[4];
-    logits(t, z);
-    unsigned k[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) k[e] = logit_key((float)z[e], p.z_clamp);
-    if (!cut_k && !cut_p) {
-      u64 v = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v += kept(Prefix{0, p.V}, k[e], first(t) + e);
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
-      if (lane == 0) p.sums[((size_t)r * tiles + t) * SAMPLE_WAVES + wave] = v;
+  // One tile's share of what the row needs first: the histogram of its cut (s.bins clear), or its waves'
+  // sums.
+  __device__ __forceinline__ void share(int tile) {
+    const bool cut = cut_k || cut_p;
+    u64 v = 0;
+    sweep(tile, tile + 1, [&](float z, int) {
+      const unsigned k = logit_key(z, p.z_clamp);
+      if (k == 0) return;
+      const u64 w = cut_k ? 1 : cut ? whole_part(scaled(k)) : kept(k);
+      if (cut) atomicAdd(&s.bins[first_bin(k)], w);
+      v += w;
+    }, Nothing());
+    if (!cut) {
+      v = wave_scan(v, Add());
+      if (lane == 63) p.sums[((size_t)r * tiles + tile) * SAMPLE_WAVES + wave] = v;
       return;
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (k[e] != 0) {
-        const int b = first_bin(k[e]);
-        atomicAdd(&s.bins[b], cut_k ? (u64)1 : mass(k[e]));
-        atomicAdd(&s.counts[b], 1);
-      }
     __syncthreads();
+#pragma unroll
     for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_THREADS)
-      if (s.counts[i]) {
-        atomicAdd(p.bins + (size_t)r * SAMPLE_BINS + i, s.bins[i]);
-        atomicAdd(p.counts + (size_t)r * SAMPLE_BINS + i, s.counts[i]);
-      }
+      if (s.bins[i]) atomicAdd(p.bins + (size_t)r * SAMPLE_BINS + i, s.bins[i]);
   }
 
-  __device__ void run() {
+  // `ready`: the row's best, and the histogram or sums that it needs first, are there.
+  __device__ __forceinline__ void run(bool ready) {
     const double u = p.u_f64 ? static_cast<const double*>(p.u)[r] : (double)static_cast<const float*>(p.u)[r];
     tables();
-    const u64 c = READY ? largest(tid < tiles ? p.best[(size_t)r * tiles + tid] : 0) : best(0, tiles);
+    u64 c = ready ? (tid < tiles ? p.best[(size_t)r * tiles + tid] : 0) : 0;
+    c = ready ? largest(c) : best(0, tiles);
     if (!begin(c)) return;
-    Prefix in{0, p.V};
-    int listed = 0;
-    u64 need = 0;
-    if (cut_k)
-      select(in, listed, need, true, [](unsigned, int) { return (u64)1; },
-             [&](u64 tokens) { return (u64)top_k < tokens ? (u64)top_k : (u64)0; });
-    const auto wanted = [&](u64 total) { return max((u64)ceil((double)top_p * (double)total), (u64)1); };
-    const int first_k = listed ? top_k : 0;  // of the list
-    if (cut_p && !listed) select(in, listed, need, !cut_k, [&](unsigned k, int) { return mass(k); }, wanted);
 
-    // u as a share of `total`, and the tokens that it passes; below 0 or NaN as 0, 1 or more as the largest below.
-    const auto target = [&](u64 total) {
-      const double at = floor((u >= 0.0 ? u : 0.0) * (double)total);
-      return at < (double)total ? min((u64)at, total - 1) : total - 1;
-    };
-    if (listed) {
-      // The list's tokens, a lane each, by falling logit; then the kept ones by their index.
-      const u64 mine = s.list[tid];
-      const bool is = tid < (first_k ? first_k : listed);
-      const double v = is ? scaled((unsigned)(mine >> 32)) : 0.0;
-      const u64 m = is ? whole_part(v) : 0;
-      u64 total, kept_total;
-      const u64 upto = scan(m, total);
-      if (first_k) need = cut_p ? wanted(total) : total;
-      const bool keep = is && v >= floor_v && (tid == 0 || upto - m < need);
-      s.value[tid] = m;
-      int size = 64;
-      while (size < listed) size <<= 1;
-      const unsigned index = ~(unsigned)mine;
-      const unsigned by_index = sorted(keep ? ~(index << 10 | (unsigned)tid) : 0u, size);
-      __syncthreads();
-      const unsigned slot = ~by_index & 1023;
-      const u64 w = by_index ? s.value[slot] : 0;
-      const u64 sum = scan(w, kept_total), t = target(kept_total);
-      if (by_index && sum - w <= t && sum > t) {
-        p.token[r] = (int)(~by_index >> 10);
-        p.logprob[r] = (float)log((double)w / (double)kept_total);
+    // The cuts: by_mass false top-k, true top-p. Each asks for the shortest prefix, within `in`, of whose tokens' values
+    // (1, or the weight) the sum reaches `need`; [lo, hi] holds the key where it does, `above` is the sum over it.
+    Prefix in{0, p.V};
+    bool by_mass = !cut_k, cut = cut_k || cut_p, fresh = true, ties = false;
+    unsigned lo = 0, hi = top;
+    u64 above = 0, need = 0, wanted_tie = 0;
+    int listed = 0, first_k = 0;
+    const auto share_of = [&](u64 total) { return max((u64)ceil((double)top_p * (double)total), (u64)1); };
+#pragma unroll 1
+    while (true) {
+      if (cut) {
+        const int shift = max(0, 21 - (int)__builtin_clz((hi - lo) | 1u));  // (hi - lo) >> shift < 2048
+        const auto bin = [&](unsigned k) { return fresh ? first_bin(k) : (int)((hi - k) >> shift); };
+        u64 a, b;
+        if (ready) {
+          const ulonglong2 sums = reinterpret_cast<const ulonglong2*>(p.bins + (size_t)r * SAMPLE_BINS)[tid];
+          a = sums.x;
+          b = sums.y;
+          ready = false;
+        } else {
+          __syncthreads();
+#pragma unroll
+          for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_THREADS) s.bins[i] = 0;
+          __syncthreads();
+          sweep(0, tiles, [&](float z, int i) {
+            const unsigned k = logit_key(z, p.z_clamp);
+            if (k == 0 || k < lo || k > hi || !in_prefix(in, k, i)) return;
+            atomicAdd(&s.bins[bin(k)], by_mass ? whole_part(scaled(k)) : 1);
+          }, Nothing());
+          __syncthreads();
+          a = s.bins[2 * tid];
+          b = s.bins[2 * tid + 1];
+        }
+        u64 total;
+        const u64 upto = above + scan(a + b, total, Add()), before = upto - a - b;
+        if (fresh) need = by_mass ? share_of(total) : (u64)top_k;
+        if (!by_mass && fresh && need >= total) {  // top-k takes all
+          by_mass = true;
+          cut = cut_p;
+          continue;
+        }
+        if (before < need && upto >= need) {
+          const bool second = before + a < need;
+          s.bin = 2 * tid + second;
+          s.above = before + (second ? a : 0);
+        }
+        // The tokens of that range, and all above if they fit the list.
+        bool all = fresh;
+        int n;
+#pragma unroll 1
+        while (true) {
+          if (tid == 0) {
+            s.lo = 0xFFFFFFFFu;
+            s.hi = s.count = 0;
+          }
+          __syncthreads();
+          const int at = s.bin;
+          sweep(0, tiles, [&](float z, int i) {
+            const unsigned k = logit_key(z, p.z_clamp);
+            if (k == 0 || k < lo || k > hi || !in_prefix(in, k, i)) return;
+            const int b = bin(k);
+            if (b > at || (b < at && !all)) return;
+            if (!all) {
+              atomicMin(&s.lo, k);
+              atomicMax(&s.hi, k);
+            }
+            const unsigned n = atomicAdd(&s.count, 1u);
+            if (n < SAMPLE_LIST) s.list[n] = (u64)k << 32 | (unsigned)~i;
+          }, Nothing());
+          __syncthreads();
+          n = (int)s.count;
+          if (n <= SAMPLE_LIST || !all) break;
+          all = false;
+          __syncthreads();
+        }
+        above = s.above;
+        if (!all) {
+          lo = s.lo;
+          hi = s.hi;
+        }
+        fresh = false;
+        if (n <= SAMPLE_LIST) {
+          u64 mine = tid < n ? s.list[tid] : 0;
+          if (n <= SAMPLE_RANKED) {
+            int rank = 0;
+            if (tid < n)
+#pragma unroll 4
+              for (int i = 0; i < n; ++i) rank += s.list[i] > mine;
+            __syncthreads();
+            s.list[tid < n ? rank : tid] = mine;
+            __syncthreads();
+            mine = s.list[tid];
+          } else {
+            int size = 64;
+            while (size < n) size <<= 1;
+            mine = sorted(mine, size);
+            __syncthreads();
+            s.list[tid] = mine;
+          }
+          if (all) {
+            listed = n;
+            first_k = by_mass ? 0 : top_k;
+            break;
+          }
+          u64 ignored;
+          const unsigned k = (unsigned)(mine >> 32);
+          const u64 v = tid < n ? (by_mass ? whole_part(scaled(k)) : 1) : 0;
+          const u64 sum = above + scan(v, ignored, Add());
+          if (sum - v < need && sum >= need) s.found = Prefix{k, (int)~(unsigned)mine};
+          __syncthreads();
+          in = s.found;
+        } else if (lo == hi) {  // one logit: as many of its tokens as it takes
+          const u64 each = by_mass ? whole_part(scaled(lo)) : 1;
+          wanted_tie = (need - above + each - 1) / each;
+          ties = true;
+        } else {
+          continue;
+        }
+        if (!ties) {  // the next cut
+          cut = !by_mass && cut_p;
+          by_mass = true;
+          fresh = true;
+          lo = 0;
+          hi = top;
+          above = 0;
+          continue;
+        }
       }
+      // A draw: of the wanted one of equal logits, or of the kept tokens. The sums of waves say which wave's.
+      const auto value = [&](float z, int i) -> u64 {
+        const unsigned k = logit_key(z, p.z_clamp);
+        if (k == 0 || !in_prefix(in, k, i)) return 0;
+        return ties ? (u64)(k == lo) : kept(k);
+      };
+      if (ready) {
+        for (int i = tid; i < tiles * SAMPLE_WAVES; i += SAMPLE_THREADS)
+          (&s.tile[0][0])[i] = p.sums[(size_t)r * tiles * SAMPLE_WAVES + i];
+      } else {
+        u64 v = 0;
+        sweep(0, tiles, [&](float z, int i) { v += value(z, i); }, [&](int t) {
+          v = wave_scan(v, Add());
+          if (lane == 63) s.tile[t][wave] = v;
+          v = 0;
+        });
+      }
+      __syncthreads();
+      u64 v = 0, total;
+      for (int i = tid; i < tiles * SAMPLE_WAVES; i += SAMPLE_THREADS) v += (&s.tile[0][0])[i];
+      scan(v, total, Add());
+      const u64 target = ties ? wanted_tie - 1 : drawn(u, total);
+      int t = 0, w = 0;
+      u64 below = 0;
+#pragma unroll 1
+      for (; t < tiles - 1; ++t) {
+        u64 sum = 0;
+#pragma unroll
+        for (int i = 0; i < SAMPLE_WAVES; ++i) sum += s.tile[t][i];
+        if (below + sum > target) break;
+        below += sum;
+      }
+#pragma unroll 1
+      for (; w < SAMPLE_WAVES - 1; ++w) {
+        if (below + s.tile[t][w] > target) break;
+        below += s.tile[t][w];
+      }
+      if (wave == w) {
+        Four z = logits(t);
+        u64 got[4], sum = 0;
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+          const u64 x = value((float)z.z[0], first(t) + e);
+          got[0] = got[1];
+          got[1] = got[2];
+          got[2] = got[3];
+          got[3] = x;
+          sum += x;
+          z.z[0] = z.z[1];
+          z.z[1] = z.z[2];
+          z.z[2] = z.z[3];
+        }
+        below += wave_scan(sum, Add()) - sum;  // up to this lane's tokens
+        if (below <= target && below + sum > target) {
+          int e = 0;
+          u64 mine = got[0];
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            below += got[i];
+            if (below <= target) {
+              ++e;
+              mine = got[i + 1];
+            }
+          }
+          if (ties) s.token = first(t) + e;
+          else answer(first(t) + e, log_share(mine, total));
+        }
+      }
+      if (!ties) return;
+      __syncthreads();
+      in = Prefix{lo, s.token};
+      ties = false;
+      cut = !by_mass && cut_p;
+      by_mass = true;
+      fresh = true;
+      lo = 0;
+      hi = top;
+      above = 0;
+    }
+
+    // The list's tokens, a lane each, by falling logit; then the kept ones by their index.
+    const u64 mine = s.list[tid];
+    const bool is = tid < (first_k ? first_k : listed);
+    const double v = is ? scaled((unsigned)(mine >> 32)) : 0.0;
+    const u64 m = is ? whole_part(v) : 0;
+    u64 total;
+    const u64 upto = scan(m, total, Add());
+    if (first_k) need = cut_p ? share_of(total) : total;
+    const bool keep = is && v >= floor_v && (tid == 0 || upto - m < need);
+    const unsigned index = ~(unsigned)mine;
+    s.value[tid] = keep ? m : 0;
+    u64 sum = 0, all = 0;  // what the kept tokens of lower index have, and all
+    if (listed <= SAMPLE_RANKED) {
+      s.list[tid] = index;
+      __syncthreads();
+      if (!keep) return;
+#pragma unroll 4
+      for (int i = 0; i < listed; ++i) {
+        const u64 w = s.value[i];
+        all += w;
+        sum += s.list[i] < index ? w : 0;
+      }
+      const u64 t = drawn(u, all);
+      if (sum <= t && sum + m > t) answer((int)index, log_share(m, all));
       return;
     }
-    const auto value = [&](unsigned k, int i) { return kept(in, k, i); };
-    u64 total;
-    if (READY && !cut_k && !cut_p) {
-      u64 v = 0;
-      for (int i = tid; i < tiles * SAMPLE_WAVES; i += SAMPLE_THREADS)
-        v += (&s.tile[0][0])[i] = p.sums[(size_t)r * tiles * SAMPLE_WAVES + i];
-      scan(v, total);
-    } else {
-      total = sums(value);
-    }
-    const int token = pick(target(total), value);
-    answer(token, tid == 0 ? log((double)value(logit_key((float)row[token], p.z_clamp), token) / (double)total) : 0.0);
+    int size = 64;
+    while (size < listed) size <<= 1;
+    const unsigned by_index = (unsigned)sorted(keep ? (u64) ~(index << 10 | (unsigned)tid) : 0, size);
+    __syncthreads();
+    const u64 w = by_index ? s.value[~by_index & 1023] : 0;
+    sum = scan(w, all, Add());
+    const u64 t = drawn(u, all);
+    if (by_index && sum - w <= t && sum > t) answer((int)(~by_index >> 10), log_share(w, all));
+  }
+  // u as a share of `total`, in whole numbers below it: below 0 or NaN as 0, 1 or more as the largest below.
+  static __device__ __forceinline__ u64 drawn(double u, u64 total) {
+    const double at = floor((u >= 0.0 ? u : 0.0) * (double)total);
+    return at < (double)total ? min((u64)at, total - 1) : total - 1;
   }
 };
 
 }  // namespace
 
-template <typename T, bool READY>
+template <typename T>
 __global__ __launch_bounds__(SAMPLE_THREADS) void head_sample_kernel(HeadSampleParams p) {
   __shared__ SampleShared s;
-  Sampler<T, READY>(p, s, blockIdx.x).run();
+  Sampler<T>(p, s, blockIdx.x).run(p.best != nullptr);
 }
 
 // Few rows leave most CUs without one, so the passes over a whole row are spread over its tiles, a workgroup each:
@@ -546,20 +612,20 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void head_sample_kernel(HeadSampleP
 template <typename T>
 __global__ __launch_bounds__(SAMPLE_THREADS) void head_sample_best_kernel(HeadSampleParams p) {
   __shared__ SampleShared s;
-  Sampler<T, false> row(p, s, blockIdx.y);
+  Sampler<T> row(p, s, blockIdx.y);
   const u64 c = row.best(blockIdx.x, blockIdx.x + 1);
   if (threadIdx.x == 0) p.best[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = c;
   for (int i = blockIdx.x * SAMPLE_THREADS + threadIdx.x; i < SAMPLE_BINS; i += gridDim.x * SAMPLE_THREADS) {
     p.bins[(size_t)blockIdx.y * SAMPLE_BINS + i] = 0;
-    p.counts[(size_t)blockIdx.y * SAMPLE_BINS + i] = 0;
   }
 }
 template <typename T>
 __global__ __launch_bounds__(SAMPLE_THREADS) void head_sample_share_kernel(HeadSampleParams p) {
   __shared__ SampleShared s;
-  Sampler<T, true> row(p, s, blockIdx.y);
+  Sampler<T> row(p, s, blockIdx.y);
   row.tables();
-  for (int i = threadIdx.x; i < SAMPLE_BINS; i += SAMPLE_THREADS) s.bins[i] = s.counts[i] = 0;
+#pragma unroll
+  for (int i = threadIdx.x; i < SAMPLE_BINS; i += SAMPLE_THREADS) s.bins[i] = 0;
   const int tiles = gridDim.x;
   const u64 c = row.largest((int)threadIdx.x < tiles ? p.best[(size_t)blockIdx.y * tiles + threadIdx.x] : 0);
   if (c != ~0ull && c >> 32 && row.temperature > 0.0f) {
@@ -571,14 +637,12 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void head_sample_share_kernel(HeadS
 template <typename T>
 static void launch_sample(const HeadSampleParams& p, hipStream_t st) {
   const dim3 threads(SAMPLE_THREADS);
-  if (!p.best) {
-    hipLaunchKernelGGL((head_sample_kernel<T, false>), dim3(p.N), threads, 0, st, p);
-    return;
+  if (p.best) {
+    const dim3 grid(sample_tiles(p.V), p.N);
+    hipLaunchKernelGGL(head_sample_best_kernel<T>, grid, threads, 0, st, p);
+    hipLaunchKernelGGL(head_sample_share_kernel<T>, grid, threads, 0, st, p);
   }
-  const dim3 grid(sample_tiles(p.V), p.N);
-  hipLaunchKernelGGL(head_sample_best_kernel<T>, grid, threads, 0, st, p);
-  hipLaunchKernelGGL(head_sample_share_kernel<T>, grid, threads, 0, st, p);
-  hipLaunchKernelGGL((head_sample_kernel<T, true>), dim3(p.N), threads, 0, st, p);
+  hipLaunchKernelGGL(head_sample_kernel<T>, dim3(p.N), threads, 0, st, p);
 }
 
 hipError_t launch_head_sample(const HeadSampleParams& p, hipStream_t st) {
