@@ -190,7 +190,8 @@ struct Sampler {
     }
     return f;
   }
-  // f(logit, token) for every token of tiles [begin, end), and g(t) after each tile; four tiles' loads are under way.
+  // f(logit, token) for every token of tiles [begin, end), and g(t) after each tile, which may end it;
+  // four tiles' loads are under way.
   template <typename F, typename G>
   __device__ __forceinline__ void sweep(int begin, int end, F f, G g) const {
     const auto load = [&](int t) { return logits(min(t, end - 1)); };
@@ -209,11 +210,11 @@ struct Sampler {
         now.z[1] = now.z[2];
         now.z[2] = now.z[3];
       }
-      g(t);
+      if (g(t)) break;
     }
   }
   struct Nothing {
-    __device__ __forceinline__ void operator()(int) const {}
+    __device__ __forceinline__ bool operator()(int) const { return false; }
   };
 
   // log2 rho(x) = log2(|x| + sqrt(1 + x^2)), to 2^-43: the root is q rsqrt(q), the hardware's with one step of
@@ -395,6 +396,7 @@ struct Sampler {
           s.above = before + (second ? a : 0);
         }
         // The tokens of that range, and all above if they fit the list.
+        const bool round0 = fresh;
         bool all = fresh;
         int n;
 #pragma unroll 1
@@ -405,7 +407,13 @@ struct Sampler {
           }
           __syncthreads();
           const int at = s.bin;
+          // What is surely under that range (the first histogram's: by two ranges, and what floats round) is passed
+          // over before anything is formed of it; a list that has run over is left.
+          const float z_top = top == KEY_CLAMPED ? p.z_clamp : key_logit(top), step = (float)(64.0 * p.inv_c);
+          const float z_cut = z_top - (at + 2) / step, z_low = z_cut - 0x1p-20f * (fabsf(z_top) + fabsf(z_cut));
+          const float z_min = round0 && at < SAMPLE_BINS - 1 && z_low > -INFINITY && z_low < INFINITY ? z_low : -INFINITY;
           sweep(0, tiles, [&](float z, int i) {
+            if (!(z >= z_min)) return;
             const unsigned k = logit_key(z, p.z_clamp);
             if (k == 0 || k < lo || k > hi || !in_prefix(in, k, i)) return;
             const int b = bin(k);
@@ -416,7 +424,7 @@ struct Sampler {
             }
             const unsigned n = atomicAdd(&s.count, 1u);
             if (n < SAMPLE_LIST) s.list[n] = (u64)k << 32 | (unsigned)~i;
-          }, Nothing());
+          }, [&](int) { return all && *(volatile unsigned*)&s.count > SAMPLE_LIST; });
           __syncthreads();
           n = (int)s.count;
           if (n <= SAMPLE_LIST || !all) break;
@@ -491,6 +499,7 @@ struct Sampler {
           v = wave_scan(v, Add());
           if (lane == 63) s.tile[t][wave] = v;
           v = 0;
+          return false;
         });
       }
       __syncthreads();
