@@ -1284,14 +1284,17 @@ int alg_head_logits(alg_stream_t stream, int dtype, int N, int d, int V, const v
   return hip_status(alg::launch_head_logits(p, (hipStream_t)stream), "alg_head_logits");
 }
 
-// Few rows are spread over their tiles (head_sample.hip): [best][bins][sums].
+// Few rows of more than two tiles are spread over them (head_sample.hip): [best][bins][sums]. us of one workgroup a
+// row and spread, without cuts, top-k 50, top-p 0.9: V 8000, 1 row 15 17, 17 19, 19 20; V 16000, 64 rows 25 20, 21 23, 30
+// 26, 128 rows 25 24, 21 25, 35 35; V 32000, 1 row 39 20, 28 22, 43 23, 128 rows 42 35, 29 33, 46 41, 192 rows 42
+// 44, 30 40, 48 52; V 100000, 128 rows 110 80, 66 71, 120 91.
 struct SampleWs {
   size_t bins, sums, total;
 };
 static SampleWs sample_ws(int N, int V) {
   SampleWs w{0, 0, 0};
   const size_t tiles = alg::sample_tiles(V);
-  if (tiles < 2 || N > 256) return w;
+  if (tiles < 3 || N > 128 || (size_t)N > 16 * tiles) return w;
   w.bins = align256(N * tiles * 8);
   w.sums = w.bins + (size_t)N * alg::SAMPLE_BINS * 8;
   w.total = w.sums + N * tiles * alg::SAMPLE_WAVES * 8;
