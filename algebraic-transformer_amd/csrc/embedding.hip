@@ -100,8 +100,9 @@ __global__ __launch_bounds__(SORT_BLOCK) void embedding_hist_kernel(EmbeddingPar
 // Each token to its place in the order of these 8 bits, equal ones as they stand: a workgroup 1024 tokens, a wave
 // 64, whose lanes of equal bits find each other by ballots. With few tokens every workgroup counts them all
 // itself, which takes as long as a launch that counts them, and saves it (16384 tokens, two passes: 18 us so, 25).
+// Tokens of one block are one workgroup's, which makes all passes.
 template <bool COUNT>
-__global__ __launch_bounds__(SORT_BLOCK) void embedding_scatter_kernel(EmbeddingParams p, int pass) {
+__device__ __forceinline__ void scatter(const EmbeddingParams& p, int pass) {
   __shared__ int base[SORT_WAVES][256], sums[256], before[256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, begin = blockIdx.x * SORT_BLOCK;
   const int i = begin + tid;
@@ -173,6 +174,16 @@ __global__ __launch_bounds__(SORT_BLOCK) void embedding_scatter_kernel(Embedding
     const int to = base[wave][bits] + rank;
     p.keys[pass & 1][to] = key;
     p.pos[pass & 1][to] = where;
+  }
+}
+template <bool COUNT>
+__global__ __launch_bounds__(SORT_BLOCK) void embedding_scatter_kernel(EmbeddingParams p, int pass) {
+  scatter<COUNT>(p, pass);
+}
+__global__ __launch_bounds__(SORT_BLOCK) void embedding_sort_kernel(EmbeddingParams p) {
+  for (int pass = 0; pass < p.passes; ++pass) {
+    if (pass) __syncthreads();  // what the pass before wrote
+    scatter<true>(p, pass);
   }
 }
 
@@ -336,7 +347,8 @@ hipError_t launch_embedding_fwd(const EmbeddingParams& p, hipStream_t st) {
 hipError_t launch_embedding_bwd(const EmbeddingParams& p, hipStream_t st) {
   if (p.N) {
     KTimer t("embedding_sort", st);
-    for (int pass = 0; pass < p.passes; ++pass) {
+    if (p.blocks == 1) hipLaunchKernelGGL(embedding_sort_kernel, dim3(1), dim3(SORT_BLOCK), 0, st, p);
+    for (int pass = 0; pass < p.passes && p.blocks > 1; ++pass) {
       if (p.blocks <= SORT_COUNT) {
         hipLaunchKernelGGL(embedding_scatter_kernel<true>, dim3(p.blocks), dim3(SORT_BLOCK), 0, st, p, pass);
       } else {
