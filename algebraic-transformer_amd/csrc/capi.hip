@@ -1564,10 +1564,17 @@ static int check_table(int width, int page, int pages) {
 // heads over 4 of 128, us of tiles of 16, 32, 128 rows with their joins: 16 rows each 52 54 63, 32 rows 80 55
 // 63, 40 rows 94 82 64, 128 rows 153 98 73; 64 of 2000, 32 over 8: 16 rows 97 99 111, 32 rows 112 101 112,
 // 48 rows 147 121 114.
-// Ranges, the former: at most one workgroup a CU, none under DECODE_RANGE keys of a sequence as long
+// Ranges, the former, bf16: at most one workgroup a CU, none under DECODE_RANGE keys of a sequence as long
 // as the table allows. One token over 131001 keys, 4 heads of 128: 64 workgroups 82 us, 128 to 256
 // 47 to 49, 320 60, 512 50; over 8000 keys, 8 heads: 64 20 us, 256 (250 keys each) 14, 512 17. (All of
 // D = 128; D = 64 takes the same. From 129 workgroups on nothing is split, whatever the lengths.)
+// Over a cache of 8 bits two workgroups a CU where there are several sequences, since the longest ends last, none
+// split under a reach of 1280 keys. us of one range, of 256, 512 and 768 workgroups, calls included: 64
+// groups (sequences x key heads) of 4000 keys on average, the longest 12000: 80 31.5 26.8 26.5; of 16000 and 48000: 60
+// 60 and 88 64 63 (256, 512 and 768); 256 groups, the same 4000: 84 84 66 65, all
+// of 4000 59 59 60 61; 320 groups, the longest thrice the average, of 4000: 84 84 78 78 (2 ranges from 512 on; 3 76); 512
+// groups of 3170 91, of 2 ranges 88, others 101 and 106; 600 keys: 20 unsplit, 23 to 24 split. One
+// sequence of 131001 keys, 4 heads: 38 of 256, 40 of 512, 42 to 45 of 384 and 768.
 // The latter: the n ranges of the least estimate, 17 ns a key and workgroup (a second one on a CU takes as
 // much from the first), 6 us and 33 ns a workgroup and range for joining. One sequence: rounds of equal
 // workgroups, ceil(workgroups n / 256) / n. Several, the longest first: the longest range or the CUs'
@@ -1594,7 +1601,8 @@ static PagedPlan paged_plan(int N, int S, int H, int Hkv, int D, int width, int 
   const long most = std::min({cap / alg::DECODE_RANGE, 65536 / slots, (long)alg::MAX_RANGES});
   pl.nsplit = 1;
   if (pl.row_tiles) {
-    pl.nsplit = (int)std::max(1L, std::min(256 / groups, most));
+    const long want = !fp8 ? 256 / groups : cap < 1280 ? 1 : seqs == 1 ? 256 / groups : (512 + groups / 2) / groups;
+    pl.nsplit = (int)std::max(1L, std::min(want, most));
   } else {
     double best = INFINITY;
     for (int n = 1; n <= std::min({768 / groups, most, 64L}) || n == 1; ++n) {
