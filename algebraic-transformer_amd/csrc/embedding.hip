@@ -23,7 +23,7 @@ namespace {
 constexpr int EMB_THREADS = 256;
 constexpr int SORT_BLOCK = 1024;  // tokens a workgroup of a pass takes, one a lane
 constexpr int SORT_WAVES = SORT_BLOCK / 64;
-constexpr int SORT_COUNT = 32;    // blocks up to which each counts all tokens
+constexpr int SORT_COUNT = 4;     // blocks up to which each counts all tokens
 constexpr int ZERO_ROWS = 32;     // rows of the table that a workgroup looks after for zeros
 constexpr int EMB_COLS = 512;     // columns a wave takes: 8 a lane
 
@@ -99,8 +99,9 @@ __global__ __launch_bounds__(SORT_BLOCK) void embedding_hist_kernel(EmbeddingPar
 
 // Each token to its place in the order of these 8 bits, equal ones as they stand: a workgroup 1024 tokens, a wave
 // 64, whose lanes of equal bits find each other by ballots. With few tokens every workgroup counts them all
-// itself, which takes as long as a launch that counts them, and saves it (16384 tokens, two passes: 18 us so, 25).
-// Tokens of one block are one workgroup's, which makes all passes.
+// itself, which saves a launch that counts them (both passes: 4096 tokens 15 to 16 us so, 17 with it; 8161 19 to 22,
+// 18; 16384 25 to 32, the more so the more tokens are equal, 18). Tokens of one block are one workgroup's,
+// which makes all passes (1024 tokens 10 us).
 template <bool COUNT>
 __device__ __forceinline__ void scatter(const EmbeddingParams& p, int pass) {
   __shared__ int base[SORT_WAVES][256], sums[256], before[256];
@@ -132,6 +133,7 @@ __device__ __forceinline__ void scatter(const EmbeddingParams& p, int pass) {
     }
     __syncthreads();
   } else if (tid < 256) {
+#pragma unroll 8
     for (int b = 0; b < p.blocks; ++b) {
       const int c = p.hist[tid * p.blocks + b];
       if (b < (int)blockIdx.x) earlier += c;
@@ -187,13 +189,13 @@ __global__ __launch_bounds__(SORT_BLOCK) void embedding_sort_kernel(EmbeddingPar
   }
 }
 
-// The first of n sorted keys that is not below v: 64 of them looked at each time.
-__device__ __forceinline__ int lower_bound(const int* keys, int n, int v) {
+// The first of n sorted keys, `apart` from each other, that is not below v: 64 of them looked at each time.
+__device__ __forceinline__ int lower_bound(const int* keys, int n, int v, int apart = 1) {
   const int lane = threadIdx.x & 63;
   int lo = 0;
   while (n > 0) {
     const int step = (n + 63) / 64, at = lane * step;
-    const int c = __popcll(__ballot(at < n && keys[lo + at] < v));
+    const int c = __popcll(__ballot(at < n && keys[(size_t)(lo + at) * apart] < v));
     if (c == 0) break;
     lo += (c - 1) * step + 1;
     n = min(step, n - (c - 1) * step) - 1;
@@ -281,42 +283,53 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_bwd_kernel(EmbeddingPar
   leave(tail);
 }
 
-// Runs over several chunks: the wave of the chunk where one begins adds up its parts, in order.
+// Runs over several chunks: the workgroup of the chunk where one begins adds up its parts, each wave a quarter of
+// them in order, then the quarters in order. (16384 tokens of 64 columns, a
+// third of them one, 14 us, of one wave for all 47; a text's, 2048 columns, 8 and 10.)
 template <typename E>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(EmbeddingParams p) {
-  constexpr int BATCH = 8;
+  constexpr int WAVES = EMB_THREADS / 64;
+  __shared__ float quarter[WAVES - 1][EMB_COLS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int* keys = p.keys[(p.passes - 1) & 1];
-  const int strips = (p.d + EMB_COLS - 1) / EMB_COLS;
-  const int unit = blockIdx.x * (EMB_THREADS / 64) + wave;
-  const int j = unit / strips, col = (unit - j * strips) * EMB_COLS + 8 * lane;
+  const int strips = (p.d + EMB_COLS - 1) / EMB_COLS, j = blockIdx.x / strips;
+  const int col = (blockIdx.x - j * strips) * EMB_COLS + 8 * lane;
   const int end = (j + 1) * p.chunk;
-  if (j >= p.chunks || end >= p.N) return;
+  if (end >= p.N) return;
   const int run = keys[end - 1], next = keys[end], last = j > 0 ? keys[j * p.chunk - 1] : -1;
   if (run >= p.V || next != run || last == run) return;
+  // The chunks that begin with the run: j + 1 to j + n.
+  const int n = lower_bound(keys + end, p.chunks - j - 1, run + 1, p.chunk);
+  const int each = (n + WAVES - 1) / WAVES, stop = min(n, (wave + 1) * each);
   const bool live = col < p.d;
+  const float* part = p.part + (live ? col : 0);
   float sum[8] = {};
-  if (live) load8(p.part + ((size_t)2 * j + 1) * p.d + col, sum);
-  for (int i0 = j + 1; i0 < p.chunks; i0 += 64) {
-    // How many of these chunks begin with the run.
-    const int i = i0 + lane;
-    const unsigned long long more = __ballot(i < p.chunks && keys[min(i, p.chunks - 1) * p.chunk] == run);
-    const int n = more == ~0ull ? 64 : __builtin_ctzll(~more);
-    for (int b = 0; b < n; b += BATCH) {
-      float x[BATCH][8];
+  if (wave == 0) load8(part + ((size_t)2 * j + 1) * p.d, sum);
+  const auto add = [&](int b, auto batch) {
+    constexpr int B = decltype(batch)::value;
+    float x[B][8];
 #pragma unroll
-      for (int e = 0; e < BATCH; ++e)
-        load8(p.part + (size_t)2 * (i0 + min(b + e, n - 1)) * p.d + (live ? col : 0), x[e]);
+    for (int e = 0; e < B; ++e) load8(part + (size_t)2 * (j + 1 + min(b + e, stop - 1)) * p.d, x[e]);
 #pragma unroll
-      for (int e = 0; e < BATCH; ++e) {
-        if (b + e >= n) break;
+    for (int e = 0; e < B; ++e) {
+      if (b + e >= stop) break;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) sum[c] += x[e][c];
-      }
+      for (int c = 0; c < 8; ++c) sum[c] += x[e][c];
     }
-    if (n < 64) break;
+  };
+  int b = wave * each;
+  for (; b + 8 < stop; b += 16) add(b, std::integral_constant<int, 16>{});
+  for (; b < stop; b += 2) add(b, std::integral_constant<int, 2>{});
+  if (wave) store8(&quarter[wave - 1][8 * lane], sum);
+  __syncthreads();
+  if (wave || !live) return;
+#pragma unroll
+  for (int w = 0; w < WAVES - 1; ++w) {
+    float x[8];
+    load8(&quarter[w][8 * lane], x);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) sum[c] += x[c];
   }
-  if (!live) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[e] *= p.scale;
   store8(static_cast<E*>(p.grad) + (size_t)run * p.d + col, sum);
@@ -367,8 +380,8 @@ hipError_t launch_embedding_bwd(const EmbeddingParams& p, hipStream_t st) {
   }
   if (p.chunks > 1) {
     KTimer t("embedding_join", st);
-    if (p.table_bf16) hipLaunchKernelGGL(embedding_join_kernel<bf16>, dim3((unsigned)work), dim3(EMB_THREADS), 0, st, p);
-    else hipLaunchKernelGGL(embedding_join_kernel<float>, dim3((unsigned)work), dim3(EMB_THREADS), 0, st, p);
+    if (p.table_bf16) hipLaunchKernelGGL(embedding_join_kernel<bf16>, dim3((unsigned)(p.chunks * strips)), dim3(EMB_THREADS), 0, st, p);
+    else hipLaunchKernelGGL(embedding_join_kernel<float>, dim3((unsigned)(p.chunks * strips)), dim3(EMB_THREADS), 0, st, p);
   }
   return hipGetLastError();
 }

@@ -375,6 +375,14 @@ def test_embedding(N, V, d, kind):
     _check_embedding(tokens, rn(V, d), rn(N, d).to(BF), 3.3, BF)
 
 
+@pytest.mark.parametrize("kind", ["even", "common", "padded"])
+@pytest.mark.parametrize("N,V", [(1024, 256), (1025, 777), (4096, 65535), (4097, 50257), (16384, 1 << 18)])
+def test_embedding_where_sorts_meet(N, V, kind):
+    g, rn = _gen(N ^ V)
+    print(f"[embedding] N{N} V{V} {kind}", flush=True)
+    _check_embedding(_tokens(N, V, kind, g), rn(V, 8), rn(N, 8).to(BF), 1.5, BF)
+
+
 @pytest.mark.parametrize("table", [BF, F32])
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("ints", [torch.int32, torch.int64])
