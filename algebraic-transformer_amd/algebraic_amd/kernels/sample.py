@@ -61,8 +61,8 @@ def _setting(name, x, N, dtype, device, least):
         raise ValueError(f"{name} must be on {device}")
     if dtype is torch.int32 and x.is_floating_point():
         raise ValueError(f"{name} must hold whole numbers")
-    if x.dtype is not dtype:  # a top_k past int32 is past every vocabulary too
-        x = x.clamp(max=2 ** 31 - 1).to(dtype) if x.dtype is torch.int64 and dtype is torch.int32 else x.detach().to(dtype)
+    if x.dtype is not dtype:  # a top_k past int32 is past every vocabulary too, and all below 0 are alike
+        x = x.clamp(0, 2 ** 31 - 1).to(dtype) if x.dtype is torch.int64 and dtype is torch.int32 else x.detach().to(dtype)
     return x.expand(N).contiguous(), 0
 
 
@@ -78,7 +78,8 @@ def head_sample(logits, uniforms, *, n: int = 8, c: float = 2.0, temperature=1.0
     the first of the largest logits.
 
     ``logits`` float32 or bfloat16, rows with a contiguous last axis any distance apart, V up to 2^20; ``uniforms`` (N,)
-    float32 or float64 in [0, 1) (``torch.rand``). Each setting is a number or a tensor (N,) of one a row. Weights are
+    float32 or float64 in [0, 1) (``torch.rand``). Each setting is a number or a tensor (N,) of one a row, in which
+    what is below 0 counts as 0 (but for temperatures). Weights are
     formed in 64 bits and summed in whole numbers, so that a row's token depends on nothing but the row. A
     logit of -inf is never drawn; a row without another, with a NaN, or with a temperature that is negative or
     NaN has token -1 and logprob NaN. No gradient.

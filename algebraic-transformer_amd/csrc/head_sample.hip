@@ -356,7 +356,7 @@ struct Sampler {
     unsigned lo = 0, hi = top;
     u64 above = 0, need = 0, wanted_tie = 0;
     int listed = 0, first_k = 0;
-    const auto share_of = [&](u64 total) { return max((u64)ceil((double)top_p * (double)total), (u64)1); };
+    const auto share_of = [&](u64 total) { return max((u64)ceil(fmax((double)top_p, 0.0) * (double)total), (u64)1); };
 #pragma unroll 1
     while (true) {
       if (cut) {

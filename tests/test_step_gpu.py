@@ -246,6 +246,17 @@ def test_sample_settings_of_each_row():
         assert torch.equal(one[0], each[0][i:i + 1]) and torch.equal(one[1], each[1][i:i + 1])
 
 
+def test_sample_settings_below_zero():
+    """In tensors, which are not read on the host: as zero."""
+    g, rn = _gen(41)
+    z, u = 2 * rn(5, 9001), torch.rand(5, device="cuda", generator=g)
+    low = torch.tensor([-0.5, -1e30, -math.inf, -1e-30, -0.0], device="cuda")
+    far = torch.tensor([-(1 << 33) + 5, -1, -(1 << 63), -(1 << 31), 0], device="cuda")
+    for a, b in ((dict(top_p=low), dict(top_k=1)), (dict(top_p=low, top_k=3000), dict(top_k=1)), (dict(min_p=low), {}), (dict(top_k=far), {})):
+        for x, y in zip(_sample()(z, u, **a), _sample()(z, u, **b)):
+            assert torch.equal(x, y), (a, b)
+
+
 def test_sample_whole_range_of_uniforms():
     """Every kept token is drawn over its own stretch of [0, 1), and no other token."""
     g, rn = _gen(6)
@@ -376,7 +387,8 @@ def test_embedding(N, V, d, kind):
 
 
 @pytest.mark.parametrize("kind", ["even", "common", "padded"])
-@pytest.mark.parametrize("N,V", [(1024, 256), (1025, 777), (4096, 65535), (4097, 50257), (16384, 1 << 18)])
+@pytest.mark.parametrize("N,V", [(1024, 256), (1025, 777), (4096, 65535), (4097, 50257), (16384, 1 << 18), (131072, 300), (131073, 70001),
+                                 (1100000, 32000)])
 def test_embedding_where_sorts_meet(N, V, kind):
     g, rn = _gen(N ^ V)
     print(f"[embedding] N{N} V{V} {kind}", flush=True)
