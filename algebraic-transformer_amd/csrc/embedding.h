@@ -18,7 +18,7 @@ struct EmbeddingParams {
   void* grad;          // (V, d), of the table's type
   int* keys[2];        // (N) tokens, and where they stood, sorted from one into the other
   int* pos[2];
-  int* hist;           // (256, blocks)
+  int* hist;           // (256, blocks), then 256 sums
   int blocks, passes;
   float* part;         // (2 chunks, d): sums of the runs that reach over a chunk's borders
   int chunk, chunks;   // sorted tokens in chunks of this many

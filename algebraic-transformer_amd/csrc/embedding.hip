@@ -24,6 +24,7 @@ constexpr int EMB_THREADS = 256;
 constexpr int SORT_BLOCK = 1024;  // tokens a workgroup of a pass takes, one a lane
 constexpr int SORT_WAVES = SORT_BLOCK / 64;
 constexpr int SORT_COUNT = 4;     // blocks up to which each counts all tokens
+constexpr int SORT_SUM = 128;      // blocks up to which each adds up the counts of all
 constexpr int ZERO_ROWS = 32;     // rows of the table that a workgroup looks after for zeros
 constexpr int EMB_COLS = 512;     // columns a wave takes: 8 a lane
 
@@ -97,6 +98,35 @@ __global__ __launch_bounds__(SORT_BLOCK) void embedding_hist_kernel(EmbeddingPar
   if (threadIdx.x < 256) p.hist[threadIdx.x * p.blocks + blockIdx.x] = count[threadIdx.x];
 }
 
+// Of many blocks, each value's counts made those of the blocks before, and their sum: a workgroup a value. (All passes
+// of 65536 tokens 26 us so, 22 without; 131072 26 and 27; 1048576 47 to 51 and 270.)
+__global__ __launch_bounds__(SORT_BLOCK) void embedding_sum_kernel(EmbeddingParams p) {
+  __shared__ int sums[SORT_WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int* counts = p.hist + (size_t)blockIdx.x * p.blocks;
+  int before = 0;
+  for (int b0 = 0; b0 < p.blocks; b0 += SORT_BLOCK) {
+    const int b = b0 + threadIdx.x, c = b < p.blocks ? counts[b] : 0;
+    int upto = c;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int below = __shfl_up(upto, m, 64);
+      if (lane >= m) upto += below;
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      if (w < wave) upto += sums[w];
+      all += sums[w];
+    }
+    if (b < p.blocks) counts[b] = before + upto - c;
+    before += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) p.hist[(size_t)256 * p.blocks + blockIdx.x] = before;
+}
+
 // Each token to its place in the order of these 8 bits, equal ones as they stand: a workgroup 1024 tokens, a wave
 // 64, whose lanes of equal bits find each other by ballots. With few tokens every workgroup counts them all
 // itself, which saves a launch that counts them (both passes: 4096 tokens 15 to 16 us so, 17 with it; 8161 19 to 22,
@@ -132,6 +162,11 @@ __device__ __forceinline__ void scatter(const EmbeddingParams& p, int pass) {
       total = earlier + sums[tid];
     }
     __syncthreads();
+  } else if (p.blocks > SORT_SUM) {
+    if (tid < 256) {
+      earlier = p.hist[(size_t)tid * p.blocks + blockIdx.x];
+      total = p.hist[(size_t)256 * p.blocks + tid];
+    }
   } else if (tid < 256) {
 #pragma unroll 8
     for (int b = 0; b < p.blocks; ++b) {
@@ -366,6 +401,7 @@ hipError_t launch_embedding_bwd(const EmbeddingParams& p, hipStream_t st) {
         hipLaunchKernelGGL(embedding_scatter_kernel<true>, dim3(p.blocks), dim3(SORT_BLOCK), 0, st, p, pass);
       } else {
         hipLaunchKernelGGL(embedding_hist_kernel, dim3(p.blocks), dim3(SORT_BLOCK), 0, st, p, pass);
+        if (p.blocks > SORT_SUM) hipLaunchKernelGGL(embedding_sum_kernel, dim3(256), dim3(SORT_BLOCK), 0, st, p);
         hipLaunchKernelGGL(embedding_scatter_kernel<false>, dim3(p.blocks), dim3(SORT_BLOCK), 0, st, p, pass);
       }
     }
