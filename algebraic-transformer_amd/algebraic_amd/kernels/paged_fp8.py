@@ -87,10 +87,10 @@ def _check_cache8(k_pages, v_pages, k_scales, v_scales, page_table, cu_seqlens, 
 def paged_append_fp8(q, k, v, k_pages, v_pages, k_scales, v_scales, page_table, cu_seqlens, kv_lens, q_gain=None,
                      k_gain=None, cos=None, sin=None, *, eps: float = 1e-5):
     """``paged_append`` into a cache of 8 bits: the new tokens' q (N, H, D) and k (N, Hkv, D) normed and
-    rotated in f32, k rounded once, to 8 bits, v to 8 bits, with a scale a row; returns the queries in bf16.
+    rotated in f64, k rounded (through f32) to 8 bits, v to 8 bits, with a scale a row; returns the queries in bf16.
 
     Positions, tables, gains, and what is out of range, as in ``paged_append``. Pages and scales are
-    written in place, one place a token.
+    written in place, one place a token (two tokens' one place may hold parts of both, a scale of the other's bytes).
     """
     _check_heads(q, k, v)
     (N, H, D), Hkv, dev = q.shape, k.shape[1], q.device

