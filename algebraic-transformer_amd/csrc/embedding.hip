@@ -11,8 +11,9 @@
 // of sorted tokens, not into runs: a chunk writes the runs that lie within it, and leaves the sums of those
 // that reach over its borders for a second launch, which adds them in order.
 //
-// Bytes bound it. 16384 tokens of a text, d 2048, V 32000, f32 table: lookup 28 us (156 MB, 5.7 TB/s), the gradient 77
-// (336 MB, 4.4 TB/s, 268 of them written; stores that pass the caches by took 116 for 82 then), its sort 16, the join 6.
+// Bytes bound it. 16384 tokens of a text, d 2048, V 32000, f32 table: lookup 28 us (156 MB, 5.7 TB/s), the gradient 69
+// (333 MB, 4.8 TB/s, 265 of them written; zeros in stores of 16 neighbouring bytes a lane: 6 less than of 32; stores
+// that pass the caches by took 116 for 82 then), its sort 16, the join 5.
 #include <type_traits>
 
 #include "common.h"
@@ -28,7 +29,7 @@ constexpr int SORT_BLOCK = 1024;  // tokens a workgroup of a pass takes, one a l
 constexpr int SORT_WAVES = SORT_BLOCK / 64;
 constexpr int SORT_COUNT = 4;     // blocks up to which each counts all tokens
 constexpr int SORT_SUM = 128;      // blocks up to which each adds up the counts of all
-constexpr int ZERO_ROWS = 32;     // rows of the table that a workgroup looks after for zeros
+constexpr int ZERO_ROWS = 16;     // rows of the table that a workgroup looks after for zeros
 constexpr int EMB_COLS = 512;     // columns a wave takes: 8 a lane
 
 template <typename T>
@@ -265,10 +266,11 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_bwd_kernel(EmbeddingPar
     for (int i = ends[0] + threadIdx.x; i < ends[1]; i += EMB_THREADS)
       if (keys[i] < p.V) held[keys[i] - v0] = 1;
     __syncthreads();
-    const float zero[8] = {};
+    const int pieces = p.d * (int)sizeof(E) / 16;
     for (int r = 0; r < min(ZERO_ROWS, p.V - v0); ++r)
       if (!held[r])
-        for (int c = 8 * threadIdx.x; c < p.d; c += 8 * EMB_THREADS) store8(grad + (size_t)(v0 + r) * p.d + c, zero);
+        for (int c = threadIdx.x; c < pieces; c += EMB_THREADS)
+          reinterpret_cast<float4*>(grad + (size_t)(v0 + r) * p.d)[c] = float4{};
     return;
   }
   const int unit = blockIdx.x * (EMB_THREADS / 64) + wave;

@@ -93,8 +93,8 @@ __device__ __forceinline__ TokenPlace token_place(const P& p, int tok) {
 
 // Into 8 bits the norm and rotation run in f64: a key that f32's few roundings carry over the border
 // between two of its steps is 2^-3 away. Results go through f32 on their way to 8 bits or (queries) bf16, 2^-24
-// beside half a step of 2^-4 or 2^-8. 7688 prompt tokens, 16 heads of 64, 80 MB: 30 us, 2.7 TB/s, of which f64
-// instructions, at the rate of f32's here, make 14 by count; neighbouring tokens on one XCD: no difference. 64 single
+// beside half a step of 2^-4 or 2^-8. 7688 prompt tokens, 16 heads of 64, 80 MB: 30 us, 2.7 TB/s; in f32 it
+// took 6 less, without the scales' bytes 2; neighbouring tokens on one XCD: no difference. 64 single
 // tokens, 32 heads over 8 of 128: 6 us.
 template <int D, bool FP8>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) {
