@@ -4,8 +4,11 @@
 //
 // Which token a number selects depends on sums over the vocabulary to their last bits wherever the number lies
 // next to a border, and V = 32000 borders lie everywhere. So the weights are f64, relative to the
-// row's largest (to 2^-40 or better), and are summed as whole numbers of 2^-bits (2^62 / V): such sums are
+// row's largest, and are summed as whole numbers of 2^-bits (2^62 / V): such sums are
 // equal in any order, among any number of lanes and atomics, and a row's token depends on the row alone.
+// log2 rho is good to 2^-44.8 (log2_rho), so a weight to (n / T) 2^-44 of itself, beside 2^-50 for the power of two:
+// 2^-41 at n / T = 8, 2^-34 at 1024, and nothing is left of it where n / T passes 2^44. Which logit is the largest, and
+// the order by logits, are exact at any temperature.
 //
 // Order: logits falling, equal ones by their index. The kept tokens are a prefix of it. Where a
 // histogram over 2048 ranges of the logits (by count for top-k, by weight for top-p) says that no more than
@@ -220,17 +223,20 @@ struct Sampler {
     __device__ __forceinline__ bool operator()(int) const { return false; }
   };
 
-  // log2 rho(x) = log2(|x| + sqrt(1 + x^2)), to 2^-43: the root is q rsqrt(q), the hardware's with one step of
-  // Newton's method.
+  // log2 rho(x) = log2(|x| + sqrt(1 + x^2)), to 2^-44.8: the root is q rsqrt(q), the hardware's (to 2^-23 of itself)
+  // with one step of Newton's method, which leaves 3/2 of the square, 2^-45.4; log2 2^-48. (2^22 of both signs: 2^-47.4.)
   __device__ __forceinline__ double log2_rho(unsigned key) const {
     const double x = key == KEY_CLAMPED ? p.clamp : (double)key_logit(key) * p.inv_c, a = __builtin_fabs(x);
     const double q = __builtin_fma(a, a, 1.0), y = __builtin_amdgcn_rsq(q), h = q * y;
     const double l = log2_of(a + __builtin_fma(0.5 * h, __builtin_fma(-h, y, 1.0), h), (TablesPtr)&s.tables);
     return x < 0.0 ? -l : l;
   }
-  // The weight times 2^bits: 2^d by the table's nearest 64th and five terms of the series.
+  // The weight times 2^bits: 2^d by the table's nearest 64th and five terms of the series. No key is over the
+  // largest, so d is 0 at most. But log2_rho rounds, and logits within 2^-20 c of zero may lie closer than its error
+  // (floats further out differ by more): times any n / T such an error could pass every exponent. Held at 0, weights
+  // stay within 2^bits, and V of them under 2^62, at any temperature.
   __device__ __forceinline__ double scaled(unsigned key) const {
-    const double d = fmax(power * (log2_rho(key) - log_top), -1000.0), j = __builtin_rint(d * 64.0);
+    const double d = fmin(fmax(power * (log2_rho(key) - log_top), -1000.0), 0.0), j = __builtin_rint(d * 64.0);
     const double f = __builtin_fma(j, -0.015625, d);
     const int ji = (int)j;
     double poly = __builtin_fma(f, LN2 * LN2 * LN2 * LN2 * LN2 / 120, LN2 * LN2 * LN2 * LN2 / 24);
