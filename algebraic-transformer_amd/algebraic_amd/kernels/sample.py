@@ -54,6 +54,8 @@ def _setting(name, x, N, dtype, device, least):
     if not torch.is_tensor(x):
         if not x >= least:
             raise ValueError(f"{name} must be {least} or more (got {x})")
+        if dtype is torch.int32 and x // 1 != x:  # (infinity // 1 is NaN)
+            raise ValueError(f"{name} must hold whole numbers")
         return None, x
     if x.dim() > 1 or (x.dim() == 1 and x.shape[0] != N):
         raise ValueError(f"{name} must be a number or a tensor ({N},)")
