@@ -81,8 +81,10 @@ def head_sample(logits, uniforms, *, n: int = 8, c: float = 2.0, temperature=1.0
 
     ``logits`` float32 or bfloat16, rows with a contiguous last axis any distance apart, V up to 2^20; ``uniforms`` (N,)
     float32 or float64 in [0, 1) (``torch.rand``). Each setting is a number or a tensor (N,) of one a row, in which
-    what is below 0 counts as 0 (but for temperatures). Weights are
-    formed in 64 bits and summed in whole numbers, so that a row's token depends on nothing but the row. A
+    what is below 0 counts as 0 (but for temperatures), and a NaN ``top_p`` as 1, a NaN ``min_p`` as 0. ``c``,
+    ``temperature``, ``top_p`` and ``min_p`` are taken as float32 numbers, however given (0.6 is 0.60000002...); from
+    there on weights are formed in 64 bits, good to (n / temperature) 2^-44 of themselves, and
+    summed in whole numbers, so that a row's token depends on nothing but the row. A
     logit of -inf is never drawn; a row without another, with a NaN, or with a temperature that is negative or
     NaN has token -1 and logprob NaN. No gradient.
     """

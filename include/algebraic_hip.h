@@ -456,9 +456,11 @@ int alg_head_logits(alg_stream_t stream, int dtype, int N, int d, int V, const v
  * weight (all if that is 1 or more; one at least), of those the ones of min_p times the largest weight
  * or more. token = the first kept one, by index, at which the running sum of the kept weights passes
  * u times their sum; logprob = the log of the probability that it was drawn with. temperature 0: the first
- * of the largest. Weights are f64 relative to the row's largest and summed as whole multiples of
+ * of the largest. Weights are f64 relative to the row's largest (good to (n / temperature) 2^-44 of
+ * themselves, for the f32 c and settings as they are given) and summed as whole multiples of
  * 2^-62 V (rounded up to a power of two), so that results depend on nothing but the row. Each setting
- * is an array (N) or, where the array is NULL, one value for all. u (N) f32 or f64 in [0, 1); below or
+ * is an array (N) or, where the array is NULL, one value for all; below 0 (but for temperatures) is 0,
+ * a top_p of NaN 1, a min_p of NaN 0. u (N) f32 or f64 in [0, 1); below or
  * NaN counts as 0, 1 or more as the largest number below 1. Logits of -infinity are never drawn; a row
  * without another, with a NaN, or whose temperature is negative or NaN gets token -1 and
  * logprob NaN. V up to 2^20. Workspace: alg_head_sample_workspace_size bytes (0: none), in which few
