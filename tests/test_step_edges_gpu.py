@@ -4,7 +4,7 @@ import math
 
 import pytest
 
-from test_step_gpu import BF, F32, F64, _check_sample, _gen, _sample
+from test_step_gpu import BF, F32, F64, SETTINGS, _check_sample, _gen, _sample
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -67,3 +67,104 @@ def test_sample_settings_that_are_nan(V):
     for a, b in ((dict(top_p=nan), {}), (dict(top_p=nan, top_k=20), dict(top_k=20)), (dict(min_p=nan), {}), (dict(min_p=nan, top_p=0.5), dict(top_p=0.5))):
         for x, y in zip(_sample()(z, u, **a), _sample()(z, u, **b)):
             assert torch.equal(x, y), (a, b)
+
+
+# Few rows of a large vocabulary (up to 128 of more than 8192) are spread over several workgroups each; others are one
+# workgroup's. The cases of test_step_gpu.py that a small vocabulary has, with a large one:
+
+WIDE = 12301  # four tiles, the last one nearly empty, rows that start anywhere
+
+
+@pytest.mark.parametrize("setting", SETTINGS, ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("what", ["any", "few values", "one value", "masked", "lowest", "huge", "signed zeros"])
+def test_sample_spread_rows_of_every_kind(what, dtype, setting):
+    g, rn = _gen(13)
+    N = 8
+    z = 2.0 * rn(N, WIDE) + 9.0 * torch.rand(N, WIDE, device="cuda", generator=g).pow(100.0)
+    out = torch.rand(N, WIDE, device="cuda", generator=g) < 0.9
+    if what == "few values":
+        z = z.round()
+    elif what == "one value":
+        z = torch.full_like(z, -1.5)
+    elif what == "masked":
+        z = torch.where(out, -math.inf, z)
+        z[0], z[0, 9000], z[1, :12288] = -math.inf, 3.0, -math.inf  # one token; the last tile alone
+    elif what == "lowest":
+        z = torch.where(out, torch.finfo(dtype).min, z)
+    elif what == "huge":
+        z = z * 10.0 ** torch.linspace(-3, 37, N, device="cuda")[:, None]
+        z[1, 5], z[2, 9], z[2, 12300] = math.inf, math.inf, 3e38
+        z = z.clamp(min=torch.finfo(dtype).min)
+    elif what == "signed zeros":
+        z = torch.where(out, 0.0, -0.0)
+    # (Masses of equal tokens are multiples of one another: more borders are met, and left out.)
+    _check_sample(z.to(dtype), torch.rand(N, device="cuda", generator=g), **setting, left_out=0.05 if what == "any" and dtype is F32 else 0.5)
+
+
+@pytest.mark.parametrize("n,c", [(1, 2.0), (2, 0.5), (16, 8.0), (1024, 30.0)])
+def test_sample_spread_rows_of_other_exponents(n, c):
+    g, rn = _gen(n)
+    z = 3.0 * rn(6, WIDE)
+    for setting in (dict(), dict(top_p=0.7, temperature=0.9), dict(top_k=9)):
+        _check_sample(z, torch.rand(6, device="cuda", generator=g), n=n, c=c, **setting)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_sample_spread_rows_without_an_answer(dtype):
+    z = torch.zeros(6, WIDE, device="cuda", dtype=dtype)
+    z[0], z[1, 7], z[2, :12300], z[3, 0], z[5, 12300] = -math.inf, math.nan, -math.inf, math.inf, -math.nan
+    for setting in (dict(), dict(top_k=3), dict(top_p=0.5), dict(temperature=0.0)):
+        token, logp = _check_sample(z, torch.full((6,), 0.3, device="cuda"), **setting, left_out=0.5)
+        assert token[:3].tolist() == [-1, -1, 12300] and int(token[5]) == -1 and torch.isnan(logp[[0, 1, 5]]).all()
+        assert logp[2] == 0 and int(token[3]) == 0
+    T = torch.tensor([1.0, 1.0, math.nan, -1.0, math.inf, 1e-30], device="cuda")
+    z = torch.arange(WIDE, device="cuda").to(dtype).expand(6, WIDE).contiguous()
+    for setting in (dict(), dict(top_k=WIDE), dict(top_p=0.99999)):
+        token, logp = _sample()(z, torch.full((6,), 0.999999, device="cuda"), temperature=T, **setting)
+        assert token[2:4].tolist() == [-1, -1] and torch.isnan(logp[2:4]).all() and int(token[4]) >= WIDE - 3
+        assert abs(float(logp[4]) + math.log(WIDE)) < 1e-4 and z[5, token[5]] == z[5].max()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_sample_spread_rows_of_any_stride(dtype):
+    g, rn = _gen(14)
+    wide = (2 * rn(9, WIDE + 13)).to(dtype)
+    u = torch.rand(9, device="cuda", generator=g)
+    for z in (wide[:, :WIDE], wide[:, 3:WIDE], wide[::2, 1:], wide.t().contiguous().t(), wide[:1, :WIDE]):
+        for setting in (dict(), dict(top_p=0.9), dict(top_k=70)):
+            _check_sample(z, u[:z.shape[0]], **setting, left_out=0.2 if dtype is BF else 0.05)
+
+
+def _settings_of_each_row(N):
+    row = torch.arange(N, device="cuda")
+    return dict(temperature=torch.where(row % 5 == 0, 0.0, 0.4 + 0.005 * row), top_k=torch.where(row % 3 == 0, 0, row * 9),
+                top_p=torch.where(row % 4 == 0, 1.0, 0.3 + 0.003 * row), min_p=torch.where(row % 7 == 0, 0.1, 0.0))
+
+
+def test_sample_spread_rows_with_settings_of_their_own():
+    g, rn = _gen(15)
+    _check_sample(2.5 * rn(64, WIDE), torch.rand(64, device="cuda", generator=g), **_settings_of_each_row(64))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("V", [8193, WIDE, 50257])
+def test_sample_the_same_from_one_workgroup_and_from_many(V, dtype):
+    """200 rows are a workgroup each, fewer are spread: the same tokens, and the same bits of their probabilities."""
+    g, rn = _gen(V)
+    N = 200
+    z = (2 * rn(N, V)).to(dtype)
+    z[5], z[6, 4000:], z[7, 8000], z[8] = -math.inf, -math.inf, math.nan, 1.0
+    u = torch.rand(N, device="cuda", generator=g)
+    for setting in [*SETTINGS, _settings_of_each_row(N)]:
+        whole = _sample()(z, u, **setting)
+        for a, b in ((0, 3), (3, 4), (4, 12), (12, 60), (60, 188), (188, 200)):
+            part = _sample()(z[a:b], u[a:b], **{k: x[a:b] if torch.is_tensor(x) else x for k, x in setting.items()})
+            for x, y in zip(part, whole):
+                assert torch.equal(x.nan_to_num(7.0), y[a:b].nan_to_num(7.0)), (setting, a)
+
+
+def test_sample_a_share_of_equal_logits_in_the_largest_vocabulary():
+    z, u = torch.zeros(2, 1 << 20, device="cuda"), torch.tensor([0.25, 0.9], device="cuda")
+    _check_sample(z, u, top_k=700001, left_out=0)
+    _check_sample(z.to(BF), u, top_k=3, left_out=0)
