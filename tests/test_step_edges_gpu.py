@@ -168,3 +168,40 @@ def test_sample_a_share_of_equal_logits_in_the_largest_vocabulary():
     z, u = torch.zeros(2, 1 << 20, device="cuda"), torch.tensor([0.25, 0.9], device="cuda")
     _check_sample(z, u, top_k=700001, left_out=0)
     _check_sample(z.to(BF), u, top_k=3, left_out=0)
+
+
+# --- the 8-bit cache --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D,heads", [(64, 16), (128, 8)])
+def test_append_stores_the_bytes_of_the_64_bit_statement(D, heads):
+    """Keys' bytes and scales against norm and rotation in float64, rounded to float32 and then to 8 bits, each of them
+    equal: float64's own error, 2^-40 here, is allowed for by a statement a little above and below, which differ
+    next to a border alone. (float32 arithmetic, off by 2^-23, would carry one key in 2^19 over one.)"""
+    from algebraic_amd import paged_append_fp8
+    from test_paged_fp8_gpu import E4M3, E8M0, _quantised
+    from test_paged_gpu import _i32, _tables
+    N, page, eps = 8000, 64, 2.0 ** -17  # (eps is a float32)
+    g, rn = _gen(D)
+    q, k, v = ((1.5 * rn(N, heads, D)).to(BF) for _ in range(3))
+    pages = N // page
+    kp, vp = (torch.zeros(pages, heads, page, D, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros(pages, heads, page, dtype=torch.uint8, device="cuda") for _ in range(2))
+    gq, gk = 1 + 0.1 * rn(D), 1 + 0.1 * rn(D)
+    cos, sin = _tables(N, D // 2)
+    paged_append_fp8(q, k, v, kp.view(E4M3), vp.view(E4M3), ks.view(E8M0), vs.view(E8M0),
+                     torch.arange(pages, dtype=torch.int32, device="cuda")[None], _i32([0, N]), _i32([N]), gq, gk, cos, sin, eps=eps)
+    x = k.double()
+    y = x / (x.pow(2).mean(-1, keepdim=True) + eps).sqrt() * gk.double()
+    a, b = y.chunk(2, -1)
+    c, s = cos.double()[:, None], sin.double()[:, None]
+    y = torch.cat([a * c - b * s, a * s + b * c], -1)
+    off = 2.0 ** -40 * torch.cat([(a * c).abs() + (b * s).abs(), (a * s).abs() + (b * c).abs()], -1)
+    got, scale = kp.transpose(1, 2).reshape(N, heads, D), ks.transpose(1, 2).reshape(N, heads)
+    sides = [_quantised((y + t * off).float()) for t in (-1, 0, 1)]
+    near = (sides[0][0] != sides[2][0]) | (sides[0][1] != sides[2][1])[..., None]
+    print(f"  {int(near.sum())} of {near.numel()} next to a border", flush=True)
+    assert near.sum() <= 8
+    assert torch.equal(torch.where(near, sides[1][0], got), sides[1][0])
+    assert torch.equal(torch.where(near.any(-1), sides[1][1], scale), sides[1][1])
+    kind, unit = _quantised(v)[:2]
+    assert torch.equal(vp.transpose(1, 2).reshape(N, heads, D), kind) and torch.equal(vs.transpose(1, 2).reshape(N, heads), unit)
