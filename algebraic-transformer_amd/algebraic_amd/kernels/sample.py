@@ -26,7 +26,9 @@ def head_logits(h, embed):
     """The logits ``h @ embed.T``, (N, V) float32 with float32 sums.
 
     ``h`` (N, d) bfloat16 or float32, ``embed`` (V, d), cast to ``h``'s dtype as ``fused_head`` does (keep a copy
-    of that dtype for serving: the cast reads and writes the whole table), d a multiple of 8. No gradient.
+    of that dtype for serving: the cast reads and writes the whole table), d a multiple of 8. The order of the sums
+    goes by the shapes, N among them: a row's logits may differ in their last bits between batches of different
+    sizes (never between calls of one shape). No gradient.
     """
     if h.dim() != 2 or embed.dim() != 2 or h.shape[1] != embed.shape[1] or embed.shape[0] == 0:
         raise ValueError(f"h {tuple(h.shape)} and embed {tuple(embed.shape)}: (N, d) and (V, d)")

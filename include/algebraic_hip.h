@@ -446,7 +446,8 @@ int alg_embedding_bwd(alg_stream_t stream, int N, int d, int V, const void* toke
                       int dy_dtype, float scale, void* dtable, int table_dtype, void* workspace, size_t workspace_bytes);
 
 /* The head's logits z (N, V) f32 = h E^T, f32 sums (model.py:225-230's logits): h (N, d) and E (V, d)
- * of one dtype, contiguous, 16-byte aligned, d a multiple of 8. */
+ * of one dtype, contiguous, 16-byte aligned, d a multiple of 8. The order of the sums goes by N, d, V
+ * and the dtype. */
 int alg_head_logits(alg_stream_t stream, int dtype, int N, int d, int V, const void* h, const void* E, float* z);
 
 /* One token a row drawn from the algebraic likelihood (algebraic.py:223-265) of logits z (N, V), f32 or
