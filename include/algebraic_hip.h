@@ -65,7 +65,9 @@ enum { ALG_ATTN_INRANGE = 0, ALG_ATTN_CLIPPED = 1, ALG_ATTN_SHIFTED = 2, ALG_ATT
  * Version 3: adds alg_attn_bwd_sink_logit, alg_head_eval_index64, alg_ffn_block_*, alg_head_plan
  * and alg_ffn_plan; nothing else changed.
  * Version 4: adds alg_add_rms_norm_*, alg_packed_attn_*, alg_paged_attn* and alg_paged_append;
- * nothing else changed. */
+ * nothing else changed.
+ * Version 5: adds alg_paged_*_fp8, alg_embedding_*, alg_head_logits, alg_head_sample* and the dtypes
+ * ALG_DTYPE_F64, _I32 and _I64; nothing else changed. */
 #define ALG_ABI_VERSION 5
 
 const char* alg_last_error(void);
@@ -409,8 +411,8 @@ int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, c
  * the scale 255 and reads as NaN, where it is seen and nowhere else. k_pages, v_pages (pages, Hkv,
  * page, D) bytes, strides in bytes, multiples of 16; k_scales, v_scales (pages, Hkv, page) bytes,
  * places contiguous, strides between pages (_ps) and heads (_hs) multiples of 16; bases 16-byte
- * aligned. Everything else as in the calls without _fp8: alg_paged_append_fp8 forms y in f32 and
- * rounds it once, to 8 bits; alg_paged_attn_fp8 is the attention over the stored values, with their
+ * aligned. Everything else as in the calls without _fp8: alg_paged_append_fp8 forms y in f64, rounds
+ * it to f32 and that to 8 bits (keys) or bf16 (queries); v goes to 8 bits as it is; alg_paged_attn_fp8 is the attention over the stored values, with their
  * products and sums as over a bf16 cache that held them. alg_paged_read_fp8 reads the N tokens'
  * places back into k_out, v_out (N, Hkv, D) bf16, contiguous: behind the last sequence and before
  * position 0 zeros, at a page number outside [0, pages) or a position that the table does not reach
