@@ -39,13 +39,6 @@ __device__ __forceinline__ void loadf8(const float* p, float (&x)[8]) {
   *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
 }
 
-__device__ __forceinline__ float inv_root(float v) { return 1.0f / sqrtf(v); }
-// In f64 the hardware's 1 / sqrt(v), good to half the bits, and one step of Newton's method.
-__device__ __forceinline__ double inv_root(double v) {
-  const double y = __builtin_amdgcn_rsq(v), e = __builtin_fma(-v * y, y, 1.0);
-  return v < INFINITY ? __builtin_fma(0.5 * y, e, y) : y;
-}
-
 // e4m3 of eight values, a power of two scaled away.
 __device__ __forceinline__ uint2 bytes8(const float (&x)[8], float unit) {
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * unit, x[1] * unit, 0, false);
@@ -133,7 +126,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) 
 #pragma unroll
     for (int m = 1; m < LPR; m <<= 1) ss += __shfl_xor(ss, m, 64);
     if (!isv) {
-      const W tau = inv_root(ss * ((W)1 / D) + (W)p.eps);
+      const W tau = (W)1 / sqrt(ss * ((W)1 / D) + (W)p.eps);
       const void* gain = isq ? p.q_gain : p.k_gain;
       float ga[8], gb[8];
 #pragma unroll
