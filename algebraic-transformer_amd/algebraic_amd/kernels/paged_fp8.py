@@ -161,7 +161,8 @@ def paged_flash_attention_fp8(q, k_pages, v_pages, k_scales, v_scales, page_tabl
     """``paged_flash_attention`` of the new tokens q (N, H, D) bf16 over a cache of 8 bits, (N, H, D) bf16.
 
     The values attended to are the stored ones; sinks, positions, zeros and NaN as in
-    ``paged_flash_attention``. The order of every sum is fixed by the shapes.
+    ``paged_flash_attention``. The order of every sum is fixed by the shapes, and so is a weight's form in the second
+    product, as there: two bfloat16 numbers for up to 32 rows a sequence on average, one above.
     """
     if k_pages.dim() != 4:
         raise ValueError("k_pages and v_pages must be (pages, Hkv, page, D)")

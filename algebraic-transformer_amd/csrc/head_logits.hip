@@ -4,8 +4,8 @@
 // Few tokens (and f32): a wave takes 16 rows of E and up to 64 tokens. E goes from memory to registers in
 // its own order, 128 bytes of each row at a time (16x16 MFMA, A = E; lane group g holds 16-byte pieces g and
 // g + 4 of the 128, and h is laid out alike), h through LDS, which the workgroup's waves share. Lane l then
-// holds four neighbouring logits of token l % 16. 5 tokens, d 2048, V 32000, the table from memory: 27 us, 4.9
-// TB/s.
+// holds four neighbouring logits of token l % 16. 5 tokens, d 2048, V 32000, the table from memory: 29 us, 4.5
+// TB/s (22 of two tables in turn, which the last cache holds).
 #include <type_traits>
 
 #include "gemm_core.h"

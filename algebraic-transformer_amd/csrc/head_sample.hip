@@ -17,8 +17,9 @@
 // where the sum is reached, or if that is crowded too, histograms of its keys' bits (at most three more);
 // tokens of one single logit are counted.
 //
-// Latency bounds it. 64 rows of 32000 with settings of each kind: 31 us (best 5, share 10, row 16), 3 rows of 50257,
-// top-p: 24 (3.5, 6.5, 14).
+// 64 rows of 32000 with settings of each kind: 31 us (best 5, share 10, row 16), 3 rows of 50257, top-p: 24 (3.5, 6.5,
+// 14). Instructions bound the first two (VALU 64 and 72 % busy: a token at a time, f64 weights), latency the last: one
+// workgroup a row, which goes over its row once more for the list and then from barrier to barrier (VALU 43 %).
 //
 // One workgroup a row, 16 waves. A lane takes four neighbouring tokens of a tile of 4096, so that a wave's
 // tokens are neighbours and a draw among all tokens needs the sums of waves, then of one wave's lanes.

@@ -25,7 +25,8 @@
 // 203 us, 0.79 PFLOP/s (65, 43: more of their tiles are at the diagonal); 13 documents, 8161 tokens, 16
 // heads, D = 64: 38 us (73, 22). Over a cache, 701 tokens each of 3 requests over 24000 keys, 16 heads over 4: 172 us,
 // 0.77 PFLOP/s, and 12 for joining two ranges.
-// Over a cache of 8 bits the same takes 197 with the join (VALU busy 65 %, matrix cores 39 %).
+// Over a cache of 8 bits the same takes 186 and 10 for the join (VALU busy 65 %, matrix cores 39 %; the first twenty of
+// a process 212).
 // A key head's workgroups are neighbours in steps of Hkv: with 2, 4, 8 key heads each XCD's L2 holds the
 // keys of one, or of the same few, and K and V leave memory about once.
 #include <type_traits>
