@@ -4,7 +4,7 @@ import math
 
 import pytest
 
-from test_step_gpu import BF, F32, F64, SETTINGS, _check_sample, _gen, _sample
+from test_step_gpu import BF, F32, F64, SETTINGS, _captured, _check_embedding, _check_sample, _gen, _logits, _sample, _within
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -170,6 +170,53 @@ def test_sample_a_share_of_equal_logits_in_the_largest_vocabulary():
     _check_sample(z.to(BF), u, top_k=3, left_out=0)
 
 
+def test_sample_more_rows_than_65536():
+    g, rn = _gen(16)
+    z, u = 2 * rn(70001, 40), torch.rand(70001, device="cuda", generator=g)
+    token, logp = _sample()(z, u, top_k=7, top_p=0.9)
+    for rows in (slice(0, 9), slice(65530, 65540), slice(69992, 70001)):
+        _check_sample(z[rows], u[rows], top_k=7, top_p=0.9, left_out=0.2)
+        one = _sample()(z[rows], u[rows], top_k=7, top_p=0.9)
+        assert torch.equal(one[0], token[rows]) and torch.equal(one[1], logp[rows])
+
+
+# --- logits and embedding at the largest sizes that they take ----------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("N,d,V", [(1 << 20, 8, 9), (1, 8, 1 << 24), (33, 8, (1 << 24) - 5), (2, 1 << 20, 20), (70, 1 << 20, 130)])
+def test_logits_at_their_largest(N, d, V, dtype):
+    print(f"[logits] N{N} d{d} V{V} {dtype}", flush=True)
+    g, rn = _gen(N)
+    h, E = rn(N, d).to(dtype), rn(V, d).to(dtype)
+    rows = torch.cat([torch.arange(min(N, 40)), torch.arange(max(0, N - 40), N)]).unique().cuda()
+    cols = torch.cat([torch.arange(min(V, 500)), torch.arange(max(0, V - 500), V), torch.randint(0, V, (500,))]).unique().cuda()
+    z = _logits()(h, E)[rows][:, cols]
+    a, b = h[rows].double(), E[cols].double()
+    _within(z, a @ b.T, (d + 1) * 2.0 ** -24 * (a.abs() @ b.abs().T), "logits")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_logits_of_many_tokens_over_a_table_past_32_bit_offsets(dtype):
+    """Tokens that take the tiled products (bf16), over a table of more than 2^32 bytes."""
+    V, d, N = 1200000, 2048 if dtype is BF else 1024, 600
+    E = torch.zeros(V, d, dtype=dtype, device="cuda")
+    E[-1], E[0], E[700000], E[1048575], E[1048576] = 1.0, 2.0, 3.0, 4.0, 5.0
+    h = torch.ones(N, d, dtype=dtype, device="cuda")
+    h[7] = 2.0
+    z = _logits()(h, E)
+    for v, x in ((-1, 1), (0, 2), (700000, 3), (1048575, 4), (1048576, 5)):
+        assert (z[:7, v] == x * d).all() and (z[7, v] == 2 * x * d).all() and (z[8:, v] == x * d).all(), v
+    assert int(torch.count_nonzero(z)) == 5 * N
+
+
+@pytest.mark.parametrize("N,V,d", [((1 << 24) - 1, 300, 8), ((1 << 24) - 1, (1 << 24) - 1, 8), (100, 70, 1 << 16), (3000, 9, 1 << 16)])
+def test_embedding_at_its_largest(N, V, d):
+    print(f"[embedding] N{N} V{V} d{d}", flush=True)
+    g, rn = _gen(N ^ V)
+    tokens = torch.randint(-1, V + 1, (N,), device="cuda", generator=g)
+    _check_embedding(tokens, rn(V, d), rn(N, d).to(BF), 0.5, BF)
+
+
 # --- the 8-bit cache --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("D,heads", [(64, 16), (128, 8)])
@@ -205,3 +252,106 @@ def test_append_stores_the_bytes_of_the_64_bit_statement(D, heads):
     assert torch.equal(torch.where(near.any(-1), sides[1][1], scale), sides[1][1])
     kind, unit = _quantised(v)[:2]
     assert torch.equal(vp.transpose(1, 2).reshape(N, heads, D), kind) and torch.equal(vs.transpose(1, 2).reshape(N, heads), unit)
+
+
+def _held8(S, width, page, new, H, Hkv, D, seed):
+    """Queries, an 8-bit cache whose every place is filled, its table, and each sequence's stored keys and values."""
+    from test_paged_fp8_gpu import E4M3, E8M0, _quantised
+    from test_serving_edges_gpu import _held
+    q, kp, vp, table, s, _, _ = _held(S, width, page, new, H, Hkv, D, seed)
+    (k8, ksc, k), (v8, vsc, v) = _quantised(kp), _quantised(vp)
+    rows = lambda t, i: t[table[i].long()].transpose(1, 2).flatten(0, 1)  # noqa: E731
+    return q, (k8.view(E4M3), v8.view(E4M3), ksc.view(E8M0), vsc.view(E8M0)), table, s, [rows(k, i) for i in range(S)], [rows(v, i) for i in range(S)]
+
+
+def _check_attention8(q, cache, table, new, kv, sink, ks, vs, what=""):
+    """Each sequence's tokens against float64; before position 0 zeros, from the table's end on NaN."""
+    from algebraic_amd import paged_flash_attention_fp8
+    from packed_ref import check
+    from test_paged_gpu import _i32, _starts
+    from test_serving_edges_gpu import _row
+    at, reach = _starts(new), table.shape[1] * cache[0].shape[2]
+    o = paged_flash_attention_fp8(q, *cache, table, _i32(at), _i32(kv), sink, n=16, c=8.0)
+    for i, m in enumerate(new):
+        pos = torch.arange(kv[i] - m, kv[i], device="cuda") if kv[i] < 1 << 30 else torch.full((m,), reach, device="cuda")
+        rows = o[at[i]:at[i + 1]]
+        assert not rows[pos < 0].any() and torch.isnan(rows[pos >= reach]).all(), (what, i)
+        live = (pos >= 0) & (pos < reach)
+        if live.any():
+            held = min(kv[i], reach)
+            check({"o": rows[live]}, *_row(q[at[i]:at[i + 1]][live], ks[i][:held], vs[i][:held], sink, pos[live]), f"{what} {i}")
+    assert not o[at[-1]:].any()
+    return o
+
+
+@pytest.mark.parametrize("new,width,past,H,Hkv", [([2, 1], 2, 1, 4, 2), ([1, 1], 3, 1, 4, 2), ([40, 1], 4, 39, 4, 1), ([150, 3], 10, 40, 4, 2),
+                                                  ([150, 3], 11, 150, 4, 2), ([2], 562, 1, 4, 1), ([200], 375, 50, 2, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("sink", [False, True])
+def test_attention8_of_lengths_past_the_table(new, width, past, H, Hkv, D, sink):
+    q, cache, table, s, ks, vs = _held8(len(new), width, 16, new, H, Hkv, D, seed=sum(new) + D)
+    for kv in ([16 * width + past] + [16 * width - 1] * (len(new) - 1), [(1 << 31) - 1] + [min(20, 16 * width)] * (len(new) - 1)):
+        _check_attention8(q, cache, table, new, kv, s if sink else None, ks, vs, f"{new} {kv}")
+
+
+@pytest.mark.parametrize("new,width", [([1, 1], 4), ([1, 1], 2000), ([1], 8192), ([2, 1], 40), ([60, 40], 4), ([150], 400)],
+                         ids=["whole", "ranges", "many-ranges", "two", "chunks", "chunk-in-ranges"])
+@pytest.mark.parametrize("G", [1, 4])
+def test_attention8_of_a_switched_off_sink_and_rows_without_keys(new, width, G):
+    q, cache, table, s, ks, vs = _held8(len(new), width, 16, new, 2 * G, 2, 64, seed=width + G)
+    s[0] = s[-1] = -math.inf
+    _check_attention8(q, cache, table, new, [0] * len(new), s, ks, vs)
+    _check_attention8(q, cache, table, new, [new[0] // 2] + [50] * (len(new) - 1), s, ks, vs)
+
+
+@pytest.mark.parametrize("S,H,Hkv,D,m", [(65, 2, 1, 64, 1), (100, 2, 1, 128, 1), (66, 2, 1, 64, 40), (70, 2, 1, 128, 40)])
+def test_attention8_of_many_sequences_in_ranges(S, H, Hkv, D, m):
+    from algebraic_amd import _lib
+    new = [m + (i % 11 if m > 1 else 0) for i in range(S)]
+    kv = [1000 + (811 * i) % 2000 for i in range(S)]
+    kv[3], kv[5] = new[3], new[5]  # ranges without a key
+    width = -(-max(kv) // 16)
+    assert _lib.load().alg_paged_attn_fp8_workspace_size(sum(new), S, H, Hkv, D, width, 16) > 0
+    q, cache, table, s, ks, vs = _held8(S, width, 16, new, H, Hkv, D, seed=S)
+    _check_attention8(q, cache, table, new, kv, s, ks, vs)
+
+
+@pytest.mark.parametrize("H,Hkv", [(128, 1), (64, 2), (4, 2)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention8_of_prompts_and_single_tokens_in_one_call(H, Hkv, D):
+    """The average of the rows chooses the kernel; single tokens with many heads to a key head take the prompts'."""
+    for new, kv in (([300, 1, 1, 1, 1], [300, 900, 17, 1, 500]), ([1, 1, 20, 1], [1400, 3, 20, 64]), ([1, 1], [200, 31])):
+        width = -(-max(kv) // 16)
+        q, cache, table, s, ks, vs = _held8(len(new), width, 16, new, H, Hkv, D, seed=H + D)
+        _check_attention8(q, cache, table, new, kv, s, ks, vs, f"{new}")
+
+
+def test_append_and_attention8_captured_over_ranges():
+    """A step of single tokens over two ranges and more, captured twice over the same buffers, whose replays alone write
+    the cache; every replay is checked against the eager calls over a copy."""
+    from algebraic_amd import paged_append_fp8, paged_flash_attention_fp8
+    from test_paged_gpu import _i32
+    S, H, Hkv, D, width, page = 3, 8, 2, 64, 130, 16
+    q, cache, table, sink, _, _ = _held8(S, width, page, [1] * S, H, Hkv, D, seed=3)
+    g, rn = _gen(17)
+    k, v = (rn(S, Hkv, D).to(BF) for _ in range(2))
+    cu, kv = _i32([0, 1, 2, 3]), _i32([1200, 2000, 1])
+    copy = tuple(t.clone() for t in cache)
+
+    def step(cache):
+        return paged_flash_attention_fp8(paged_append_fp8(q, k, v, *cache, table, cu, kv), *cache, table, cu, kv, sink, n=16, c=8.0)
+
+    graphs = _captured(lambda: step(cache))
+    for t, c in zip(cache, copy):  # as before the warm-up
+        t.view(torch.uint8).copy_(c.view(torch.uint8))
+    for i in range(6):
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, device="cuda"))
+        kv += 1
+        want = step(copy)
+        torch.cuda.synchronize()
+        graph, out = graphs[i % 2]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, copy)), i
