@@ -1574,8 +1574,8 @@ static int check_table(int width, int page, int pages) {
 // one range, 2, 4: 4 to 128 groups (sequences x key heads) of 600 keys 18 22 22, 850 keys 18 22 22, 1210 keys 20.5 to
 // 22 22 22, 1700 keys 26 to 28 22 22; 256 groups of 600 18 22 22, 1210 23 26 30, 1700 29 31 33. (In a captured graph,
 // without the host, splitting would gain sooner: 4 to 64 groups of 600 keys 15 14.5 14.5, 850 18 15 15, 1210 21 17.7
-// 15.4; 256 groups lose as above, 9 % at 1300 keys each, where the rule takes 2.) us of one range, of 256, 512 and 768 workgroups, calls included: 64
-// groups (sequences x key heads) of 4000 keys on average, the longest 12000: 80 31.5 26.8 26.5; of 16000 and 48000: 60
+// 15.4; 256 groups lose as above, 7 % at 1300 keys each, where the rule takes 2.) us of one range, of 256, 512 and 768
+// workgroups, calls included: 64 groups of 4000 keys on average, the longest 12000: 80 31.5 26.8 26.5; of 16000 and 48000: 60
 // 60 and 88 64 63 (256, 512 and 768); 256 groups, the same 4000: 84 84 66 65, all
 // of 4000 59 59 60 61; 320 groups, the longest thrice the average, of 4000: 84 84 78 78 (2 ranges from 512 on; 3 76); 512
 // groups of 3170 91, of 2 ranges 88, others 101 and 106; 600 keys: 20 unsplit, 23 to 24 split. One
@@ -1589,7 +1589,7 @@ static int check_table(int width, int page, int pages) {
 // 9000, 16 over 4 (240): 178 117 104 106 113, 2, a tenth over the best; 46 each over 12000 to 40000, 32 over 8 (112): 749 401 290
 // 234 210, 6; 459 each over 12 x 2393, 8 over 1 (348): 87 89 100 103 108, 1; 645 over 9319, 32 over 4 (164):
 // 187 158 129 144 147, 3; 300 over 30000, 16 over 4 (40): 562 300 210 163 137, 119 of 6, 135 of 8, takes 6.
-// A key of 8 bits takes 15 % more, and the estimate is the same: of 1 to 8 ranges it takes the best or one within 9 %
+// A key of 8 bits takes 15 % more, and the estimate is the same: of 1 to 8 ranges it takes the best or one within 12 %
 // at D = 128 (the first of those calls 283 202 201 203 197, takes 2; 100 each of 8 over 24000 in all 130 80 64 57 63, 3),
 // within 20 % at D = 64 (211 151 137 132 131, 2; 99 61 49 45 43, 3), whose keys take three quarters as long.
 struct PagedPlan {

@@ -6,7 +6,7 @@
 // next to a border, and V = 32000 borders lie everywhere. So the weights are f64, relative to the
 // row's largest, and are summed as whole numbers of 2^-bits (2^62 / V): such sums are
 // equal in any order, among any number of lanes and atomics, and a row's token depends on the row alone.
-// log2 rho is good to 2^-44.8 (log2_rho), so a weight to (n / T) 2^-44 of itself, beside 2^-50 for the power of two:
+// log2 rho is good to 2^-44.7 (log2_rho), so a weight to (n / T) 2^-44 of itself, beside 2^-50 for the power of two:
 // 2^-41 at n / T = 8, 2^-34 at 1024, and nothing is left of it where n / T passes 2^44. Which logit is the largest, and
 // the order by logits, are exact at any temperature.
 //
@@ -224,7 +224,7 @@ struct Sampler {
     __device__ __forceinline__ bool operator()(int) const { return false; }
   };
 
-  // log2 rho(x) = log2(|x| + sqrt(1 + x^2)), to 2^-44.8: the root is q rsqrt(q), the hardware's (to 2^-23 of itself)
+  // log2 rho(x) = log2(|x| + sqrt(1 + x^2)), to 2^-44.7: the root is q rsqrt(q), the hardware's (to 2^-23 of itself)
   // with one step of Newton's method, which leaves 3/2 of the square, 2^-45.4; log2 2^-48. (2^22 of both signs: 2^-47.4.)
   __device__ __forceinline__ double log2_rho(unsigned key) const {
     const double x = key == KEY_CLAMPED ? p.clamp : (double)key_logit(key) * p.inv_c, a = __builtin_fabs(x);
