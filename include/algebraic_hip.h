@@ -414,9 +414,9 @@ int alg_paged_append(alg_stream_t stream, int N, int S, int H, int Hkv, int D, c
  * aligned. Everything else as in the calls without _fp8: alg_paged_append_fp8 forms y in f64, rounds
  * it to f32 and that to 8 bits (keys) or bf16 (queries); v goes to 8 bits as it is;
  * alg_paged_attn_fp8 is the attention over the stored values, with their products and sums as over a
- * bf16 cache that held them. alg_paged_read_fp8 reads the N tokens' places back into k_out, v_out (N, Hkv, D) bf16, contiguous: behind the last sequence and before
- * position 0 zeros, at a page number outside [0, pages) or a position that the table does not reach
- * NaN. */
+ * bf16 cache that held them. alg_paged_read_fp8 reads the N tokens' places back into k_out, v_out
+ * (N, Hkv, D) bf16, contiguous: behind the last sequence and before position 0 zeros, at a page
+ * number outside [0, pages) or a position that the table does not reach NaN. */
 int alg_paged_append_fp8(alg_stream_t stream, int N, int S, int H, int Hkv, int D, const void* q, long q_ts, long q_hs,
                          const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, void* k_pages, long k_ps,
                          long kp_hs, long kp_ts, void* v_pages, long v_ps, long vp_hs, long vp_ts, void* k_scales, long ks_ps,
